@@ -1444,6 +1444,58 @@ extern "C" int moe_swiglu_fwd_fp8(const void* xq, const float* sx, const void* w
   return launch<2, 2, 0, 0, kNW_fp8>("k_gemm_swiglu_fwd2_fp8", s, b, R);
 }
 
+namespace moe {
+// The row-grouped products of the backward, over the tile table that swiglu_tiles has put into the workspace (common.h).
+int swiglu_tiles(const int* offsets, int64_t E, void* workspace, hipStream_t s) {
+  launch_tiles(s, offsets, E, static_cast<int*>(workspace), nullptr);
+  return check_launch("k_gemm_tiles");
+}
+
+// dA: dh = epilogue(dy . Wd)   (B[n=f][k=h] = Wd[h][f])
+int swiglu_dact(const void* dy, const void* hgu, const void* w_down, const int* offsets, int64_t R, int64_t H, int64_t F,
+                int64_t E, void* dh, const void* workspace, hipStream_t s) {
+  GemmArgs a{};
+  a.offsets = offsets;
+  a.tile_off = static_cast<const int*>(workspace);
+  a.E = (int)E;
+  a.F = (int)F;
+  a.A = static_cast<const uint16_t*>(dy);
+  a.lda = H;
+  a.B = static_cast<const uint16_t*>(w_down);
+  a.ldb = F;
+  a.b_estride = H * F;
+  a.C = static_cast<uint16_t*>(dh);
+  a.ldc = 2 * F;
+  a.X = static_cast<const uint16_t*>(hgu);
+  a.N = (int)F;
+  a.K = (int)H;
+  return launch<0, 1, 0, 2, kNW_dact>("k_gemm_swiglu_dact", s, a, R);
+}
+
+// dxp = dh . [Wg ; Wu]   (B[n=h][k=j] = W1[j][h])
+int swiglu_dxp(const void* dh, const void* w_gate, const void* w_up, const int* offsets, int64_t R, int64_t H, int64_t F,
+               int64_t E, void* dxp, void* workspace, size_t ws_bytes, hipStream_t s) {
+  GemmArgs a{};
+  a.offsets = offsets;
+  a.tile_off = static_cast<const int*>(workspace);
+  a.E = (int)E;
+  a.F = (int)F;
+  a.A = static_cast<const uint16_t*>(dh);
+  a.lda = 2 * F;
+  a.B = static_cast<const uint16_t*>(w_gate);
+  a.B2 = static_cast<const uint16_t*>(w_up);
+  a.b_split = (int)F;
+  a.ldb = H;
+  a.b_estride = F * H;
+  a.C = static_cast<uint16_t*>(dxp);
+  a.ldc = H;
+  a.N = (int)H;
+  a.K = (int)(2 * F);
+  take_split(a, R, workspace, ws_bytes, moe_swiglu_workspace(E));
+  return launch<0, 1, 0, 0, kNW_dxp>("k_gemm_swiglu_dxp", s, a, R);
+}
+}  // namespace moe
+
 extern "C" int moe_swiglu_bwd(const void* dy, const void* xp, const void* act, const void* hgu, const void* w_gate,
                               const void* w_up, const void* w_down, const int32_t* offsets, int64_t R, int64_t H,
                               int64_t F, int64_t E, void* dh, void* dxp, void* dw_gate, void* dw_up, void* dw_down,
@@ -1456,48 +1508,11 @@ extern "C" int moe_swiglu_bwd(const void* dy, const void* xp, const void* act, c
     return fail_arg("moe_swiglu_bwd: null pointer argument");
   if (ws_bytes < moe_swiglu_workspace(E) || !workspace) return set_error("moe_swiglu_bwd: workspace"), MOE_EWORKSPACE;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  int* tile_off = static_cast<int*>(workspace);
-  int* korder = tile_off + (E + 1);
-  launch_tiles(s, offsets, E, tile_off, korder);
-  // dA: dh = epilogue(dy . Wd)   (B[n=f][k=h] = Wd[h][f])
+  int* korder = static_cast<int*>(workspace) + (E + 1);
+  launch_tiles(s, offsets, E, static_cast<int*>(workspace), korder);
   if (R > 0) {
-    GemmArgs a{};
-    a.offsets = offsets;
-    a.tile_off = tile_off;
-    a.E = (int)E;
-    a.F = (int)F;
-    a.A = static_cast<const uint16_t*>(dy);
-    a.lda = H;
-    a.B = static_cast<const uint16_t*>(w_down);
-    a.ldb = F;
-    a.b_estride = H * F;
-    a.C = static_cast<uint16_t*>(dh);
-    a.ldc = 2 * F;
-    a.X = static_cast<const uint16_t*>(hgu);
-    a.N = (int)F;
-    a.K = (int)H;
-    if (int rc = launch<0, 1, 0, 2, kNW_dact>("k_gemm_swiglu_dact", s, a, R)) return rc;
-  }
-  // dxp = dh . [Wg ; Wu]   (B[n=h][k=j] = W1[j][h])
-  if (R > 0) {
-    GemmArgs a{};
-    a.offsets = offsets;
-    a.tile_off = tile_off;
-    a.E = (int)E;
-    a.F = (int)F;
-    a.A = static_cast<const uint16_t*>(dh);
-    a.lda = 2 * F;
-    a.B = static_cast<const uint16_t*>(w_gate);
-    a.B2 = static_cast<const uint16_t*>(w_up);
-    a.b_split = (int)F;
-    a.ldb = H;
-    a.b_estride = F * H;
-    a.C = static_cast<uint16_t*>(dxp);
-    a.ldc = H;
-    a.N = (int)H;
-    a.K = (int)(2 * F);
-    take_split(a, R, workspace, ws_bytes, moe_swiglu_workspace(E));
-    if (int rc = launch<0, 1, 0, 0, kNW_dxp>("k_gemm_swiglu_dxp", s, a, R)) return rc;
+    if (int rc = swiglu_dact(dy, hgu, w_down, offsets, R, H, F, E, dh, workspace, s)) return rc;
+    if (int rc = swiglu_dxp(dh, w_gate, w_up, offsets, R, H, F, E, dxp, workspace, ws_bytes, s)) return rc;
   }
   // dWd_e = dy_e^T . act_e   (M = H, N = F, K = rows of e)
   {

@@ -451,6 +451,111 @@ std::vector<at::Tensor> op_swiglu_backward(const at::Tensor& dy, const at::Tenso
   return {dxp, dwg, dwu, dwd};
 }
 
+// ---- MXFP4 experts ----
+
+std::tuple<at::Tensor, at::Tensor> op_quant_mxfp4(const at::Tensor& t_in) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(t_in.device());
+  const at::Tensor t = t_in.contiguous();
+  std::vector<int64_t> qs = t.sizes().vec(), ss = qs;
+  const int64_t cols = qs.back(), rows = t.numel() / cols;
+  qs.back() = cols / 2;
+  ss.back() = cols / 32;
+  const auto u8 = t.options().dtype(at::kByte);
+  at::Tensor q = at::empty(qs, u8), sc = at::empty(ss, u8);
+  check_rc(moe_quant_mxfp4(t.data_ptr(), code_of(t), rows, cols, q.data_ptr(), sc.data_ptr(), stream_of(t)),
+           "moe_quant_mxfp4");
+  return {q, sc};
+}
+
+at::Tensor op_dequant_mxfp4(const at::Tensor& q_in, const at::Tensor& sc_in, bool bf16) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q_in.device());
+  const at::Tensor q = q_in.contiguous(), sc = sc_in.contiguous();
+  std::vector<int64_t> vs = q.sizes().vec();
+  vs.back() *= 2;
+  at::Tensor v = at::empty(vs, q.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  const int64_t cols = vs.back(), rows = v.numel() / cols;
+  check_rc(moe_dequant_mxfp4(q.data_ptr(), sc.data_ptr(), rows, cols, v.data_ptr(), bf16 ? MOE_BF16 : MOE_F32, stream_of(q)),
+           "moe_dequant_mxfp4");
+  return v;
+}
+
+// wq, ws: the quantized gate [E, F, H], up [E, F, H] and down [E, H, F] matrices and their scales, contiguous.
+std::tuple<OptTensor, at::Tensor> op_swiglu_forward_mxfp4(const at::Tensor& xp_in, const std::vector<at::Tensor>& wq,
+                                                          const std::vector<at::Tensor>& ws, const at::Tensor& offsets,
+                                                          bool keep_preact) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(xp_in.device());
+  const at::Tensor xp = xp_in.contiguous();
+  const int64_t R = xp.size(0), H = xp.size(1), E = wq[0].size(0), F = wq[0].size(1);
+  at::Tensor y = at::empty({R, H}, xp.options());
+  OptTensor hgu;
+  if (keep_preact) hgu = at::empty({R, 2 * F}, xp.options());
+  const size_t nbytes = moe_swiglu_fwd_mxfp4_workspace(R, H, F, E);
+  const at::Tensor w = scratch(nbytes, xp);
+  check_rc(moe_swiglu_fwd_mxfp4(xp.data_ptr(), wq[0].data_ptr(), ws[0].data_ptr(), wq[1].data_ptr(), ws[1].data_ptr(),
+                                wq[2].data_ptr(), ws[2].data_ptr(), offsets.data_ptr<int>(), R, H, F, E,
+                                const_cast<void*>(ptr(hgu)), y.data_ptr(), w.data_ptr(), nbytes, stream_of(xp)),
+           "moe_swiglu_fwd_mxfp4");
+  return {hgu, y};
+}
+
+at::Tensor op_swiglu_backward_mxfp4(const at::Tensor& dy_in, const at::Tensor& hgu_in, const std::vector<at::Tensor>& wq,
+                                    const std::vector<at::Tensor>& ws, const at::Tensor& offsets) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dy_in.device());
+  const at::Tensor dy = dy_in.contiguous(), hgu = hgu_in.contiguous();
+  const int64_t R = dy.size(0), H = dy.size(1), E = wq[0].size(0), F = wq[0].size(1);
+  at::Tensor dxp = at::empty({R, H}, dy.options());
+  const size_t nbytes = moe_swiglu_bwd_mxfp4_workspace(R, H, F, E);
+  const at::Tensor w = scratch(nbytes, dy);
+  check_rc(moe_swiglu_bwd_mxfp4(dy.data_ptr(), hgu.data_ptr(), wq[0].data_ptr(), ws[0].data_ptr(), wq[1].data_ptr(),
+                                ws[1].data_ptr(), wq[2].data_ptr(), ws[2].data_ptr(), offsets.data_ptr<int>(), R, H, F, E,
+                                dxp.data_ptr(), w.data_ptr(), nbytes, stream_of(dy)),
+           "moe_swiglu_bwd_mxfp4");
+  return dxp;
+}
+
+// ---- the balance loss of sequences ----
+
+std::vector<at::Tensor> op_balance_forward(const at::Tensor& logits_in, const at::Tensor& idx_in, const OptTensor& off_in,
+                                           const OptTensor& mask_in, double balance_coef, double z_coef) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits_in.device());
+  const at::Tensor logits = logits_in.contiguous(), idx = idx_in.contiguous();
+  OptTensor off, mask;
+  if (off_in.has_value()) off = off_in->to(at::kLong).contiguous();
+  if (mask_in.has_value()) mask = mask_in->contiguous();
+  const int64_t N = logits.size(0), E = logits.size(1), K = idx.size(1), S = off.has_value() ? off->size(0) - 1 : 1;
+  const auto f32 = logits.options();
+  const auto i64 = logits.options().dtype(at::kLong);
+  at::Tensor balance = at::empty({}, f32), z = at::empty({}, f32), counts = at::empty({S, E}, i64);
+  at::Tensor tokens = at::empty({S + 2}, i64), mean_prob = at::empty({S, E}, f32);
+  const hipStream_t s = stream_of(logits);
+  const size_t nbytes = moe_balance_fwd_workspace(N, E, S);
+  const FwdWorkspace ws(nbytes, logits.device(), s);
+  check_rc(moe_balance_fwd(logits.data_ptr<float>(), idx.data_ptr<int64_t>(), static_cast<const int64_t*>(ptr(off)),
+                           static_cast<const uint8_t*>(ptr(mask)), N, E, K, S, (float)balance_coef, (float)z_coef,
+                           balance.data_ptr<float>(), z.data_ptr<float>(), counts.data_ptr<int64_t>(),
+                           tokens.data_ptr<int64_t>(), mean_prob.data_ptr<float>(), ws.data_ptr(), nbytes, s),
+           "moe_balance_fwd");
+  return {balance, z, counts, tokens, mean_prob};
+}
+
+at::Tensor op_balance_backward(const at::Tensor& logits_in, const at::Tensor& counts_in, const at::Tensor& tokens_in,
+                               int64_t K, const OptTensor& off_in, const OptTensor& mask_in, const OptTensor& grad_b,
+                               const OptTensor& grad_z, double balance_coef, double z_coef) {
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits_in.device());
+  const at::Tensor logits = logits_in.contiguous(), counts = counts_in.contiguous(), tokens = tokens_in.contiguous();
+  OptTensor off, mask;
+  if (off_in.has_value()) off = off_in->to(at::kLong).contiguous();
+  if (mask_in.has_value()) mask = mask_in->contiguous();
+  const int64_t N = logits.size(0), E = logits.size(1), S = counts.size(0);
+  at::Tensor d = at::empty_like(logits);
+  check_rc(moe_balance_bwd(logits.data_ptr<float>(), counts.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(),
+                           static_cast<const int64_t*>(ptr(off)), static_cast<const uint8_t*>(ptr(mask)),
+                           static_cast<const float*>(ptr(grad_b)), static_cast<const float*>(ptr(grad_z)), N, E, K, S,
+                           (float)balance_coef, (float)z_coef, d.data_ptr<float>(), stream_of(logits)),
+           "moe_balance_bwd");
+  return d;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_moe_torch, m) {
@@ -471,4 +576,10 @@ PYBIND11_MODULE(_moe_torch, m) {
   m.def("unpermute_sum", &op_unpermute_sum, nogil);
   m.def("swiglu_forward", &op_swiglu_forward, nogil);
   m.def("swiglu_backward", &op_swiglu_backward, nogil);
+  m.def("quant_mxfp4", &op_quant_mxfp4, nogil);
+  m.def("dequant_mxfp4", &op_dequant_mxfp4, nogil);
+  m.def("swiglu_forward_mxfp4", &op_swiglu_forward_mxfp4, nogil);
+  m.def("swiglu_backward_mxfp4", &op_swiglu_backward_mxfp4, nogil);
+  m.def("balance_forward", &op_balance_forward, nogil);
+  m.def("balance_backward", &op_balance_backward, nogil);
 }

@@ -82,6 +82,23 @@ _SIGNATURES = {
     "moe_swiglu_fwd_fp8": (
         _I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ, _P]
     ),
+    "moe_quant_mxfp4": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P]),
+    "moe_dequant_mxfp4": (_I32, [_P, _P, _I64, _I64, _P, _I32, _P]),
+    "moe_swiglu_fwd_mxfp4_workspace": (_SZ, [_I64, _I64, _I64, _I64]),
+    "moe_swiglu_fwd_mxfp4": (
+        _I32, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _SZ, _P]
+    ),
+    "moe_swiglu_bwd_mxfp4_workspace": (_SZ, [_I64, _I64, _I64, _I64]),
+    "moe_swiglu_bwd_mxfp4": (
+        _I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _SZ, _P]
+    ),
+    "moe_balance_fwd_workspace": (_SZ, [_I64, _I64, _I64]),
+    "moe_balance_fwd": (
+        _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _F32, _F32, _P, _P, _P, _P, _P, _P, _SZ, _P]
+    ),
+    "moe_balance_bwd": (
+        _I32, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _F32, _F32, _P, _P]
+    ),
     "moe_telemetry_fields": (_I32, []),
     "moe_telemetry_record": (_I32, [_P, _I64, _I64, _I64, _F32, _P, _I64, _P, _I64, _P]),
     "moe_swiglu_workspace": (_SZ, [_I64]),

@@ -459,3 +459,169 @@ def swiglu_backward(dy, xp, act, hgu, w_gate, w_up, w_down, offsets):
     _, _ = xp.shape
     _, _, _ = w_gate.shape
     return tuple(L.native().swiglu_backward(dy, xp, act, hgu, w_gate, w_up, w_down, offsets))
+
+
+# ---------------------------------------------------------------------------
+# Experts held in 4 bits (MXFP4)
+# ---------------------------------------------------------------------------
+MXFP4_BLOCK = 32
+
+
+def quant_mxfp4(t: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of ``t`` [..., cols] (bf16 / fp32, cols % 32 == 0) in MXFP4: (e2m1 pairs uint8 [..., cols / 2], the even
+    column in the low half; E8M0 scale bytes uint8 [..., cols / 32]).  Every 32 consecutive elements share the scale
+    2^e, e the smallest integer with absmax <= 6 * 2^e (in [-124, 125]), stored as e + 127; elements are x * 2^-e rounded
+    to nearest even, at most 6.  A block that holds an infinity or a NaN stands for NaNs (scale byte 255)."""
+    L.require_device(t)
+    L.dtype_code(t.dtype)
+    if t.dim() < 1 or t.shape[-1] % MXFP4_BLOCK or t.shape[-1] == 0:
+        raise ValueError(f"quant_mxfp4: the last dim must be a positive multiple of {MXFP4_BLOCK}, got {list(t.shape)}")
+    return L.native().quant_mxfp4(t.detach())
+
+
+def dequant_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [..., cols] that :func:`quant_mxfp4`'s bytes stand for (exact in bf16 and fp32)."""
+    L.require_device(q, scale)
+    L.dtype_code(dtype)
+    if q.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        raise TypeError("dequant_mxfp4: q and scale are uint8")
+    if q.dim() < 1 or q.shape[-1] == 0 or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != scale.shape[-1] * 16:
+        raise ValueError(f"dequant_mxfp4: q {list(q.shape)} needs scales [..., {q.shape[-1] // 16}], "
+                         f"got {list(scale.shape)}")
+    return L.native().dequant_mxfp4(q, scale, dtype == torch.bfloat16)
+
+
+def _mxfp4_experts(what: str, wq, wscale, H: int, offsets: torch.Tensor):
+    """Checks of the three quantized matrices (gate, up [E, F, H]; down [E, H, F]) and the row offsets [E + 1]."""
+    wg, wu, wd = wq
+    sg, su, sd = wscale
+    for t in (wg, wu, wd, sg, su, sd):
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.dim() != 3:
+            raise TypeError(f"{what}: quantized weights and scales are contiguous uint8 of rank 3")
+    E, F, _ = wg.shape
+    if H % MXFP4_BLOCK or F % MXFP4_BLOCK:
+        raise ValueError(f"{what}: hidden and ffn dims must be multiples of {MXFP4_BLOCK} (got {H} and {F})")
+    for name, t, shape in (("gate", wg, (E, F, H // 2)), ("up", wu, (E, F, H // 2)), ("down", wd, (E, H, F // 2)),
+                           ("gate scale", sg, (E, F, H // 32)), ("up scale", su, (E, F, H // 32)),
+                           ("down scale", sd, (E, H, F // 32))):
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{what}: {name} must be {list(shape)}, got {list(t.shape)}")
+    if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or not offsets.is_contiguous():
+        raise ValueError(f"{what}: offsets must be contiguous int32 [{E + 1}]")
+    return [wg, wu, wd], [sg, su, sd], F
+
+
+def swiglu_forward_mxfp4(xp, wq, wscale, offsets, keep_preact: bool = True):
+    """Forward of the SwiGLU experts on 4-bit weights: ``xp`` [R, H] bf16 rows grouped by expert (``offsets`` [E + 1]
+    int32), ``wq`` = (gate [E, F, H / 2], up [E, F, H / 2], down [E, H, F / 2]) with ``wscale`` = their scales, as
+    :func:`quant_mxfp4` gives them for [E, F, H], [E, F, H] and [E, H, F] -> (hgu [R, 2F] or None, y [R, H]) bf16.
+    ``act = silu(g) u`` is rounded to bf16 between the projections.  From one row to many; rows past offsets[E] are left
+    unwritten.  ``keep_preact=False`` (no backward follows) skips storing the pre-activations: hgu is None."""
+    L.require_device(xp, *wq, *wscale, offsets)
+    if xp.dtype != torch.bfloat16:
+        raise TypeError(f"swiglu_forward_mxfp4: rows are bfloat16, got {xp.dtype}")
+    R, H = xp.shape
+    wq, wscale, F = _mxfp4_experts("swiglu_forward_mxfp4", wq, wscale, H, offsets)
+    if R == 0:
+        return (xp.new_empty((0, 2 * F)) if keep_preact else None), xp.new_empty((0, H))
+    return L.native().swiglu_forward_mxfp4(xp, wq, wscale, offsets, bool(keep_preact))
+
+
+def swiglu_backward_mxfp4(dy, hgu, wq, wscale, offsets):
+    """Gradient of the rows of :func:`swiglu_forward_mxfp4` (the 4-bit weights are constants): ``dy`` [R, H] and the
+    forward's ``hgu`` [R, 2F], bf16 -> dxp [R, H] bf16."""
+    L.require_device(dy, hgu, *wq, *wscale, offsets)
+    if dy.dtype != torch.bfloat16 or hgu.dtype != torch.bfloat16:
+        raise TypeError("swiglu_backward_mxfp4: dy and hgu are bfloat16")
+    R, H = dy.shape
+    wq, wscale, F = _mxfp4_experts("swiglu_backward_mxfp4", wq, wscale, H, offsets)
+    if tuple(hgu.shape) != (R, 2 * F):
+        raise ValueError(f"swiglu_backward_mxfp4: hgu must be [{R}, {2 * F}], got {list(hgu.shape)}")
+    if R == 0:
+        return dy.new_empty((0, H))
+    return L.native().swiglu_backward_mxfp4(dy, hgu, wq, wscale, offsets)
+
+
+# ---------------------------------------------------------------------------
+# Balance loss of sequences
+# ---------------------------------------------------------------------------
+def _balance_check(what, logits, N, seq_offsets, token_mask):
+    if logits.dtype != torch.float32 or logits.dim() != 2:
+        raise TypeError(f"{what}: logits must be float32 [N, E]")
+    if seq_offsets is not None:
+        if seq_offsets.dtype not in (torch.int64, torch.int32) or seq_offsets.dim() != 1 or seq_offsets.shape[0] < 2:
+            raise ValueError(f"{what}: seq_offsets must be int64 or int32 [S + 1], S >= 1")
+    if token_mask is not None:
+        if token_mask.dtype != torch.bool or token_mask.numel() != N:
+            raise ValueError(f"{what}: token_mask must be bool with one value a token ({N})")
+        token_mask = token_mask.reshape(-1)
+    return token_mask
+
+
+def balance_loss_forward(
+    logits: torch.Tensor,
+    idx: torch.Tensor,
+    seq_offsets: Optional[torch.Tensor] = None,
+    token_mask: Optional[torch.Tensor] = None,
+    balance_coef: float = 1.0,
+    z_coef: float = 0.0,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Load balance of the choices ``idx`` [N, K] (int64) within each sequence, and the z-loss, over valid tokens.
+
+    Sequence s holds the tokens [seq_offsets[s], seq_offsets[s + 1]) (nondecreasing, in [0, N]; None: one sequence of all
+    tokens); ``token_mask`` (bool, one value a token) marks the valid ones (None: all).  Tokens of no sequence, and those
+    that are not valid, are left out whatever they hold.  With n_s valid tokens in sequence s, c_se their choices of expert
+    e and p = softmax(logits):
+
+        balance = balance_coef * mean over sequences with n_s > 0 of sum_e (E c_se / (K n_s)) mean_t p[t, e]
+        z       = z_coef * mean over valid tokens of logsumexp(logits_t)^2
+
+    Returns ``(balance, z, counts int64 [S, E], tokens int64 [S + 2], mean_prob f32 [S, E])``: counts is c, tokens the
+    valid tokens of each sequence, then of all, then the number of sequences that have any.  With one sequence and no mask
+    ``balance`` is the router's aux loss."""
+    L.require_device(logits, idx, seq_offsets, token_mask)
+    N, E = logits.shape
+    token_mask = _balance_check("balance_loss_forward", logits, N, seq_offsets, token_mask)
+    if idx.dtype != torch.int64 or idx.dim() != 2 or idx.shape[0] != N:
+        raise ValueError(f"balance_loss_forward: idx must be int64 [{N}, K]")
+    S = 1 if seq_offsets is None else seq_offsets.shape[0] - 1
+    if N == 0:
+        f32 = dict(dtype=torch.float32, device=logits.device)
+        i64 = dict(dtype=torch.int64, device=logits.device)
+        return (torch.zeros((), **f32), torch.zeros((), **f32), torch.zeros((S, E), **i64),
+                torch.zeros((S + 2,), **i64), torch.zeros((S, E), **f32))
+    return tuple(L.native().balance_forward(logits.detach(), idx, seq_offsets, token_mask, float(balance_coef),
+                                            float(z_coef)))
+
+
+def balance_loss_backward(
+    logits: torch.Tensor,
+    counts: torch.Tensor,
+    tokens: torch.Tensor,
+    k: int,
+    seq_offsets: Optional[torch.Tensor] = None,
+    token_mask: Optional[torch.Tensor] = None,
+    grad_balance: Optional[torch.Tensor] = None,
+    grad_z: Optional[torch.Tensor] = None,
+    balance_coef: float = 1.0,
+    z_coef: float = 0.0,
+) -> torch.Tensor:
+    """Gradient of :func:`balance_loss_forward` with respect to the logits, from its ``counts`` and ``tokens``: dlogits
+    [N, E] f32, zeros for tokens that are not valid or in no sequence.  ``grad_balance`` / ``grad_z`` (0-d; None: 1) are
+    the upstream gradients; a term is left out by its coefficient 0."""
+    L.require_device(logits, counts, tokens, seq_offsets, token_mask, grad_balance, grad_z)
+    N, E = logits.shape
+    token_mask = _balance_check("balance_loss_backward", logits, N, seq_offsets, token_mask)
+    S = 1 if seq_offsets is None else seq_offsets.shape[0] - 1
+    if counts.dtype != torch.int64 or tuple(counts.shape) != (S, E):
+        raise ValueError(f"balance_loss_backward: counts must be int64 [{S}, {E}]")
+    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (S + 2,):
+        raise ValueError(f"balance_loss_backward: tokens must be int64 [{S + 2}]")
+    if N == 0:
+        return torch.zeros_like(logits)
+    if grad_balance is not None:
+        grad_balance = grad_balance.detach().to(torch.float32).reshape(1)
+    if grad_z is not None:
+        grad_z = grad_z.detach().to(torch.float32).reshape(1)
+    return L.native().balance_backward(logits.detach(), counts, tokens, int(k), seq_offsets, token_mask, grad_balance,
+                                       grad_z, float(balance_coef), float(z_coef))

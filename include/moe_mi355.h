@@ -324,6 +324,63 @@ int moe_swiglu_fwd_fp8(const void* xq, const float* sx, const void* wg_q, const 
                        size_t ws_bytes, void* stream);
 
 /* ----------------------------------------------------------------------
+ * MXFP4 experts: weights held in 4 bits (e2m1: 0, 1/2, 1, 3/2, 2, 3, 4, 6 and negatives), every 32 consecutive
+ * elements of a row with one power-of-two scale (OCP MX, E8M0 byte e + 127); a variant of moe_quant_rows_fp8 /
+ * moe_swiglu_fwd_fp8 (the expert loop, moe_layer.py L:166-198, L:326-337) with bf16 rows.  The reference has no 4-bit
+ * path: its results are the bf16 path's up to this quantization of the weights.
+ *
+ * moe_quant_mxfp4: src [rows, cols] (MOE_BF16 / MOE_F32, contiguous) -> q [rows, cols / 2] bytes, the even column in
+ * the low half, and scale [rows, cols / 32] bytes.  e is the smallest integer with absmax <= 6 * 2^e, clamped to
+ * [-124, 125]; elements x * 2^-e rounded to nearest even, at most 6.  A block with an infinity or a NaN gets the scale
+ * byte 255 and stands for NaNs.  moe_dequant_mxfp4 gives the values back (exact in either dtype); it takes any scale
+ * bytes up to 252 (and 255).  cols % 32 == 0; src, q and dst 16-byte aligned.
+ *
+ * moe_swiglu_fwd_mxfp4: for the rows of each expert segment  g = Wg x, u = Wu x, act = silu(g) u (rounded to bf16),
+ * y = Wd act, with xp [R, H] bf16 and the quantized weights wg_q, wu_q [E, F, H / 2] (scales sg, su [E, F, H / 32]),
+ * wd_q [E, H, F / 2] (sd [E, H, F / 32]).  hgu [R, 2F] (bf16, [g | u], for the backward) may be NULL.  Rows past
+ * offsets[E] are left unwritten.  One row to many: no entry point of its own for decoding.
+ *
+ * moe_swiglu_bwd_mxfp4: the gradient of the rows (the weights are constants): dxp = Wg^T dg + Wu^T du with
+ * da = Wd^T dy, dg = da u silu'(g), du = da silu(g), g and u from hgu.
+ * Limits: H % 32 == 0, F % 32 == 0, E <= 1024; all pointers but the scales 16-byte aligned.
+ * ---------------------------------------------------------------------- */
+int moe_quant_mxfp4(const void* src, int src_dtype, int64_t rows, int64_t cols, void* q, void* scale, void* stream);
+int moe_dequant_mxfp4(const void* q, const void* scale, int64_t rows, int64_t cols, void* dst, int dst_dtype, void* stream);
+size_t moe_swiglu_fwd_mxfp4_workspace(int64_t R, int64_t H, int64_t F, int64_t E);
+int moe_swiglu_fwd_mxfp4(const void* xp, const void* wg_q, const void* sg, const void* wu_q, const void* su,
+                         const void* wd_q, const void* sd, const int32_t* offsets, int64_t R, int64_t H, int64_t F,
+                         int64_t E, void* hgu, void* y, void* workspace, size_t ws_bytes, void* stream);
+size_t moe_swiglu_bwd_mxfp4_workspace(int64_t R, int64_t H, int64_t F, int64_t E);
+int moe_swiglu_bwd_mxfp4(const void* dy, const void* hgu, const void* wg_q, const void* sg, const void* wu_q,
+                         const void* su, const void* wd_q, const void* sd, const int32_t* offsets, int64_t R, int64_t H,
+                         int64_t F, int64_t E, void* dxp, void* workspace, size_t ws_bytes, void* stream);
+
+/* ----------------------------------------------------------------------
+ * Balance loss and z-loss over the valid tokens of each sequence, with per-expert counts, and their gradient (no
+ * counterpart in the reference; moe_router_fwd's losses are over the whole batch, padding included).
+ *
+ * Sequence s holds the tokens [seq_offsets[s], seq_offsets[s + 1]) (S + 1 nondecreasing values in [0, N]; NULL with
+ * S == 1: all tokens); token_mask [N] marks the valid ones (NULL: all).  What the tokens of no sequence and those that
+ * are not valid hold is not used, whatever it is.  With n_s valid tokens in sequence s, c_se their choices of expert e
+ * (an id outside [0, E) counts for none) and p = softmax(logits):
+ *   balance = balance_coef / S+ * sum_s sum_e (E c_se / (K n_s)) (mean over valid t of p[t, e]),  S+ sequences with n_s > 0
+ *   z       = z_coef / n * sum over valid t of logsumexp(logits[t])^2,  n valid tokens
+ * (0 without valid tokens).  counts [S, E] = c, tokens [S + 2] = n_s of each sequence, then n, then S+;
+ * mean_prob [S, E] = the means (0 where n_s is 0).
+ * Workspace and its first word as moe_router_fwd's (zero before the first use, calls that share it in order).
+ * moe_balance_bwd: dlogits [N, E] = grad_balance d(balance)/dlogits + grad_z d(z)/dlogits (NULL = 1), from the forward's
+ * counts and tokens; rows of tokens that are not valid or in no sequence are zeros.
+ * Limits: 1 <= K <= min(E, 32), E <= 256, N >= 1, S >= 1.
+ * ---------------------------------------------------------------------- */
+size_t moe_balance_fwd_workspace(int64_t N, int64_t E, int64_t S);
+int moe_balance_fwd(const float* logits, const int64_t* idx, const int64_t* seq_offsets, const uint8_t* token_mask,
+                    int64_t N, int64_t E, int64_t K, int64_t S, float balance_coef, float z_coef, float* balance, float* z,
+                    int64_t* counts, int64_t* tokens, float* mean_prob, void* workspace, size_t ws_bytes, void* stream);
+int moe_balance_bwd(const float* logits, const int64_t* counts, const int64_t* tokens, const int64_t* seq_offsets,
+                    const uint8_t* token_mask, const float* grad_balance, const float* grad_z, int64_t N, int64_t E,
+                    int64_t K, int64_t S, float balance_coef, float z_coef, float* dlogits, void* stream);
+
+/* ----------------------------------------------------------------------
  * RMSNorm in front of the router (the caller step before the routed path):
  * replaces RMSNorm.forward (moe-engine/pkg/models/moe.py L:83-86) as used by
  * ToyMoEBlock.forward (L:125-126, x + moe(norm(x))):

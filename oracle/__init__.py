@@ -13,6 +13,9 @@ algorithm of the reference moe-engine hot path:
 * ``oracle.norm``    -- the RMSNorm in front of the router and its backward.
 * ``oracle.fp8``     -- the e4m3 row quantization and the fp8 expert forward
   (this build's own variant: the reference has no fp8 path).
+* ``oracle.mxfp4``   -- the experts held in 4 bits, forward and backward to the rows
+  (likewise without a counterpart).
+* ``oracle.balance`` -- the balance loss of sequences and the z-loss over valid tokens.
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and ``bench.py``'s CPU-baseline
 leg may import this package, and only as the checker (or the timed CPU
