@@ -7,12 +7,14 @@
 //   balance = coef / S+ * sum_s L_s   (S+ sequences have a valid token),   z = zcoef / n * sum over valid t of lse_t^2,
 //   d balance / dl[t, j] = coef / (S+ n_s) p[t, j] (f_sj - sum_e p[t, e] f_se),   dz / dl[t, j] = 2 zcoef / n lse_t p[t, j].
 //
-// Both directions are one read of the logits (and one write of the gradient): N E 4 bytes, bound by memory for large
-// batches and by two launches for small ones.  A wave owns a run of consecutive tokens and walks the sequences that meet
-// it; LPT lanes share a token, each with every LPT-th expert.  A sequence's sums stay in registers until the wave leaves
-// it, and go to a row of their own: run c and sequence s meet in row c + s, which is distinct for every pair that meets
-// (along a walk one of the two grows by one), and a sequence's rows are consecutive.  k_balance_sum then adds each
-// sequence's rows in order (64 bits), so every result is the same from run to run; its last block adds the sequences.
+// Both directions are one read of the logits (and one write of the gradient), N E 4 bytes: bound by memory for large
+// batches, by launches and chains of dependent loads for small ones.  A block owns a run of consecutive tokens.  LPT lanes
+// share a token, each with four neighbouring experts (one 16-byte load); a lane group's U tokens are loaded and their
+// softmax formed while the block finds the sequences that meet its run, and then it walks them.  A sequence's probabilities
+// are summed in registers and over the block's waves, its counts by LDS atomics of integers, and go to a row of their own:
+// run c and sequence s meet in row c + s, which is distinct for every pair that meets (along a walk one of the two grows by
+// one), and a sequence's rows are consecutive.  Its rows are then added in order (64 bits), so every result is the same from
+// run to run: by one block that also forms the losses where there are few rows, else by a block a sequence and a third launch.
 #include <algorithm>
 
 #include "common.h"
@@ -21,6 +23,9 @@ namespace moe {
 namespace {
 
 constexpr int kMaxBalanceE = 256;
+constexpr int kBalanceNT = 512;  // threads of a block of the two kernels over tokens
+constexpr int kFewSeqs = 64;     // sequences, and rows of sums, that one block adds up
+constexpr int kFewRows = 128;
 
 struct BalanceArgs {
   const float* logits;    // [N][E]
@@ -28,7 +33,7 @@ struct BalanceArgs {
   const int64_t* off;     // [S + 1]; null: one sequence of all tokens
   const uint8_t* mask;    // [N] nonzero: valid; null: all are
   int64_t N, S;
-  int E, K, run;          // run: tokens of a wave
+  int E, K;
   float* part_p;          // [rows][E]
   int* part_c;            // [rows][E]
   int* part_n;            // [rows]
@@ -76,168 +81,247 @@ __device__ __forceinline__ int64_t first_seq(const BalanceArgs& a, int64_t t, in
   return lo;
 }
 
-// softmax of the token whose logits these lanes hold: p and logsumexp.
-template <int LPT, int EPL>
-__device__ __forceinline__ float softmax_token(float (&p)[EPL]) {
-  float m = p[0];
+// The four logits of this lane of one token; -inf past E.
+template <bool VEC>
+__device__ __forceinline__ f32x4 load_logits(const BalanceArgs& a, int64_t t, int e0) {
+  const float* const p = a.logits + t * a.E + e0;
+  f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  if constexpr (VEC) {
+    if (e0 < a.E) v = *reinterpret_cast<const f32x4*>(p);
+  } else {
 #pragma unroll
-  for (int j = 1; j < EPL; ++j) m = fmaxf(m, p[j]);
-  m = team_max<LPT>(m);
-  float s = 0.f;
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    p[j] = expf(p[j] - m);
-    s += p[j];
+    for (int j = 0; j < 4; ++j)
+      if (e0 + j < a.E) v[j] = p[j];
   }
-  s = team_sum<LPT>(s);
+  return v;
+}
+
+// softmax of the token whose logits these lanes hold: p in their place, logsumexp returned.
+template <int LPT>
+__device__ __forceinline__ float softmax_token(f32x4& p) {
+  const float m = team_max<LPT>(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p[j] = expf(p[j] - m);
+  const float s = team_sum<LPT>((p[0] + p[1]) + (p[2] + p[3]));
   const float inv = 1.f / s;
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) p[j] *= inv;
+  for (int j = 0; j < 4; ++j) p[j] *= inv;
   return m + logf(s);
 }
 
-// Walks the sequences that meet tokens [c0, c1): visit(s, lo, hi) for each, gap(lo, hi) for the tokens of none.
-template <class V, class G>
-__device__ __forceinline__ void walk(const BalanceArgs& a, int64_t c0, int64_t c1, int lane, V visit, G gap) {
-  int64_t s0 = first_seq(a, c0, lane), pos = c0;
-  for (; s0 < a.S && pos < c1; s0 += 63) {
-    // the bounds of up to 63 sequences, one a lane
-    const int64_t mine = seq_off(a, min(s0 + lane, a.S));
-    const int n = (int)min((int64_t)63, a.S - s0);
-    // the first of them that starts past the run (starts grow)
-    for (int i = 0; i < n && pos < c1; ++i) {
-      const int64_t b = __shfl(mine, i), e = __shfl(mine, i + 1);
+// The bounds of up to 63 sequences from s0 on, one a lane (the last one's end in the next lane).
+struct SeqWindow {
+  int64_t s0, bound;
+};
+__device__ __forceinline__ SeqWindow seq_window(const BalanceArgs& a, int64_t s0, int lane) {
+  return SeqWindow{s0, s0 < a.S ? seq_off(a, min(s0 + lane, a.S)) : a.N};
+}
+// The window that the walk of a run starting at c0 begins with.
+__device__ __forceinline__ SeqWindow first_window(const BalanceArgs& a, int64_t c0, int lane) {
+  return seq_window(a, a.S <= 63 ? 0 : first_seq(a, c0, lane), lane);
+}
+
+// Walks the sequences that meet tokens [c0, c1): visit(s, lo, hi) for each.
+template <class V>
+__device__ __forceinline__ void walk(const BalanceArgs& a, SeqWindow w, int64_t c0, int64_t c1, int lane, V visit) {
+  int64_t pos = c0;
+  while (w.s0 < a.S && pos < c1) {
+    const int n = (int)min((int64_t)63, a.S - w.s0);
+    // of these, from the first that ends past the tokens walked so far
+    const unsigned long long past = __ballot(w.bound > pos) >> 1;
+    for (int i = past ? __builtin_ctzll(past) : 63; i < n && pos < c1; ++i) {
+      const int64_t b = __shfl(w.bound, i), e = __shfl(w.bound, i + 1);
       const int64_t lo = max(b, pos), hi = min(e, c1);
-      if (lo >= c1) {
-        s0 = a.S;
-        break;
-      }
+      if (lo >= c1) return;  // starts grow: none after it meets the run
       if (lo < hi) {
-        if (pos < lo) gap(pos, lo);
-        visit(s0 + i, lo, hi);
+        visit(w.s0 + i, lo, hi);
         pos = hi;
       }
     }
+    w = seq_window(a, w.s0 + 63, lane);
   }
-  if (pos < c1) gap(pos, c1);
 }
 
-template <int LPT, int EPL>
-__global__ __launch_bounds__(256) void k_balance_fwd(BalanceArgs a) {
-  constexpr int TPW = 64 / LPT;
-  const int lane = threadIdx.x & 63, sub = lane % LPT, team = lane / LPT;
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t c0 = c * a.run, c1 = min(a.N, c0 + a.run);
-  if (c0 >= c1) return;
+// A block's run is U tokens for each of its lane groups.
+template <int LPT, int U>
+constexpr int run_tokens() {
+  return U * (kBalanceNT / LPT);
+}
+
+template <int LPT, int U, bool VEC>
+__global__ __launch_bounds__(kBalanceNT) void k_balance_fwd(BalanceArgs a) {
+  constexpr int TEAMS = kBalanceNT / LPT, NW = kBalanceNT / 64, EW = LPT * 4;
+  __shared__ f32x4 s_p[2][NW][LPT];
+  __shared__ int s_c[2][EW];
+  __shared__ int s_n[2][NW];
+  __shared__ float s_z[NW];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, sub = lane % LPT, team = tid / LPT;
+  const int64_t c = blockIdx.x;
+  const int64_t c0 = c * run_tokens<LPT, U>(), c1 = min(a.N, c0 + run_tokens<LPT, U>());
   const int E = a.E, K = a.K;
+  f32x4 p[U];
+  int64_t id[U];  // the first of the lane's share of its tokens' choices
+  bool ok[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t t = min(c0 + u * TEAMS + team, c1 - 1);
+    p[u] = load_logits<VEC>(a, t, sub * 4);
+    id[u] = sub < K ? a.idx[t * K + sub] : -1;
+    ok[u] = a.mask == nullptr || a.mask[t] != 0;
+  }
+  const SeqWindow w0 = first_window(a, c0, lane);
+  for (int i = tid; i < 2 * EW; i += kBalanceNT) s_c[i / EW][i % EW] = 0;
+  float lse[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) lse[u] = softmax_token<LPT>(p[u]);
+  __syncthreads();
   float z = 0.f;
+  int b = 0;
   walk(
-      a, c0, c1, lane,
-      [&](int64_t s, int64_t lo, int64_t hi) {
-        float P[EPL];
-        int C[EPL], n = 0;
+      a, w0, c0, c1, lane, [&](int64_t s, int64_t lo, int64_t hi) {
+        f32x4 P = {0.f, 0.f, 0.f, 0.f};
+        int n = 0;
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) P[j] = 0.f, C[j] = 0;
-        for (int64_t t0 = lo; t0 < hi; t0 += TPW) {
-          const int64_t t = t0 + team;
-          const bool ok = t < hi && (a.mask == nullptr || a.mask[min(t, hi - 1)] != 0);
-          const int64_t tr = min(t, hi - 1);
-          float p[EPL];
-#pragma unroll
-          for (int j = 0; j < EPL; ++j) {
-            const int e = sub + LPT * j;
-            p[j] = e < E ? a.logits[tr * E + e] : -INFINITY;
-          }
-          const float lse = softmax_token<LPT, EPL>(p);
-#pragma unroll
-          for (int j = 0; j < EPL; ++j) P[j] += ok ? p[j] : 0.f;
-          z += ok ? lse * lse : 0.f;
-          n += ok;
-          for (int k = 0; k < K; ++k) {
-            const int64_t id = a.idx[tr * K + k];
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) C[j] += ok && id == sub + LPT * j;
+        for (int u = 0; u < U; ++u) {
+          const int64_t t = c0 + u * TEAMS + team;
+          if (ok[u] && t >= lo && t < hi) {
+            P += p[u];
+            z += lse[u] * lse[u];
+            ++n;
+            if (id[u] >= 0 && id[u] < E) atomicAdd(&s_c[b][id[u]], 1);
+            for (int k = sub + LPT; k < K; k += LPT) {
+              const int64_t i = a.idx[t * K + k];
+              if (i >= 0 && i < E) atomicAdd(&s_c[b][i], 1);
+            }
           }
         }
-        // sums over the wave's teams
 #pragma unroll
-        for (int o = LPT; o < 64; o <<= 1) {
+        for (int o = LPT; o < 64; o <<= 1) {  // over the wave's lane groups
           n += __shfl_xor(n, o);
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) {
-            P[j] += __shfl_xor(P[j], o);
-            C[j] += __shfl_xor(C[j], o);
-          }
+          for (int j = 0; j < 4; ++j) P[j] += __shfl_xor(P[j], o);
         }
+        if (lane < LPT) s_p[b][wv][sub] = P;
+        if (lane == 0) s_n[b][wv] = n;
+        __syncthreads();
         const int64_t row = c + s;
-        if (team == 0) {
+        if (tid < E) {
+          float v = 0.f;
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) {
-            const int e = sub + LPT * j;
-            if (e < E) {
-              a.part_p[row * E + e] = P[j];
-              a.part_c[row * E + e] = C[j];
-            }
-          }
+          for (int w = 0; w < NW; ++w) v += reinterpret_cast<const float*>(s_p[b][w])[tid];
+          a.part_p[row * E + tid] = v;
+          a.part_c[row * E + tid] = s_c[b][tid];
+          s_c[b][tid] = 0;  // used again two sequences on, behind the next one's barrier
         }
-        if (lane == 0) a.part_n[row] = n;
-      },
-      [](int64_t, int64_t) {});
+        if (tid == kBalanceNT - 1) {
+          int v = 0;
+#pragma unroll
+          for (int w = 0; w < NW; ++w) v += s_n[b][w];
+          a.part_n[row] = v;
+        }
+        b ^= 1;
+      });
 #pragma unroll
   for (int o = LPT; o < 64; o <<= 1) z += __shfl_xor(z, o);
-  if (lane == 0) a.part_z[c] = z;
+  if (lane == 0) s_z[wv] = z;
+  __syncthreads();
+  if (tid == 0) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += s_z[w];
+    a.part_z[c] = v;
+  }
 }
 
-template <int LPT, int EPL>
-__global__ __launch_bounds__(256) void k_balance_bwd(BalanceArgs a) {
-  constexpr int TPW = 64 / LPT;
-  const int lane = threadIdx.x & 63, sub = lane % LPT, team = lane / LPT;
-  const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t c0 = c * a.run, c1 = min(a.N, c0 + a.run);
-  if (c0 >= c1) return;
-  const int E = a.E;
+// Gradient: each token finds its own sequence among the windows of bounds (in LDS), so the counts of a lane group's U tokens
+// are in flight together whatever sequences they are of.
+template <int LPT, int U, bool VEC>
+__global__ __launch_bounds__(kBalanceNT) void k_balance_bwd(BalanceArgs a) {
+  constexpr int TEAMS = kBalanceNT / LPT;
+  __shared__ int64_t s_b[64];
+  const int lane = threadIdx.x & 63, sub = lane % LPT, team = threadIdx.x / LPT;
+  const int64_t c0 = (int64_t)blockIdx.x * run_tokens<LPT, U>(), c1 = min(a.N, c0 + run_tokens<LPT, U>());
+  const int E = a.E, e0 = sub * 4;
+  f32x4 p[U];
+  bool ok[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t t = min(c0 + u * TEAMS + team, c1 - 1);
+    p[u] = load_logits<VEC>(a, t, e0);
+    ok[u] = a.mask == nullptr || a.mask[t] != 0;
+  }
   const float gb = a.bcoef * (a.grad_b ? a.grad_b[0] : 1.f), gz = a.zcoef * (a.grad_z ? a.grad_z[0] : 1.f);
   const float total = (float)max(a.tokens[a.S], (int64_t)1), used = (float)max(a.tokens[a.S + 1], (int64_t)1);
-  const float cz = gz * 2.f / total;
-  auto zeros = [&](int64_t lo, int64_t hi) {
-    for (int64_t i = lo * E + lane; i < hi * E; i += 64) a.dlogits[i] = 0.f;
-  };
-  walk(
-      a, c0, c1, lane,
-      [&](int64_t s, int64_t lo, int64_t hi) {
-        const float n = (float)max(a.tokens[s], (int64_t)1);
-        const float cb = gb / (used * n), fs = (float)E / ((float)a.K * n);
-        float f[EPL];
+  SeqWindow w = first_window(a, c0, lane);
+  const float cz = gz * 2.f / total, cs = (float)E / (float)a.K;
+  int64_t seq[U];
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-          const int e = sub + LPT * j;
-          f[j] = e < E ? (float)a.counts[s * E + e] * fs : 0.f;
-        }
-        for (int64_t t0 = lo; t0 < hi; t0 += TPW) {
-          const int64_t t = t0 + team, tr = min(t, hi - 1);
-          const bool ok = a.mask == nullptr || a.mask[tr] != 0;
-          float p[EPL];
+  for (int u = 0; u < U; ++u) seq[u] = -1;
+  for (;;) {  // windows until one ends past the run
+    if (threadIdx.x < 64) s_b[threadIdx.x] = w.bound;
+    __syncthreads();
+    const int n = (int)min((int64_t)63, a.S - w.s0);
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) {
-            const int e = sub + LPT * j;
-            p[j] = e < E ? a.logits[tr * E + e] : -INFINITY;
-          }
-          const float lse = softmax_token<LPT, EPL>(p);
-          float pf = 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = min(c0 + u * TEAMS + team, c1 - 1);
+      int lo = 0, len = n;  // the first of the window's sequences that ends past t
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) pf += p[j] * f[j];
-          pf = team_sum<LPT>(pf);
-          if (t < hi) {
+      for (int i = 0; i < 6; ++i) {
+        const int half = len >> 1;
+        const bool on = len > 0 && s_b[lo + half + 1] <= t;
+        lo = on ? lo + half + 1 : lo;
+        len = len > 0 ? (on ? len - half - 1 : half) : 0;
+      }
+      if (seq[u] < 0 && lo < n && s_b[lo] <= t) seq[u] = w.s0 + lo;
+    }
+    const bool more = w.s0 + n < a.S && s_b[n] < c1;
+    if (!more) break;
+    w = seq_window(a, w.s0 + n, lane);
+    __syncthreads();
+  }
+  uint32_t cnt[U][4], n[U];  // all counts are below 2^31: their low halves
 #pragma unroll
-            for (int j = 0; j < EPL; ++j) {
-              const int e = sub + LPT * j;
-              const float d = p[j] * (cb * (f[j] - pf) + cz * lse);
-              if (e < E) a.dlogits[t * E + e] = ok ? d : 0.f;
-            }
-          }
-        }
-      },
-      zeros);
+  for (int u = 0; u < U; ++u) {
+    const int64_t s = max(seq[u], (int64_t)0);
+    n[u] = reinterpret_cast<const uint32_t*>(a.tokens + s)[0];
+    const uint32_t* const c = reinterpret_cast<const uint32_t*>(a.counts + s * E + e0);
+    if constexpr (VEC) {  // a lane past E (fewer experts than lanes) has no counts
+      const bool in = e0 < E;
+      const u32x4 lo = *reinterpret_cast<const u32x4*>(in ? c : reinterpret_cast<const uint32_t*>(a.counts));
+      const u32x4 hi = *reinterpret_cast<const u32x4*>((in ? c : reinterpret_cast<const uint32_t*>(a.counts)) + 4);
+      cnt[u][0] = in ? lo[0] : 0u, cnt[u][1] = in ? lo[2] : 0u, cnt[u][2] = in ? hi[0] : 0u, cnt[u][3] = in ? hi[2] : 0u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cnt[u][j] = e0 + j < E ? c[2 * j] : 0u;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t t = c0 + u * TEAMS + team;
+    const float lse = softmax_token<LPT>(p[u]);
+    const float in = 1.f / (float)max(n[u], 1u), cb = gb / used * in, fs = cs * in;
+    f32x4 d;
+    float pf = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      d[j] = (float)cnt[u][j] * fs;
+      pf += p[u][j] * d[j];
+    }
+    pf = team_sum<LPT>(pf);
+    const bool live = ok[u] && seq[u] >= 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = live ? p[u][j] * (cb * (d[j] - pf) + cz * lse) : 0.f;
+    if (t < c1) {
+      float* const o = a.dlogits + t * E + e0;
+      if constexpr (VEC) {
+        if (e0 < E) *reinterpret_cast<f32x4*>(o) = d;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (e0 + j < E) o[j] = d[j];
+      }
+    }
+  }
 }
 
 struct BalanceSumArgs {
@@ -247,7 +331,7 @@ struct BalanceSumArgs {
   const int* part_n;
   const float* part_z;
   int64_t N, S, runs;
-  int E, K, run, EP;      // EP: lanes of a row of experts, a power of two
+  int E, K, run;
   float bcoef, zcoef;
   int64_t* counts;        // [S][E]
   int64_t* tokens;        // [S + 2]
@@ -255,93 +339,195 @@ struct BalanceSumArgs {
   double* seq_loss;       // [S]
   float* balance;
   float* z;
-  unsigned* ticket;
 };
 
 template <typename T>
-__device__ __forceinline__ T block_sum(T v, T* red) {
+__device__ __forceinline__ T wave_sum_of(T v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  const int wv = threadIdx.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[wv] = v;
-  __syncthreads();
-  T t = 0;
-  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) t += red[i];
-  return t;
+  return v;
 }
 
-// One block a sequence: EP threads side by side on a row of experts, the block's other threads on further rows.
-__global__ __launch_bounds__(1024) void k_balance_sum(BalanceSumArgs a) {
-  __shared__ double s_p[1024];
-  __shared__ int64_t s_c[1024];
-  __shared__ double s_red[16];
-  __shared__ int64_t s_redi[16];
-  __shared__ bool s_last;
-  const int tid = threadIdx.x, nt = blockDim.x;
-  const int64_t s = blockIdx.x;
-  const int e = tid & (a.EP - 1), rg = tid / a.EP, nrg = nt / a.EP;
-  const int64_t b = min(max(a.off ? a.off[s] : (int64_t)0, (int64_t)0), a.N);
-  const int64_t h = min(max(a.off ? a.off[s + 1] : a.N, (int64_t)0), a.N);
-  const int64_t r0 = b / a.run + s, r1 = h > b ? (h - 1) / a.run + s + 1 : r0;
-  double p = 0.;
-  int64_t c = 0, n = 0;
-  if (e < a.E)
-    for (int64_t r = r0 + rg; r < r1; r += nrg) {
-      p += (double)a.part_p[r * a.E + e];
-      c += a.part_c[r * a.E + e];
+// One sequence's rows, added by W waves of a block (a power of two; wave w of them).  Lanes lie side by side on a row's
+// experts, 64 at a time, and with fewer experts on several rows.  Every wave of the block calls it, with live false where
+// it has no sequence.  EJ: 64-wide pieces of a row.  sm: a row for each of the block's waves.  Returns the sequence's loss and valid tokens to wave 0's lanes.
+template <int EJ>
+__device__ __forceinline__ double sum_sequence(const BalanceSumArgs& a, int64_t s, bool live, int W, int w, int lane,
+                                               double* sm_p, int64_t* sm_c, int64_t* sm_n, int64_t& n) {
+  const int E = a.E;
+  int64_t r0 = 0, r1 = 0;
+  if (live) {
+    const int64_t b = min(max(a.off ? a.off[s] : (int64_t)0, (int64_t)0), a.N);
+    const int64_t h = min(max(a.off ? a.off[s + 1] : a.N, (int64_t)0), a.N);
+    r0 = b / a.run + s;
+    r1 = h > b ? (h - 1) / a.run + s + 1 : r0;
+  }
+  int EP = 1;
+  while (EP < E && EP < 64) EP *= 2;
+  const int el = lane & (EP - 1), rl = lane / EP, rows = 64 / EP;
+  double p[EJ];
+  int64_t c[EJ];
+#pragma unroll
+  for (int j = 0; j < EJ; ++j) p[j] = 0., c[j] = 0;
+  for (int64_t r = r0 + w * rows + rl; r < r1; r += 4 * W * rows) {
+    float pv[4][EJ];
+    int cv[4][EJ];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t ri = r + i * W * rows;
+#pragma unroll
+      for (int j = 0; j < EJ; ++j) {
+        const int e = el + 64 * j;
+        const bool in = ri < r1 && e < E;
+        pv[i][j] = in ? a.part_p[ri * E + e] : 0.f;
+        cv[i][j] = in ? a.part_c[ri * E + e] : 0;
+      }
     }
-  for (int64_t r = r0 + tid; r < r1; r += nt) n += a.part_n[r];
-  n = block_sum(n, s_redi);
-  s_p[tid] = p;
-  s_c[tid] = c;
-  __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < EJ; ++j) {
+        p[j] += (double)pv[i][j];
+        c[j] += cv[i][j];
+      }
+  }
+  n = 0;
+  for (int64_t r = r0 + w * 64 + lane; r < r1; r += W * 64) n += a.part_n[r];
+  n = wave_sum_of(n);
+#pragma unroll
+  for (int j = 0; j < EJ; ++j)
+    for (int o = EP; o < 64; o <<= 1) {
+      p[j] += __shfl_xor(p[j], o);
+      c[j] += __shfl_xor(c[j], o);
+    }
+  if (W > 1) {
+#pragma unroll
+    for (int j = 0; j < EJ; ++j) {
+      sm_p[w * (64 * EJ) + lane + 64 * j] = p[j];
+      sm_c[w * (64 * EJ) + lane + 64 * j] = c[j];
+    }
+    if (lane == 0) sm_n[w] = n;
+    __syncthreads();
+    if (w == 0) {
+      for (int x = 1; x < W; ++x) {
+#pragma unroll
+        for (int j = 0; j < EJ; ++j) {
+          p[j] += sm_p[x * (64 * EJ) + lane + 64 * j];
+          c[j] += sm_c[x * (64 * EJ) + lane + 64 * j];
+        }
+        n += sm_n[x];
+      }
+    }
+    __syncthreads();
+  }
   double l = 0.;
-  if (tid < a.E) {
-    for (int g = 1; g < nrg; ++g) {
-      p += s_p[g * a.EP + tid];
-      c += s_c[g * a.EP + tid];
-    }
+  if (live && w == 0) {
     const double inv = n > 0 ? 1. / (double)n : 0.;
-    p *= inv;
-    a.counts[s * a.E + tid] = c;
-    a.mean_p[s * a.E + tid] = (float)p;
-    l = (double)a.E * (double)c * inv / (double)a.K * p;
+#pragma unroll
+    for (int j = 0; j < EJ; ++j) {
+      const int e = el + 64 * j;
+      if (rl == 0 && e < E) {
+        const double m = p[j] * inv;
+        a.counts[s * E + e] = c[j];
+        a.mean_p[s * E + e] = (float)m;
+        l += (double)E * (double)c[j] * inv / (double)a.K * m;
+      }
+    }
+    l = wave_sum_of(l);
+    if (lane == 0) a.tokens[s] = n;
   }
-  l = block_sum(l, s_red);
-  if (tid == 0) {
-    a.tokens[s] = n;
-    a.seq_loss[s] = l;
-    __threadfence();
-    s_last = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  double sum = 0., zs = 0.;
-  int64_t all = 0, used = 0;
+  return l;
+}
+
+// This thread's share of the runs' z sums.
+__device__ __forceinline__ double z_share(const BalanceSumArgs& a) {
+  double zs = 0.;
+  for (int64_t i = threadIdx.x; i < a.runs; i += blockDim.x) zs += (double)a.part_z[i];
+  return zs;
+}
+
+// The losses from the sequences' losses and the threads' shares of the z sums, by a whole block.
+template <typename F, typename G>
+__device__ __forceinline__ void total_losses(const BalanceSumArgs& a, double zs, F loss_of, G tokens_of, double* red) {
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wv = tid >> 6;
+  double sum = 0., all = 0., used = 0.;  // whole numbers below 2^53 are exact
   for (int64_t i = tid; i < a.S; i += nt) {
-    sum += __hip_atomic_load(a.seq_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int64_t m = __hip_atomic_load(a.tokens + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    all += m;
-    used += m > 0;
+    sum += loss_of(i);
+    const int64_t m = tokens_of(i);
+    all += (double)m;
+    used += m > 0 ? 1. : 0.;
   }
-  for (int64_t i = tid; i < a.runs; i += nt) zs += (double)a.part_z[i];
-  sum = block_sum(sum, s_red);
-  zs = block_sum(zs, s_red);
-  all = block_sum(all, s_redi);
-  used = block_sum(used, s_redi);
+  double v[4] = {wave_sum_of(sum), wave_sum_of(zs), wave_sum_of(all), wave_sum_of(used)};
+  __syncthreads();
+  if (lane < 4) red[wv * 4 + lane] = lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
+  __syncthreads();
   if (tid == 0) {
-    a.tokens[a.S] = all;
-    a.tokens[a.S + 1] = used;
-    *a.balance = (float)((double)a.bcoef * sum / (double)max(used, (int64_t)1));
-    *a.z = (float)((double)a.zcoef * zs / (double)max(all, (int64_t)1));
-    *a.ticket = 0u;
+    for (int w = 1; w < (nt >> 6); ++w)
+      for (int i = 0; i < 4; ++i) v[i] += red[w * 4 + i];
+    a.tokens[a.S] = (int64_t)v[2];
+    a.tokens[a.S + 1] = (int64_t)v[3];
+    *a.balance = (float)((double)a.bcoef * v[0] / fmax(v[3], 1.));
+    *a.z = (float)((double)a.zcoef * v[1] / fmax(v[2], 1.));
   }
 }
 
-// Tokens of a wave: enough waves for every SIMD to hold a few (16 tokens each below 65536 tokens), and at most 4096 of them.
-int run_of(int64_t N) { return (int)std::max<int64_t>(16, ((N + 4095) / 4096 + 15) / 16 * 16); }
+// Up to kFewSeqs sequences: one block of 16 waves, W of them a sequence.
+template <int EJ>
+__global__ __launch_bounds__(1024) void k_balance_sum_few(BalanceSumArgs a, int W) {
+  __shared__ double s_p[16 * 64 * EJ];
+  __shared__ int64_t s_c[16 * 64 * EJ];
+  __shared__ int64_t s_n[16];
+  __shared__ double s_loss[kFewSeqs];
+  __shared__ int64_t s_tok[kFewSeqs];
+  __shared__ double red[64];
+  const double zs = z_share(a);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, grp = wv / W, groups = 16 / W;
+  for (int64_t s0 = 0; s0 < a.S; s0 += groups) {
+    const int64_t s = s0 + grp;
+    int64_t n;
+    const double l = sum_sequence<EJ>(a, s, s < a.S, W, wv & (W - 1), lane, s_p + grp * W * 64 * EJ,
+                                      s_c + grp * W * 64 * EJ, s_n + grp * W, n);
+    if (s < a.S && (wv & (W - 1)) == 0 && lane == 0) {
+      s_loss[s] = l;
+      s_tok[s] = n;
+    }
+  }
+  __syncthreads();
+  total_losses(
+      a, zs, [&](int64_t i) { return s_loss[i]; }, [&](int64_t i) { return s_tok[i]; }, red);
+}
+
+template <int EJ>
+__global__ __launch_bounds__(1024) void k_balance_sum(BalanceSumArgs a) {
+  __shared__ double s_p[16 * 64 * EJ];
+  __shared__ int64_t s_c[16 * 64 * EJ];
+  __shared__ int64_t s_n[16];
+  int64_t n;
+  const double l = sum_sequence<EJ>(a, blockIdx.x, true, blockDim.x >> 6, threadIdx.x >> 6, threadIdx.x & 63, s_p, s_c, s_n, n);
+  if (threadIdx.x == 0) a.seq_loss[blockIdx.x] = l;
+}
+
+__global__ __launch_bounds__(1024) void k_balance_total(BalanceSumArgs a) {
+  __shared__ double red[64];
+  total_losses(
+      a, z_share(a), [&](int64_t i) { return a.seq_loss[i]; }, [&](int64_t i) { return a.tokens[i]; }, red);
+}
+
+// Lane groups of a token and tokens of a group.  A group's U tokens are in flight together and a block's run is 128 or 256
+// tokens (64 past 128 experts); batches that give fewer than 256 such runs take one token a group, for more blocks.
+struct BalanceForm {
+  int lpt, u, run;
+};
+BalanceForm balance_form(int64_t N, int64_t E, bool fwd) {
+  BalanceForm f;
+  f.lpt = 2;
+  while (f.lpt * 4 < E) f.lpt *= 2;
+  f.u = f.lpt <= 2 ? 1 : f.lpt <= 4 ? 2 : f.lpt <= 16 ? 4 : 8;
+  if (N < (int64_t)256 * f.u * (kBalanceNT / f.lpt)) f.u = 1;
+  if (!fwd) f.u = std::min(f.u, 2);
+  f.run = f.u * (kBalanceNT / f.lpt);
+  return f;
+}
 
 size_t al256b(size_t v) { return (v + 255) & ~(size_t)255; }
 struct BalanceWs {
@@ -350,9 +536,10 @@ struct BalanceWs {
 };
 BalanceWs balance_ws(int64_t N, int64_t E, int64_t S) {
   BalanceWs w;
-  w.runs = (N + run_of(N) - 1) / run_of(N);
+  const int run = balance_form(N, E, true).run;
+  w.runs = (N + run - 1) / run;
   w.rows = w.runs + S;
-  w.off_loss = 256;  // the ticket's line first
+  w.off_loss = 0;
   w.off_p = w.off_loss + al256b((size_t)S * 8);
   w.off_c = w.off_p + al256b((size_t)w.rows * E * 4);
   w.off_n = w.off_c + al256b((size_t)w.rows * E * 4);
@@ -363,22 +550,49 @@ BalanceWs balance_ws(int64_t N, int64_t E, int64_t S) {
 
 int balance_check(const char* what, int64_t N, int64_t E, int64_t K, int64_t S) {
   const int64_t lim = INT32_MAX;
-  if (N < 1 || N > lim || E < 1 || E > kMaxBalanceE || K < 1 || K > 32 || K > E || S < 1 || S > lim - 1)
-    return fail_arg("%s: bad shape N=%lld E=%lld K=%lld S=%lld (need N, S >= 1, E <= %d, K <= min(E, 32))", what, (long long)N,
+  if (N < 1 || N > lim / 32 || E < 1 || E > kMaxBalanceE || K < 1 || K > 32 || K > E || S < 1 || S > lim - 1)
+    return fail_arg("%s: bad shape N=%lld E=%lld K=%lld S=%lld (need N, S >= 1, N < 2^26, E <= %d, K <= min(E, 32))", what, (long long)N,
                     (long long)E, (long long)K, (long long)S, kMaxBalanceE);
   return 0;
 }
 
-#define MOE_BALANCE(KERNEL, name)                                                                                       \
-  do {                                                                                                                  \
-    const dim3 grid((unsigned)cdiv(runs, 4));                                                                           \
-    if (E <= 8) MOE_LAUNCH(name, (KERNEL<8, 1>), grid, dim3(256), 0, s, a);                                             \
-    else if (E <= 16) MOE_LAUNCH(name, (KERNEL<16, 1>), grid, dim3(256), 0, s, a);                                      \
-    else if (E <= 32) MOE_LAUNCH(name, (KERNEL<16, 2>), grid, dim3(256), 0, s, a);                                      \
-    else if (E <= 64) MOE_LAUNCH(name, (KERNEL<16, 4>), grid, dim3(256), 0, s, a);                                      \
-    else if (E <= 128) MOE_LAUNCH(name, (KERNEL<16, 8>), grid, dim3(256), 0, s, a);                                     \
-    else MOE_LAUNCH(name, (KERNEL<32, 8>), grid, dim3(256), 0, s, a);                                                   \
+// VEC: every lane's four logits are one aligned 16-byte word.
+#define MOE_BALANCE_FWD(VEC)                                                                                  \
+  do {                                                                                                        \
+    const dim3 grid((unsigned)runs), block(kBalanceNT);                                                       \
+    switch (f.lpt * 16 + f.u) {                                                                               \
+      case 2 * 16 + 1: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<2, 1, VEC>), grid, block, 0, s, a); break;  \
+      case 4 * 16 + 1: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<4, 1, VEC>), grid, block, 0, s, a); break;  \
+      case 4 * 16 + 2: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<4, 2, VEC>), grid, block, 0, s, a); break;  \
+      case 8 * 16 + 1: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<8, 1, VEC>), grid, block, 0, s, a); break;  \
+      case 8 * 16 + 4: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<8, 4, VEC>), grid, block, 0, s, a); break;  \
+      case 16 * 16 + 1: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<16, 1, VEC>), grid, block, 0, s, a); break;\
+      case 16 * 16 + 4: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<16, 4, VEC>), grid, block, 0, s, a); break;\
+      case 32 * 16 + 1: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<32, 1, VEC>), grid, block, 0, s, a); break;\
+      case 32 * 16 + 8: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<32, 8, VEC>), grid, block, 0, s, a); break;\
+      case 64 * 16 + 1: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<64, 1, VEC>), grid, block, 0, s, a); break;\
+      case 64 * 16 + 8: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<64, 8, VEC>), grid, block, 0, s, a); break;\
+    }                                                                                                         \
   } while (0)
+#define MOE_BALANCE_BWD(VEC)                                                                                  \
+  do {                                                                                                        \
+    const dim3 grid((unsigned)runs), block(kBalanceNT);                                                       \
+    switch (f.lpt * 16 + f.u) {                                                                               \
+      case 2 * 16 + 1: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<2, 1, VEC>), grid, block, 0, s, a); break;  \
+      case 4 * 16 + 1: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<4, 1, VEC>), grid, block, 0, s, a); break;  \
+      case 4 * 16 + 2: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<4, 2, VEC>), grid, block, 0, s, a); break;  \
+      case 8 * 16 + 1: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<8, 1, VEC>), grid, block, 0, s, a); break;  \
+      case 8 * 16 + 2: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<8, 2, VEC>), grid, block, 0, s, a); break;  \
+      case 16 * 16 + 1: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<16, 1, VEC>), grid, block, 0, s, a); break;\
+      case 16 * 16 + 2: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<16, 2, VEC>), grid, block, 0, s, a); break;\
+      case 32 * 16 + 1: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<32, 1, VEC>), grid, block, 0, s, a); break;\
+      case 32 * 16 + 2: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<32, 2, VEC>), grid, block, 0, s, a); break;\
+      case 64 * 16 + 1: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<64, 1, VEC>), grid, block, 0, s, a); break;\
+      case 64 * 16 + 2: MOE_LAUNCH("k_balance_bwd", (k_balance_bwd<64, 2, VEC>), grid, block, 0, s, a); break;\
+    }                                                                                                         \
+  } while (0)
+
+bool al16b(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
 }  // namespace moe
@@ -412,12 +626,13 @@ extern "C" int moe_balance_fwd(const float* logits, const int64_t* idx, const in
   a.S = S;
   a.E = (int)E;
   a.K = (int)K;
-  a.run = run_of(N);
+  const BalanceForm f = balance_form(N, E, true);
   a.part_p = reinterpret_cast<float*>(ws + w.off_p);
   a.part_c = reinterpret_cast<int*>(ws + w.off_c);
   a.part_n = reinterpret_cast<int*>(ws + w.off_n);
   a.part_z = reinterpret_cast<float*>(ws + w.off_z);
-  MOE_BALANCE(k_balance_fwd, "k_balance_fwd");
+  if (E % 4 == 0 && al16b(logits)) MOE_BALANCE_FWD(true);
+  else MOE_BALANCE_FWD(false);
   if (int rc = check_launch("k_balance_fwd")) return rc;
   BalanceSumArgs b{};
   b.off = seq_offsets;
@@ -430,9 +645,7 @@ extern "C" int moe_balance_fwd(const float* logits, const int64_t* idx, const in
   b.runs = runs;
   b.E = (int)E;
   b.K = (int)K;
-  b.run = a.run;
-  b.EP = 1;
-  while (b.EP < E) b.EP *= 2;
+  b.run = f.run;
   b.bcoef = balance_coef;
   b.zcoef = z_coef;
   b.counts = counts;
@@ -441,8 +654,21 @@ extern "C" int moe_balance_fwd(const float* logits, const int64_t* idx, const in
   b.seq_loss = reinterpret_cast<double*>(ws + w.off_loss);
   b.balance = balance;
   b.z = z;
-  b.ticket = reinterpret_cast<unsigned*>(ws);
-  MOE_LAUNCH("k_balance_sum", k_balance_sum, dim3((unsigned)S), dim3(256), 0, s, b);
+#define MOE_BALANCE_SUM(KERNEL, name, grid, block, ...)                               \
+  do {                                                                                \
+    if (E <= 64) MOE_LAUNCH(name, KERNEL<1>, grid, block, 0, s, __VA_ARGS__);         \
+    else if (E <= 128) MOE_LAUNCH(name, KERNEL<2>, grid, block, 0, s, __VA_ARGS__);   \
+    else MOE_LAUNCH(name, KERNEL<4>, grid, block, 0, s, __VA_ARGS__);                 \
+  } while (0)
+  if (S <= kFewSeqs && w.rows <= kFewRows) {
+    int W = 16;
+    while (W > 1 && W * S > 16) W /= 2;
+    MOE_BALANCE_SUM(k_balance_sum_few, "k_balance_sum_few", dim3(1), dim3(1024), b, W);
+    return check_launch("moe_balance_fwd");
+  }
+  // a sequence's rows by 16 waves where sequences are long on average, by 4 where they are many
+  MOE_BALANCE_SUM(k_balance_sum, "k_balance_sum", dim3((unsigned)S), dim3(runs / S >= 16 ? 1024 : 256), b);
+  MOE_LAUNCH("k_balance_total", k_balance_total, dim3(1), dim3(1024), 0, s, b);
   return check_launch("moe_balance_fwd");
 }
 
@@ -461,7 +687,7 @@ extern "C" int moe_balance_bwd(const float* logits, const int64_t* counts, const
   a.S = S;
   a.E = (int)E;
   a.K = (int)K;
-  a.run = run_of(N);
+  const BalanceForm f = balance_form(N, E, false);
   a.counts = counts;
   a.tokens = tokens;
   a.grad_b = grad_balance;
@@ -469,7 +695,8 @@ extern "C" int moe_balance_bwd(const float* logits, const int64_t* counts, const
   a.bcoef = balance_coef;
   a.zcoef = z_coef;
   a.dlogits = dlogits;
-  const int64_t runs = (N + a.run - 1) / a.run;
-  MOE_BALANCE(k_balance_bwd, "k_balance_bwd");
+  const int64_t runs = (N + f.run - 1) / f.run;
+  if (E % 4 == 0 && al16b(logits) && al16b(counts) && al16b(dlogits)) MOE_BALANCE_BWD(true);
+  else MOE_BALANCE_BWD(false);
   return check_launch("moe_balance_bwd");
 }

@@ -527,13 +527,12 @@ std::vector<at::Tensor> op_balance_forward(const at::Tensor& logits_in, const at
   const auto i64 = logits.options().dtype(at::kLong);
   at::Tensor balance = at::empty({}, f32), z = at::empty({}, f32), counts = at::empty({S, E}, i64);
   at::Tensor tokens = at::empty({S + 2}, i64), mean_prob = at::empty({S, E}, f32);
-  const hipStream_t s = stream_of(logits);
   const size_t nbytes = moe_balance_fwd_workspace(N, E, S);
-  const FwdWorkspace ws(nbytes, logits.device(), s);
+  const at::Tensor ws = scratch(nbytes, logits);
   check_rc(moe_balance_fwd(logits.data_ptr<float>(), idx.data_ptr<int64_t>(), static_cast<const int64_t*>(ptr(off)),
                            static_cast<const uint8_t*>(ptr(mask)), N, E, K, S, (float)balance_coef, (float)z_coef,
                            balance.data_ptr<float>(), z.data_ptr<float>(), counts.data_ptr<int64_t>(),
-                           tokens.data_ptr<int64_t>(), mean_prob.data_ptr<float>(), ws.data_ptr(), nbytes, s),
+                           tokens.data_ptr<int64_t>(), mean_prob.data_ptr<float>(), ws.data_ptr(), nbytes, stream_of(logits)),
            "moe_balance_fwd");
   return {balance, z, counts, tokens, mean_prob};
 }

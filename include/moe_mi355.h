@@ -367,10 +367,9 @@ int moe_swiglu_bwd_mxfp4(const void* dy, const void* hgu, const void* wg_q, cons
  *   z       = z_coef / n * sum over valid t of logsumexp(logits[t])^2,  n valid tokens
  * (0 without valid tokens).  counts [S, E] = c, tokens [S + 2] = n_s of each sequence, then n, then S+;
  * mean_prob [S, E] = the means (0 where n_s is 0).
- * Workspace and its first word as moe_router_fwd's (zero before the first use, calls that share it in order).
  * moe_balance_bwd: dlogits [N, E] = grad_balance d(balance)/dlogits + grad_z d(z)/dlogits (NULL = 1), from the forward's
  * counts and tokens; rows of tokens that are not valid or in no sequence are zeros.
- * Limits: 1 <= K <= min(E, 32), E <= 256, N >= 1, S >= 1.
+ * Limits: 1 <= K <= min(E, 32), E <= 256, 1 <= N < 2^26, S >= 1.
  * ---------------------------------------------------------------------- */
 size_t moe_balance_fwd_workspace(int64_t N, int64_t E, int64_t S);
 int moe_balance_fwd(const float* logits, const int64_t* idx, const int64_t* seq_offsets, const uint8_t* token_mask,
