@@ -191,9 +191,10 @@ int swiglu_small_fwd(bool f32, const void* xp, const void* w_gate, const void* w
                      const int* offsets, int64_t R, int64_t H, int64_t F, int64_t E, void* act, void* hgu, void* y,
                      hipStream_t s);
 
-// ---- the row-grouped products of the bf16 backward (csrc/gemm.hip): a tile table in the workspace's first
-// moe_swiglu_workspace(E) bytes, dh [R, 2F] = epilogue(dy Wd), dxp = dh [Wg ; Wu] (ws_bytes past the table: partial tiles) ----
-int swiglu_tiles(const int* offsets, int64_t E, void* workspace, hipStream_t s);
+// ---- the row-grouped products of the bf16 backward (csrc/gemm.hip): a table of tiles of bm rows (theirs: kGemmRows) in the
+// workspace's first moe_swiglu_workspace(E) bytes, dh [R, 2F] = epilogue(dy Wd), dxp = dh [Wg ; Wu] (ws_bytes past the table: partial tiles) ----
+constexpr int kGemmRows = 256;
+int swiglu_tiles(const int* offsets, int64_t E, int bm, void* workspace, hipStream_t s);
 int swiglu_dact(const void* dy, const void* hgu, const void* w_down, const int* offsets, int64_t R, int64_t H, int64_t F,
                 int64_t E, void* dh, const void* workspace, hipStream_t s);
 int swiglu_dxp(const void* dh, const void* w_gate, const void* w_up, const int* offsets, int64_t R, int64_t H, int64_t F,

@@ -1231,9 +1231,9 @@ namespace {
 bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 unsigned round8(int64_t v) { return (unsigned)((v + 7) / 8 * 8); }
 
-void launch_tiles(hipStream_t s, const int* offsets, int64_t E, int* tile_off, int* korder) {
+void launch_tiles(hipStream_t s, const int* offsets, int64_t E, int* tile_off, int* korder, int bm = GBM) {
   const unsigned threads = (unsigned)((E + 63) / 64 * 64);
-  MOE_LAUNCH("k_gemm_tiles", k_gemm_tiles, dim3(1), dim3(threads), 0, s, offsets, (int)E, GBM, tile_off, korder);
+  MOE_LAUNCH("k_gemm_tiles", k_gemm_tiles, dim3(1), dim3(threads), 0, s, offsets, (int)E, bm, tile_off, korder);
 }
 
 template <int AM, int BMD, int GR, int EP, int NW>
@@ -1446,8 +1446,8 @@ extern "C" int moe_swiglu_fwd_fp8(const void* xq, const float* sx, const void* w
 
 namespace moe {
 // The row-grouped products of the backward, over the tile table that swiglu_tiles has put into the workspace (common.h).
-int swiglu_tiles(const int* offsets, int64_t E, void* workspace, hipStream_t s) {
-  launch_tiles(s, offsets, E, static_cast<int*>(workspace), nullptr);
+int swiglu_tiles(const int* offsets, int64_t E, int bm, void* workspace, hipStream_t s) {
+  launch_tiles(s, offsets, E, static_cast<int*>(workspace), nullptr, bm);
   return check_launch("k_gemm_tiles");
 }
 

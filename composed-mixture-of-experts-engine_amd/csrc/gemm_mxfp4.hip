@@ -15,6 +15,7 @@
 // agree: lane 16 q + r holds block 4 c + q of row r, and takes elements 128 c + 32 q + 8 s + [0, 8) of token row r for the
 // s-th of the four.  The waves' partial sums meet in LDS in wave order.
 #include <algorithm>
+#include <utility>
 
 #include "common.h"
 
@@ -34,6 +35,7 @@ struct MxArgs {
   int N;               // output columns: F (gate/up) or H
   int Tn;              // column tiles
   int E;
+  const int* tile_off; // [E+1] row-tile prefix (tiled form)
 };
 
 __device__ __forceinline__ float sig_mx(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
@@ -48,6 +50,8 @@ __device__ __forceinline__ bf16x8 mx_frag(uint32_t w, float sc) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
+struct __attribute__((packed)) MxBytes8 { uint32_t v[2]; };
+
 // One pass: rows [row0, row0 + min(rows, 16 MT)) of the segment against the block's 16 NF weight rows.
 template <bool GU, int NF, int NW, int MT>
 __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, int rows, int n0, uint32_t tile, float* red) {
@@ -56,43 +60,70 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
   const int nb = g.K / 32;          // blocks of a row
   constexpr int RP = NF * 16 + 4;   // floats a row of the partial sums
   const int64_t eb = (int64_t)e * g.N * nb;  // blocks before this expert
-  const uint8_t* const wb[2] = {g.B + eb * 16, GU ? g.B2 + eb * 16 : nullptr};
-  const uint8_t* const sb[2] = {g.S + eb, GU ? g.S2 + eb : nullptr};
+  const uint8_t* const wb[2] = {g.B + eb * 16, (GU ? g.B2 : g.B) + eb * 16};
+  const uint8_t* const sb[2] = {g.S + eb, (GU ? g.S2 : g.S) + eb};
   // fragment f of the 16 NF weight rows: GU: the first NF / 2 gate rows, the others up rows; rows past N repeat the last
-  uint32_t wo[NF], ao[MT];  // in blocks of 32 elements
+  uint32_t wo[NF], ao[MT];  // the row's first block, and the row's first byte
 #pragma unroll
   for (int f = 0; f < NF; ++f)
     wo[f] = (uint32_t)min(n0 + (GU ? f % (NF / 2) : f) * 16 + r, g.N - 1) * (uint32_t)nb;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) ao[m] = (uint32_t)min(m * 16 + r, rows - 1) * (uint32_t)nb;
-  const uint16_t* const arow = g.A + row0 * g.K;
+  for (int m = 0; m < MT; ++m) ao[m] = (uint32_t)min(m * 16 + r, rows - 1) * (uint32_t)g.K * 2u;
+  const uint8_t* const arow = reinterpret_cast<const uint8_t*>(g.A + row0 * g.K);
 
-  u32x4 w[2][NF], a[2][MT][4];
-  uint32_t sc[2][NF];
-  auto load = [&](int b, int c) {
-    const bool in = c * 4 + q < nb;  // blocks past the row's end are zeros on both sides
-    const uint32_t blk = in ? c * 4 + q : 0;
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      const int o = GU && f >= NF / 2;
-      w[b][f] = *reinterpret_cast<const u32x4*>(wb[o] + (int64_t)(wo[f] + blk) * 16);
-      sc[b][f] = sb[o][wo[f] + blk];
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        a[b][m][s] = *reinterpret_cast<const u32x4*>(arow + (int64_t)(ao[m] + blk) * 32 + s * 8);
-    if (!in) {
+  // a unit: 256 columns, one 128-byte line of 4-bit values of each weight row, as two halves of four blocks
+  u32x4 w[2][NF][2], a[MT][2][4];
+  uint32_t sc[2][NF][2];
+  auto load_w = [&](int b, int u) {
+    if (u * 8 + 8 <= nb) {
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        w[b][f] = u32x4{0u, 0u, 0u, 0u};
-        sc[b][f] = 127u;
+        const int o = GU && f >= NF / 2;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          w[b][f][j] = *reinterpret_cast<const u32x4*>(wb[o] + u * 128 + j * 64 + (wo[f] + (uint32_t)q) * 16u);
+        const MxBytes8 s = *reinterpret_cast<const MxBytes8*>(sb[o] + u * 8 + wo[f]);
+        sc[b][f][0] = s.v[0];
+        sc[b][f][1] = s.v[1];
       }
+    } else {  // the row's last, partial unit: blocks past its end have any values and a finite scale (their tokens are zeros)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const int o = GU && f >= NF / 2;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int blk = u * 8 + j * 4 + q;
+          const uint32_t at = wo[f] + (uint32_t)min(blk, nb - 1);
+          w[b][f][j] = *reinterpret_cast<const u32x4*>(wb[o] + at * 16u);
+          const uint32_t s = sb[o][at];
+          sc[b][f][j] = (blk < nb ? s : 127u) << (8 * q);
+        }
+      }
+    }
+  };
+  auto load_a = [&](int u) {
+    if (u * 8 + 8 <= nb) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) a[b][m][s] = u32x4{0u, 0u, 0u, 0u};
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            a[m][j][s] = *reinterpret_cast<const u32x4*>(arow + u * 512 + j * 256 + s * 16 + (ao[m] + (uint32_t)q * 64u));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int blk = u * 8 + j * 4 + q;
+        const bool in = blk < nb;
+        const u32x4 z = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(arow + (ao[m] + (in ? (uint32_t)blk * 64u : 0u) + s * 16u));
+            a[m][j][s] = in ? v : z;
+          }
+      }
     }
   };
   f32x4 acc[NF][MT];
@@ -102,32 +133,41 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
     for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto mma = [&](int b) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int j = 0; j < 2; ++j) {
+      float sf[NF];
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const bf16x8 wf = mx_frag(w[b][f][s], __uint_as_float(sc[b][f] << 23));
+      for (int f = 0; f < NF; ++f) sf[f] = __uint_as_float(((sc[b][f][j] >> (8 * q)) & 0xffu) << 23);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[f][m] = mfma16x16x32(wf, __builtin_bit_cast(bf16x8, a[b][m][s]), acc[f][m]);
-      }
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const bf16x8 wf = mx_frag(w[b][f][j][s], sf[f]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[f][m] = mfma16x16x32(wf, __builtin_bit_cast(bf16x8, a[m][j][s]), acc[f][m]);
+        }
+    }
   };
-  const int nc = (nb + 3) / 4;
-  const int start = (int)__umulhi(tile * 0x9E3779B1u, (uint32_t)nc);
+  // the waves take every NW-th unit, from one on that differs between blocks
+  const int nu = (nb + 7) / 8;
+  const int start = (int)__umulhi(tile * 0x9E3779B1u, (uint32_t)nu);
   auto at = [&](int i) {
-    const int c = i + start;
-    return c < nc ? c : c - nc;
+    const int u = i + start;
+    return u < nu ? u : u - nu;
   };
-  int c = wv;
-  if (c < nc) {
-    load(0, at(c));
+  int u = wv;
+  if (u < nu) {
+    load_w(0, at(u));
     for (;;) {
-      if (c + NW < nc) load(1, at(c + NW));
+      load_a(at(u));
+      if (u + NW < nu) load_w(1, at(u + NW));
       mma(0);
-      c += NW;
-      if (c >= nc) break;
-      if (c + NW < nc) load(0, at(c + NW));
+      u += NW;
+      if (u >= nu) break;
+      load_a(at(u));
+      if (u + NW < nu) load_w(0, at(u + NW));
       mma(1);
-      c += NW;
-      if (c >= nc) break;
+      u += NW;
+      if (u >= nu) break;
     }
   }
 
@@ -175,7 +215,7 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
 constexpr int kMxPass = 32;  // rows of a pass
 
 template <bool GU, int NF, int NW>
-__global__ __launch_bounds__(NW * 64) void k_mx_small(MxArgs g) {
+__global__ __launch_bounds__(NW * 64, 8 / NW) void k_mx_small(MxArgs g) {
   __shared__ __attribute__((aligned(16))) float red[NW * 16 * (NF * 16 + 4)];
   const int slot = (int)(blockIdx.x / g.Tn), nt = (int)(blockIdx.x % g.Tn);
   int e = slot, pass = 0;
@@ -212,14 +252,307 @@ __global__ __launch_bounds__(NW * 64) void k_mx_small(MxArgs g) {
   else mx_pass<GU, NF, NW, 1>(g, e, m0, hi - m0, n0, tile, red);
 }
 
+// 64 weight rows and four waves a block; where that leaves fewer than 512 blocks with rows, 32 rows and eight waves.
 template <bool GU>
 int launch_small(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
   a.E = (int)E;
   const int64_t slots = E + R / kMxPass;  // every expert's first pass, and as many more as R rows can need
-  a.Tn = cdiv(a.N, GU ? 32 : 64);
+  const bool wide = cdiv(a.N, GU ? 32 : 64) * std::min(E, R) >= 512;
+  a.Tn = cdiv(a.N, (GU ? 16 : 32) * (wide ? 2 : 1));
   if (a.Tn * slots > INT32_MAX) return fail_arg("%s: too many tiles", name);
-  MOE_LAUNCH(name, (k_mx_small<GU, 4, 4>), dim3((unsigned)(a.Tn * slots)), dim3(256), 0, s, a);
+  if (wide) MOE_LAUNCH(name, (k_mx_small<GU, 4, 4>), dim3((unsigned)(a.Tn * slots)), dim3(256), 0, s, a);
+  else MOE_LAUNCH(name, (k_mx_small<GU, 2, 8>), dim3((unsigned)(a.Tn * slots)), dim3(512), 0, s, a);
   return check_launch(name);
+}
+
+// ---- many rows ----
+template <int P>
+__device__ __forceinline__ uint32_t mx_pair(uint32_t w, float sc) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, P));
+}
+
+// BM: rows of a tile.  MW: 32-row weight fragments of a wave (the block's four waves lie side by side on the weights).
+// WS: 64-wide slices of weights that a wave loads together.
+template <int BM, int MW, int WS, bool GU>
+__global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs g) {
+  constexpr int NB = BM / 32;                       // token fragments, and 16-byte pieces of a thread's share of a slice
+  constexpr int BN = 128 * MW;                      // weight rows of the tile
+  constexpr int CW = GU ? BN / 2 : BN;              // output columns of the tile
+  constexpr int WC = CW / 4;                        // ... and of a wave
+  constexpr int SLICE = BM * 128;                   // LDS bytes of a 64-wide slice of the rows
+  constexpr int CP = BN + 8;                        // pitch of the output tile (bf16)
+  constexpr int SMEM = 2 * SLICE > BM * CP * 2 ? 2 * SLICE : BM * CP * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i32 = lane & 31, h = lane >> 5;
+
+  // XCD-contiguous logical order over a 1-D grid sized for the most tiles any routing can produce: the tiles that there
+  // are, split into 8 contiguous ranges (blockIdx mod 8), row tiles of a column tile next to each other
+  const int total = g.tile_off[g.E] * g.Tn;
+  const int chunk = (total + 7) >> 3;
+  const int slot = (int)(blockIdx.x >> 3), L = (int)(blockIdx.x & 7) * chunk + slot;
+  if (slot >= chunk || L >= total) return;
+  int e = 0;  // the experts whose tiles all come before L
+  for (int e0 = 0; e0 < g.E; e0 += 64) {
+    const int i = e0 + lane;
+    const int n = __popcll(__ballot(i < g.E && g.tile_off[min(i, g.E - 1) + 1] * g.Tn <= L));
+    e += n;
+    if (n < 64) break;
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
+  const int cnt = g.tile_off[e + 1] - g.tile_off[e], local = L - g.tile_off[e] * g.Tn;
+  const int nt = local / cnt, mt = local - nt * cnt;
+  const int mbase = g.offsets[e] + mt * BM, mlen = min(BM, g.offsets[e + 1] - mbase);
+  const int n0 = nt * CW;
+  const int K = g.K, nb = K / 32;
+
+  // Slices: an even number, so that two fill the LDS ring.  What does not divide comes first, where the loads are checked:
+  // of the first `lead` slices (0 to 2) the last holds a row's last 32 values if K is no multiple of 64, and another is
+  // zeros; slice i >= lead holds values 64 (i - lead) on.
+  const int ns = ((K + 63) / 64 + 1) & ~1, lead = ns - K / 64;
+  const bool partial = (K & 63) != 0;  // K >= 128, so ns - 2 >= lead: a clamped load stays inside the rows
+
+  // rows: instruction j = NB wv + p of a slice fills rows 8 j + lane / 8; a row's eight 16-byte chunks are swizzled so that
+  // the 16 rows a fragment read touches at once lie in distinct banks
+  const uint8_t* const xbase = reinterpret_cast<const uint8_t*>(g.A + (int64_t)mbase * K);
+  uint32_t xo[NB];  // the piece's row and chunk, in bytes
+#pragma unroll
+  for (int p = 0; p < NB; ++p) {
+    const int row = 8 * (NB * wv + p) + (lane >> 3);
+    xo[p] = ((uint32_t)min(row, mlen - 1) * (uint32_t)K + (uint32_t)(((lane & 7) ^ ((row >> 1) & 7)) * 8)) * 2u;
+  }
+  // weights: the wave's MW fragments of 32 rows, straight to registers; GU: gate rows, then the same up rows
+  const int64_t eb = (int64_t)e * g.N * nb;
+  auto wbase = [&](int m) { return (GU && m >= MW / 2 ? g.B2 : g.B) + eb * 16; };
+  auto sbase = [&](int m) { return (GU && m >= MW / 2 ? g.S2 : g.S) + eb; };
+  uint32_t wo[MW];  // the row's first block
+#pragma unroll
+  for (int m = 0; m < MW; ++m)
+    wo[m] = (uint32_t)min(n0 + wv * WC + (GU ? m % (MW / 2) : m) * 32 + i32, g.N - 1) * (uint32_t)nb;
+
+  u32x4 xs[NB], w[2][WS][MW];
+  uint32_t sw[2][MW];  // scale bytes of a set's slices: 16 j + 8 h bits up for slice j (shifted where they are used: a use waits)
+  auto load_x = [&](int i, int p) {
+    xs[p] = *reinterpret_cast<const u32x4*>(xbase + (int64_t)(min(i, ns - 1) - lead) * 128 + xo[p]);
+  };
+  auto load_x_checked = [&](int i, int p) {
+    const int row = 8 * (NB * wv + p) + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+    const bool half = i == lead - 1 && partial;
+    const bool in = i >= lead || (half && c < 4);
+    const int k = i >= lead ? (i - lead) * 64 : K - 32;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(xbase + (in ? xo[p] + (uint32_t)k * 2u : xo[p] - (uint32_t)c * 16u));
+    xs[p] = in ? v : u32x4{0u, 0u, 0u, 0u};
+  };
+  auto write_x = [&](int i, int p) {
+    __asm__ volatile("" ::: "memory");
+    *reinterpret_cast<u32x4*>(smem + (i & 1) * SLICE + (NB * wv + p) * 1024 + lane * 16) = xs[p];
+    __asm__ volatile("" ::: "memory");
+  };
+  struct __attribute__((packed)) Bytes4 { uint32_t v; };
+  struct __attribute__((packed)) Bytes2 { uint16_t v; };
+  // the weights of slices [i, i + WS); those of a set wholly behind the last slice are never used
+  auto load_w = [&](int set, int i) {
+    const int at = min(i, ns - WS) - lead;
+#pragma unroll
+    for (int m = 0; m < MW; ++m) {
+#pragma unroll
+      for (int j = 0; j < WS; ++j)
+        w[set][j][m] = *reinterpret_cast<const u32x4*>(wbase(m) + (int64_t)(at + j) * 32 + (wo[m] + (uint32_t)h) * 16u);
+      const uint8_t* const s = sbase(m) + (int64_t)at * 2 + wo[m];
+      sw[set][m] = WS == 2 ? reinterpret_cast<const Bytes4*>(s)->v : (uint32_t)reinterpret_cast<const Bytes2*>(s)->v;
+    }
+  };
+  // ... of a set that may hold leading slices, whose missing weights are any (their rows are zeros) with a finite scale
+  auto load_w_checked = [&](int set, int i) {
+#pragma unroll
+    for (int m = 0; m < MW; ++m) {
+      sw[set][m] = 0u;
+#pragma unroll
+      for (int j = 0; j < WS; ++j) {
+        const int l = i + j;
+        const bool in = (l >= lead && l < ns) || (l == lead - 1 && partial && h == 0);
+        const uint32_t o = wo[m] + (uint32_t)(!in ? 0 : l >= lead ? 2 * (l - lead) + h : nb - 1);
+        w[set][j][m] = *reinterpret_cast<const u32x4*>(wbase(m) + o * 16u);
+        const uint32_t s = *(sbase(m) + o);
+        sw[set][m] |= (in ? s : 127u) << (16 * j + 8 * h);
+      }
+    }
+  };
+  float sf[MW];  // the scales of the slice whose weights are used next
+  auto scales = [&](int set, int j) {
+#pragma unroll
+    for (int m = 0; m < MW; ++m) sf[m] = __uint_as_float(((sw[set][m] >> (16 * j + 8 * h)) & 0xffu) << 23);
+  };
+  auto frag = [&](int i, int s, int n) {
+    const int row = n * 32 + i32;
+    return *reinterpret_cast<const bf16x8*>(smem + (i & 1) * SLICE + row * 128 + (((4 * h + s) ^ ((row >> 1) & 7)) << 4));
+  };
+
+  f32x16 acc[MW][NB];
+#pragma unroll
+  for (int m = 0; m < MW; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[m][n][j] = 0.f;
+  bf16x8 fb0[NB], fb1[NB];
+  u32x4 wf0[MW], wf1[MW];
+
+  // One 16-wide step of slice i: MW NB MFMAs, and between them the next step's token fragments, its weights' conversion and
+  // refill pieces [PLO, PHI) (slice i + 1 to LDS, i + 2 from memory)
+  auto step = [&](auto plo_c, auto phi_c, auto ns_c, const bf16x8(&cb)[NB], const u32x4(&cw)[MW], bf16x8(&nb_)[NB],
+                  u32x4(&nw)[MW], int ni, auto nset_c, auto nj_c, int i) {
+    constexpr int PLO = decltype(plo_c)::value, PHI = decltype(phi_c)::value;
+    constexpr int NS = decltype(ns_c)::value, NSET = decltype(nset_c)::value, NJ = decltype(nj_c)::value;
+    constexpr int SLOTS = MW * NB, CV = MW * 4;
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      (([&] {
+         constexpr int n = I / MW, m = I % MW;
+         acc[m][n] = mfma32x32x16(__builtin_bit_cast(bf16x8, cw[m]), cb[n], acc[m][n]);
+         __builtin_amdgcn_sched_barrier(0);
+         if constexpr (I < NB) nb_[I] = frag(ni, NS, I);
+         constexpr int C0 = I * CV / SLOTS, C1 = (I + 1) * CV / SLOTS;
+         [&]<int... C>(std::integer_sequence<int, C...>) {
+           ((nw[(C0 + C) / 4][(C0 + C) % 4] = mx_pair<(C0 + C) % 4>(w[NSET][NJ][(C0 + C) / 4][NS], sf[(C0 + C) / 4])), ...);
+         }(std::make_integer_sequence<int, C1 - C0>{});
+         constexpr int p = PLO + I - NB;
+         if constexpr (I >= NB && p < PHI) {
+           write_x(i + 1, p);
+           load_x(i + 2, p);
+         }
+         __builtin_amdgcn_sched_barrier(0);
+       }()), ...);
+    }(std::make_integer_sequence<int, SLOTS>{});
+  };
+  constexpr int P1 = (NB + 2) / 3, P2 = (2 * NB + 2) / 3;
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  using IP1 = std::integral_constant<int, P1>;
+  using IP2 = std::integral_constant<int, P2>;
+  using IPN = std::integral_constant<int, NB>;
+  // slice i, the J-th of set SET
+  auto slice = [&](auto set_c, auto j_c, int i) {
+    constexpr int SET = decltype(set_c)::value, J = decltype(j_c)::value;
+    using NSet = std::integral_constant<int, J + 1 < WS ? SET : 1 - SET>;
+    using NJ = std::integral_constant<int, (J + 1) % WS>;
+    step(I0{}, IP1{}, I1{}, fb0, wf0, fb1, wf1, i, set_c, j_c, i);
+    step(IP1{}, IP2{}, I2{}, fb1, wf1, fb0, wf0, i, set_c, j_c, i);
+    step(IP2{}, IPN{}, I3{}, fb0, wf0, fb1, wf1, i, set_c, j_c, i);
+    if constexpr (WS == 1) load_w(SET, i + 2);
+    lds_sync();  // every wave's pieces of slice i + 1 are written and its reads of slice i done
+    scales(NSet::value, NJ::value);
+    __builtin_amdgcn_sched_barrier(0);
+    step(I0{}, I0{}, I0{}, fb1, wf1, fb0, wf0, i + 1, NSet{}, NJ{}, i);
+  };
+#pragma unroll
+  for (int p = 0; p < NB; ++p) load_x_checked(0, p);
+  load_w_checked(0, 0);
+#pragma unroll
+  for (int p = 0; p < NB; ++p) {
+    write_x(0, p);
+    load_x_checked(1, p);
+  }
+  load_w_checked(1, WS);
+  __syncthreads();
+  scales(0, 0);
+#pragma unroll
+  for (int n = 0; n < NB; ++n) fb0[n] = frag(0, 0, n);
+#pragma unroll
+  for (int m = 0; m < MW; ++m) wf0[m] = __builtin_bit_cast(u32x4, mx_frag(w[0][0][m][0], sf[m]));
+  for (int i = 0; i < ns; i += 2) {
+    slice(I0{}, I0{}, i);
+    if constexpr (WS == 1) {
+      slice(I1{}, I0{}, i + 1);
+    } else {
+      slice(I0{}, I1{}, i + 1);
+#pragma unroll
+      for (int m = 0; m < MW; ++m) {  // the next pair's weights, which have arrived, make room for those behind them
+#pragma unroll
+        for (int j = 0; j < WS; ++j) w[0][j][m] = w[1][j][m];
+        sw[0][m] = sw[1][m];
+      }
+      load_w(1, i + 4);
+    }
+  }
+  __syncthreads();
+
+  // acc[m][n][j]: weight row 32 m + (j & 3) + 8 (j >> 2) + 4 h of the wave's, token row 32 n + i32.  The tile goes through
+  // LDS so that its rows leave as whole segments.
+  uint16_t* const ct = reinterpret_cast<uint16_t*>(smem);
+  auto put = [&](int n, int col, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(ct + (n * 32 + i32) * CP + col + 4 * h) = uint2{pack2bf(a, b), pack2bf(c, d)};
+  };
+  auto out = [&](auto cols_c, auto at) {
+    constexpr int UR = decltype(cols_c)::value / 8;  // 16-byte units of a row
+    __syncthreads();
+    for (int u = tid; u < BM * UR; u += 256) {
+      const int row = u / UR, c = (u % UR) * 8;
+      uint16_t* const dst = at(row, c);
+      if (row < mlen && dst != nullptr) *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(ct + row * CP + c);
+    }
+  };
+  if constexpr (GU) {
+#pragma unroll
+    for (int m = 0; m < MW / 2; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float a[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = acc[m][n][4 * q + j];
+            a[j] = x * sig_mx(x) * acc[MW / 2 + m][n][4 * q + j];
+          }
+          put(n, wv * WC + m * 32 + q * 8, a[0], a[1], a[2], a[3]);
+        }
+    out(std::integral_constant<int, CW>{}, [&](int row, int c) {
+      return n0 + c < g.N ? g.C + (int64_t)(mbase + row) * g.N + n0 + c : nullptr;
+    });
+    if (g.C2 == nullptr) return;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int m = 0; m < MW; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        put(n, (GU ? m / (MW / 2) * CW + m % (MW / 2) * 32 : m * 32) + wv * WC + q * 8, acc[m][n][4 * q],
+            acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]);
+  out(std::integral_constant<int, BN>{}, [&](int row, int c) -> uint16_t* {
+    if constexpr (GU) {
+      const int f = n0 + c % CW;
+      return f < g.N ? g.C2 + (int64_t)(mbase + row) * 2 * g.N + (c < CW ? f : g.N + f) : nullptr;
+    } else {
+      return n0 + c < g.N ? g.C + (int64_t)(mbase + row) * g.N + n0 + c : nullptr;
+    }
+  });
+}
+
+template <int BM, int MW, int WS, bool GU>
+int launch_tile_as(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
+  a.E = (int)E;
+  a.Tn = cdiv(a.N, GU ? 64 * MW : 128 * MW);
+  const int64_t blocks = ((R + BM - 1) / BM + E) * a.Tn;
+  if (blocks > INT32_MAX - 8) return fail_arg("%s: too many tiles", name);
+  MOE_LAUNCH(name, (k_mx_tile<BM, MW, WS, GU>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(256), 0, s, a);
+  return check_launch(name);
+}
+template <int BM, bool GU>
+int launch_tile(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
+  if constexpr (BM == 256) return launch_tile_as<256, 2, 1, GU>(name, s, a, E, R);
+  else if constexpr (BM == 128) return launch_tile_as<128, 2, 2, GU>(name, s, a, E, R);
+  else return launch_tile_as<64, 2, 2, GU>(name, s, a, E, R);
+}
+
+// Rows of a tile (0: the few-row form).  The tiled loop loads two whole slices of a row at a time, also behind the last one
+// (clamped to it): it takes reductions of 128 and more.
+int mx_rows(int64_t R, int64_t H, int64_t F, int64_t E) {
+  if (H < 128 || F < 128) return 0;
+  return R <= 24 * E ? 0 : R <= 64 * E ? 64 : R <= 160 * E ? 128 : 256;
 }
 
 bool al16x(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -227,8 +560,8 @@ size_t al256x(size_t v) { return (v + 255) & ~(size_t)255; }
 
 int mx_shape(const char* what, int64_t R, int64_t H, int64_t F, int64_t E) {
   const int64_t lim = INT32_MAX;
-  if (R < 0 || R > lim || H < 32 || F < 32 || E < 1 || E > 1024 || H % 32 || F % 32 || H > lim / 64 || F > lim / 64 ||
-      H * F > lim * 16)
+  if (R < 0 || R > lim || H < 32 || F < 32 || E < 1 || E > 1024 || H % 32 || F % 32 || H > lim / 512 || F > lim / 512 ||
+      H * F > lim * 2)
     return fail_arg("%s: bad shape R=%lld H=%lld F=%lld E=%lld (need H%%32==0, F%%32==0, E<=1024)", what, (long long)R,
                     (long long)H, (long long)F, (long long)E);
   return 0;
@@ -268,8 +601,17 @@ extern "C" int moe_swiglu_fwd_mxfp4(const void* xp, const void* wg_q, const void
   a.C2 = static_cast<uint16_t*>(hgu);
   a.K = (int)H;
   a.N = (int)F;
-  if (int rc = launch_small<true>("k_mx_small_fwd1", s, a, E, R)) return rc;
+  const int bm = mx_rows(R, H, F, E);
+  a.tile_off = static_cast<const int*>(workspace);
+  if (bm > 0)
+    if (int rc = swiglu_tiles(offsets, E, bm, workspace, s)) return rc;
+  if (int rc = bm == 256   ? launch_tile<256, true>("k_mx_tile_fwd1", s, a, E, R)
+               : bm == 128 ? launch_tile<128, true>("k_mx_tile_fwd1", s, a, E, R)
+               : bm == 64  ? launch_tile<64, true>("k_mx_tile_fwd1", s, a, E, R)
+                           : launch_small<true>("k_mx_small_fwd1", s, a, E, R))
+    return rc;
   MxArgs b{};
+  b.tile_off = a.tile_off;
   b.offsets = offsets;
   b.A = act;
   b.B = static_cast<const uint8_t*>(wd_q);
@@ -277,7 +619,10 @@ extern "C" int moe_swiglu_fwd_mxfp4(const void* xp, const void* wg_q, const void
   b.C = static_cast<uint16_t*>(y);
   b.K = (int)F;
   b.N = (int)H;
-  return launch_small<false>("k_mx_small_fwd2", s, b, E, R);
+  return bm == 256   ? launch_tile<256, false>("k_mx_tile_fwd2", s, b, E, R)
+         : bm == 128 ? launch_tile<128, false>("k_mx_tile_fwd2", s, b, E, R)
+         : bm == 64  ? launch_tile<64, false>("k_mx_tile_fwd2", s, b, E, R)
+                     : launch_small<false>("k_mx_small_fwd2", s, b, E, R);
 }
 
 // ---- backward to the rows ----
@@ -307,7 +652,7 @@ extern "C" int moe_swiglu_bwd_mxfp4(const void* dy, const void* hgu, const void*
   char* w1 = w0 + al256x((size_t)E * F * H * 2);
   const int64_t n = E * F * H;
   if (int rc = dequant_mxfp4_bf16(wd_q, sd, n, w0, s)) return rc;
-  if (int rc = swiglu_tiles(offsets, E, workspace, s)) return rc;
+  if (int rc = swiglu_tiles(offsets, E, kGemmRows, workspace, s)) return rc;
   if (int rc = swiglu_dact(dy, hgu, w0, offsets, R, H, F, E, dh, workspace, s)) return rc;
   if (int rc = dequant_mxfp4_bf16(wg_q, sg, n, w0, s)) return rc;
   if (int rc = dequant_mxfp4_bf16(wu_q, su, n, w1, s)) return rc;

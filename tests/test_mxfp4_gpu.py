@@ -85,6 +85,10 @@ CASES = [
     (96, 160, [5, 17, 1]),                   # a partial 128-column chunk in both products
     (128, 128, [16, 32, 33, 64, 65, 1]),     # at the row passes' edges
     (160, 96, [3] * 130),                    # more than 128 experts
+    (32, 32, [70, 5, 300]),                  # one block a row, many rows
+    (96, 64, [100, 0, 257, 64]),             # rows of an odd number of blocks
+    (288, 416, [500, 130]),                  # reductions that leave 32 of 128 columns
+    (192, 224, [260, 0, 129]),               # ... 64 and 96
     (544, 1056, [127, 0, 129, 40]),          # odd blocks of a row
     (2048, 768, [9, 3, 0, 70]),
     (1024, 4096, [300, 0, 513, 1]),
