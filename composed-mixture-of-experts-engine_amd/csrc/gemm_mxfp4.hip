@@ -15,6 +15,7 @@
 // agree: lane 16 q + r holds block 4 c + q of row r, and takes elements 128 c + 32 q + 8 s + [0, 8) of token row r for the
 // s-th of the four.  The waves' partial sums meet in LDS in wave order.
 #include <algorithm>
+#include <cstdlib>
 #include <utility>
 
 #include "common.h"
@@ -36,6 +37,8 @@ struct MxArgs {
   int Tn;              // column tiles
   int E;
   const int* tile_off; // [E+1] row-tile prefix (tiled form)
+  float* part;         // partial tiles of a split last round (tiled down projection; null: no split)
+  int npart;           // ... and how many of them an XCD has room for
 };
 
 __device__ __forceinline__ float sig_mx(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
@@ -271,10 +274,52 @@ __device__ __forceinline__ uint32_t mx_pair(uint32_t w, float sc) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, P));
 }
 
+// The expert of logical tile L: the experts whose tiles all come before it.
+__device__ __forceinline__ int mx_expert(const MxArgs& g, int L, int lane) {
+  int e = 0;
+  for (int e0 = 0; e0 < g.E; e0 += 64) {
+    const int i = e0 + lane;
+    const int n = __popcll(__ballot(i < g.E && g.tile_off[min(i, g.E - 1) + 1] * g.Tn <= L));
+    e += n;
+    if (n < 64) break;
+  }
+  return __builtin_amdgcn_readfirstlane(e);
+}
+
+// Blocks of a tiled product that an XCD's 32 CUs hold at once.
+__host__ __device__ constexpr int mx_resident(int bm) { return bm == 256 ? 32 : 64; }
+
+// The last round of a product: an XCD's n tiles run `resident` at a time, and its last n % resident leave the rest of it
+// idle; with few rows that round is all there is.  Those tiles are split over their slices, in rounds of G, into `parts`
+// blocks each, whose fp32 tiles go to memory and are added in order by k_mx_reduce.  parts (1 to 8) is the one with the
+// least estimated time in slices: the rounds that the parts take, plus 16 slices a part for writing and reading back its
+// tile, plus the reduction's launch.  Every block computes it from the device's tile count, and the reduction again.
+struct MxSplit {
+  int full, rest, parts;  // whole tiles; split tiles; blocks of each
+};
+__device__ __forceinline__ MxSplit mx_split(int n, int ns, int npart, int resident, int G) {
+  MxSplit s{0, 0, 1};
+  if (n <= 0) return s;
+  s.rest = n % resident;
+  s.full = n - s.rest;
+  int cost = ns;
+  for (int S = 2; s.rest > 0 && S <= 8; ++S) {
+    if (s.rest * S > npart || S * G > ns) break;
+    const int c = (s.rest * S + resident - 1) / resident * ((ns + S - 1) / S + 16) + 5;
+    if (c < cost) {
+      cost = c;
+      s.parts = S;
+    }
+  }
+  return s;
+}
+
 // BM: rows of a tile.  MW: 32-row weight fragments of a wave (the block's four waves lie side by side on the weights).
-// WS: 64-wide slices of weights that a wave loads together.
-template <int BM, int MW, int WS, bool GU>
+// G: 64-wide slices of weights in flight or in use (a slice's registers are loaded with slice i + G as soon as slice i is
+// converted).  XD: slices of the rows on their way from memory to LDS.
+template <int BM, int MW, int G, int XD, bool GU>
 __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs g) {
+  constexpr bool EVEN = BM == 256;                  // K % 128 == 0: rounds of two whole slices, nothing to mask
   constexpr int NB = BM / 32;                       // token fragments, and 16-byte pieces of a thread's share of a slice
   constexpr int BN = 128 * MW;                      // weight rows of the tile
   constexpr int CW = GU ? BN / 2 : BN;              // output columns of the tile
@@ -289,32 +334,41 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
   // XCD-contiguous logical order over a 1-D grid sized for the most tiles any routing can produce: the tiles that there
   // are, split into 8 contiguous ranges (blockIdx mod 8), row tiles of a column tile next to each other
   const int total = g.tile_off[g.E] * g.Tn;
-  const int chunk = (total + 7) >> 3;
-  const int slot = (int)(blockIdx.x >> 3), L = (int)(blockIdx.x & 7) * chunk + slot;
-  if (slot >= chunk || L >= total) return;
-  int e = 0;  // the experts whose tiles all come before L
-  for (int e0 = 0; e0 < g.E; e0 += 64) {
-    const int i = e0 + lane;
-    const int n = __popcll(__ballot(i < g.E && g.tile_off[min(i, g.E - 1) + 1] * g.Tn <= L));
-    e += n;
-    if (n < 64) break;
+  const int chunk = (total + 7) >> 3, xcd = (int)(blockIdx.x & 7);
+  int slot = (int)(blockIdx.x >> 3);
+  int b0 = 0, b1 = (g.K + 63) / 64;   // the block's slices of the reduction
+  float* part_out = nullptr;
+  if constexpr (!GU) {
+    if (g.part != nullptr) {
+      const MxSplit sp = mx_split(min(chunk, total - xcd * chunk), b1, g.npart, mx_resident(BM), G);
+      if (sp.parts > 1 && slot >= sp.full) {
+        const int j = slot - sp.full, t = j / sp.parts, p = j - t * sp.parts;
+        if (t >= sp.rest) return;
+        slot = sp.full + t;
+        b0 = __builtin_amdgcn_readfirstlane(b1 / G * p / sp.parts * G);
+        b1 = __builtin_amdgcn_readfirstlane(p + 1 == sp.parts ? b1 : b1 / G * (p + 1) / sp.parts * G);
+        part_out = g.part + (int64_t)(xcd * g.npart + j) * (BM * BN);
+      }
+    }
   }
-  e = __builtin_amdgcn_readfirstlane(e);
+  const int L = xcd * chunk + slot;
+  if (slot >= chunk || L >= total) return;
+  const int e = mx_expert(g, L, lane);
   const int cnt = g.tile_off[e + 1] - g.tile_off[e], local = L - g.tile_off[e] * g.Tn;
   const int nt = local / cnt, mt = local - nt * cnt;
   const int mbase = g.offsets[e] + mt * BM, mlen = min(BM, g.offsets[e + 1] - mbase);
   const int n0 = nt * CW;
   const int K = g.K, nb = K / 32;
 
-  // Slices: an even number, so that two fill the LDS ring.  What does not divide comes first, where the loads are checked:
-  // of the first `lead` slices (0 to 2) the last holds a row's last 32 values if K is no multiple of 64, and another is
-  // zeros; slice i >= lead holds values 64 (i - lead) on.
-  const int ns = ((K + 63) / 64 + 1) & ~1, lead = ns - K / 64;
-  const bool partial = (K & 63) != 0;  // K >= 128, so ns - 2 >= lead: a clamped load stays inside the rows
+  // Slices: if K is no multiple of 64, slice 0 holds a row's last 32 values (its loads are the checked ones) and slice i the
+  // 64 from 64 (i - 1) on.  The loop takes them in rounds of G; a slice behind the last, ns, is zeros.
+  // A part of a split tile starts at slice b0.
+  const int lead = b0 > 0 ? 0 : (K + 63) / 64 - K / 64, ns = b1 - b0;  // ns - lead >= 2: K >= 128, parts have rounds of G
+  const int first = b0 > 0 ? b0 - ((K + 63) / 64 - K / 64) : 0;         // whole slices of the row in front of the block's
 
   // rows: instruction j = NB wv + p of a slice fills rows 8 j + lane / 8; a row's eight 16-byte chunks are swizzled so that
   // the 16 rows a fragment read touches at once lie in distinct banks
-  const uint8_t* const xbase = reinterpret_cast<const uint8_t*>(g.A + (int64_t)mbase * K);
+  const uint8_t* const xbase = reinterpret_cast<const uint8_t*>(g.A + (int64_t)mbase * K + first * 64);
   uint32_t xo[NB];  // the piece's row and chunk, in bytes
 #pragma unroll
   for (int p = 0; p < NB; ++p) {
@@ -323,65 +377,70 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
   }
   // weights: the wave's MW fragments of 32 rows, straight to registers; GU: gate rows, then the same up rows
   const int64_t eb = (int64_t)e * g.N * nb;
-  auto wbase = [&](int m) { return (GU && m >= MW / 2 ? g.B2 : g.B) + eb * 16; };
-  auto sbase = [&](int m) { return (GU && m >= MW / 2 ? g.S2 : g.S) + eb; };
+  auto wbase = [&](int m) { return (GU && m >= MW / 2 ? g.B2 : g.B) + eb * 16 + first * 32; };
+  auto sbase = [&](int m) { return (GU && m >= MW / 2 ? g.S2 : g.S) + eb + first * 2; };
   uint32_t wo[MW];  // the row's first block
 #pragma unroll
   for (int m = 0; m < MW; ++m)
     wo[m] = (uint32_t)min(n0 + wv * WC + (GU ? m % (MW / 2) : m) * 32 + i32, g.N - 1) * (uint32_t)nb;
 
-  u32x4 xs[NB], w[2][WS][MW];
-  uint32_t sw[2][MW];  // scale bytes of a set's slices: 16 j + 8 h bits up for slice j (shifted where they are used: a use waits)
-  auto load_x = [&](int i, int p) {
-    xs[p] = *reinterpret_cast<const u32x4*>(xbase + (int64_t)(min(i, ns - 1) - lead) * 128 + xo[p]);
+  // scale bytes: of a slice (G == 2), or of two slices in one word; a lane's byte is 8 h (+ 16) bits up
+  constexpr int SJ = G == 2 ? 1 : 2;
+  u32x4 xs[XD][NB], w[G][MW];
+  uint32_t sw[G / SJ][MW];
+  auto load_x = [&](int slot, int i, int p) {
+    xs[slot][p] = *reinterpret_cast<const u32x4*>(xbase + (int64_t)(min(i, ns - 1) - lead) * 128 + xo[p]);
   };
-  auto load_x_checked = [&](int i, int p) {
+  auto load_x_first = [&](int p) {
     const int row = 8 * (NB * wv + p) + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-    const bool half = i == lead - 1 && partial;
-    const bool in = i >= lead || (half && c < 4);
-    const int k = i >= lead ? (i - lead) * 64 : K - 32;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(xbase + (in ? xo[p] + (uint32_t)k * 2u : xo[p] - (uint32_t)c * 16u));
-    xs[p] = in ? v : u32x4{0u, 0u, 0u, 0u};
+    const bool in = lead == 0 || c < 4;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(
+        xbase + (in ? xo[p] + (lead ? (uint32_t)(K - 32) * 2u : 0u) : xo[p] - (uint32_t)c * 16u));
+    xs[0][p] = in ? v : u32x4{0u, 0u, 0u, 0u};
   };
-  auto write_x = [&](int i, int p) {
+  auto write_x = [&](int slot, int i, int p) {
+    const uint32_t keep = EVEN || i < ns ? ~0u : 0u;
     __asm__ volatile("" ::: "memory");
-    *reinterpret_cast<u32x4*>(smem + (i & 1) * SLICE + (NB * wv + p) * 1024 + lane * 16) = xs[p];
+    *reinterpret_cast<u32x4*>(smem + (i & 1) * SLICE + (NB * wv + p) * 1024 + lane * 16) = xs[slot][p] & keep;
     __asm__ volatile("" ::: "memory");
   };
   struct __attribute__((packed)) Bytes4 { uint32_t v; };
   struct __attribute__((packed)) Bytes2 { uint16_t v; };
-  // the weights of slices [i, i + WS); those of a set wholly behind the last slice are never used
-  auto load_w = [&](int set, int i) {
-    const int at = min(i, ns - WS) - lead;
+  // slice i's weights; those behind the last slice are never used
+  auto load_w = [&](int slot, int i) {
+    const int at = min(i, ns - 1) - lead;
+#pragma unroll
+    for (int m = 0; m < MW; ++m)
+      w[slot][m] = *reinterpret_cast<const u32x4*>(wbase(m) + (int64_t)at * 32 + (wo[m] + (uint32_t)h) * 16u);
+  };
+  // the scales of slices [i, i + SJ); of the last slice alone, those of the last two
+  auto load_s = [&](int slot, int i) {
+    const int at = min(i, ns - SJ) - lead;
 #pragma unroll
     for (int m = 0; m < MW; ++m) {
-#pragma unroll
-      for (int j = 0; j < WS; ++j)
-        w[set][j][m] = *reinterpret_cast<const u32x4*>(wbase(m) + (int64_t)(at + j) * 32 + (wo[m] + (uint32_t)h) * 16u);
       const uint8_t* const s = sbase(m) + (int64_t)at * 2 + wo[m];
-      sw[set][m] = WS == 2 ? reinterpret_cast<const Bytes4*>(s)->v : (uint32_t)reinterpret_cast<const Bytes2*>(s)->v;
+      sw[slot][m] = SJ == 2 ? reinterpret_cast<const Bytes4*>(s)->v : (uint32_t)reinterpret_cast<const Bytes2*>(s)->v;
     }
   };
-  // ... of a set that may hold leading slices, whose missing weights are any (their rows are zeros) with a finite scale
-  auto load_w_checked = [&](int set, int i) {
+  // both of the first round, in which slice 0 may be half a slice (its second half: any weights, a finite scale)
+  auto load_w_first = [&](int l) {
+    const bool in = l < ns && (l >= lead || h == 0);
 #pragma unroll
     for (int m = 0; m < MW; ++m) {
-      sw[set][m] = 0u;
-#pragma unroll
-      for (int j = 0; j < WS; ++j) {
-        const int l = i + j;
-        const bool in = (l >= lead && l < ns) || (l == lead - 1 && partial && h == 0);
-        const uint32_t o = wo[m] + (uint32_t)(!in ? 0 : l >= lead ? 2 * (l - lead) + h : nb - 1);
-        w[set][j][m] = *reinterpret_cast<const u32x4*>(wbase(m) + o * 16u);
-        const uint32_t s = *(sbase(m) + o);
-        sw[set][m] |= (in ? s : 127u) << (16 * j + 8 * h);
-      }
+      const uint32_t o = wo[m] + (uint32_t)(!in ? 0 : l >= lead ? 2 * (l - lead) + h : nb - 1);
+      w[l][m] = *reinterpret_cast<const u32x4*>(wbase(m) + o * 16u);
+      const uint32_t s = (in ? (uint32_t)*(sbase(m) + o) : 127u) << (16 * (l % SJ) + 8 * h);
+      sw[l / SJ][m] = l % SJ == 0 ? s : sw[l / SJ][m] | s;
     }
   };
-  float sf[MW];  // the scales of the slice whose weights are used next
-  auto scales = [&](int set, int j) {
+  float sf[MW];  // the scales of the slice whose weights are used next (finite behind the last one)
+  auto scales = [&](int l, int i) {
+    const int up = 16 * (l % SJ) + (SJ == 2 && l % 2 == 0 && i >= G && i == ns - 1 ? 16 : 0);
 #pragma unroll
-    for (int m = 0; m < MW; ++m) sf[m] = __uint_as_float(((sw[set][m] >> (16 * j + 8 * h)) & 0xffu) << 23);
+    for (int m = 0; m < MW; ++m) {
+      const uint32_t b = ((sw[l / SJ][m] >> (up + 8 * h)) & 0xffu) << 23;
+      sf[m] = __uint_as_float(EVEN || i < ns ? b : 0x3f800000u);
+    }
   };
   auto frag = [&](int i, int s, int n) {
     const int row = n * 32 + i32;
@@ -399,11 +458,11 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
   u32x4 wf0[MW], wf1[MW];
 
   // One 16-wide step of slice i: MW NB MFMAs, and between them the next step's token fragments, its weights' conversion and
-  // refill pieces [PLO, PHI) (slice i + 1 to LDS, i + 2 from memory)
+  // refill pieces [PLO, PHI) (slice i + 1 to LDS, i + 1 + XD from memory)
   auto step = [&](auto plo_c, auto phi_c, auto ns_c, const bf16x8(&cb)[NB], const u32x4(&cw)[MW], bf16x8(&nb_)[NB],
-                  u32x4(&nw)[MW], int ni, auto nset_c, auto nj_c, int i) {
+                  u32x4(&nw)[MW], int ni, auto nl_c, auto xl_c, int i) {
     constexpr int PLO = decltype(plo_c)::value, PHI = decltype(phi_c)::value;
-    constexpr int NS = decltype(ns_c)::value, NSET = decltype(nset_c)::value, NJ = decltype(nj_c)::value;
+    constexpr int NS = decltype(ns_c)::value, NL = decltype(nl_c)::value, XL = decltype(xl_c)::value;
     constexpr int SLOTS = MW * NB, CV = MW * 4;
     [&]<int... I>(std::integer_sequence<int, I...>) {
       (([&] {
@@ -413,12 +472,12 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
          if constexpr (I < NB) nb_[I] = frag(ni, NS, I);
          constexpr int C0 = I * CV / SLOTS, C1 = (I + 1) * CV / SLOTS;
          [&]<int... C>(std::integer_sequence<int, C...>) {
-           ((nw[(C0 + C) / 4][(C0 + C) % 4] = mx_pair<(C0 + C) % 4>(w[NSET][NJ][(C0 + C) / 4][NS], sf[(C0 + C) / 4])), ...);
+           ((nw[(C0 + C) / 4][(C0 + C) % 4] = mx_pair<(C0 + C) % 4>(w[NL][(C0 + C) / 4][NS], sf[(C0 + C) / 4])), ...);
          }(std::make_integer_sequence<int, C1 - C0>{});
          constexpr int p = PLO + I - NB;
          if constexpr (I >= NB && p < PHI) {
-           write_x(i + 1, p);
-           load_x(i + 2, p);
+           write_x(XL, i + 1, p);
+           load_x(XL, i + 1 + XD, p);
          }
          __builtin_amdgcn_sched_barrier(0);
        }()), ...);
@@ -432,51 +491,59 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
   using IP1 = std::integral_constant<int, P1>;
   using IP2 = std::integral_constant<int, P2>;
   using IPN = std::integral_constant<int, NB>;
-  // slice i, the J-th of set SET
-  auto slice = [&](auto set_c, auto j_c, int i) {
-    constexpr int SET = decltype(set_c)::value, J = decltype(j_c)::value;
-    using NSet = std::integral_constant<int, J + 1 < WS ? SET : 1 - SET>;
-    using NJ = std::integral_constant<int, (J + 1) % WS>;
-    step(I0{}, IP1{}, I1{}, fb0, wf0, fb1, wf1, i, set_c, j_c, i);
-    step(IP1{}, IP2{}, I2{}, fb1, wf1, fb0, wf0, i, set_c, j_c, i);
-    step(IP2{}, IPN{}, I3{}, fb0, wf0, fb1, wf1, i, set_c, j_c, i);
-    if constexpr (WS == 1) load_w(SET, i + 2);
+  // slice i, at position J of a round of G
+  auto slice = [&](auto j_c, int i) {
+    constexpr int J = decltype(j_c)::value;
+    using NJ = std::integral_constant<int, (J + 1) % G>;
+    using X = std::integral_constant<int, (J + 1) % XD>;
+    step(I0{}, IP1{}, I1{}, fb0, wf0, fb1, wf1, i, j_c, X{}, i);
+    step(IP1{}, IP2{}, I2{}, fb1, wf1, fb0, wf0, i, j_c, X{}, i);
+    step(IP2{}, IPN{}, I3{}, fb0, wf0, fb1, wf1, i, j_c, X{}, i);
+    load_w(J, i + G);
+    if constexpr (SJ == 1) load_s(J, i + G);
+    else if constexpr (J % 2 == 1) load_s(J / 2, i - 1 + G);
     lds_sync();  // every wave's pieces of slice i + 1 are written and its reads of slice i done
-    scales(NSet::value, NJ::value);
+    scales(NJ::value, i + 1);
     __builtin_amdgcn_sched_barrier(0);
-    step(I0{}, I0{}, I0{}, fb1, wf1, fb0, wf0, i + 1, NSet{}, NJ{}, i);
+    step(I0{}, I0{}, I0{}, fb1, wf1, fb0, wf0, i + 1, NJ{}, X{}, i);
   };
 #pragma unroll
-  for (int p = 0; p < NB; ++p) load_x_checked(0, p);
-  load_w_checked(0, 0);
+  for (int p = 0; p < NB; ++p) load_x_first(p);
 #pragma unroll
-  for (int p = 0; p < NB; ++p) {
-    write_x(0, p);
-    load_x_checked(1, p);
-  }
-  load_w_checked(1, WS);
+  for (int l = 0; l < G; ++l) load_w_first(l);
+#pragma unroll
+  for (int p = 0; p < NB; ++p) write_x(0, 0, p);
+#pragma unroll
+  for (int x = 1; x <= XD; ++x)
+#pragma unroll
+    for (int p = 0; p < NB; ++p) load_x(x % XD, x, p);
   __syncthreads();
   scales(0, 0);
 #pragma unroll
   for (int n = 0; n < NB; ++n) fb0[n] = frag(0, 0, n);
 #pragma unroll
-  for (int m = 0; m < MW; ++m) wf0[m] = __builtin_bit_cast(u32x4, mx_frag(w[0][0][m][0], sf[m]));
-  for (int i = 0; i < ns; i += 2) {
-    slice(I0{}, I0{}, i);
-    if constexpr (WS == 1) {
-      slice(I1{}, I0{}, i + 1);
-    } else {
-      slice(I0{}, I1{}, i + 1);
-#pragma unroll
-      for (int m = 0; m < MW; ++m) {  // the next pair's weights, which have arrived, make room for those behind them
-#pragma unroll
-        for (int j = 0; j < WS; ++j) w[0][j][m] = w[1][j][m];
-        sw[0][m] = sw[1][m];
-      }
-      load_w(1, i + 4);
-    }
+  for (int m = 0; m < MW; ++m) wf0[m] = __builtin_bit_cast(u32x4, mx_frag(w[0][m][0], sf[m]));
+  for (int i = 0; i < ns; i += G) {
+    [&]<int... J>(std::integer_sequence<int, J...>) {
+      (slice(std::integral_constant<int, J>{}, i + J), ...);
+    }(std::make_integer_sequence<int, G>{});
   }
   __syncthreads();
+
+  if constexpr (!GU) {
+    if (part_out != nullptr) {
+      f32x4* const o = reinterpret_cast<f32x4*>(part_out) + wv * (MW * NB * 256) + lane;
+#pragma unroll
+      for (int m = 0; m < MW; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            o[((m * NB + n) * 4 + q) * 64] =
+                f32x4{acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]};
+      return;
+    }
+  }
 
   // acc[m][n][j]: weight row 32 m + (j & 3) + 8 (j >> 2) + 4 h of the wave's, token row 32 n + i32.  The tile goes through
   // LDS so that its rows leave as whole segments.
@@ -532,27 +599,91 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
   });
 }
 
-template <int BM, int MW, int WS, bool GU>
+// The split tiles' sums: blockIdx = (XCD, split tile), blockIdx.y an eighth of its 32 x 32 blocks.
+template <int BM, int MW, int G>
+__global__ __launch_bounds__(256) void k_mx_reduce(MxArgs g) {
+  constexpr int NB = BM / 32, BN = 128 * MW, RES = mx_resident(BM), U = BM * BN / 4, BLOCKS = BM * BN / 1024;
+  constexpr int BP = 36;  // pitch of a 32 x 32 block (bf16): 8-byte writes, rows 18 banks apart
+  __shared__ __attribute__((aligned(16))) uint16_t blk[2][32 * BP];
+  const int tid = threadIdx.x, lane = tid & 63, q = tid >> 6;
+  const int xcd = (int)blockIdx.x / RES, t = (int)blockIdx.x % RES;
+  const int total = g.tile_off[g.E] * g.Tn, chunk = (total + 7) >> 3;
+  const MxSplit sp = mx_split(min(chunk, total - xcd * chunk), (g.K + 63) / 64, g.npart, RES, G);
+  if (sp.parts == 1 || t >= sp.rest) return;
+  const int L = xcd * chunk + sp.full + t, e = mx_expert(g, L, lane);
+  const int cnt = g.tile_off[e + 1] - g.tile_off[e], local = L - g.tile_off[e] * g.Tn;
+  const int nt = local / cnt, mt = local - nt * cnt;
+  const int mbase = g.offsets[e] + mt * BM, mlen = min(BM, g.offsets[e + 1] - mbase);
+  const f32x4* const src = reinterpret_cast<const f32x4*>(g.part + (int64_t)(xcd * g.npart + t * sp.parts) * (BM * BN));
+  int buf = 0;
+  for (int b = (int)blockIdx.y * (BLOCKS / 8); b < (int)(blockIdx.y + 1) * (BLOCKS / 8); ++b) {
+    const int n = b % NB, m = b / NB;  // m: 32 weight rows of all waves'
+    const int rb = n * 32, cb = nt * BN + m * 32;
+    if (rb >= mlen || cb >= g.N) continue;  // the same for the whole block
+    f32x4 s = src[b * 256 + q * 64 + lane];
+    for (int p = 1; p < sp.parts; ++p) s += src[(int64_t)p * U + b * 256 + q * 64 + lane];
+    *reinterpret_cast<uint2*>(&blk[buf][(lane & 31) * BP + q * 8 + (lane >> 5) * 4]) =
+        uint2{pack2bf(s[0], s[1]), pack2bf(s[2], s[3])};
+    __syncthreads();  // between a buffer's readers and its next writers lies the other buffer's barrier
+    const int r = tid >> 3, c = (tid & 7) * 4;
+    if (rb + r < mlen)  // N % 32 == 0
+      *reinterpret_cast<uint2*>(g.C + (int64_t)(mbase + rb + r) * g.N + cb + c) =
+          *reinterpret_cast<const uint2*>(&blk[buf][r * BP + c]);
+    buf ^= 1;
+  }
+}
+
+template <int BM, int MW, int G, int XD, bool GU>
 int launch_tile_as(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
   a.E = (int)E;
   a.Tn = cdiv(a.N, GU ? 64 * MW : 128 * MW);
   const int64_t blocks = ((R + BM - 1) / BM + E) * a.Tn;
   if (blocks > INT32_MAX - 8) return fail_arg("%s: too many tiles", name);
-  MOE_LAUNCH(name, (k_mx_tile<BM, MW, WS, GU>), dim3((unsigned)((blocks + 7) / 8 * 8)), dim3(256), 0, s, a);
+  const int64_t more = a.part ? 8 * a.npart : 0;
+  MOE_LAUNCH(name, (k_mx_tile<BM, MW, G, XD, GU>), dim3((unsigned)((blocks + 7) / 8 * 8 + more)), dim3(256), 0, s, a);
+  if constexpr (!GU) {
+    if (a.part != nullptr)
+      MOE_LAUNCH("k_mx_reduce", (k_mx_reduce<BM, MW, G>), dim3(8 * mx_resident(BM), 8), dim3(256), 0, s, a);
+  }
   return check_launch(name);
 }
 template <int BM, bool GU>
 int launch_tile(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
-  if constexpr (BM == 256) return launch_tile_as<256, 2, 1, GU>(name, s, a, E, R);
-  else if constexpr (BM == 128) return launch_tile_as<128, 2, 2, GU>(name, s, a, E, R);
-  else return launch_tile_as<64, 2, 2, GU>(name, s, a, E, R);
+  const char* f = getenv("MOE_MX_MW");
+  if (f && f[0] == '0') a.part = nullptr;
+  if constexpr (BM == 256) return launch_tile_as<256, 2, 2, 1, GU>(name, s, a, E, R);
+  else if constexpr (BM == 128) return launch_tile_as<128, 2, 4, 1, GU>(name, s, a, E, R);
+  else return launch_tile_as<64, 2, 4, 2, GU>(name, s, a, E, R);
 }
 
-// Rows of a tile (0: the few-row form).  The tiled loop loads two whole slices of a row at a time, also behind the last one
-// (clamped to it): it takes reductions of 128 and more.
+// Rows of a tile (0: the few-row form), by the rows an expert has on average (the host does not know more) and by the gate/up
+// product's tiles, which have to fill the chip: 512 blocks of 64 or 128 rows are resident at once, 256 of 256 rows.  The tiled
+// loop takes reductions of 128 and more, and with 256 rows only multiples of 128.  Both products, us, by rows an expert
+// (routed; few-row form | 64 | 128 | 256 rows):
+//   E 8,   H 4096, F 14336   16: 224 | 326 | 381 | 616   32: 375 | 336 | 393 | 620   64: 628 | 440 | 405 | 631   128: - | 597 | 536 | 648
+//   E 128, H 2048, F 768     16: 106 | 114 | 145 | 244   32: 170 | 122 | 152 | 247   64: 303 | 171 | 160 | 257   256: - | 476 | 386 | 450
+//   E 8,   H 1024, F 4096    16: 25 | 53 | 68 | 104      32: 40 | 53 | 70 | 105      64: 70 | 63 | 72 | 106      256: - | 95 | 98 | 133
+// and at 512 rows 128 | 256: 1585 | 1516, 710 | 696, 150 | 163.
 int mx_rows(int64_t R, int64_t H, int64_t F, int64_t E) {
   if (H < 128 || F < 128) return 0;
-  return R <= 24 * E ? 0 : R <= 64 * E ? 64 : R <= 160 * E ? 128 : 256;
+  const bool even = H % 128 == 0 && F % 128 == 0;
+  if (const char* f = getenv("MOE_MX_FORM")) return atoi(f) == 256 && !even ? 128 : atoi(f);
+  const int64_t tn = (F + 127) / 128;
+  if (R <= (E * tn < 512 ? 40 : 24) * E) return 0;
+  if (even && R > 400 * E && R / 256 * tn >= 1024) return 256;
+  return R > 48 * E && std::max(R / 128, E) * tn >= 512 ? 128 : 64;
+}
+
+// Room for the partial tiles of an XCD (tiles of bm rows, 256 columns): two rounds of parts, 8 a tile.  None for products of
+// 16 rounds of tiles and more, of which the last is too little to pay for the reduction.
+int mx_parts(int bm, int64_t R, int64_t E, int64_t N) {
+  if (bm == 0) return 0;
+  const int64_t tiles = ((R + bm - 1) / bm + E) * ((N + 255) / 256);
+  if (R / bm * ((N + 255) / 256) >= 16 * 8 * mx_resident(bm)) return 0;
+  return (int)std::min<int64_t>(2 * mx_resident(bm), 8 * ((tiles + 7) / 8));
+}
+size_t mx_part_bytes(int bm, int64_t R, int64_t E, int64_t N) {
+  return (size_t)8 * mx_parts(bm, R, E, N) * bm * 256 * sizeof(float);
 }
 
 bool al16x(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -572,9 +703,8 @@ int mx_shape(const char* what, int64_t R, int64_t H, int64_t F, int64_t E) {
 using namespace moe;
 
 extern "C" size_t moe_swiglu_fwd_mxfp4_workspace(int64_t R, int64_t H, int64_t F, int64_t E) {
-  (void)H;
-  if (R <= 0 || F <= 0 || E <= 0) return 0;
-  return moe_swiglu_workspace(E) + al256x((size_t)R * F * 2);
+  if (R <= 0 || H <= 0 || F <= 0 || E <= 0) return 0;
+  return moe_swiglu_workspace(E) + al256x((size_t)R * F * 2) + mx_part_bytes(mx_rows(R, H, F, E), R, E, H);
 }
 
 extern "C" int moe_swiglu_fwd_mxfp4(const void* xp, const void* wg_q, const void* sg, const void* wu_q, const void* su,
@@ -619,6 +749,9 @@ extern "C" int moe_swiglu_fwd_mxfp4(const void* xp, const void* wg_q, const void
   b.C = static_cast<uint16_t*>(y);
   b.K = (int)F;
   b.N = (int)H;
+  b.npart = mx_parts(bm, R, E, H);
+  if (b.npart > 0)
+    b.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + moe_swiglu_workspace(E) + al256x((size_t)R * F * 2));
   return bm == 256   ? launch_tile<256, false>("k_mx_tile_fwd2", s, b, E, R)
          : bm == 128 ? launch_tile<128, false>("k_mx_tile_fwd2", s, b, E, R)
          : bm == 64  ? launch_tile<64, false>("k_mx_tile_fwd2", s, b, E, R)
