@@ -15,7 +15,6 @@
 // agree: lane 16 q + r holds block 4 c + q of row r, and takes elements 128 c + 32 q + 8 s + [0, 8) of token row r for the
 // s-th of the four.  The waves' partial sums meet in LDS in wave order.
 #include <algorithm>
-#include <cstdlib>
 #include <utility>
 
 #include "common.h"
@@ -649,8 +648,6 @@ int launch_tile_as(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t
 }
 template <int BM, bool GU>
 int launch_tile(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
-  const char* f = getenv("MOE_MX_MW");
-  if (f && f[0] == '0') a.part = nullptr;
   if constexpr (BM == 256) return launch_tile_as<256, 2, 2, 1, GU>(name, s, a, E, R);
   else if constexpr (BM == 128) return launch_tile_as<128, 2, 4, 1, GU>(name, s, a, E, R);
   else return launch_tile_as<64, 2, 4, 2, GU>(name, s, a, E, R);
@@ -667,7 +664,6 @@ int launch_tile(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R)
 int mx_rows(int64_t R, int64_t H, int64_t F, int64_t E) {
   if (H < 128 || F < 128) return 0;
   const bool even = H % 128 == 0 && F % 128 == 0;
-  if (const char* f = getenv("MOE_MX_FORM")) return atoi(f) == 256 && !even ? 128 : atoi(f);
   const int64_t tn = (F + 127) / 128;
   if (R <= (E * tn < 512 ? 40 : 24) * E) return 0;
   if (even && R > 400 * E && R / 256 * tn >= 1024) return 256;
