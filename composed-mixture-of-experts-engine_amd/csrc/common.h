@@ -200,8 +200,11 @@ int swiglu_dact(const void* dy, const void* hgu, const void* w_down, const int* 
 int swiglu_dxp(const void* dh, const void* w_gate, const void* w_up, const int* offsets, int64_t R, int64_t H, int64_t F,
                int64_t E, void* dxp, void* workspace, size_t ws_bytes, hipStream_t s);
 
-// ---- n MXFP4 elements to bf16 (csrc/mxfp4.hip) ----
-int dequant_mxfp4_bf16(const void* q, const void* scale, int64_t n, void* dst, hipStream_t s);
+// The same on MXFP4 weights, dequantized inside the products.
+int swiglu_dact_mxfp4(const void* dy, const void* hgu, const void* wd_q, const void* sd, const int* offsets, int64_t R,
+                      int64_t H, int64_t F, int64_t E, void* dh, const void* workspace, hipStream_t s);
+int swiglu_dxp_mxfp4(const void* dh, const void* wg_q, const void* sg, const void* wu_q, const void* su, const int* offsets,
+                     int64_t R, int64_t H, int64_t F, int64_t E, void* dxp, void* workspace, size_t ws_bytes, hipStream_t s);
 
 // ---- optional per-kernel timing (host side; off unless moe_prof_enable(1)) ----
 // Brackets one launch with two hipEvents recorded on the launch stream.

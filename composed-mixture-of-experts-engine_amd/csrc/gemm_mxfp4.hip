@@ -758,8 +758,7 @@ extern "C" int moe_swiglu_fwd_mxfp4(const void* xp, const void* wg_q, const void
 
 extern "C" size_t moe_swiglu_bwd_mxfp4_workspace(int64_t R, int64_t H, int64_t F, int64_t E) {
   if (R <= 0 || H <= 0 || F <= 0 || E <= 0) return 0;
-  return moe_swiglu_workspace(E) + moe_swiglu_split_workspace(R, H, F, E) + al256x((size_t)R * F * 4) +
-         2 * al256x((size_t)E * F * H * 2);
+  return moe_swiglu_workspace(E) + moe_swiglu_split_workspace(R, H, F, E) + al256x((size_t)R * F * 4);
 }
 
 extern "C" int moe_swiglu_bwd_mxfp4(const void* dy, const void* hgu, const void* wg_q, const void* sg, const void* wu_q,
@@ -775,15 +774,8 @@ extern "C" int moe_swiglu_bwd_mxfp4(const void* dy, const void* hgu, const void*
     return set_error("moe_swiglu_bwd_mxfp4: workspace"), MOE_EWORKSPACE;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t gemm_ws = moe_swiglu_workspace(E) + moe_swiglu_split_workspace(R, H, F, E);
-  char* ws = static_cast<char*>(workspace);
-  void* dh = ws + gemm_ws;
-  char* w0 = ws + gemm_ws + al256x((size_t)R * F * 4);
-  char* w1 = w0 + al256x((size_t)E * F * H * 2);
-  const int64_t n = E * F * H;
-  if (int rc = dequant_mxfp4_bf16(wd_q, sd, n, w0, s)) return rc;
+  void* dh = static_cast<char*>(workspace) + gemm_ws;
   if (int rc = swiglu_tiles(offsets, E, kGemmRows, workspace, s)) return rc;
-  if (int rc = swiglu_dact(dy, hgu, w0, offsets, R, H, F, E, dh, workspace, s)) return rc;
-  if (int rc = dequant_mxfp4_bf16(wg_q, sg, n, w0, s)) return rc;
-  if (int rc = dequant_mxfp4_bf16(wu_q, su, n, w1, s)) return rc;
-  return swiglu_dxp(dh, w0, w1, offsets, R, H, F, E, dxp, workspace, gemm_ws, s);
+  if (int rc = swiglu_dact_mxfp4(dy, hgu, wd_q, sd, offsets, R, H, F, E, dh, workspace, s)) return rc;
+  return swiglu_dxp_mxfp4(dh, wg_q, sg, wu_q, su, offsets, R, H, F, E, dxp, workspace, gemm_ws, s);
 }

@@ -128,11 +128,6 @@ unsigned mx_blocks(int64_t n) { return (unsigned)std::min<int64_t>(2048, (n + 4 
 
 }  // namespace
 
-int dequant_mxfp4_bf16(const void* q, const void* scale, int64_t n, void* dst, hipStream_t s) {
-  MOE_LAUNCH("k_dequant_mxfp4", k_dequant_mxfp4<uint16_t>, dim3(mx_blocks(n)), dim3(256), 0, s,
-             static_cast<const uint32_t*>(q), static_cast<const uint8_t*>(scale), n, static_cast<uint16_t*>(dst));
-  return check_launch("k_dequant_mxfp4");
-}
 }  // namespace moe
 
 using namespace moe;
@@ -168,8 +163,11 @@ extern "C" int moe_dequant_mxfp4(const void* q, const void* scale, int64_t rows,
   if (!q || !scale || !dst || !al16m(q) || !al16m(dst)) return fail_arg("moe_dequant_mxfp4: null or misaligned pointer");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t n = rows * cols;
-  if (dst_dtype == MOE_BF16) return dequant_mxfp4_bf16(q, scale, n, dst, s);
-  MOE_LAUNCH("k_dequant_mxfp4", k_dequant_mxfp4<float>, dim3(mx_blocks(n)), dim3(256), 0, s,
-             static_cast<const uint32_t*>(q), static_cast<const uint8_t*>(scale), n, static_cast<float*>(dst));
+  if (dst_dtype == MOE_BF16)
+    MOE_LAUNCH("k_dequant_mxfp4", k_dequant_mxfp4<uint16_t>, dim3(mx_blocks(n)), dim3(256), 0, s,
+               static_cast<const uint32_t*>(q), static_cast<const uint8_t*>(scale), n, static_cast<uint16_t*>(dst));
+  else
+    MOE_LAUNCH("k_dequant_mxfp4", k_dequant_mxfp4<float>, dim3(mx_blocks(n)), dim3(256), 0, s,
+               static_cast<const uint32_t*>(q), static_cast<const uint8_t*>(scale), n, static_cast<float*>(dst));
   return check_launch("moe_dequant_mxfp4");
 }
