@@ -998,13 +998,13 @@ extern "C" size_t moe_rmsnorm_router_bwd_workspace(int64_t N, int64_t H, int64_t
   return plan_norm_route_bwd(N, H, E, K, x_dtype, wg_dtype).total;
 }
 
-extern "C" int moe_rmsnorm_router_bwd(const void* x, int x_dtype, const void* gamma, int gamma_dtype,
-                                      const float* rstd, const void* xn, const void* wg, int wg_dtype,
-                                      const float* logits, const int64_t* idx, const void* grad_w, int gw_dtype,
-                                      const int64_t* cnt, const float* grad_aux, const float* grad_z, float aux_coef,
-                                      float z_coef, const void* dxn, int64_t N, int64_t H, int64_t E, int64_t K,
-                                      void* dx_out, void* dgamma_out, void* dwg_out, void* workspace, size_t ws_bytes,
-                                      void* stream) {
+extern "C" int moe_rmsnorm_router_bwd_logits(const void* x, int x_dtype, const void* gamma, int gamma_dtype,
+                                             const float* rstd, const void* xn, const void* wg, int wg_dtype,
+                                             const float* logits, const int64_t* idx, const void* grad_w, int gw_dtype,
+                                             const int64_t* cnt, const float* grad_aux, const float* grad_z,
+                                             float aux_coef, float z_coef, const float* grad_logits, const void* dxn,
+                                             int64_t N, int64_t H, int64_t E, int64_t K, void* dx_out, void* dgamma_out,
+                                             void* dwg_out, void* workspace, size_t ws_bytes, void* stream) {
   if (int rc = norm_check("moe_rmsnorm_router_bwd", N, H, x_dtype, gamma_dtype)) return rc;
   if (E < 1 || E > kMaxE || K < 1 || K > E)
     return fail_arg("moe_rmsnorm_router_bwd: bad shape E=%lld K=%lld", (long long)E, (long long)K);
@@ -1030,16 +1030,16 @@ extern "C" int moe_rmsnorm_router_bwd(const void* x, int x_dtype, const void* ga
   if (!p.fused) {
     // the router backward over xn (its dxn into the workspace), then the norm backward of dxn + that
     void* dxr = ws + p.off_g;
-    if (int rc = moe_router_bwd(xn, x_dtype, wg, wg_dtype, logits, idx, grad_w, gw_dtype, cnt, grad_aux, grad_z,
-                                aux_coef, z_coef, N, H, E, K, dxr, dwg_out, ws + p.off_rw, p.off_dg - p.off_rw,
-                                stream))
+    if (int rc = moe_router_bwd_logits(xn, x_dtype, wg, wg_dtype, logits, idx, grad_w, gw_dtype, cnt, grad_aux, grad_z,
+                                       aux_coef, z_coef, grad_logits, N, H, E, K, nullptr, dxr, dwg_out, ws + p.off_rw,
+                                       p.off_dg - p.off_rw, stream))
       return rc;
     return moe_rmsnorm_bwd(x, x_dtype, gamma, gamma_dtype, rstd, dxn ? dxn : dxr, dxn ? dxr : nullptr, N, H, dx_out,
                            dgamma_out, part, p.total - p.off_dg, stream);
   }
   uint16_t* G = reinterpret_cast<uint16_t*>(ws + p.off_g);
   if (int rc = router_dw_g(static_cast<const uint16_t*>(xn), static_cast<const uint16_t*>(wg), logits, idx, grad_w,
-                           gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, N, H, E, K, dwg_out, G, p.ep,
+                           gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, grad_logits, N, H, E, K, dwg_out, G, p.ep,
                            ws + p.off_rw, s))
     return rc;
   NormBwdArgs a{};
@@ -1063,4 +1063,16 @@ extern "C" int moe_rmsnorm_router_bwd(const void* x, int x_dtype, const void* ga
                                    : launch_norm_bwd<uint16_t, uint16_t, NCHv, 16>(p.nblk, s, a)));
   if (rc) return rc;
   return launch_dgamma(s, part, p.nblk, H, dgamma_out, gamma_dtype);
+}
+
+extern "C" int moe_rmsnorm_router_bwd(const void* x, int x_dtype, const void* gamma, int gamma_dtype,
+                                      const float* rstd, const void* xn, const void* wg, int wg_dtype,
+                                      const float* logits, const int64_t* idx, const void* grad_w, int gw_dtype,
+                                      const int64_t* cnt, const float* grad_aux, const float* grad_z, float aux_coef,
+                                      float z_coef, const void* dxn, int64_t N, int64_t H, int64_t E, int64_t K,
+                                      void* dx_out, void* dgamma_out, void* dwg_out, void* workspace, size_t ws_bytes,
+                                      void* stream) {
+  return moe_rmsnorm_router_bwd_logits(x, x_dtype, gamma, gamma_dtype, rstd, xn, wg, wg_dtype, logits, idx, grad_w,
+                                       gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, nullptr, dxn, N, H, E, K, dx_out,
+                                       dgamma_out, dwg_out, workspace, ws_bytes, stream);
 }

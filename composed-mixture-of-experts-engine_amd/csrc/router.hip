@@ -1573,8 +1573,9 @@ __global__ __launch_bounds__(256) void k_router_glogits(const float* __restrict_
                                                         int gw_dt, const int64_t* __restrict__ cnt,
                                                         const float* __restrict__ grad_aux,
                                                         const float* __restrict__ grad_z, float aux_coef,
-                                                        float z_coef, int N, int E, int K, int round_bf16,
-                                                        float* __restrict__ G, uint16_t* __restrict__ gb, int ekp) {
+                                                        float z_coef, const float* __restrict__ grad_l, int N, int E,
+                                                        int K, int round_bf16, float* __restrict__ G,
+                                                        uint16_t* __restrict__ gb, int ekp) {
   constexpr int TPW = 64 / LPT;  // tokens per wave
   const int lane = threadIdx.x & 63;
   const int sub = lane % LPT;
@@ -1594,6 +1595,7 @@ __global__ __launch_bounds__(256) void k_router_glogits(const float* __restrict_
         const int e = sub + LPT * j;
         if (e < E) {
           float v = gl[j];
+          if (grad_l != nullptr) v += grad_l[(int64_t)t * E + e];
           if (round_bf16) v = bf2f(f2bf(v));
           if (G) G[(int64_t)t * E + e] = v;
           if (gb) gb[(int64_t)t * ekp + e] = f2bf(v);
@@ -1794,7 +1796,7 @@ __global__ __launch_bounds__(64 * WPB) __attribute__((amdgpu_waves_per_eu(NTE ==
                                                             int nht, uint16_t* __restrict__ dx,
                                                             const uint16_t* __restrict__ dx_add,
                                                             float* __restrict__ ws_dw, uint16_t* __restrict__ g_out,
-                                                            int g_pitch) {
+                                                            int g_pitch, const float* __restrict__ grad_l) {
   constexpr int GS = NTE * 16;       // expert slots of a token-major G row
   constexpr int GP = GS + 8;         // its pitch: 16 rows of one 16-byte read hit distinct bank groups
   constexpr int GTP = kSTC + 8;      // expert-major G row pitch
@@ -1893,6 +1895,11 @@ __global__ __launch_bounds__(64 * WPB) __attribute__((amdgpu_waves_per_eu(NTE ==
         glogit_token_regs<EL, KR>(lgv, fv, ikv, gkv, gw != nullptr, cf, K, gl);
       } else if constexpr (KR != 2) {
         glogit_token<1, EL>(logits, idx, gw, gw_dt, cnt, cf, t, E, K, 0, gl);
+      }
+      if (grad_l != nullptr) {
+#pragma unroll
+        for (int e = 0; e < EL; ++e)
+          if (e < E) gl[e] += grad_l[(int64_t)t * E + e];
       }
     } else {
 #pragma unroll
@@ -2646,12 +2653,12 @@ template <int NTE>
 void launch_dxdw_stream(hipStream_t s, const uint16_t* x, const uint16_t* wg, const float* logits, const int64_t* idx,
                         const void* gw, int gw_dt, const int64_t* cnt, const float* grad_aux, const float* grad_z,
                         float aux_coef, float z_coef, int N, int H, int E, int K, int tc_len, int nchunk, uint16_t* dx,
-                        float* ws, uint16_t* g_out = nullptr, int g_pitch = 0, const uint16_t* dx_add = nullptr) {
+                        float* ws, uint16_t* g_out, int g_pitch, const uint16_t* dx_add, const float* grad_l) {
   const char* name = dx ? "k_router_dxdw_bf16" : "k_router_dw_bf16";
 #define MOE_DXDW_STREAM(EL_, KR_, WPB_)                                                                               \
   MOE_LAUNCH(name, (k_router_dxdw_stream<NTE, EL_, KR_, WPB_>), dim3((unsigned)(nchunk * cdiv(H, 64 * WPB_))),         \
              dim3(64 * WPB_), 0, s, x, wg, logits, idx, gw, gw_dt, cnt, grad_aux, grad_z, aux_coef, z_coef, N, H, E, K,  \
-             tc_len, cdiv(H, 64 * WPB_), dx, dx_add, ws, g_out, g_pitch)
+             tc_len, cdiv(H, 64 * WPB_), dx, dx_add, ws, g_out, g_pitch, grad_l)
   // G over 8 expert slots when E <= 8 (fewer registers while the first x tiles are in flight); the top-k
   // slots preloaded: 2 when K <= 2 (shorter code: the prologue runs on a cold instruction cache), else 4;
   // 16-wave blocks (1024 columns) when H allows
@@ -2689,12 +2696,12 @@ size_t router_dw_g_workspace(int64_t N, int64_t H, int64_t E) {
 
 int router_dw_g(const uint16_t* x, const uint16_t* wg, const float* logits, const int64_t* idx, const void* grad_w,
                 int gw_dtype, const int64_t* cnt, const float* grad_aux, const float* grad_z, float aux_coef,
-                float z_coef, int64_t N, int64_t H, int64_t E, int64_t K, void* dwg_out, uint16_t* g_out, int g_pitch,
-                void* ws, hipStream_t s) {
+                float z_coef, const float* grad_l, int64_t N, int64_t H, int64_t E, int64_t K, void* dwg_out, uint16_t* g_out,
+                int g_pitch, void* ws, hipStream_t s) {
   const BwdPlan p = plan_bwd(N, H, E, MOE_BF16, MOE_BF16);
   float* wsdw = static_cast<float*>(ws);
   launch_dxdw_stream<1>(s, x, wg, logits, idx, grad_w, gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, (int)N,
-                        (int)H, (int)E, (int)K, p.tc_len, p.nchunk, nullptr, wsdw, g_out, g_pitch);
+                        (int)H, (int)E, (int)K, p.tc_len, p.nchunk, nullptr, wsdw, g_out, g_pitch, nullptr, grad_l);
   if (int rc = check_launch("k_router_dw_bf16")) return rc;
   launch_reduce(s, wsdw, p.nchunk, H * E, dwg_out, MOE_BF16);
   return check_launch("router_dw_g");
@@ -2886,11 +2893,12 @@ extern "C" size_t moe_router_bwd_workspace(int64_t N, int64_t H, int64_t E, int6
   return plan_bwd(N, H, E, x_dtype, wg_dtype).total;
 }
 
-extern "C" int moe_router_bwd_acc(const void* x, int x_dtype, const void* wg, int wg_dtype, const float* logits,
-                                  const int64_t* idx, const void* grad_w, int gw_dtype, const int64_t* cnt,
-                                  const float* grad_aux, const float* grad_z, float aux_coef, float z_coef, int64_t N,
-                                  int64_t H, int64_t E, int64_t K, const void* dx_add, void* dx_out, void* dwg_out,
-                                  void* workspace, size_t ws_bytes, void* stream) {
+extern "C" int moe_router_bwd_logits(const void* x, int x_dtype, const void* wg, int wg_dtype, const float* logits,
+                                     const int64_t* idx, const void* grad_w, int gw_dtype, const int64_t* cnt,
+                                     const float* grad_aux, const float* grad_z, float aux_coef, float z_coef,
+                                     const float* grad_logits, int64_t N, int64_t H, int64_t E, int64_t K,
+                                     const void* dx_add, void* dx_out, void* dwg_out, void* workspace, size_t ws_bytes,
+                                     void* stream) {
   if (N < 0 || H <= 0 || E < 1 || E > kMaxE || K < 1 || K > E)
     return fail_arg("moe_router_bwd: bad shape N=%lld H=%lld E=%lld K=%lld", (long long)N, (long long)H,
                     (long long)E, (long long)K);
@@ -2933,7 +2941,7 @@ extern "C" int moe_router_bwd_acc(const void* x, int x_dtype, const void* wg, in
     uint16_t* dxb = static_cast<uint16_t*>(dx_out);
 #define MOE_DXDWS(NTEv)                                                                                          \
   launch_dxdw_stream<NTEv>(s, xb, wb, logits, idx, grad_w, gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef,    \
-                           (int)N, (int)H, (int)E, (int)K, p.tc_len, p.nchunk, dxb, wsdw, nullptr, 0, addb)
+                           (int)N, (int)H, (int)E, (int)K, p.tc_len, p.nchunk, dxb, wsdw, nullptr, 0, addb, grad_logits)
     if (p.NTE == 1) MOE_DXDWS(1);
     else MOE_DXDWS(2);
 #undef MOE_DXDWS
@@ -2948,7 +2956,7 @@ extern "C" int moe_router_bwd_acc(const void* x, int x_dtype, const void* wg, in
 #define MOE_GLOGW(EPL)                                                                                         \
   MOE_LAUNCH("k_router_glogits", (k_router_glogits<16, EPL>),                                                  \
              dim3((unsigned)std::min<int64_t>(4096, (N * 16 + 255) / 256)), dim3(256), 0, s, logits, idx,      \
-             grad_w, gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, (int)N, (int)E, (int)K, 1,            \
+             grad_w, gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, grad_logits, (int)N, (int)E, (int)K, 1, \
              static_cast<float*>(nullptr), gb, ekp)
     if (E <= 64) MOE_GLOGW(4);
     else MOE_GLOGW(8);
@@ -2976,7 +2984,7 @@ extern "C" int moe_router_bwd_acc(const void* x, int x_dtype, const void* wg, in
 #define MOE_GLOG(LPT, EPL)                                                                                     \
   MOE_LAUNCH("k_router_glogits", (k_router_glogits<LPT, EPL>),                                                 \
              dim3((unsigned)std::min<int64_t>(4096, (N * LPT + 255) / 256)), dim3(256), 0, s, logits, idx,     \
-             grad_w, gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, (int)N, (int)E, (int)K, rb, G, gb, ekp)
+             grad_w, gw_dtype, cnt, grad_aux, grad_z, aux_coef, z_coef, grad_logits, (int)N, (int)E, (int)K, rb, G, gb, ekp)
     if (E <= 8) MOE_GLOG(8, 1);
     else if (E <= 16) MOE_GLOG(16, 1);
     else if (E <= 32) MOE_GLOG(32, 1);
@@ -3040,6 +3048,15 @@ extern "C" int moe_router_bwd_acc(const void* x, int x_dtype, const void* wg, in
   launch_reduce(s,
                      wsdw, nchunk, len, dwg_out, wg_dtype);
   return check_launch("moe_router_bwd");
+}
+
+extern "C" int moe_router_bwd_acc(const void* x, int x_dtype, const void* wg, int wg_dtype, const float* logits,
+                                  const int64_t* idx, const void* grad_w, int gw_dtype, const int64_t* cnt,
+                                  const float* grad_aux, const float* grad_z, float aux_coef, float z_coef, int64_t N,
+                                  int64_t H, int64_t E, int64_t K, const void* dx_add, void* dx_out, void* dwg_out,
+                                  void* workspace, size_t ws_bytes, void* stream) {
+  return moe_router_bwd_logits(x, x_dtype, wg, wg_dtype, logits, idx, grad_w, gw_dtype, cnt, grad_aux, grad_z, aux_coef,
+                               z_coef, nullptr, N, H, E, K, dx_add, dx_out, dwg_out, workspace, ws_bytes, stream);
 }
 
 extern "C" int moe_router_bwd(const void* x, int x_dtype, const void* wg, int wg_dtype, const float* logits,

@@ -218,7 +218,7 @@ bool router_dw_g_applies(int64_t H, int64_t E);
 size_t router_dw_g_workspace(int64_t N, int64_t H, int64_t E);
 int router_dw_g(const uint16_t* x, const uint16_t* wg, const float* logits, const int64_t* idx, const void* grad_w,
                 int gw_dtype, const int64_t* cnt, const float* grad_aux, const float* grad_z, float aux_coef,
-                float z_coef, int64_t N, int64_t H, int64_t E, int64_t K, void* dwg_out, uint16_t* g_out, int g_pitch,
-                void* ws, hipStream_t s);
+                float z_coef, const float* grad_l, int64_t N, int64_t H, int64_t E, int64_t K, void* dwg_out, uint16_t* g_out,
+                int g_pitch, void* ws, hipStream_t s);
 
 }  // namespace moe

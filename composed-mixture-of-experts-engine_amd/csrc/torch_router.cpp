@@ -120,7 +120,8 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
   // (the expert path's gradient of x) then arrives here as an upstream gradient and is added inside the dx
   // kernel, instead of autograd summing the two contributions to x's gradient in a separate addition.
   static variable_list forward(AutogradContext* ctx, const Variable& x_in, const Variable& gw_in, int64_t k,
-                               double aux_coef, double z_coef, const std::optional<Variable>& bias_in, bool link_x) {
+                               double aux_coef, double z_coef, const std::optional<Variable>& bias_in, bool link_x,
+                               bool diff_logits) {
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x_in.device());
     const at::Tensor x = x_in.contiguous();
     const at::Tensor gw = gw_in.contiguous();
@@ -160,14 +161,16 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
     ctx->saved_data["aux_coef"] = aux_coef;
     ctx->saved_data["z_coef"] = z_coef;
     ctx->set_materialize_grads(false);
-    ctx->mark_non_differentiable({idx, logits, cnt, stats});
+    // diff_logits: a loss of the caller's formed on the logits sends its gradient back through them
+    if (diff_logits) ctx->mark_non_differentiable({idx, cnt, stats});
+    else ctx->mark_non_differentiable({idx, logits, cnt, stats});
     if (link_x) return {idx, w, aux, z, logits, cnt, stats, x_in};
     return {idx, w, aux, z, logits, cnt, stats};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
-    variable_list out(7);
+    variable_list out(8);
     if (!(need_x || need_w)) return out;
     const auto saved = ctx->get_saved_variables();
     const at::Tensor& x = saved[0];
@@ -182,6 +185,8 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
     // the linked x output's gradient (the expert path's gradient of x), if any
     at::Tensor dx_add;
     if (need_x && grads.size() > 7 && grads[7].defined()) dx_add = grads[7].to(x.scalar_type()).contiguous();
+    at::Tensor g_logits;  // undefined unless the forward left the logits differentiable
+    if (grads[4].defined()) g_logits = grads[4].to(at::kFloat).contiguous();
     const float aux_coef = g_aux.defined() ? (float)ctx->saved_data["aux_coef"].toDouble() : 0.f;
     const float z_coef = g_z.defined() ? (float)ctx->saved_data["z_coef"].toDouble() : 0.f;
     int gdt = MOE_F32;
@@ -204,12 +209,13 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
       const size_t nbytes = moe_router_bwd_workspace(N, H, E, K, xdt, wdt);
       const at::Tensor ws = at::empty({std::max<int64_t>((int64_t)nbytes, 1)}, x.options().dtype(at::kByte));
       const hipStream_t s = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).stream();
-      const int rc = moe_router_bwd_acc(x.data_ptr(), xdt, gw.data_ptr(), wdt, logits.data_ptr<float>(),
-                                        idx.data_ptr<int64_t>(), g_w.defined() ? g_w.data_ptr() : nullptr, gdt,
-                                        cnt.data_ptr<int64_t>(), g_aux.defined() ? g_aux.data_ptr<float>() : nullptr,
-                                        g_z.defined() ? g_z.data_ptr<float>() : nullptr, aux_coef, z_coef, N, H, E, K,
-                                        dx_add.defined() ? dx_add.data_ptr() : nullptr, dx.data_ptr(), dw.data_ptr(),
-                                        ws.data_ptr(), nbytes, s);
+      const int rc = moe_router_bwd_logits(x.data_ptr(), xdt, gw.data_ptr(), wdt, logits.data_ptr<float>(),
+                                           idx.data_ptr<int64_t>(), g_w.defined() ? g_w.data_ptr() : nullptr, gdt,
+                                           cnt.data_ptr<int64_t>(), g_aux.defined() ? g_aux.data_ptr<float>() : nullptr,
+                                           g_z.defined() ? g_z.data_ptr<float>() : nullptr, aux_coef, z_coef,
+                                           g_logits.defined() ? g_logits.data_ptr<float>() : nullptr, N, H, E, K,
+                                           dx_add.defined() ? dx_add.data_ptr() : nullptr, dx.data_ptr(), dw.data_ptr(),
+                                           ws.data_ptr(), nbytes, s);
       if (rc != 0) raise_rc(rc, "moe_router_bwd");
     }
     if (need_x) out[0] = dx;
@@ -219,8 +225,8 @@ struct RouterFn : public torch::autograd::Function<RouterFn> {
 };
 
 variable_list router_core(const at::Tensor& x, const at::Tensor& gate_w, int64_t k, double aux_coef,
-                          double z_coef, const std::optional<at::Tensor>& bias, bool link_x) {
-  return RouterFn::apply(x, gate_w, k, aux_coef, z_coef, bias, link_x);
+                          double z_coef, const std::optional<at::Tensor>& bias, bool link_x, bool diff_logits) {
+  return RouterFn::apply(x, gate_w, k, aux_coef, z_coef, bias, link_x, diff_logits);
 }
 
 // ---- the operations of moe_mi355/ops.py: outputs from ATen, one C ABI call, no autograd.  ops.py has checked device,
@@ -292,7 +298,7 @@ std::vector<at::Tensor> op_rmsnorm_router_backward(const at::Tensor& x_in, const
                                                    const at::Tensor& logits_in, const at::Tensor& idx_in,
                                                    const OptTensor& grad_w, const OptTensor& dxn, const OptTensor& cnt,
                                                    const OptTensor& grad_aux, const OptTensor& grad_z, double aux_coef,
-                                                   double z_coef) {
+                                                   double z_coef, const OptTensor& grad_logits) {
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(x_in.device());
   const at::Tensor x = x_in.contiguous(), weight = weight_in.contiguous(), xn = xn_in.contiguous();
   const at::Tensor gw = gw_in.contiguous(), logits = logits_in.contiguous(), idx = idx_in.contiguous();
@@ -301,12 +307,12 @@ std::vector<at::Tensor> op_rmsnorm_router_backward(const at::Tensor& x_in, const
   const int xdt = code_of(x), wdt = code_of(gw);
   const size_t nbytes = moe_rmsnorm_router_bwd_workspace(N, H, E, K, xdt, wdt);
   const at::Tensor ws = scratch(nbytes, x);
-  check_rc(moe_rmsnorm_router_bwd(
+  check_rc(moe_rmsnorm_router_bwd_logits(
                x.data_ptr(), xdt, weight.data_ptr(), code_of(weight), rstd.data_ptr<float>(), xn.data_ptr(), gw.data_ptr(),
                wdt, logits.data_ptr<float>(), idx.data_ptr<int64_t>(), ptr(grad_w),
                grad_w.has_value() && grad_w->defined() ? code_of(*grad_w) : MOE_F32, static_cast<const int64_t*>(ptr(cnt)),
                static_cast<const float*>(ptr(grad_aux)), static_cast<const float*>(ptr(grad_z)), (float)aux_coef,
-               (float)z_coef, ptr(dxn), N, H, E, K, dx.data_ptr(), dweight.data_ptr(), dgate.data_ptr(), ws.data_ptr(),
+               (float)z_coef, static_cast<const float*>(ptr(grad_logits)), ptr(dxn), N, H, E, K, dx.data_ptr(), dweight.data_ptr(), dgate.data_ptr(), ws.data_ptr(),
                nbytes, stream_of(x)),
            "moe_rmsnorm_router_bwd");
   return {dx, dweight, dgate};
@@ -564,7 +570,8 @@ PYBIND11_MODULE(_moe_torch, m) {
   const pybind11::call_guard<pybind11::gil_scoped_release> nogil;
   m.def("router_core", &router_core, "(x, gate_w, k, aux_coef, z_coef, bias) -> (idx, w, aux, z, logits, cnt, stats)",
         pybind11::arg("x"), pybind11::arg("gate_w"), pybind11::arg("k"), pybind11::arg("aux_coef"),
-        pybind11::arg("z_coef"), pybind11::arg("bias") = pybind11::none(), pybind11::arg("link_x") = false, nogil);
+        pybind11::arg("z_coef"), pybind11::arg("bias") = pybind11::none(), pybind11::arg("link_x") = false,
+        pybind11::arg("diff_logits") = false, nogil);
   m.def("router_forward", &op_router_forward, nogil);
   m.def("rmsnorm_router_forward", &op_rmsnorm_router_forward, nogil);
   m.def("rmsnorm_router_backward", &op_rmsnorm_router_backward, nogil);

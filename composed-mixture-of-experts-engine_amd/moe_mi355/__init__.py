@@ -7,6 +7,7 @@ the ``pkg`` package next to this one.
 """
 
 from . import _lib, ops  # noqa: F401
+from .balance import balance_loss  # noqa: F401
 from .router import RouterCore, route  # noqa: F401
 
 __version__ = "0.1.0"

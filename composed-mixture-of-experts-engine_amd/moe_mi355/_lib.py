@@ -51,6 +51,11 @@ _SIGNATURES = {
         [_P, _I32, _P, _I32, _P, _P, _P, _I32, _P, _P, _P, _F32, _F32, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ,
          _P],
     ),
+    "moe_router_bwd_logits": (
+        _I32,
+        [_P, _I32, _P, _I32, _P, _P, _P, _I32, _P, _P, _P, _F32, _F32, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ,
+         _P],
+    ),
     "moe_plan_workspace": (_SZ, [_I64, _I64, _I64]),
     "moe_plan": (_I32, [_P, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "moe_plan_noalloc": (_I32, [_P, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P]),
@@ -74,6 +79,11 @@ _SIGNATURES = {
     "moe_rmsnorm_router_bwd": (
         _I32,
         [_P, _I32, _P, _I32, _P, _P, _P, _I32, _P, _P, _P, _I32, _P, _P, _P, _F32, _F32, _P, _I64, _I64, _I64, _I64,
+         _P, _P, _P, _P, _SZ, _P],
+    ),
+    "moe_rmsnorm_router_bwd_logits": (
+        _I32,
+        [_P, _I32, _P, _I32, _P, _P, _P, _I32, _P, _P, _P, _I32, _P, _P, _P, _F32, _F32, _P, _P, _I64, _I64, _I64, _I64,
          _P, _P, _P, _P, _SZ, _P],
     ),
     "moe_quant_rows_fp8": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),

@@ -36,12 +36,12 @@ class RMSNormFn(torch.autograd.Function):
 
 
 class NormRouterCore(torch.autograd.Function):
-    """(x [N,H], norm_weight [H], eps, gate_w [H,E], k, aux_coef, z_coef, bias|None) ->
-    (xn, idx, w, aux, z, logits, cnt, stats)."""
+    """(x [N,H], norm_weight [H], eps, gate_w [H,E], k, aux_coef, z_coef, bias|None, diff_logits) ->
+    (xn, idx, w, aux, z, logits, cnt, stats).  ``diff_logits`` as :meth:`moe_mi355.router.RouterCore.apply`."""
 
     @staticmethod
     def forward(ctx, x, norm_weight, eps: float, gate_w, k: int, aux_coef: float, z_coef: float,
-                bias: Optional[torch.Tensor] = None):
+                bias: Optional[torch.Tensor] = None, diff_logits: bool = False):
         xn, rstd, idx, w, logits, _lse, cnt, stats, aux, z = ops.rmsnorm_router_forward(
             x, norm_weight, eps, gate_w, k, bias, aux_coef=aux_coef, z_coef=z_coef
         )
@@ -49,7 +49,7 @@ class NormRouterCore(torch.autograd.Function):
         ctx.aux_coef = float(aux_coef)
         ctx.z_coef = float(z_coef)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(idx, logits, cnt, stats)
+        ctx.mark_non_differentiable(*((idx, cnt, stats) if diff_logits else (idx, logits, cnt, stats)))
         return xn, idx, w, aux, z, logits, cnt, stats
 
     @staticmethod
@@ -57,13 +57,13 @@ class NormRouterCore(torch.autograd.Function):
         x, norm_weight, rstd, xn, gate_w, logits, idx, cnt = ctx.saved_tensors
         need_x, need_nw, need_gw = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3]
         dx = dnw = dgate = None
-        if g_w is not None or g_aux is not None or g_z is not None:
+        if g_w is not None or g_aux is not None or g_z is not None or g_logits is not None:
             # the router backward and the norm backward in one call: the router's gradient of xn is formed
             # inside the norm kernel
             aux_coef = ctx.aux_coef if g_aux is not None else 0.0
             z_coef = ctx.z_coef if g_z is not None else 0.0
             dx, dnw, dgate = ops.rmsnorm_router_backward(x, norm_weight, rstd, xn, gate_w, logits, idx, g_w, g_xn,
-                                                         cnt, g_aux, g_z, aux_coef, z_coef)
+                                                         cnt, g_aux, g_z, aux_coef, z_coef, grad_logits=g_logits)
         elif need_x or need_nw:
             if g_xn is None:
                 dx, dnw = torch.zeros_like(x), torch.zeros_like(norm_weight)
@@ -72,4 +72,4 @@ class NormRouterCore(torch.autograd.Function):
         if need_gw and dgate is None:
             dgate = torch.zeros_like(gate_w)
         return (dx if need_x else None), (dnw if need_nw else None), None, (dgate if need_gw else None), \
-            None, None, None, None
+            None, None, None, None, None

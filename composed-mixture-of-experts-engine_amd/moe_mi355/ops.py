@@ -71,11 +71,13 @@ def router_backward(
     aux_coef: float = 0.0,
     z_coef: float = 0.0,
     dx_add: Optional[torch.Tensor] = None,
+    grad_logits: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Fused router backward: returns ``(dx [N,H] x.dtype, dgate_w [H,E] gate_w.dtype)``; with ``dx_add``
     ([N, H], x's dtype) dx is the router's gradient of x plus dx_add, summed inside the dx kernel
-    (moe_router_bwd_acc)."""
-    dev = L.require_device(x, gate_w, logits, idx, grad_w, cnt, dx_add)
+    (moe_router_bwd_acc); ``grad_logits`` ([N, E] f32) is a gradient of the logits from a loss formed on them, added to
+    dL/dlogits (moe_router_bwd_logits)."""
+    dev = L.require_device(x, gate_w, logits, idx, grad_w, cnt, dx_add, grad_logits)
     x = x.contiguous()
     gate_w = gate_w.contiguous()
     logits = logits.contiguous()
@@ -101,7 +103,19 @@ def router_backward(
     dw = torch.empty((H, E), dtype=gate_w.dtype, device=dev)
     nbytes = lib.moe_router_bwd_workspace(N, H, E, K, xdt, wdt)
     ws = L.workspace(nbytes, dev)
-    if dx_add is None:
+    if grad_logits is not None:
+        if grad_logits.shape != (N, E) or grad_logits.dtype != torch.float32:
+            raise ValueError(f"router_backward: grad_logits must be [{N}, {E}] float32")
+        if dx_add is not None and (dx_add.shape != (N, H) or dx_add.dtype != x.dtype):
+            raise ValueError(f"router_backward: dx_add must be [{N}, {H}] {x.dtype}")
+        grad_logits, dx_add = grad_logits.contiguous(), _c(dx_add)
+        rc = lib.moe_router_bwd_logits(
+            x.data_ptr(), xdt, gate_w.data_ptr(), wdt, logits.data_ptr(), idx.data_ptr(),
+            L.ptr(grad_w), gdt, L.ptr(cnt), L.ptr(grad_aux), L.ptr(grad_z),
+            float(aux_coef), float(z_coef), grad_logits.data_ptr(), N, H, E, K,
+            L.ptr(dx_add), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes, L.stream_of(dev),
+        )
+    elif dx_add is None:
         rc = lib.moe_router_bwd(
             x.data_ptr(), xdt, gate_w.data_ptr(), wdt, logits.data_ptr(), idx.data_ptr(),
             L.ptr(grad_w), gdt, L.ptr(cnt), L.ptr(grad_aux), L.ptr(grad_z),
@@ -223,13 +237,18 @@ def rmsnorm_router_backward(
     grad_z: Optional[torch.Tensor] = None,
     aux_coef: float = 0.0,
     z_coef: float = 0.0,
+    grad_logits: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Backward of :func:`rmsnorm_router_forward` for the router's upstream gradients (as
     :func:`router_backward`) and a gradient ``dxn`` of ``xn`` from the expert path (or None).
 
     Returns ``(dx [N,H] x.dtype, dweight [H] weight.dtype, dgate_w [H,E] gate_w.dtype)``."""
-    L.require_device(x, weight, rstd, xn, gate_w, logits, idx, grad_w, dxn, cnt)
+    L.require_device(x, weight, rstd, xn, gate_w, logits, idx, grad_w, dxn, cnt, grad_logits)
     _, _ = x.shape
+    if grad_logits is not None:
+        if grad_logits.shape != logits.shape or grad_logits.dtype != torch.float32:
+            raise ValueError(f"rmsnorm_router_backward: grad_logits must be {list(logits.shape)} float32")
+        grad_logits = grad_logits.contiguous()
     for t in (x, weight, gate_w):
         L.dtype_code(t.dtype)
     if dxn is not None:
@@ -243,7 +262,7 @@ def rmsnorm_router_backward(
     if grad_z is not None:
         grad_z = grad_z.detach().to(torch.float32).reshape(1).contiguous()
     return tuple(L.native().rmsnorm_router_backward(x, weight, rstd, xn, gate_w, logits, idx, grad_w, dxn, cnt, grad_aux,
-                                                    grad_z, float(aux_coef), float(z_coef)))
+                                                    grad_z, float(aux_coef), float(z_coef), grad_logits))
 
 
 # ---------------------------------------------------------------------------

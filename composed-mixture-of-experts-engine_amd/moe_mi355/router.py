@@ -44,16 +44,18 @@ class RouterCore:
     ``apply`` runs a torch C++ autograd Function (csrc/torch_router.cpp): the forward launches moe_router_fwd
     and saves (x, gate_w, logits, idx, cnt); the backward, run by the autograd engine without a return to
     Python, launches moe_router_bwd with the upstream gradients of w, aux and z (an aux or z output that gets
-    no gradient contributes no term).  idx, logits, cnt and stats are not differentiable; no gradient flows
+    no gradient contributes no term).  idx, cnt and stats (and logits, without ``diff_logits``) are not differentiable; no gradient flows
     to k, the coefficients or the bias.  The checks below raise the errors the ctypes path raises."""
 
     @staticmethod
     def apply(x, gate_w, k: int, aux_coef: float, z_coef: float, bias: Optional[torch.Tensor] = None,
-              link_x: bool = False):
+              link_x: bool = False, diff_logits: bool = False):
         """``link_x``: also return x itself as an eighth output.  A caller that feeds that output (rather than
         x) to its other consumer of the tokens hands that consumer's gradient of x to this Function's backward,
         which adds it inside the dx kernel (moe_router_bwd_acc) instead of autograd summing the two
-        contributions to x's gradient in a separate addition."""
+        contributions to x's gradient in a separate addition.  ``diff_logits``: the logits output is differentiable,
+        for a loss formed on it (:func:`moe_mi355.balance.balance_loss`), whose gradient joins dL/dlogits inside the
+        backward kernel (moe_router_bwd_logits)."""
         L.require_device(x, gate_w, bias)
         N, H = x.shape
         H2, E = gate_w.shape
@@ -61,7 +63,8 @@ class RouterCore:
             raise ValueError(f"router_forward: hidden dims differ ({H} vs {H2})")
         L.dtype_code(x.dtype)
         L.dtype_code(gate_w.dtype)
-        return tuple(L.native().router_core(x, gate_w, int(k), float(aux_coef), float(z_coef), bias, bool(link_x)))
+        return tuple(L.native().router_core(x, gate_w, int(k), float(aux_coef), float(z_coef), bias, bool(link_x),
+                                            bool(diff_logits)))
 
 
 def route(x: torch.Tensor, gate_w: torch.Tensor, k: int, aux_coef: float = 0.0, z_coef: float = 0.0,

@@ -45,7 +45,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from moe_mi355 import ops
-from moe_mi355.layer import CombineFn, ExpertsFn, PermuteFn
+from moe_mi355.layer import CombineFn, ExpertsFn, ExpertsMxfp4Fn, PermuteFn
 from pkg.kernels.moe_router import MoERouter
 
 __all__ = ["DistributedMoELayer", "compute_capacity_drop_mask", "_cumcount"]
@@ -167,6 +167,7 @@ class DistributedMoELayer(nn.Module):
         aux_loss_coef: float = 0.0,
         z_loss_coef: float = 0.0,
         check_numerics: bool = True,
+        seq_balance_coef: float = 0.0,
     ):
         super().__init__()
         if getattr(topology, "ep_size", 1) != 1 or getattr(topology, "tp_size", 1) != 1:
@@ -197,7 +198,8 @@ class DistributedMoELayer(nn.Module):
         ref = weakref.ref(self)
         self.experts = nn.ModuleList([_SwiGLUExpert(ref, i) for i in range(E)])
         self.router = MoERouter(hidden_dim, num_experts, top_k, dtype=dtype, aux_loss_coef=aux_loss_coef,
-                                z_loss_coef=z_loss_coef, sync_profile=check_numerics)
+                                z_loss_coef=z_loss_coef, sync_profile=check_numerics,
+                                seq_balance_coef=seq_balance_coef)
         if dev is not None:
             self.router.to(dev)
         self.last_dispatch_ms: float = 0.0
@@ -268,14 +270,26 @@ class DistributedMoELayer(nn.Module):
             and len(self.experts) == self.num_experts
         )
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+    def _seq_kwargs(self, tokens: torch.Tensor, seq_offsets, token_mask) -> dict:
+        """The router's arguments for the balance loss of sequences, the rows of a [B, S, H] batch by default."""
+        r = self.router
+        if seq_offsets is None and token_mask is None and getattr(r, "seq_balance_coef", 0.0) == 0.0:
+            return {}
+        if seq_offsets is None and tokens.dim() == 3 and tokens.shape[0] > 0 and tokens.shape[1] > 0:
+            seq_offsets = torch.arange(0, tokens.shape[0] * tokens.shape[1] + 1, tokens.shape[1], device=tokens.device)
+        return {"seq_offsets": seq_offsets, "token_mask": token_mask}
+
+    def forward(self, tokens: torch.Tensor, seq_offsets: Optional[torch.Tensor] = None,
+                token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``seq_offsets`` and ``token_mask`` go to the router's balance loss of sequences (:meth:`MoERouter.forward`; the
+        rows of a [B, S, H] batch are its sequences unless told otherwise): every token is routed and dispatched."""
         original_shape = tokens.shape
         if tokens.dim() not in (2, 3):
             raise ValueError(f"tokens must be rank 2 or 3, got {tokens.dim()}")
         H = tokens.shape[-1]
         flat = tokens.reshape(-1, H)
         with self._deferred_router_check(), self._linked_tokens():
-            idx, weights, _cnt = self.router(flat)
+            idx, weights, _cnt = self.router(flat, **self._seq_kwargs(tokens, seq_offsets, token_mask))
         # the router hands the tokens back as a linked output (a view of the same memory): the expert path's
         # gradient of the tokens then reaches the router's backward, which adds it inside its dx kernel, so
         # x's gradient is formed in one pass instead of autograd adding the two paths' gradients afterwards
@@ -305,7 +319,9 @@ class DistributedMoELayer(nn.Module):
         finally:
             r._defer_check = False
 
-    def forward_normed(self, tokens: torch.Tensor, norm_weight: torch.Tensor, eps: float) -> torch.Tensor:
+    def forward_normed(self, tokens: torch.Tensor, norm_weight: torch.Tensor, eps: float,
+                       seq_offsets: Optional[torch.Tensor] = None,
+                       token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``forward(rmsnorm(tokens))`` with the norm fused into the router's read of the hidden state
         (moe-engine/pkg/models/moe.py L:125-126): the normalised rows feed both the router and the experts."""
         original_shape = tokens.shape
@@ -314,17 +330,23 @@ class DistributedMoELayer(nn.Module):
         H = tokens.shape[-1]
         flat = tokens.reshape(-1, H)
         with self._deferred_router_check():
-            xn, idx, weights, _cnt = self.router.forward_with_norm(flat, norm_weight, eps)
+            xn, idx, weights, _cnt = self.router.forward_with_norm(flat, norm_weight, eps,
+                                                                   **self._seq_kwargs(tokens, seq_offsets, token_mask))
         return self._experts_forward(xn, idx, weights).reshape(original_shape)
 
-    def _experts_forward(self, flat: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+    def _experts_forward(self, flat: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor,
+                         mxfp4=None) -> torch.Tensor:
         N = flat.shape[0]
         capacity = (
             math.ceil(self.capacity_factor * N * self.top_k / self.num_experts) if self.capacity_dropping else -1
         )
         p = ops.plan(idx, self.num_experts, capacity=capacity, layout=_LAYOUTS[self.layout])
         self.last_plan = p
-        if self._fused():
+        if mxfp4 is not None:
+            train = torch.is_grad_enabled() and (flat.requires_grad or weights.requires_grad)
+            timer = _ExpertTimer.new(flat)
+            out = ExpertsMxfp4Fn.apply(flat, weights, *mxfp4, p, train, timer)
+        elif self._fused():
             train = torch.is_grad_enabled() and any(
                 t.requires_grad for t in (flat, weights, self.w_gate, self.w_up, self.w_down))
             timer = _ExpertTimer.new(flat)
@@ -379,6 +401,41 @@ class DistributedMoELayer(nn.Module):
         _act, _hgu, y = ops.swiglu_forward_fp8(xq, sx, wq, ws, p.offsets, keep_preact=False)
         out = ops.combine(y, weights, p)
         return out.reshape(shape)
+
+    # ------------------------------------------------------------------
+    # experts held in 4 bits (MXFP4), new: serving, and training around frozen experts
+    # ------------------------------------------------------------------
+    @torch.no_grad()
+    def quantize_mxfp4(self):
+        """Quantize the expert weights to MXFP4 (:func:`moe_mi355.ops.quant_mxfp4`: 4-bit e2m1 values, one power-of-two scale
+        per 32 along the reduction) for :meth:`forward_mxfp4`, on the GPU.  The quantized weights stay as they are until this
+        is called again, whatever becomes of the parameters.  Returns ``((gate, up, down), (their scales))``."""
+        if self.w_gate.shape[-1] % ops.MXFP4_BLOCK or self.w_gate.shape[1] % ops.MXFP4_BLOCK:
+            raise NotImplementedError(f"quantize_mxfp4 needs hidden and ffn dims that are multiples of {ops.MXFP4_BLOCK}")
+        q = [ops.quant_mxfp4(t.detach()) for t in (self.w_gate, self.w_up, self.w_down)]
+        self._mxfp4 = (tuple(t for t, _ in q), tuple(s for _, s in q))
+        return self._mxfp4
+
+    def forward_mxfp4(self, tokens: torch.Tensor, seq_offsets: Optional[torch.Tensor] = None,
+                      token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``forward`` with the experts' weights as :meth:`quantize_mxfp4` left them: bf16 rows, 4-bit weights, from one
+        decoded token to a long prefill.  Differentiable in the tokens and the router; the 4-bit weights are constants (the
+        layer's own expert parameters get no gradient), so a router, or what lies before the layer, can be trained around
+        experts in the form that they are served in.  Needs the built-in SwiGLU experts and bfloat16 tokens."""
+        q = getattr(self, "_mxfp4", None)
+        if q is None:
+            raise RuntimeError("forward_mxfp4: call quantize_mxfp4() first")
+        if not all(type(m) is _SwiGLUExpert and m.w_gate._owner() is self for m in self.experts):
+            raise NotImplementedError("forward_mxfp4 needs the built-in SwiGLU experts")
+        if tokens.dim() not in (2, 3):
+            raise ValueError(f"tokens must be rank 2 or 3, got {tokens.dim()}")
+        if tokens.dtype != torch.bfloat16:
+            raise TypeError(f"forward_mxfp4 takes bfloat16 tokens, got {tokens.dtype}")
+        flat = tokens.reshape(-1, tokens.shape[-1])
+        with self._deferred_router_check(), self._linked_tokens():
+            idx, weights, _cnt = self.router(flat, **self._seq_kwargs(tokens, seq_offsets, token_mask))
+        linked = self.router.take_linked_tokens()
+        return self._experts_forward(flat if linked is None else linked, idx, weights, q).reshape(tokens.shape)
 
     def _forward_per_expert(self, flat: torch.Tensor, weights: torch.Tensor, p: ops.Plan,
                             timer: Optional["_ExpertTimer"] = None) -> torch.Tensor:

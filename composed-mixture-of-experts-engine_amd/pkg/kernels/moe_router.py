@@ -28,6 +28,9 @@ Differences from the reference, all deliberate:
   differentiable load-balance loss and z-loss of the last forward are kept in
   ``last_aux_loss`` / ``last_z_loss`` (0-d tensors).  With both coefficients
   at 0 (the default) behaviour matches the reference.
+* New, opt-in: ``seq_balance_coef`` with ``forward(tokens, seq_offsets=..., token_mask=...)``: the load-balance loss
+  within each sequence over its valid tokens (:mod:`moe_mi355.balance`), differentiable, in
+  ``last_seq_balance_loss``, with the sequences' per-expert counts.
 * Exact ties in the gate probabilities go to the lower expert index.
 """
 
@@ -40,6 +43,7 @@ from typing import Optional, Tuple
 import torch
 
 from moe_mi355 import _lib, ops
+from moe_mi355.balance import balance_loss
 from moe_mi355.router import STAT_CNT_MEAN, STAT_CNT_STD, STAT_CNT_TOTAL, STAT_IMBALANCE, STAT_NONFINITE, STAT_Z
 from moe_mi355.norm import NormRouterCore
 from moe_mi355.router import RouterCore
@@ -222,6 +226,7 @@ class MoERouter(torch.nn.Module):
         aux_loss_coef: float = 0.0,
         z_loss_coef: float = 0.0,
         sync_profile: bool = True,
+        seq_balance_coef: float = 0.0,
     ):
         super().__init__()
         if top_k < 1 or top_k > num_experts:
@@ -234,6 +239,8 @@ class MoERouter(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.zeros(num_experts, dtype=dtype)) if bias else None
         self.aux_loss_coef = float(aux_loss_coef)
         self.z_loss_coef = float(z_loss_coef)
+        # load balance within sequences (last_seq_*); the aux loss is over the whole batch
+        self.seq_balance_coef = float(seq_balance_coef)
         self.sync_profile = sync_profile
         self._profile: Optional[RouterProfile] = None
         self._pending = None  # what a not-yet-read profile is built from
@@ -247,6 +254,9 @@ class MoERouter(torch.nn.Module):
         self._last_logits: Optional[torch.Tensor] = None
         self.last_aux_loss: Optional[torch.Tensor] = None
         self.last_z_loss: Optional[torch.Tensor] = None
+        self.last_seq_balance_loss: Optional[torch.Tensor] = None
+        self.last_seq_counts: Optional[torch.Tensor] = None
+        self.last_seq_tokens: Optional[torch.Tensor] = None
         self.last_stats: Optional[torch.Tensor] = None
         self.last_stats_host: Optional[torch.Tensor] = None
         self.last_num_tokens = 0
@@ -265,13 +275,22 @@ class MoERouter(torch.nn.Module):
         self._pending = None
         self._profile = value
 
-    def forward(self, tokens: torch.Tensor, force_reference: bool = False):
-        """Returns ``(topk_idx [N,K] int64, topk_w [N,K] tokens.dtype, dispatch_cnt [E] int64)``."""
+    def forward(self, tokens: torch.Tensor, force_reference: bool = False,
+                seq_offsets: Optional[torch.Tensor] = None, token_mask: Optional[torch.Tensor] = None):
+        """Returns ``(topk_idx [N,K] int64, topk_w [N,K] tokens.dtype, dispatch_cnt [E] int64)``.
+
+        With ``seq_balance_coef`` (or one of the two arguments) the balance loss of the batch's sequences is formed as well:
+        ``last_seq_balance_loss`` (0-d, differentiable), ``last_seq_counts`` [S, E] and ``last_seq_tokens`` [S + 2]
+        (:func:`moe_mi355.ops.balance_loss_forward`).  ``seq_offsets`` [S + 1] bounds the sequences in the flattened tokens
+        (None: the rows of a [B, S, H] batch, or one sequence); ``token_mask`` (bool, one value a token) marks the valid
+        tokens.  With a mask ``last_z_loss`` is over the valid tokens; every token is routed and dispatched all the same,
+        and ``last_aux_loss``, the counts and the statistics are over all of them."""
         if tokens.dim() == 3:
             B, S, H = tokens.shape
             flat = tokens.reshape(B * S, H)
         else:
             flat = tokens
+        seq = self._seq_args(tokens.shape, seq_offsets, token_mask, tokens.device)
         N = flat.shape[0]
         H = flat.shape[1]
         assert H == self.hidden_dim
@@ -280,8 +299,8 @@ class MoERouter(torch.nn.Module):
 
         timing = _LaunchTiming.start(flat)
         outs = RouterCore.apply(
-            flat, self.gate_w, self.top_k, self.aux_loss_coef, self.z_loss_coef, self._logit_bias(),
-            link_x=self._link_x,
+            flat, self.gate_w, self.top_k, self.aux_loss_coef, self._kernel_z_coef(seq), self._logit_bias(),
+            link_x=self._link_x, diff_logits=seq is not None,
         )
         idx, w, aux, z, logits, cnt, stats = outs[:7]
         # with _link_x (set by DistributedMoELayer around its call) the tokens come back as an eighth output for
@@ -289,6 +308,7 @@ class MoERouter(torch.nn.Module):
         self._x_link = outs[7] if self._link_x else None
         if timing is not None:
             timing.stop()
+        z = self._seq_losses(seq, logits, idx, z)
         return self._finish(flat, idx, w, aux, z, logits, cnt, stats, timing)
 
     def take_linked_tokens(self) -> Optional[torch.Tensor]:
@@ -296,19 +316,47 @@ class MoERouter(torch.nn.Module):
         x, self._x_link = self._x_link, None
         return x
 
-    def forward_with_norm(self, tokens: torch.Tensor, norm_weight: torch.Tensor, eps: float):
+    def _seq_args(self, shape, seq_offsets, token_mask, device):
+        """(seq_offsets, token_mask) of a forward that forms the balance loss of sequences, else None."""
+        if self.seq_balance_coef == 0.0 and seq_offsets is None and token_mask is None:
+            self.last_seq_balance_loss = self.last_seq_counts = self.last_seq_tokens = None
+            return None
+        if seq_offsets is None and len(shape) == 3 and shape[0] > 0:
+            seq_offsets = torch.arange(0, shape[0] * shape[1] + 1, max(shape[1], 1), device=device)[: shape[0] + 1]
+            if shape[1] == 0:
+                seq_offsets = torch.zeros(shape[0] + 1, dtype=torch.int64, device=device)
+        return seq_offsets, token_mask
+
+    def _kernel_z_coef(self, seq) -> float:
+        """The z-loss over valid tokens is formed with the sequences' balance; the kernel's is over every token."""
+        return 0.0 if seq is not None and seq[1] is not None else self.z_loss_coef
+
+    def _seq_losses(self, seq, logits, idx, z):
+        if seq is None:
+            return z
+        masked = seq[1] is not None
+        balance, z_valid, self.last_seq_counts, self.last_seq_tokens, _ = balance_loss(
+            logits, idx, seq[0], seq[1], self.seq_balance_coef, self.z_loss_coef if masked else 0.0)
+        self.last_seq_balance_loss = balance
+        return z_valid if masked else z
+
+    def forward_with_norm(self, tokens: torch.Tensor, norm_weight: torch.Tensor, eps: float,
+                          seq_offsets: Optional[torch.Tensor] = None, token_mask: Optional[torch.Tensor] = None):
         """Route ``rmsnorm(tokens)`` with the norm fused into the router's read of ``tokens``
         (moe-engine/pkg/models/moe.py L:83-86, L:125-126).  Returns ``(xn, topk_idx, topk_w, dispatch_cnt)``:
-        ``xn`` is the normalised input the routing used, for the expert path."""
+        ``xn`` is the normalised input the routing used, for the expert path.  ``seq_offsets`` and ``token_mask`` as in
+        :meth:`forward`."""
+        seq = self._seq_args(tokens.shape, seq_offsets, token_mask, tokens.device)
         flat = tokens.reshape(-1, tokens.shape[-1])
         assert flat.shape[1] == self.hidden_dim
         timing = _LaunchTiming.start(flat)
         xn, idx, w, aux, z, logits, cnt, stats = NormRouterCore.apply(
-            flat, norm_weight, float(eps), self.gate_w, self.top_k, self.aux_loss_coef, self.z_loss_coef,
-            self._logit_bias(),
+            flat, norm_weight, float(eps), self.gate_w, self.top_k, self.aux_loss_coef, self._kernel_z_coef(seq),
+            self._logit_bias(), seq is not None,
         )
         if timing is not None:
             timing.stop()
+        z = self._seq_losses(seq, logits, idx, z)
         idx, w, cnt = self._finish(flat, idx, w, aux, z, logits, cnt, stats, timing)
         return xn, idx, w, cnt
 
@@ -333,7 +381,7 @@ class MoERouter(torch.nn.Module):
                 if self.logit_bias is not None:
                     logits = logits + self.logit_bias.float()
             z_plain = torch.logsumexp(logits, dim=-1).square().mean().reshape(1) if N else logits.new_zeros(1)
-        self._last_logits = logits
+        self._last_logits = logits.detach()
         self.last_aux_loss = aux
         self.last_z_loss = z
         self.last_stats = stats

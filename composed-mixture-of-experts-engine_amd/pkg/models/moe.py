@@ -74,9 +74,11 @@ class ToyMoEBlock(nn.Module):
             and self.moe.router.gate_w.dtype == x.dtype
         )
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, seq_offsets=None, token_mask=None) -> torch.Tensor:
+        """``seq_offsets`` and ``token_mask``: the sequences and valid tokens of the router's balance loss
+        (:meth:`DistributedMoELayer.forward`)."""
         if self._fused(x):
-            out = self.moe.forward_normed(x, self.norm.weight, self.norm.eps)
+            out = self.moe.forward_normed(x, self.norm.weight, self.norm.eps, seq_offsets, token_mask)
         else:
-            out = self.moe(self.norm(x))
+            out = self.moe(self.norm(x), seq_offsets, token_mask)
         return x + out

@@ -158,6 +158,17 @@ int moe_router_bwd_acc(const void* x, int x_dtype, const void* wg, int wg_dtype,
                        const void* dx_add, void* dx_out, void* dwg_out,
                        void* workspace, size_t ws_bytes, void* stream);
 
+/* moe_router_bwd_acc with one more upstream gradient: grad_logits [N, E] f32 (NULL = zero), the gradient of the logits from
+ * a loss formed on them (moe_balance_bwd's), is added to G before its rounding.  dx_add may be NULL.  No counterpart in the
+ * reference, whose logits carry no gradient of their own. */
+int moe_router_bwd_logits(const void* x, int x_dtype, const void* wg, int wg_dtype,
+                          const float* logits, const int64_t* idx, const void* grad_w, int gw_dtype,
+                          const int64_t* cnt, const float* grad_aux, const float* grad_z,
+                          float aux_coef, float z_coef, const float* grad_logits,
+                          int64_t N, int64_t H, int64_t E, int64_t K,
+                          const void* dx_add, void* dx_out, void* dwg_out,
+                          void* workspace, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Dispatch planner.  From the router's idx [N, K] (int64) builds, on the
  * device and deterministically:
@@ -429,6 +440,13 @@ int moe_rmsnorm_router_bwd(const void* x, int x_dtype, const void* gamma, int ga
                            const float* grad_z, float aux_coef, float z_coef, const void* dxn, int64_t N, int64_t H,
                            int64_t E, int64_t K, void* dx_out, void* dgamma_out, void* dwg_out, void* workspace,
                            size_t ws_bytes, void* stream);
+/* The same with the logits' own upstream gradient, as moe_router_bwd_logits (workspace: moe_rmsnorm_router_bwd's). */
+int moe_rmsnorm_router_bwd_logits(const void* x, int x_dtype, const void* gamma, int gamma_dtype, const float* rstd,
+                                  const void* xn, const void* wg, int wg_dtype, const float* logits, const int64_t* idx,
+                                  const void* grad_w, int gw_dtype, const int64_t* cnt, const float* grad_aux,
+                                  const float* grad_z, float aux_coef, float z_coef, const float* grad_logits,
+                                  const void* dxn, int64_t N, int64_t H, int64_t E, int64_t K, void* dx_out,
+                                  void* dgamma_out, void* dwg_out, void* workspace, size_t ws_bytes, void* stream);
 
 /* ----------------------------------------------------------------------
  * Per-step routing telemetry on the device: replaces the host-side routing
