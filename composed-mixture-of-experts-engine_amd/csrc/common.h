@@ -191,20 +191,9 @@ int swiglu_small_fwd(bool f32, const void* xp, const void* w_gate, const void* w
                      const int* offsets, int64_t R, int64_t H, int64_t F, int64_t E, void* act, void* hgu, void* y,
                      hipStream_t s);
 
-// ---- the row-grouped products of the bf16 backward (csrc/gemm.hip): a table of tiles of bm rows (theirs: kGemmRows) in the
-// workspace's first moe_swiglu_workspace(E) bytes, dh [R, 2F] = epilogue(dy Wd), dxp = dh [Wg ; Wu] (ws_bytes past the table: partial tiles) ----
-constexpr int kGemmRows = 256;
+// ---- the table of row tiles of bm rows (csrc/gemm.hip), in a workspace's first moe_swiglu_workspace(E) bytes: how many come
+// before each expert's ----
 int swiglu_tiles(const int* offsets, int64_t E, int bm, void* workspace, hipStream_t s);
-int swiglu_dact(const void* dy, const void* hgu, const void* w_down, const int* offsets, int64_t R, int64_t H, int64_t F,
-                int64_t E, void* dh, const void* workspace, hipStream_t s);
-int swiglu_dxp(const void* dh, const void* w_gate, const void* w_up, const int* offsets, int64_t R, int64_t H, int64_t F,
-               int64_t E, void* dxp, void* workspace, size_t ws_bytes, hipStream_t s);
-
-// The same on MXFP4 weights, dequantized inside the products.
-int swiglu_dact_mxfp4(const void* dy, const void* hgu, const void* wd_q, const void* sd, const int* offsets, int64_t R,
-                      int64_t H, int64_t F, int64_t E, void* dh, const void* workspace, hipStream_t s);
-int swiglu_dxp_mxfp4(const void* dh, const void* wg_q, const void* sg, const void* wu_q, const void* su, const int* offsets,
-                     int64_t R, int64_t H, int64_t F, int64_t E, void* dxp, void* workspace, size_t ws_bytes, hipStream_t s);
 
 // ---- optional per-kernel timing (host side; off unless moe_prof_enable(1)) ----
 // Brackets one launch with two hipEvents recorded on the launch stream.

@@ -48,10 +48,6 @@
 //          sa[row] * sb[col] before rounding.  The gate/up product (EPI1) writes act block-quantized
 //          (e4m3 plus an E8M0 scale per 32 values, aq / aqs), and the down projection passes those
 //          block scales to the MFMA (mxs; its sa is then 1).
-//   operand mode 3 (B, "cols fp4"): element (i, k) of a cols operand as MXFP4 along i (q4: pairs of e2m1, s4: a scale byte per
-//          32).  A thread loads one 16-byte block of a slice (k row thread / 8, columns 32 (thread % 8) on) two slices ahead
-//          and, when the slice's ring unit is free, dequantizes it into the unit's cols layout (exact in bf16), where the
-//          other modes' DMA would land.
 //
 // products (R = rows, per expert e):
 //   fwd1  [act | hgu] = xp  . [Wg_e ; Wu_e]^T      A rows(xp), B rows(W),  G0, EPI1
@@ -92,10 +88,6 @@ struct GemmArgs {
   uint8_t* aqs;        // ... and its E8M0 block scales, slice-major: [(f / 128) * srows + row] * 4 + (f / 32) % 4
   const uint8_t* mxs;  // mode 2, EPI0: the A operand's E8M0 block scales in that layout (A's rows are act's)
   int64_t srows;       // rows per slice of the block-scale layout (a multiple of 4)
-  const uint8_t* q4;   // mode 3: B's elements, two a byte (ldb, b_estride, b_split in elements) ...
-  const uint8_t* s4;   // ... its scale bytes ...
-  const uint8_t* q42;  // ... and both of the second source
-  const uint8_t* s42;
   float* part;         // row-grouped EPI0: partial tiles of the split last round (null: no split)
   int npart;           // ... and how many of them an XCD has room for
   int E;
@@ -264,8 +256,6 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
   constexpr bool MX = F8 && EPI == 0;
   constexpr int MXSTAGE = 2048;
   static_assert((AMODE == 2) == (BMODE == 2), "fp8 mode applies to both operands");
-  constexpr bool Q4 = BMODE == 3;  // the LDS tile is a cols tile
-  static_assert(!Q4 || (GROUP == 0 && NW == 8), "mode 3 has a block per thread of 512");
   __shared__ __attribute__((aligned(16))) uint8_t smem[GSMEM + (F8 ? GSCALE : 0) + (MX ? 2 * MXSTAGE : 0)];
 
   const int tid = threadIdx.x;
@@ -354,7 +344,7 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
   const int n0 = nt * GBN;
   const int nlen = (EPI == 1) ? min(GBN, 2 * (g.F - nt * (GBN / 2))) : min(GBN, g.N - n0);
   const int nk = (klen + GBK - 1) / GBK;
-  const bool has_split = GROUP == 0 && (BMODE == 1 || Q4) && g.b_split > 0;  // dxp: the second weight follows at k = bsplit
+  const bool has_split = GROUP == 0 && BMODE == 1 && g.b_split > 0;  // dxp: the second weight follows at k = bsplit
   const int bsplit = g.b_split - (GROUP == 0 ? kbase : 0);           // in this block's k (not positive: all second)
 
   // ---- per-lane DMA sources.  Wave instruction j (= QPW*wv + q, q < QPW) of an operand fills bytes
@@ -384,10 +374,7 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
       a_src[q] = g.A + (int64_t)(kbase + a_kl_[q]) * g.lda + mbase + (i < mlen ? i : 0);
     }
     b_src2[q] = nullptr;
-    if constexpr (Q4) {
-      b_kl_[q] = 0;
-      b_src[q] = nullptr;
-    } else if constexpr (BMODE != 1) {
+    if constexpr (BMODE != 1) {
       const int i = 8 * j + (lane >> 3);
       b_kl_[q] = ((lane & 7) ^ ((i >> 1) & 7)) * 8;
       const int ic = min(i, nlen - 1);
@@ -462,41 +449,8 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
   // Ring unit u (A of slice u/2 when u is even, B otherwise) lives in LDS slot u % GUNITS.
   auto unit_ptr = [&](int u) { return smem + (u & (GUNITS - 1)) * GOPB; };
   auto issue_unit = [&](int u) {
-    if (u & 1) {
-      if constexpr (!Q4) issue_b(u >> 1, unit_ptr(u));
-    } else {
-      issue_a(u >> 1, unit_ptr(u));
-    }
-  };
-  // mode 3: this thread's block of slice kt to registers, and from there to the slice's ring unit (past klen: zeros)
-  u32x4 q4v;
-  uint32_t q4s = 0;
-  const int q4k = tid >> 3, q4c = tid & 7;
-  auto q4_load = [&](int kt) {
-    const int k = min(kt * GBK + q4k, klen - 1);
-    const bool second = has_split && k >= bsplit;
-    const int64_t blk = (((int64_t)e * g.b_estride + (int64_t)((SPLIT && !second ? kbase : 0) + (second ? k - bsplit : k)) * g.ldb + n0) >> 5) +
-                        min(q4c, (nlen >> 5) - 1);
-    q4v = *reinterpret_cast<const u32x4*>((second ? g.q42 : g.q4) + blk * 16);
-    q4s = (second ? g.s42 : g.s4)[blk];
-  };
-  auto q4_write = [&](int kt) {
-    const bool in = kt * GBK + q4k < klen;
-    const float sc = __uint_as_float(in ? q4s << 23 : 0x3f800000u);
-    // the block's four 16-byte pieces lie side by side; the upper four threads of a k row start with the third, so that
-    // eight threads' writes fall in distinct banks
-    const bool up = q4c >= 4;
-    uint8_t* const dst = unit_ptr(2 * kt + 1) + q4k * 512 + ((q4c ^ (q4k & 3)) << 6);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = in ? (up ? q4v[j ^ 2] : q4v[j]) : 0u;
-      u32x4 r;
-      r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
-      r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
-      r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
-      r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
-      *reinterpret_cast<u32x4*>(dst + ((up ? j ^ 2 : j) << 4)) = r;
-    }
+    if (u & 1) issue_b(u >> 1, unit_ptr(u));
+    else issue_a(u >> 1, unit_ptr(u));
   };
 
   f32x16 acc[MI][NI];
@@ -514,7 +468,7 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
       fa[mi] = AMODE != 1 ? frag_rows(as, wm0 + mi * 32, ks, lane) : frag_cols(as, wm0 + mi * 32, ks, lane);
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni)
-      fb[ni] = BMODE != 1 && !Q4 ? frag_rows(bs, wn0 + ni * 32, ks, lane) : frag_cols(bs, wn0 + ni * 32, ks, lane);
+      fb[ni] = BMODE != 1 ? frag_rows(bs, wn0 + ni * 32, ks, lane) : frag_cols(bs, wn0 + ni * 32, ks, lane);
   };
   auto mma = [&](const i16x8 (&fa)[MI], const i16x8 (&fb)[NI]) {
 #pragma unroll
@@ -793,27 +747,14 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
     // quarter of stage kt every wave waits for stage kt+1 (the only DMA group in flight) and for its
     // own reads of stage kt; one barrier makes both visible workgroup-wide, and stage kt's two units
     // are refilled with stage kt+2 while the last quarter's MFMAs run.
-    if constexpr (Q4) {
-      issue_unit(0);
-      q4_load(0);
-      q4_write(0);
-      if (nk > 1) {
-        issue_unit(2);
-        q4_load(1);
-        q4_write(1);
-      }
-      wait_vmcnt_lgkm0<0>();
-      if (nk > 2) q4_load(2);
-    } else {
-      issue_unit(0);
-      issue_unit(1);
-      if (nk > 1) {
-        issue_unit(2);
-        issue_unit(3);
-      }
-      if (nk > 1) wait_vmcnt<2 * QPW>();  // this wave's part of stage 0 has landed
-      else wait_vmcnt<0>();
+    issue_unit(0);
+    issue_unit(1);
+    if (nk > 1) {
+      issue_unit(2);
+      issue_unit(3);
     }
+    if (nk > 1) wait_vmcnt<2 * QPW>();  // this wave's part of stage 0 has landed
+    else wait_vmcnt<0>();
     lds_barrier();                                   // every wave's part has
     // A tile of at most 128 rows (the usual end of an expert's segment): the waves of the lower half only feed the ring
     // and keep the barriers, which leaves the MFMAs of a SIMD to its wave of the upper half.  The slices then wait for
@@ -823,16 +764,11 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
     // of them and put 2% on the down projection's loop.
     if (GROUP == 0 && wm0 >= mlen) {
       for (int kt = 0; kt < nk; ++kt) {
-        if constexpr (Q4) wait_vmcnt_lgkm0<0>();
-        else wait_vmcnt<0>();  // this wave's part of stage kt+1
+        wait_vmcnt<0>();  // this wave's part of stage kt+1
         lds_barrier();
         if (kt + 2 < nk) {
           issue_unit(2 * kt + 4);
           issue_unit(2 * kt + 5);
-          if constexpr (Q4) {
-            q4_write(kt + 2);
-            if (kt + 3 < nk) q4_load(kt + 3);
-          }
         }
       }
     } else {
@@ -860,11 +796,6 @@ __global__ __launch_bounds__(NW * 64, 1) void k_gemm(GemmArgs g) {
       if (kt + 2 < nk) {
         issue_unit(2 * kt + 4);
         issue_unit(2 * kt + 5);
-        if constexpr (Q4) {
-          q4_write(kt + 2);  // its block, loaded a slice ago, arrived with the slice's DMA
-          if (kt + 3 < nk) q4_load(kt + 3);
-          __builtin_amdgcn_sched_barrier(0);
-        }
       }
       if (kt + 1 < nk) frags(unit_ptr(2 * kt + 2), unit_ptr(2 * kt + 3), 0, fa0, fb0);
       mma(fa1, fb1);
@@ -1514,80 +1445,9 @@ extern "C" int moe_swiglu_fwd_fp8(const void* xq, const float* sx, const void* w
 }
 
 namespace moe {
-// The row-grouped products of the backward, over the tile table that swiglu_tiles has put into the workspace (common.h).
 int swiglu_tiles(const int* offsets, int64_t E, int bm, void* workspace, hipStream_t s) {
   launch_tiles(s, offsets, E, static_cast<int*>(workspace), nullptr, bm);
   return check_launch("k_gemm_tiles");
-}
-
-// dA: dh = epilogue(dy . Wd)   (B[n=f][k=h] = Wd[h][f])
-static GemmArgs dact_args(const void* dy, const void* hgu, const int* offsets, int64_t H, int64_t F, int64_t E, void* dh,
-                          const void* workspace) {
-  GemmArgs a{};
-  a.offsets = offsets;
-  a.tile_off = static_cast<const int*>(workspace);
-  a.E = (int)E;
-  a.F = (int)F;
-  a.A = static_cast<const uint16_t*>(dy);
-  a.lda = H;
-  a.ldb = F;
-  a.b_estride = H * F;
-  a.C = static_cast<uint16_t*>(dh);
-  a.ldc = 2 * F;
-  a.X = static_cast<const uint16_t*>(hgu);
-  a.N = (int)F;
-  a.K = (int)H;
-  return a;
-}
-int swiglu_dact(const void* dy, const void* hgu, const void* w_down, const int* offsets, int64_t R, int64_t H, int64_t F,
-                int64_t E, void* dh, const void* workspace, hipStream_t s) {
-  GemmArgs a = dact_args(dy, hgu, offsets, H, F, E, dh, workspace);
-  a.B = static_cast<const uint16_t*>(w_down);
-  return launch<0, 1, 0, 2, kNW_dact>("k_gemm_swiglu_dact", s, a, R);
-}
-int swiglu_dact_mxfp4(const void* dy, const void* hgu, const void* wd_q, const void* sd, const int* offsets, int64_t R,
-                      int64_t H, int64_t F, int64_t E, void* dh, const void* workspace, hipStream_t s) {
-  GemmArgs a = dact_args(dy, hgu, offsets, H, F, E, dh, workspace);
-  a.q4 = static_cast<const uint8_t*>(wd_q);
-  a.s4 = static_cast<const uint8_t*>(sd);
-  return launch<0, 3, 0, 2, kNW_dact>("k_gemm_swiglu_dact_mxfp4", s, a, R);
-}
-
-// dxp = dh . [Wg ; Wu]   (B[n=h][k=j] = W1[j][h])
-static GemmArgs dxp_args(const void* dh, const int* offsets, int64_t R, int64_t H, int64_t F, int64_t E, void* dxp,
-                         void* workspace, size_t ws_bytes) {
-  GemmArgs a{};
-  a.offsets = offsets;
-  a.tile_off = static_cast<const int*>(workspace);
-  a.E = (int)E;
-  a.F = (int)F;
-  a.A = static_cast<const uint16_t*>(dh);
-  a.lda = 2 * F;
-  a.b_split = (int)F;
-  a.ldb = H;
-  a.b_estride = F * H;
-  a.C = static_cast<uint16_t*>(dxp);
-  a.ldc = H;
-  a.N = (int)H;
-  a.K = (int)(2 * F);
-  take_split(a, R, workspace, ws_bytes, moe_swiglu_workspace(E));
-  return a;
-}
-int swiglu_dxp(const void* dh, const void* w_gate, const void* w_up, const int* offsets, int64_t R, int64_t H, int64_t F,
-               int64_t E, void* dxp, void* workspace, size_t ws_bytes, hipStream_t s) {
-  GemmArgs a = dxp_args(dh, offsets, R, H, F, E, dxp, workspace, ws_bytes);
-  a.B = static_cast<const uint16_t*>(w_gate);
-  a.B2 = static_cast<const uint16_t*>(w_up);
-  return launch<0, 1, 0, 0, kNW_dxp>("k_gemm_swiglu_dxp", s, a, R);
-}
-int swiglu_dxp_mxfp4(const void* dh, const void* wg_q, const void* sg, const void* wu_q, const void* su, const int* offsets,
-                     int64_t R, int64_t H, int64_t F, int64_t E, void* dxp, void* workspace, size_t ws_bytes, hipStream_t s) {
-  GemmArgs a = dxp_args(dh, offsets, R, H, F, E, dxp, workspace, ws_bytes);
-  a.q4 = static_cast<const uint8_t*>(wg_q);
-  a.s4 = static_cast<const uint8_t*>(sg);
-  a.q42 = static_cast<const uint8_t*>(wu_q);
-  a.s42 = static_cast<const uint8_t*>(su);
-  return launch<0, 3, 0, 0, kNW_dxp>("k_gemm_swiglu_dxp_mxfp4", s, a, R);
 }
 }  // namespace moe
 
@@ -1603,11 +1463,48 @@ extern "C" int moe_swiglu_bwd(const void* dy, const void* xp, const void* act, c
     return fail_arg("moe_swiglu_bwd: null pointer argument");
   if (ws_bytes < moe_swiglu_workspace(E) || !workspace) return set_error("moe_swiglu_bwd: workspace"), MOE_EWORKSPACE;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  int* korder = static_cast<int*>(workspace) + (E + 1);
-  launch_tiles(s, offsets, E, static_cast<int*>(workspace), korder);
+  int* tile_off = static_cast<int*>(workspace);
+  int* korder = tile_off + (E + 1);
+  launch_tiles(s, offsets, E, tile_off, korder);
+  // dA: dh = epilogue(dy . Wd)   (B[n=f][k=h] = Wd[h][f])
   if (R > 0) {
-    if (int rc = swiglu_dact(dy, hgu, w_down, offsets, R, H, F, E, dh, workspace, s)) return rc;
-    if (int rc = swiglu_dxp(dh, w_gate, w_up, offsets, R, H, F, E, dxp, workspace, ws_bytes, s)) return rc;
+    GemmArgs a{};
+    a.offsets = offsets;
+    a.tile_off = tile_off;
+    a.E = (int)E;
+    a.F = (int)F;
+    a.A = static_cast<const uint16_t*>(dy);
+    a.lda = H;
+    a.B = static_cast<const uint16_t*>(w_down);
+    a.ldb = F;
+    a.b_estride = H * F;
+    a.C = static_cast<uint16_t*>(dh);
+    a.ldc = 2 * F;
+    a.X = static_cast<const uint16_t*>(hgu);
+    a.N = (int)F;
+    a.K = (int)H;
+    if (int rc = launch<0, 1, 0, 2, kNW_dact>("k_gemm_swiglu_dact", s, a, R)) return rc;
+  }
+  // dxp = dh . [Wg ; Wu]   (B[n=h][k=j] = W1[j][h])
+  if (R > 0) {
+    GemmArgs a{};
+    a.offsets = offsets;
+    a.tile_off = tile_off;
+    a.E = (int)E;
+    a.F = (int)F;
+    a.A = static_cast<const uint16_t*>(dh);
+    a.lda = 2 * F;
+    a.B = static_cast<const uint16_t*>(w_gate);
+    a.B2 = static_cast<const uint16_t*>(w_up);
+    a.b_split = (int)F;
+    a.ldb = H;
+    a.b_estride = F * H;
+    a.C = static_cast<uint16_t*>(dxp);
+    a.ldc = H;
+    a.N = (int)H;
+    a.K = (int)(2 * F);
+    take_split(a, R, workspace, ws_bytes, moe_swiglu_workspace(E));
+    if (int rc = launch<0, 1, 0, 0, kNW_dxp>("k_gemm_swiglu_dxp", s, a, R)) return rc;
   }
   // dWd_e = dy_e^T . act_e   (M = H, N = F, K = rows of e)
   {

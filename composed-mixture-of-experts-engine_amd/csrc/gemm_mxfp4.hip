@@ -291,12 +291,12 @@ __host__ __device__ constexpr int mx_resident(int bm) { return bm == 256 ? 32 : 
 // The last round of a product: an XCD's n tiles run `resident` at a time, and its last n % resident leave the rest of it
 // idle; with few rows that round is all there is.  Those tiles are split over their slices, in rounds of G, into `parts`
 // blocks each, whose fp32 tiles go to memory and are added in order by k_mx_reduce.  parts (1 to 8) is the one with the
-// least estimated time in slices: the rounds that the parts take, plus 16 slices a part for writing and reading back its
+// least estimated time in slices: the rounds that the parts take, plus `over` slices a part for writing and reading back its
 // tile, plus the reduction's launch.  Every block computes it from the device's tile count, and the reduction again.
 struct MxSplit {
   int full, rest, parts;  // whole tiles; split tiles; blocks of each
 };
-__device__ __forceinline__ MxSplit mx_split(int n, int ns, int npart, int resident, int G) {
+__device__ __forceinline__ MxSplit mx_split(int n, int ns, int npart, int resident, int G, int over = 16) {
   MxSplit s{0, 0, 1};
   if (n <= 0) return s;
   s.rest = n % resident;
@@ -304,7 +304,7 @@ __device__ __forceinline__ MxSplit mx_split(int n, int ns, int npart, int reside
   int cost = ns;
   for (int S = 2; s.rest > 0 && S <= 8; ++S) {
     if (s.rest * S > npart || S * G > ns) break;
-    const int c = (s.rest * S + resident - 1) / resident * ((ns + S - 1) / S + 16) + 5;
+    const int c = (s.rest * S + resident - 1) / resident * ((ns + S - 1) / S + over) + 5;
     if (c < cost) {
       cost = c;
       s.parts = S;
@@ -756,9 +756,514 @@ extern "C" int moe_swiglu_fwd_mxfp4(const void* xp, const void* wg_q, const void
 
 // ---- backward to the rows ----
 
+namespace moe {
+namespace {
+struct BkArgs {
+  const uint16_t* A;   // dy [R][K] / dh [R][K]
+  const uint8_t* B;    // weights [E][Ks][N / 2]: the reduction runs down their rows, their blocks lie along the columns
+  const uint8_t* B2;   // ... and those of the reduction's rows from Ks on (up weights)
+  const uint8_t* S;    // scales [E][Ks][N / 32]
+  const uint8_t* S2;
+  uint16_t* C;         // dh [R][2N] / dxp [R][N]
+  const uint16_t* X;   // hgu [R][2N] (product with Wd)
+  const int* offsets;  // [E+1]
+  const int* tile_off; // [E+1] row-tile prefix
+  int K;               // reduction length: Ks or 2 Ks
+  int Ks;
+  int N;               // output columns
+  int Tn;              // column tiles
+  int E;
+  float* part;         // partial tiles of a split last round (null: no split) ...
+  int npart;           // ... and how many of them an XCD has room for
+};
+
+constexpr int kBkCols = 256;  // columns of a tile
+
+// NF consecutive columns of a row of bf16.
+template <int NF>
+struct __attribute__((aligned(NF * 2))) BkCols {
+  uint32_t d[NF / 2];
+};
+// They leave: dxp as they are; dh = [da u silu'(g) | da silu(g)] from fp32 da, the pre-activations gv, uv in hand.
+template <int NF>
+__device__ __forceinline__ void bk_put(const BkArgs& g, int64_t row, int col, const float (&v)[NF]) {
+  BkCols<NF> o;
+#pragma unroll
+  for (int d = 0; d < NF / 2; ++d) o.d[d] = pack2bf(v[2 * d], v[2 * d + 1]);
+  *reinterpret_cast<BkCols<NF>*>(g.C + row * g.N + col) = o;
+}
+template <int NF>
+__device__ __forceinline__ void bk_put(const BkArgs& g, int64_t row, int col, const float (&v)[NF], const BkCols<NF>& gv,
+                                       const BkCols<NF>& uv) {
+  BkCols<NF> dg, du;
+#pragma unroll
+  for (int d = 0; d < NF / 2; ++d) {
+    float o[2], p[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float x = __uint_as_float(h ? gv.d[d] & 0xffff0000u : gv.d[d] << 16);
+      const float u = __uint_as_float(h ? uv.d[d] & 0xffff0000u : uv.d[d] << 16);
+      const float sg = sig_mx(x), t = v[2 * d + h] * sg;
+      o[h] = t * u * (1.f + x * (1.f - sg));
+      p[h] = t * x;
+    }
+    dg.d[d] = pack2bf(o[0], o[1]);
+    du.d[d] = pack2bf(p[0], p[1]);
+  }
+  const int64_t at = row * 2 * (int64_t)g.N + col;
+  *reinterpret_cast<BkCols<NF>*>(g.C + at) = dg;
+  *reinterpret_cast<BkCols<NF>*>(g.C + at + g.N) = du;
+}
+template <bool DACT, int NF>
+__device__ __forceinline__ void bk_store(const BkArgs& g, int64_t row, int col, const float (&v)[NF]) {
+  if constexpr (DACT) {
+    const uint16_t* const x = g.X + row * 2 * (int64_t)g.N + col;
+    const BkCols<NF> gv = *reinterpret_cast<const BkCols<NF>*>(x), uv = *reinterpret_cast<const BkCols<NF>*>(x + g.N);
+    bk_put<NF>(g, row, col, v, gv, uv);
+  } else {
+    bk_put<NF>(g, row, col, v);
+  }
+}
+
+// Where a product's tile L lies.
+struct BkTile {
+  int e, nt, mbase, mlen;
+};
+template <int BM>
+__device__ __forceinline__ BkTile bk_tile(const BkArgs& g, int L, int lane) {
+  MxArgs m{};
+  m.E = g.E;
+  m.Tn = g.Tn;
+  m.tile_off = g.tile_off;
+  BkTile t;
+  t.e = mx_expert(m, L, lane);
+  const int cnt = g.tile_off[t.e + 1] - g.tile_off[t.e], local = L - g.tile_off[t.e] * g.Tn;
+  t.nt = local / cnt;
+  t.mbase = g.offsets[t.e] + (local - t.nt * cnt) * BM;
+  t.mlen = min(BM, g.offsets[t.e + 1] - t.mbase);
+  return t;
+}
+// The backward's products reduce down the weights' rows, across their blocks: every reduction row of a block has a scale of its
+// own, and the matrix instruction wants pairs of reduction rows in a word.  So a lane loads NF consecutive columns of eight rows
+// (a scale a row), dequantizes them along the columns, two a instruction, and turns the words of two rows over with one v_perm
+// a word: a vector instruction a weight, twice the forward's, and no pass through LDS.  Column NF i + j of the wave's goes to
+// fragment j, lane i, which leaves each lane NF consecutive columns of the result: fp32 da meets the pre-activations in
+// registers, and rows leave in whole segments.  The rows go through LDS in 64-wide slices, as in k_mx_tile: fetched by the lanes
+// that use them they are 64 cache accesses a load, and those bounded the products (5.4 ms for dxp below).
+//
+// What bounds them: matrix instructions and the conversion's issue with 256 rows (one wave a SIMD, MFMA busy 62%), the
+// epilogue's 3.8 GB in the product with Wd, whose two blocks a CU run under each other's.  16384 rows, E 8, H 4096, F 14336:
+// dact 2.17 ms, dxp 3.33 ms (1.92 TFLOP and 3.85: 890 and 1160 TFLOP/s); the products on bf16 weights 2.01 and 3.35.
+
+// A form: a wave has 32 TF rows by 32 NF columns, a block's four waves lie WT on the rows, WF on the columns and KS along the
+// reduction.
+template <int TF_, int NF_, int WT_, int WF_, int KS_>
+struct BkForm {
+  static constexpr int TF = TF_, NF = NF_, WT = WT_, WF = WF_, KS = KS_, BM = 32 * TF_ * WT_;
+  static constexpr int BLOCKS = TF * NF > 8 ? 1 : 2;  // of a CU
+  static_assert(WT * WF * KS == 4 && WF * NF == 8);
+};
+// The split of an XCD's last round.  With KS waves along the reduction a block's slices pass KS times as fast, and its tile is
+// as much smaller.
+template <class Form>
+__device__ __forceinline__ MxSplit bk_split(const BkArgs& g, int n) {
+  constexpr int KS = Form::KS;
+  return mx_split(n, (g.K / 32 + 2 * KS - 1) / (2 * KS), g.npart, 32 * Form::BLOCKS, 2, 16 / KS);
+}
+
+template <class Form, bool DACT>
+__global__ __launch_bounds__(256, Form::BLOCKS) void k_mx_back(BkArgs g) {
+  constexpr int TF = Form::TF, NF = Form::NF, WT = Form::WT, WF = Form::WF, KS = Form::KS, BM = Form::BM;
+  constexpr int NP = BM / (8 * WT * WF);  // 16-byte pieces of a thread's share of a slice of the rows
+  constexpr int SL = TF * NF;     // MFMAs of a 16-wide step
+  constexpr int SLICE = BM * 128; // LDS bytes of a 64-wide slice of the rows
+  constexpr int PB = NF;          // blocks of a wave's columns
+  constexpr int SR = 36;          // a block's scales of 32 reduction rows (padded: blocks lie in distinct banks)
+  constexpr int SP = PB * SR;     // ... and a wave's
+  constexpr int SMEM = std::max(2 * KS * SLICE, 4 * (KS - 1) * 8192);
+  __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
+  __shared__ __attribute__((aligned(16))) float scl[4 * SP];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i32 = lane & 31, h = lane >> 5;
+
+  const int total = g.tile_off[g.E] * g.Tn;
+  const int chunk = (total + 7) >> 3, xcd = (int)(blockIdx.x & 7);
+  int slot = (int)(blockIdx.x >> 3);
+  int b0 = 0, b1 = g.K / 32;  // the block's units of 32 of the reduction
+  float* part_out = nullptr;
+  {
+    const MxSplit sp = bk_split<Form>(g, min(chunk, total - xcd * chunk));
+    if (sp.parts > 1 && slot >= sp.full) {
+      const int j = slot - sp.full, t = j / sp.parts, p = j - t * sp.parts;
+      if (t >= sp.rest) return;
+      slot = sp.full + t;
+      const int units = b1;
+      b0 = units * p / sp.parts;
+      b1 = units * (p + 1) / sp.parts;
+      part_out = g.part + (int64_t)(xcd * g.npart + j) * (BM * kBkCols);
+    }
+  }
+  const int L = xcd * chunk + slot;
+  if (slot >= chunk || L >= total) return;
+  const BkTile tl = bk_tile<BM>(g, L, lane);
+  const int gw = wv % (WT * WF), tw = gw % WT, fw = gw / WT, kw = wv / (WT * WF);
+  const int n0 = tl.nt * kBkCols + fw * (32 * NF);
+  const int w0 = __builtin_amdgcn_readfirstlane(b0 + (b1 - b0) * kw / KS);
+  const int w1 = __builtin_amdgcn_readfirstlane(b0 + (b1 - b0) * (kw + 1) / KS);
+  // Slices of 64: an odd number of units has a unit of zeros in front.  The KS shares run as many slices as the longest.
+  const int lead = (w1 - w0) & 1, ns = (w1 - w0 + lead) >> 1;
+  const int rounds = ((b1 - b0 + KS - 1) / KS + 1) >> 1;
+  // unit 2 i + half of the share; behind the share's last one (and in front of its first) any unit there is
+  const int units = g.K / 32;
+  auto unit = [&](int i, int half) { return max(min(w0 - lead + 2 * i + half, min(w1, units) - 1), 0); };
+  auto live = [&](int i, int half) { return i < ns && (half == 1 || lead == 0 || i > 0); };
+
+  const int N = g.N, nbk = N / 32, rowb = N / 2;
+  // rows: piece p of a slice is rows 8 (NP gw + p) + lane / 8 of the share's; a row's eight 16-byte chunks are swizzled so
+  // that the 16 rows a fragment read touches at once lie in distinct banks
+  const uint8_t* const xbase = reinterpret_cast<const uint8_t*>(g.A + (int64_t)tl.mbase * g.K);
+  uint8_t* const xs_lds = smem + kw * (2 * SLICE);
+  uint32_t xo[NP];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int row = 8 * (NP * gw + p) + (lane >> 3);
+    xo[p] = (uint32_t)min(row, tl.mlen - 1) * (uint32_t)g.K * 2u;
+  }
+  const buf_rsrc_t xr = buf_rsrc(xbase, -1);
+  u32x4 xs[NP];
+  auto load_x = [&](int i, int p) {
+    const int row = 8 * (NP * gw + p) + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+    // (behind the share's last slice any two units there are: they are written as zeros)
+    const int at = max(min(w0 - lead + 2 * i, units - 2), 0);
+    xs[p] = __builtin_bit_cast(
+        u32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, (int)(xo[p] + (uint32_t)(units > 1 ? c : c & 3) * 16u), at * 64, 0));
+  };
+  auto load_x_first = [&](int p) {
+    const int row = 8 * (NP * gw + p) + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+    xs[p] = *reinterpret_cast<const u32x4*>(xbase + (int64_t)unit(0, c >> 2) * 64 + xo[p] + (c & 3) * 16);
+    if (!live(0, c >> 2)) xs[p] = u32x4{0u, 0u, 0u, 0u};
+  };
+  auto write_x = [&](int i, int p, bool first) {
+    const uint32_t keep = KS == 1 || first || i < ns ? ~0u : 0u;  // (KS == 1: no one reads what is behind the last slice)
+    __asm__ volatile("" ::: "memory");
+    *reinterpret_cast<u32x4*>(xs_lds + (i & 1) * SLICE + (NP * gw + p) * 1024 + lane * 16) = xs[p] & keep;
+    __asm__ volatile("" ::: "memory");
+  };
+  auto frag = [&](int i, int s, int t) {
+    const int row = tw * (32 * TF) + t * 32 + i32;
+    return *reinterpret_cast<const bf16x8*>(xs_lds + (i & 1) * SLICE + row * 128 + (((2 * s + h) ^ ((row >> 1) & 7)) << 4));
+  };
+
+  // weights: lane 32 h + i has columns NF i + [0, NF) of rows 16 s + 8 h + [0, 8); columns past N repeat the last.  Buffer
+  // loads: a lane offset that stays, and a uniform one that moves.
+  const int64_t eb = (int64_t)tl.e * g.Ks;
+  const uint32_t bo = (uint32_t)(8 * h) * (uint32_t)rowb + (uint32_t)min(n0 / NF + i32, N / NF - 1) * (NF / 2u);
+  // scales: lane 32 h + i loads blocks PB / 2 h + [0, PB / 2) of row i, as a word that ends inside the array
+  const uint32_t so = (uint32_t)i32 * (uint32_t)nbk + (uint32_t)(n0 / 32 + PB / 2 * h);
+  const uint32_t slim = (uint32_t)min((int64_t)INT32_MAX, (int64_t)(g.E - tl.e) * g.Ks * nbk - 4);
+  struct __attribute__((packed)) Bytes4 { uint32_t v; };
+  typedef f32x4 __attribute__((may_alias)) f32x4a;
+  uint32_t w[4][8];         // [step][row]
+  uint32_t sw[2], sh[2];    // a unit's word, and how many of its bits are other blocks'
+  float* const sl = scl + wv * SP;
+  auto second = [&](int u) { return u * 32 >= g.Ks; };
+  const uint8_t* const wb = g.B + eb * rowb;
+  const uint8_t* const wb2 = g.B2 + eb * rowb;
+  typedef const __attribute__((address_space(1))) uint8_t gbyte;
+  gbyte* sb = (gbyte*)(g.S + eb * nbk);
+  gbyte* sb2 = (gbyte*)(g.S2 + eb * nbk);
+  __asm__("" : "+s"(sb), "+s"(sb2));  // in registers: not loaded again in the loop
+  auto wsrc = [&](int u) {
+    return buf_rsrc(second(u) ? wb2 : wb, -1);
+  };
+  auto woff = [&](int u, int x) { return (u * 32 + 16 * x - (second(u) ? g.Ks : 0)) * rowb; };
+  auto load_w = [&](int s, int j, buf_rsrc_t b, int off) {
+    if constexpr (NF == 8) w[s][j] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, (int)bo, off + j * rowb, 0);
+    else w[s][j] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, (int)bo, off + j * rowb, 0);
+  };
+  auto load_s = [&](int half, int u) {
+    const uint32_t at = (uint32_t)(u * 32 - (second(u) ? g.Ks : 0)) * (uint32_t)nbk + so, in = min(at, slim);
+    sw[half] = ((const __attribute__((address_space(1))) Bytes4*)((second(u) ? sb2 : sb) + in))->v;
+    sh[half] = min((at - in) * 8u, 31u);
+  };
+  auto put_s = [&](int i, int half) {
+    const uint32_t v = live(i, half) ? sw[half] >> sh[half] : 0x7f7f7f7fu;
+    __asm__ volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < PB / 2; ++j) sl[(PB / 2 * h + j) * SR + i32] = __uint_as_float(((v >> (8 * j)) & 0xffu) << 23);
+    __asm__ volatile("" ::: "memory");
+  };
+  f32x4 sc[2][2];  // the scales of the rows of a unit's two steps
+  auto get_s = [&](int x) {
+    const float* const at = sl + i32 * NF / 32 * SR + 16 * x + 8 * h;
+    sc[x][0] = *reinterpret_cast<const f32x4a*>(at);
+    sc[x][1] = *reinterpret_cast<const f32x4a*>(at + 4);
+    __asm__ volatile("" ::: "memory");
+  };
+
+  f32x16 acc[TF][NF];
+#pragma unroll
+  for (int t = 0; t < TF; ++t)
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[t][j][v] = 0.f;
+  u32x4 f0[NF], f1[NF];  // fragment j: column NF i + j of the wave's, 16 reduction rows
+  bf16x8 x0[TF], x1[TF];
+
+  // Piece c of a step's conversion: rows 2 t, 2 t + 1, columns 2 p, 2 p + 1 become words t of fragments 2 p, 2 p + 1.
+  constexpr int P = NF / 2, PIECES = 4 * P;
+  uint32_t cx[2], cy[2];
+  auto conv_a = [&](auto c_c, const uint32_t(&r)[8], const f32x4(&s)[2]) {
+    constexpr int c = decltype(c_c)::value, t = c / P, p = c % P;
+    cx[c & 1] = mx_pair<p>(r[2 * t], s[t / 2][t % 2 * 2]);
+    cy[c & 1] = mx_pair<p>(r[2 * t + 1], s[t / 2][t % 2 * 2 + 1]);
+  };
+  auto conv_b = [&](auto c_c, u32x4(&f)[NF]) {
+    constexpr int c = decltype(c_c)::value, t = c / P, p = c % P;
+    f[2 * p][t] = __builtin_amdgcn_perm(cy[c & 1], cx[c & 1], 0x05040100u);
+    f[2 * p + 1][t] = __builtin_amdgcn_perm(cy[c & 1], cx[c & 1], 0x07060302u);
+  };
+
+  // Step s of slice i: TF NF MFMAs, and between them the next step's row fragments, its conversion (a piece's transposition a
+  // slot behind its dequantization), each pair of its rows followed by the loads of the same rows of the next slice, and in
+  // the first three the slice's share of refill pieces (slice i + 1 to LDS, i + 2 from memory).
+  auto step = [&](auto s_c, const bf16x8(&cx_)[TF], const u32x4(&cf)[NF], bf16x8(&nx)[TF], u32x4(&nf)[NF], int i) {
+    constexpr int s = decltype(s_c)::value, sn = (s + 1) % 4, x = s & 1, half = s >> 1;
+    const int in = s == 3 ? i + 1 : i;                 // the next step's slice
+    const int un = unit(in + 1, sn >> 1);
+    const buf_rsrc_t bn = wsrc(un);
+    const int wn = woff(un, sn & 1);
+    constexpr int P0 = s == 3 ? 0 : (s * NP + 2) / 3, P1 = s == 3 ? 0 : ((s + 1) * NP + 2) / 3;
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      (([&] {
+         constexpr int t = I / NF, j = I % NF, EVERY = SL / PIECES, c = I / EVERY;
+         acc[t][j] = mfma32x32x16(cx_[t], __builtin_bit_cast(bf16x8, cf[j]), acc[t][j]);
+         __builtin_amdgcn_sched_barrier(0);
+         if constexpr (I < TF) nx[I] = frag(in, sn, I);
+         if constexpr (I % EVERY == 0) {
+           conv_a(std::integral_constant<int, c>{}, w[sn], sc[1 - x]);
+           if constexpr (c > 0) conv_b(std::integral_constant<int, c - 1>{}, nf);
+           if constexpr (c % P == P - 1) {
+             load_w(sn, 2 * (c / P), bn, wn);
+             load_w(sn, 2 * (c / P) + 1, bn, wn);
+           }
+         }
+         if constexpr (x == 0 && I == SL * 5 / 16) put_s(half == 0 ? i : i + 1, 1 - half);
+         if constexpr (x == 0 && I == SL * 7 / 16) load_s(1 - half, unit(half == 0 ? i + 1 : i + 2, 1 - half));
+         if constexpr (I == SL * 11 / 16) get_s(x);
+         constexpr int PE = SL / 8, p = P0 + (I - 5 * PE) / PE;
+         if constexpr (I >= 5 * PE && I % PE == 0 && p < P1) {
+           write_x(i + 1, p, false);
+           load_x(i + 2, p);
+         }
+         __builtin_amdgcn_sched_barrier(0);
+       }()), ...);
+    }(std::make_integer_sequence<int, SL>{});
+    conv_b(std::integral_constant<int, PIECES - 1>{}, nf);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  using S2 = std::integral_constant<int, 2>;
+  using S3 = std::integral_constant<int, 3>;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) load_x_first(p);
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) load_w(s, j, wsrc(unit(0, s >> 1)), woff(unit(0, s >> 1), s & 1));
+  load_s(0, unit(0, 0));
+  load_s(1, unit(0, 1));
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    write_x(0, p, true);
+    load_x(1, p);
+  }
+  put_s(0, 0);
+  get_s(0);
+  get_s(1);
+  load_s(0, unit(1, 0));
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < TF; ++t) x0[t] = frag(0, 0, t);
+  [&]<int... I>(std::integer_sequence<int, I...>) {
+    ((conv_a(std::integral_constant<int, I>{}, w[0], sc[0]), conv_b(std::integral_constant<int, I>{}, f0)), ...);
+  }(std::make_integer_sequence<int, PIECES>{});
+#pragma unroll
+  for (int j = 0; j < 8; ++j) load_w(0, j, wsrc(unit(1, 0)), woff(unit(1, 0), 0));
+  // (a second use of the loaded words, or the loop would carry them as 16 bits, widen them at its top and wait for them there)
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) __asm__ volatile("" ::"v"(w[s][j]));
+  // The pre-activations that the epilogue starts with are on their way while the product runs, the others' while it works on
+  // the ones in front of them: 16 rows each.
+  constexpr bool AHEAD = DACT && KS == 1 && Form::BLOCKS == 1;
+  const int col = n0 + i32 * NF;
+  BkCols<NF> pg[AHEAD ? 2 : 1][16], pu[AHEAD ? 2 : 1][16];
+  auto fetch = [&](int t) {
+    const uint8_t* const x = reinterpret_cast<const uint8_t*>(g.X + (int64_t)tl.mbase * 2 * N);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int r = tw * (32 * TF) + t * 32 + (v & 3) + (v >> 2) * 8 + 4 * h;
+      const uint32_t o = (uint32_t)min(r, tl.mlen - 1) * (uint32_t)N * 4u + (uint32_t)min(col, N - NF) * 2u;
+      pg[t & 1][v] = *reinterpret_cast<const BkCols<NF>*>(x + o);
+      pu[t & 1][v] = *reinterpret_cast<const BkCols<NF>*>(x + (int64_t)N * 2 + o);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if constexpr (AHEAD) fetch(0);
+  for (int i = 0; i < rounds; ++i) {
+    step(S0{}, x0, f0, x1, f1, i);
+    step(S1{}, x1, f1, x0, f0, i);
+    step(S2{}, x0, f0, x1, f1, i);
+    lds_sync();  // every wave's pieces of slice i + 1 are written and its reads of slice i done
+    step(S3{}, x1, f1, x0, f0, i);
+  }
+  __syncthreads();
+
+  // acc[t][j][v]: row 32 t + (v & 3) + 8 (v >> 2) + 4 h, column NF i + j: a lane has NF consecutive columns of a row, and
+  // 32 lanes a whole segment of it.  c = 16 t + v.
+  struct __attribute__((aligned(16))) Cols { float v[NF]; };
+  auto cols = [&](int c) {
+    Cols o;
+#pragma unroll
+    for (int j = 0; j < NF; ++j) o.v[j] = acc[c / 16][j][c % 16];
+    return o;
+  };
+  auto partial = [&](int c, const Cols& o) {
+    reinterpret_cast<Cols*>(part_out)[((tw * WF + fw) * (16 * TF) + c) * 64 + lane] = o;
+  };
+  auto leave = [&](int c, const Cols& o) {
+    const int r = tw * (32 * TF) + (c >> 4) * 32 + (c & 3) + ((c >> 2) & 3) * 8 + 4 * h;
+    if (r < tl.mlen && col < N) bk_store<DACT, NF>(g, tl.mbase + r, col, o.v);
+  };
+  if constexpr (KS == 1) {
+    if (part_out != nullptr) {
+#pragma unroll
+      for (int c = 0; c < 16 * TF; ++c) partial(c, cols(c));
+      return;
+    }
+#pragma unroll
+    for (int t = 0; t < TF; ++t) {
+      if constexpr (AHEAD) {
+        if (t + 1 < TF) fetch(t + 1);
+      }
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int r = tw * (32 * TF) + t * 32 + (v & 3) + (v >> 2) * 8 + 4 * h;
+        if (r >= tl.mlen || col >= N) continue;
+        const Cols o = cols(16 * t + v);
+        if constexpr (AHEAD) bk_put<NF>(g, tl.mbase + r, col, o.v, pg[t & 1][v], pu[t & 1][v]);
+        else bk_store<DACT, NF>(g, tl.mbase + r, col, o.v);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+    // The KS waves of the same rows and columns meet in LDS, each for a KS-th of the c, in rounds of 32 values a lane.
+    constexpr int PC = 16 * TF / KS, Q = 32 / NF;
+    Cols* const rd = reinterpret_cast<Cols*>(smem) + (wv % (WT * WF)) * (KS * (KS - 1) * Q * 64) + lane;
+#pragma unroll
+    for (int q0 = 0; q0 < PC; q0 += Q) {
+      if (q0 > 0) __syncthreads();
+#pragma unroll
+      for (int o = 0; o < KS; ++o) {  // owner
+        if (o == kw) continue;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) rd[((o * (KS - 1) + (kw < o ? kw : kw - 1)) * Q + q) * 64] = cols(o * PC + q0 + q);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int o = 0; o < KS; ++o) {
+        if (o != kw) continue;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int c = o * PC + q0 + q;
+          Cols sum;
+#pragma unroll
+          for (int x = 0; x < KS; ++x) {  // in the order of the reduction
+            const Cols y = x == o ? cols(c) : rd[((o * (KS - 1) + (x < o ? x : x - 1)) * Q + q) * 64];
+#pragma unroll
+            for (int j = 0; j < NF; ++j) sum.v[j] = x == 0 ? y.v[j] : sum.v[j] + y.v[j];
+          }
+          if (part_out != nullptr) partial(c, sum);
+          else leave(c, sum);
+        }
+      }
+    }
+  }
+}
+
+// The split tiles' sums: blockIdx.x = (XCD, split tile), blockIdx.y an eighth of the tile's (wave, c) pairs.
+template <class Form, bool DACT>
+__global__ __launch_bounds__(256) void k_mx_back_reduce(BkArgs g) {
+  constexpr int NF = Form::NF, BM = Form::BM, PAIRS = BM * kBkCols / (64 * NF), WC = 16 * Form::TF;
+  const int tid = threadIdx.x, lane = tid & 63;
+  constexpr int RES = 32 * Form::BLOCKS;
+  const int xcd = (int)blockIdx.x / RES, t = (int)blockIdx.x % RES;
+  const int total = g.tile_off[g.E] * g.Tn, chunk = (total + 7) >> 3;
+  const MxSplit sp = bk_split<Form>(g, min(chunk, total - xcd * chunk));
+  if (sp.parts == 1 || t >= sp.rest) return;
+  const BkTile tl = bk_tile<BM>(g, xcd * chunk + sp.full + t, lane);
+  struct __attribute__((aligned(16))) Cols { float v[NF]; };
+  const Cols* const src = reinterpret_cast<const Cols*>(g.part + (int64_t)(xcd * g.npart + t * sp.parts) * (BM * kBkCols));
+  for (int wc = (int)blockIdx.y * (PAIRS / 8) + (tid >> 6); wc < (int)(blockIdx.y + 1) * (PAIRS / 8); wc += 4) {
+    const int c = wc % WC, wave = wc / WC, tw = wave / Form::WF, fw = wave % Form::WF;
+    const int r = tw * (2 * WC) + (c >> 4) * 32 + (c & 3) + ((c >> 2) & 3) * 8 + 4 * (lane >> 5);
+    const int col = tl.nt * kBkCols + fw * (32 * NF) + (lane & 31) * NF;
+    if (r >= tl.mlen || col >= g.N) continue;
+    Cols sum = src[wc * 64 + lane];
+    for (int p = 1; p < sp.parts; ++p) {
+      const Cols y = src[(int64_t)p * (PAIRS * 64) + wc * 64 + lane];
+#pragma unroll
+      for (int j = 0; j < NF; ++j) sum.v[j] += y.v[j];
+    }
+    bk_store<DACT, NF>(g, tl.mbase + r, col, sum.v);
+  }
+}
+
+// Rows of a product's tile, by the rows an expert has on average and by the tiles there are (N: its output columns).  Both
+// products, us, by rows an expert (routed; 64 rows | 128 | 256 for dxp alone):
+//   E 8,   H 4096, F 14336   16: 252 | 366 | 524   64: 399 | 393 | 542   256: 920 | 942 | 993   2048: 7323 | 5742 | 5380
+//   E 128, H 2048, F 768     16: 161 | 175 | 255   64: 244 | 196 | 274   256: 633 | 454 | 502   2048: 4358 | 2787 | 2715
+//   E 8,   H 1024, F 4096    16: 57 | 69 | 83      64: 68 | 83 | 103     256: 137 | 116 | 126   2048: 825 | 533 | 541
+// 256 rows for the product with Wd as well cost 4% at 2048 rows: one block a CU leaves nothing to run under its epilogue.
+int bk_rows(bool dact, int64_t R, int64_t N, int64_t F, int64_t E) {
+  if (R < 64 * E || std::max(R / 128, E) * ((F + 255) / 256) < 256) return 64;
+  return !dact && R >= 1024 * E && R / 256 * ((N + 255) / 256) >= 512 ? 256 : 128;
+}
+int bk_parts(int bm, int64_t R, int64_t E, int64_t N) {
+  const int64_t tiles = ((R + bm - 1) / bm + E) * ((N + kBkCols - 1) / kBkCols);
+  return (int)std::min<int64_t>(bm == 128 ? 128 : 64, 8 * ((tiles + 7) / 8));
+}
+size_t bk_part_bytes(int bm, int64_t R, int64_t E, int64_t N) {
+  return (size_t)8 * bk_parts(bm, R, E, N) * bm * kBkCols * sizeof(float);
+}
+
+template <class Form, bool DACT>
+int launch_back_as(const char* name, hipStream_t s, BkArgs a, int64_t E, int64_t R) {
+  a.E = (int)E;
+  a.Tn = cdiv(a.N, kBkCols);
+  const int64_t blocks = ((R + Form::BM - 1) / Form::BM + E) * a.Tn;
+  if (blocks > INT32_MAX / 2) return fail_arg("%s: too many tiles", name);
+  MOE_LAUNCH(name, (k_mx_back<Form, DACT>), dim3((unsigned)((blocks + 7) / 8 * 8 + 8 * a.npart)), dim3(256), 0, s, a);
+  MOE_LAUNCH("k_mx_back_reduce", (k_mx_back_reduce<Form, DACT>), dim3(8 * 32 * Form::BLOCKS, 8), dim3(256), 0, s, a);
+  return check_launch(name);
+}
+template <bool DACT>
+int launch_back(const char* name, hipStream_t s, const BkArgs& a, int64_t E, int64_t R, int bm) {
+  return bm == 256   ? launch_back_as<BkForm<4, 4, 2, 2, 1>, DACT>(name, s, a, E, R)
+         : bm == 128 ? launch_back_as<BkForm<2, 4, 2, 2, 1>, DACT>(name, s, a, E, R)
+                     : launch_back_as<BkForm<2, 8, 1, 1, 4>, DACT>(name, s, a, E, R);
+}
+}  // namespace
+}  // namespace moe
+
 extern "C" size_t moe_swiglu_bwd_mxfp4_workspace(int64_t R, int64_t H, int64_t F, int64_t E) {
   if (R <= 0 || H <= 0 || F <= 0 || E <= 0) return 0;
-  return moe_swiglu_workspace(E) + moe_swiglu_split_workspace(R, H, F, E) + al256x((size_t)R * F * 4);
+  return moe_swiglu_workspace(E) + al256x((size_t)R * F * 4) +
+         std::max(bk_part_bytes(bk_rows(true, R, F, F, E), R, E, F), bk_part_bytes(bk_rows(false, R, H, F, E), R, E, H));
 }
 
 extern "C" int moe_swiglu_bwd_mxfp4(const void* dy, const void* hgu, const void* wg_q, const void* sg, const void* wu_q,
@@ -773,9 +1278,36 @@ extern "C" int moe_swiglu_bwd_mxfp4(const void* dy, const void* hgu, const void*
   if (ws_bytes < moe_swiglu_bwd_mxfp4_workspace(R, H, F, E) || !workspace || !al16x(workspace))
     return set_error("moe_swiglu_bwd_mxfp4: workspace"), MOE_EWORKSPACE;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const size_t gemm_ws = moe_swiglu_workspace(E) + moe_swiglu_split_workspace(R, H, F, E);
-  void* dh = static_cast<char*>(workspace) + gemm_ws;
-  if (int rc = swiglu_tiles(offsets, E, kGemmRows, workspace, s)) return rc;
-  if (int rc = swiglu_dact_mxfp4(dy, hgu, wd_q, sd, offsets, R, H, F, E, dh, workspace, s)) return rc;
-  return swiglu_dxp_mxfp4(dh, wg_q, sg, wu_q, su, offsets, R, H, F, E, dxp, workspace, gemm_ws, s);
+  const int da = bk_rows(true, R, F, F, E), dx = bk_rows(false, R, H, F, E);
+  uint16_t* const dh = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + moe_swiglu_workspace(E));
+  if (int rc = swiglu_tiles(offsets, E, da, workspace, s)) return rc;
+  BkArgs a{};
+  a.offsets = offsets;
+  a.tile_off = static_cast<const int*>(workspace);
+  a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(dh) + al256x((size_t)R * F * 4));
+  BkArgs b = a;
+  // dh = epilogue(dy . Wd): Wd's rows are the reduction
+  a.A = static_cast<const uint16_t*>(dy);
+  a.B = a.B2 = static_cast<const uint8_t*>(wd_q);
+  a.S = a.S2 = static_cast<const uint8_t*>(sd);
+  a.C = dh;
+  a.X = static_cast<const uint16_t*>(hgu);
+  a.K = a.Ks = (int)H;
+  a.N = (int)F;
+  a.npart = bk_parts(da, R, E, F);
+  if (int rc = launch_back<true>("k_mx_back_dact", s, a, E, R, da)) return rc;
+  // dxp = dh . [Wg ; Wu]
+  if (dx != da)
+    if (int rc = swiglu_tiles(offsets, E, dx, workspace, s)) return rc;
+  b.A = dh;
+  b.B = static_cast<const uint8_t*>(wg_q);
+  b.S = static_cast<const uint8_t*>(sg);
+  b.B2 = static_cast<const uint8_t*>(wu_q);
+  b.S2 = static_cast<const uint8_t*>(su);
+  b.C = static_cast<uint16_t*>(dxp);
+  b.K = (int)(2 * F);
+  b.Ks = (int)F;
+  b.N = (int)H;
+  b.npart = bk_parts(dx, R, E, H);
+  return launch_back<false>("k_mx_back_dxp", s, b, E, R, dx);
 }

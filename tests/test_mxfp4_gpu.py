@@ -129,6 +129,15 @@ def test_backward(H, F, counts):
     _inside(dx[:used], rx, tx, "dxp")
 
 
+@pytest.mark.parametrize("H,F,counts", [
+    (160, 2080, [3000, 0, 1201]),            # tiles of 128 rows; reductions and columns of odd numbers of blocks
+    (96, 544, [64, 70, 58] * 44),            # ... of many experts
+    (8224, 2016, [4133, 101]),               # of 256 rows for dxp
+], ids=lambda v: str(v)[:24])
+def test_backward_of_many_rows(H, F, counts):
+    test_backward(H, F, counts)
+
+
 def test_rows_past_the_last_segment_are_left_alone():
     """Through the C ABI, whose caller owns the outputs."""
     H, F, counts = 128, 96, [3, 0, 20]
