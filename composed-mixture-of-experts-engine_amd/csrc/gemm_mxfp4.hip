@@ -9,11 +9,21 @@
 // weights.
 //
 // Few rows (k_mx_small): the weights' stream bounds both products.  A block owns 16 NF weight rows of one expert (gate/up
-// product: 8 NF gate and the matching up rows) and its NW waves each take every NW-th 128-column chunk of them, straight
-// from HBM into MFMA fragments: a lane's 16-byte load is one 32-element block of one row, with its one scale byte, and
-// feeds four v_mfma_f32_16x16x32_bf16, 8 elements each.  The k slot that a value lands in is free as long as both operands
-// agree: lane 16 q + r holds block 4 c + q of row r, and takes elements 128 c + 32 q + 8 s + [0, 8) of token row r for the
-// s-th of the four.  The waves' partial sums meet in LDS in wave order.
+// product: 8 NF gate and the matching up rows) and its NW waves each take every NW-th unit of 256 columns of them.  Lane
+// 16 q + r of v_mfma_f32_16x16x32_bf16 wants row r's block 4 j + q, but sixteen rows' blocks side by side in a load are 64
+// cache accesses of 16 bytes, about one a clock, and the vector cache then bounds the kernel (measured: 0.9 of one a clock).  So
+// eight lanes fetch a row's 128-byte line, two units ahead, and the unit passes through the wave's own LDS, with no barrier.
+// The k slot that a value lands in is free as long as both operands agree: a lane's block feeds four MFMAs, 8 elements each,
+// and takes elements 8 s + [0, 8) of the same 32 of its token row for the s-th.  The waves' partial sums meet in LDS in wave
+// order.  16 tokens, two experts each, E 8, H 4096, F 14336: 92 us for the gate/up product (500 MB, 5.4 TB/s) and 52 for the
+// down projection (4.8 TB/s), where loads in the lanes' own order took 116 and 60.
+//
+// Many rows (k_mx_tile): 64, 128 or 256 rows of an expert by 256 weight rows.  The rows go through LDS in 64-wide slices, two
+// at a time; a wave has weight rows of its own, dequantizes them between registers and feeds v_mfma_f32_32x32x16_bf16, half a
+// conversion to 2, 4 or 8 row fragments.  64 rows read a weight so rarely that the vector cache bounds them too: their weights
+// come by whole lines through the wave's LDS (1002 rows at the sizes above, tiles of 64 rows: 600 -> 500 us), and LDS bounds
+// them after that (7/8 of its rate).  128 and 256 rows load in the lanes' own order, whose accesses the matrix instructions
+// cover; what bounds them is the matrix instructions' power (16384 rows: 4.76 ms, 5.77 TFLOP, 1210 TFLOP/s at 1.6 GHz).
 #include <algorithm>
 #include <utility>
 
@@ -54,56 +64,73 @@ __device__ __forceinline__ bf16x8 mx_frag(uint32_t w, float sc) {
 
 struct __attribute__((packed)) MxBytes8 { uint32_t v[2]; };
 
+// A wave's LDS: a unit of the block's 16 NF weight rows (128 bytes of each, swizzled) and their eight scale bytes.
+constexpr int mx_stage(int NF) { return NF * 16 * 136; }
+
 // One pass: rows [row0, row0 + min(rows, 16 MT)) of the segment against the block's 16 NF weight rows.
 template <bool GU, int NF, int NW, int MT>
-__device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, int rows, int n0, uint32_t tile, float* red) {
+__device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, int rows, int n0, uint32_t tile, uint8_t* stage,
+                                        float* red) {
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int nb = g.K / 32;          // blocks of a row
   constexpr int RP = NF * 16 + 4;   // floats a row of the partial sums
+  constexpr int NP = NF * 2;        // pieces of a unit: 8 weight rows each, GU: the first half gate rows, the others up rows
   const int64_t eb = (int64_t)e * g.N * nb;  // blocks before this expert
   const uint8_t* const wb[2] = {g.B + eb * 16, (GU ? g.B2 : g.B) + eb * 16};
   const uint8_t* const sb[2] = {g.S + eb, (GU ? g.S2 : g.S) + eb};
-  // fragment f of the 16 NF weight rows: GU: the first NF / 2 gate rows, the others up rows; rows past N repeat the last
-  uint32_t wo[NF], ao[MT];  // the row's first block, and the row's first byte
+  // the weight row of row x of the block's; rows past N repeat the last
+  auto wrow = [&](int x) { return (uint32_t)min(n0 + (GU ? x % (NF * 8) : x), g.N - 1) * (uint32_t)nb; };
+  uint32_t wo[NP], ao[MT];  // the row's first block, and the token row's first byte
 #pragma unroll
-  for (int f = 0; f < NF; ++f)
-    wo[f] = (uint32_t)min(n0 + (GU ? f % (NF / 2) : f) * 16 + r, g.N - 1) * (uint32_t)nb;
+  for (int p = 0; p < NP; ++p) wo[p] = wrow(p * 8 + (lane >> 3));
+  const uint32_t so = wrow(lane % (NF * 16));
+  const bool sup = GU && lane % (NF * 16) >= NF * 8;
 #pragma unroll
   for (int m = 0; m < MT; ++m) ao[m] = (uint32_t)min(m * 16 + r, rows - 1) * (uint32_t)g.K * 2u;
   const uint8_t* const arow = reinterpret_cast<const uint8_t*>(g.A + row0 * g.K);
 
-  // a unit: 256 columns, one 128-byte line of 4-bit values of each weight row, as two halves of four blocks
-  u32x4 w[2][NF][2], a[MT][2][4];
-  uint32_t sc[2][NF][2];
+  // A unit: 256 columns, one 128-byte line of 4-bit values of each weight row.  Eight lanes fetch a line; the matrix
+  // instruction wants a row's blocks four lanes of sixteen apart, so the unit passes through the wave's own LDS.
+  constexpr int AB = MT == 1 ? 2 : 1;  // units of token rows in flight or in use
+  u32x4 w[2][NP], a[AB][MT][2][4];
+  uint32_t sc[2][2];
   auto load_w = [&](int b, int u) {
+    const int c = lane & 7;
     if (u * 8 + 8 <= nb) {
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const int o = GU && f >= NF / 2;
+      for (int p = 0; p < NP; ++p)
+        w[b][p] = *reinterpret_cast<const u32x4*>(wb[GU && p >= NF] + u * 128 + (wo[p] + (uint32_t)c) * 16u);
+      const MxBytes8 s = *reinterpret_cast<const MxBytes8*>((sup ? sb[1] : sb[0]) + u * 8 + so);
+      sc[b][0] = s.v[0];
+      sc[b][1] = s.v[1];
+    } else {  // the row's last, partial unit: blocks past its end have any values and a scale of 1 (their tokens are zeros)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          w[b][f][j] = *reinterpret_cast<const u32x4*>(wb[o] + u * 128 + j * 64 + (wo[f] + (uint32_t)q) * 16u);
-        const MxBytes8 s = *reinterpret_cast<const MxBytes8*>(sb[o] + u * 8 + wo[f]);
-        sc[b][f][0] = s.v[0];
-        sc[b][f][1] = s.v[1];
-      }
-    } else {  // the row's last, partial unit: blocks past its end have any values and a finite scale (their tokens are zeros)
+      for (int p = 0; p < NP; ++p)
+        w[b][p] = *reinterpret_cast<const u32x4*>(wb[GU && p >= NF] + (wo[p] + (uint32_t)min(u * 8 + c, nb - 1)) * 16u);
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const int o = GU && f >= NF / 2;
+      for (int j = 0; j < 2; ++j) {
+        sc[b][j] = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int blk = u * 8 + j * 4 + q;
-          const uint32_t at = wo[f] + (uint32_t)min(blk, nb - 1);
-          w[b][f][j] = *reinterpret_cast<const u32x4*>(wb[o] + at * 16u);
-          const uint32_t s = sb[o][at];
-          sc[b][f][j] = (blk < nb ? s : 127u) << (8 * q);
+        for (int k = 0; k < 4; ++k) {
+          const int blk = u * 8 + j * 4 + k;
+          const uint32_t s = (sup ? sb[1] : sb[0])[so + (uint32_t)min(blk, nb - 1)];
+          sc[b][j] |= (blk < nb ? s : 127u) << (8 * k);
         }
       }
     }
   };
-  auto load_a = [&](int u) {
+  auto put_w = [&](int b) {
+    __asm__ volatile("" ::: "memory");
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int row = p * 8 + (lane >> 3);
+      *reinterpret_cast<u32x4*>(stage + row * 128 + (((lane & 7) ^ ((row >> 1) & 7)) << 4)) = w[b][p];
+    }
+    if (lane < NF * 16) *reinterpret_cast<uint2*>(stage + NF * 16 * 128 + lane * 8) = uint2{sc[b][0], sc[b][1]};
+    __asm__ volatile("" ::: "memory");
+  };
+  auto load_a = [&](int b, int u) {
     if (u * 8 + 8 <= nb) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -111,7 +138,7 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int s = 0; s < 4; ++s)
-            a[m][j][s] = *reinterpret_cast<const u32x4*>(arow + u * 512 + j * 256 + s * 16 + (ao[m] + (uint32_t)q * 64u));
+            a[b][m][j][s] = *reinterpret_cast<const u32x4*>(arow + u * 512 + j * 256 + s * 16 + (ao[m] + (uint32_t)q * 64u));
     } else {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -123,7 +150,7 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const u32x4 v = *reinterpret_cast<const u32x4*>(arow + (ao[m] + (in ? (uint32_t)blk * 64u : 0u) + s * 16u));
-            a[m][j][s] = in ? v : z;
+            a[b][m][j][s] = in ? v : z;
           }
       }
     }
@@ -134,18 +161,26 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[f][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto mma = [&](int b) {
+    uint2 sv[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) sv[f] = *reinterpret_cast<const uint2*>(stage + NF * 16 * 128 + (f * 16 + r) * 8);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
+      u32x4 wv4[NF];
       float sf[NF];
 #pragma unroll
-      for (int f = 0; f < NF; ++f) sf[f] = __uint_as_float(((sc[b][f][j] >> (8 * q)) & 0xffu) << 23);
+      for (int f = 0; f < NF; ++f) {
+        const int row = f * 16 + r;
+        wv4[f] = *reinterpret_cast<const u32x4*>(stage + row * 128 + (((4 * j + q) ^ ((row >> 1) & 7)) << 4));
+        sf[f] = __uint_as_float((((j ? sv[f].y : sv[f].x) >> (8 * q)) & 0xffu) << 23);
+      }
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-          const bf16x8 wf = mx_frag(w[b][f][j][s], sf[f]);
+          const bf16x8 wf = mx_frag(wv4[f][s], sf[f]);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) acc[f][m] = mfma16x16x32(wf, __builtin_bit_cast(bf16x8, a[m][j][s]), acc[f][m]);
+          for (int m = 0; m < MT; ++m) acc[f][m] = mfma16x16x32(wf, __builtin_bit_cast(bf16x8, a[b][m][j][s]), acc[f][m]);
         }
     }
   };
@@ -156,18 +191,33 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
     const int u = i + start;
     return u < nu ? u : u - nu;
   };
-  int u = wv;
-  if (u < nu) {
-    load_w(0, at(u));
-    for (;;) {
-      load_a(at(u));
-      if (u + NW < nu) load_w(1, at(u + NW));
-      mma(0);
+  if (wv < nu) {
+    load_w(0, at(wv));
+    load_a(0, at(wv));
+    if (wv + NW < nu) {
+      load_w(1, at(wv + NW));
+      if constexpr (AB == 2) load_a(1, at(wv + NW));
+    }
+    auto unit = [&](auto b_c, int u) {
+      constexpr int b = decltype(b_c)::value;
+      put_w(b);
+      if constexpr (AB == 2) {
+        if (u + 2 * NW < nu) load_w(b, at(u + 2 * NW));
+        mma(b);
+        if (u + 2 * NW < nu) load_a(b, at(u + 2 * NW));
+      } else {
+        __builtin_amdgcn_sched_barrier(0);
+        mma(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (u + NW < nu) load_a(0, at(u + NW));
+        if (u + 2 * NW < nu) load_w(b, at(u + 2 * NW));
+      }
+    };
+    for (int u = wv;;) {
+      unit(std::integral_constant<int, 0>{}, u);
       u += NW;
       if (u >= nu) break;
-      load_a(at(u));
-      if (u + NW < nu) load_w(0, at(u + NW));
-      mma(1);
+      unit(std::integral_constant<int, 1>{}, u);
       u += NW;
       if (u >= nu) break;
     }
@@ -217,8 +267,10 @@ __device__ __forceinline__ void mx_pass(const MxArgs& g, int e, int64_t row0, in
 constexpr int kMxPass = 32;  // rows of a pass
 
 template <bool GU, int NF, int NW>
-__global__ __launch_bounds__(NW * 64, 8 / NW) void k_mx_small(MxArgs g) {
+__global__ __launch_bounds__(NW * 64, 2) void k_mx_small(MxArgs g) {
   __shared__ __attribute__((aligned(16))) float red[NW * 16 * (NF * 16 + 4)];
+  __shared__ __attribute__((aligned(16))) uint8_t stages[NW * mx_stage(NF)];
+  uint8_t* const stage = stages + (threadIdx.x >> 6) * mx_stage(NF);
   const int slot = (int)(blockIdx.x / g.Tn), nt = (int)(blockIdx.x % g.Tn);
   int e = slot, pass = 0;
   if (slot >= g.E) {  // the (slot - E)-th of the passes past the experts' first ones
@@ -250,16 +302,18 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void k_mx_small(MxArgs g) {
   if (m0 >= hi) return;
   const int n0 = nt * NF * (GU ? 8 : 16);
   const uint32_t tile = (uint32_t)(e * g.Tn + nt);
-  if (hi - m0 > 16) mx_pass<GU, NF, NW, 2>(g, e, m0, min(kMxPass, hi - m0), n0, tile, red);
-  else mx_pass<GU, NF, NW, 1>(g, e, m0, hi - m0, n0, tile, red);
+  if (hi - m0 > 16) mx_pass<GU, NF, NW, 2>(g, e, m0, min(kMxPass, hi - m0), n0, tile, stage, red);
+  else mx_pass<GU, NF, NW, 1>(g, e, m0, hi - m0, n0, tile, stage, red);
 }
 
-// 64 weight rows and four waves a block; where that leaves fewer than 512 blocks with rows, 32 rows and eight waves.
+// 64 weight rows and four waves a block; where that leaves fewer than 256 blocks with rows, 32 rows and eight waves.  Down
+// projection, us, (4, 4) | (2, 8): one token at H 4096, F 14336 (128 blocks) 20 | 14; 16 tokens (512 blocks) 52 | 55; 64 rows of
+// E 128, H 2048, F 768 (2048 blocks, three units a row) 20 | 43.
 template <bool GU>
 int launch_small(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
   a.E = (int)E;
   const int64_t slots = E + R / kMxPass;  // every expert's first pass, and as many more as R rows can need
-  const bool wide = cdiv(a.N, GU ? 32 : 64) * std::min(E, R) >= 512;
+  const bool wide = cdiv(a.N, GU ? 32 : 64) * std::min(E, R) >= 256;
   a.Tn = cdiv(a.N, (GU ? 16 : 32) * (wide ? 2 : 1));
   if (a.Tn * slots > INT32_MAX) return fail_arg("%s: too many tiles", name);
   if (wide) MOE_LAUNCH(name, (k_mx_small<GU, 4, 4>), dim3((unsigned)(a.Tn * slots)), dim3(256), 0, s, a);
@@ -325,7 +379,10 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
   constexpr int WC = CW / 4;                        // ... and of a wave
   constexpr int SLICE = BM * 128;                   // LDS bytes of a 64-wide slice of the rows
   constexpr int CP = BN + 8;                        // pitch of the output tile (bf16)
-  constexpr int SMEM = 2 * SLICE > BM * CP * 2 ? 2 * SLICE : BM * CP * 2;
+  constexpr bool VIA = BM == 64;                     // weights by whole 128-byte lines and through the wave's own LDS
+  constexpr int WST = VIA ? mx_stage(4) : 0;        // ... a round of 64 rows and their scales
+  static_assert(!VIA || (MW == 2 && G == 4));
+  constexpr int SMEM = std::max(2 * SLICE + 4 * WST, BM * CP * 2);
   __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i32 = lane & 31, h = lane >> 5;
@@ -432,12 +489,74 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
       sw[l / SJ][m] = l % SJ == 0 ? s : sw[l / SJ][m] | s;
     }
   };
+  // VIA: a round of four slices of the wave's 64 rows.  Eight lanes fetch a row's 128 bytes (piece p: rows 8 p + lane / 8), a
+  // lane the scales of row `lane`; a row's chunks are swizzled in LDS as the token rows' are.
+  uint8_t* const wst = smem + 2 * SLICE + wv * WST;
+  u32x4(&wr)[G * MW] = reinterpret_cast<u32x4(&)[G * MW]>(w);
+  uint32_t sr[2];
+  // (N % 32 == 0: a fragment's 32 rows lie inside the matrix or past it; those past it repeat the last ones)
+  auto row0 = [&](int m) { return min(n0 + wv * WC + (GU ? 0 : m * 32), g.N - 32); };
+  auto piece = [&](int p) { return wbase(p / 4) + (int64_t)(row0(p / 4) + p % 4 * 8) * nb * 16; };
+  const uint32_t wp = (uint32_t)(lane >> 3) * (uint32_t)nb;
+  const uint32_t sp = (uint32_t)(lane < 32 ? row0(0) : row0(MW - 1)) * (uint32_t)nb + (uint32_t)i32 * (uint32_t)nb;
+  const uint8_t* const srow = lane < 32 ? sbase(0) : sbase(MW - 1);
+  auto load_round = [&](int i) {  // slices [i, i + 4); those behind the last one again
+    const int at = min(i + ((lane & 7) >> 1), ns - 1) - lead;
+    const uint32_t o = (wp + (uint32_t)(2 * at + (lane & 1))) * 16u;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) wr[p] = *reinterpret_cast<const u32x4*>(piece(p) + o);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      sr[k] = reinterpret_cast<const Bytes4*>(srow + (int64_t)(min(i + 2 * k, ns - 2) - lead) * 2 + sp)->v;
+  };
+  auto load_round_first = [&] {
+    auto block = [&](int l, int hh) {
+      return (uint32_t)(l >= ns || (l < lead && hh) ? 0 : l >= lead ? 2 * (l - lead) + hh : nb - 1);
+    };
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+      wr[p] = *reinterpret_cast<const u32x4*>(piece(p) + (wp + block((lane & 7) >> 1, lane & 1)) * 16u);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      sr[k] = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int l = 2 * k + b / 2, hh = b & 1;
+        const uint32_t v = srow[sp + block(l, hh)];
+        sr[k] |= (l < lead && hh ? 127u : v) << (8 * b);
+      }
+    }
+  };
+  auto put_round = [&](int i) {
+    __asm__ volatile("" ::: "memory");
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int row = p * 8 + (lane >> 3);
+      *reinterpret_cast<u32x4*>(wst + row * 128 + (((lane & 7) ^ ((row >> 1) & 7)) << 4)) = wr[p];
+    }
+    // (the last slice alone comes with the one in front of it)
+    const uint32_t s0 = i > 0 && i == ns - 1 ? sr[0] >> 16 : sr[0], s1 = i > 0 && i + 2 == ns - 1 ? sr[1] >> 16 : sr[1];
+    *reinterpret_cast<uint2*>(wst + 64 * 128 + lane * 8) = uint2{s0, s1};
+    __asm__ volatile("" ::: "memory");
+  };
+  u32x4 wl[MW];     // the slice in use
+  uint32_t sl[MW];  // its scale bytes
+  auto take = [&](auto l_c) {  // slice l of the round in LDS
+    constexpr int l = decltype(l_c)::value;
+#pragma unroll
+    for (int m = 0; m < MW; ++m) {
+      const int row = m * 32 + i32;
+      wl[m] = *reinterpret_cast<const u32x4*>(wst + row * 128 + (((2 * l + h) ^ ((row >> 1) & 7)) << 4));
+      sl[m] = wst[64 * 128 + row * 8 + 2 * l + h];
+    }
+    __asm__ volatile("" ::: "memory");
+  };
   float sf[MW];  // the scales of the slice whose weights are used next (finite behind the last one)
   auto scales = [&](int l, int i) {
     const int up = 16 * (l % SJ) + (SJ == 2 && l % 2 == 0 && i >= G && i == ns - 1 ? 16 : 0);
 #pragma unroll
     for (int m = 0; m < MW; ++m) {
-      const uint32_t b = ((sw[l / SJ][m] >> (up + 8 * h)) & 0xffu) << 23;
+      const uint32_t b = VIA ? sl[m] << 23 : ((sw[l / SJ][m] >> (up + 8 * h)) & 0xffu) << 23;
       sf[m] = __uint_as_float(EVEN || i < ns ? b : 0x3f800000u);
     }
   };
@@ -471,7 +590,8 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
          if constexpr (I < NB) nb_[I] = frag(ni, NS, I);
          constexpr int C0 = I * CV / SLOTS, C1 = (I + 1) * CV / SLOTS;
          [&]<int... C>(std::integer_sequence<int, C...>) {
-           ((nw[(C0 + C) / 4][(C0 + C) % 4] = mx_pair<(C0 + C) % 4>(w[NL][(C0 + C) / 4][NS], sf[(C0 + C) / 4])), ...);
+           ((nw[(C0 + C) / 4][(C0 + C) % 4] = mx_pair<(C0 + C) % 4>(VIA ? wl[(C0 + C) / 4][NS] : w[NL][(C0 + C) / 4][NS],
+                                                                     sf[(C0 + C) / 4])), ...);
          }(std::make_integer_sequence<int, C1 - C0>{});
          constexpr int p = PLO + I - NB;
          if constexpr (I >= NB && p < PHI) {
@@ -496,11 +616,17 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
     using NJ = std::integral_constant<int, (J + 1) % G>;
     using X = std::integral_constant<int, (J + 1) % XD>;
     step(I0{}, IP1{}, I1{}, fb0, wf0, fb1, wf1, i, j_c, X{}, i);
+    if constexpr (VIA && J == G - 1) put_round(i + 1);
     step(IP1{}, IP2{}, I2{}, fb1, wf1, fb0, wf0, i, j_c, X{}, i);
     step(IP2{}, IPN{}, I3{}, fb0, wf0, fb1, wf1, i, j_c, X{}, i);
-    load_w(J, i + G);
-    if constexpr (SJ == 1) load_s(J, i + G);
-    else if constexpr (J % 2 == 1) load_s(J / 2, i - 1 + G);
+    if constexpr (VIA) {
+      if constexpr (J == G - 1) load_round(i + 1 + G);
+      take(NJ{});
+    } else {
+      load_w(J, i + G);
+      if constexpr (SJ == 1) load_s(J, i + G);
+      else if constexpr (J % 2 == 1) load_s(J / 2, i - 1 + G);
+    }
     lds_sync();  // every wave's pieces of slice i + 1 are written and its reads of slice i done
     scales(NJ::value, i + 1);
     __builtin_amdgcn_sched_barrier(0);
@@ -508,20 +634,29 @@ __global__ __launch_bounds__(256, BM * MW >= 512 ? 1 : 2) void k_mx_tile(MxArgs 
   };
 #pragma unroll
   for (int p = 0; p < NB; ++p) load_x_first(p);
+  if constexpr (VIA) {
+    load_round_first();
+  } else {
 #pragma unroll
-  for (int l = 0; l < G; ++l) load_w_first(l);
+    for (int l = 0; l < G; ++l) load_w_first(l);
+  }
 #pragma unroll
   for (int p = 0; p < NB; ++p) write_x(0, 0, p);
 #pragma unroll
   for (int x = 1; x <= XD; ++x)
 #pragma unroll
     for (int p = 0; p < NB; ++p) load_x(x % XD, x, p);
+  if constexpr (VIA) {
+    put_round(0);
+    load_round(G);
+    take(I0{});
+  }
   __syncthreads();
   scales(0, 0);
 #pragma unroll
   for (int n = 0; n < NB; ++n) fb0[n] = frag(0, 0, n);
 #pragma unroll
-  for (int m = 0; m < MW; ++m) wf0[m] = __builtin_bit_cast(u32x4, mx_frag(w[0][m][0], sf[m]));
+  for (int m = 0; m < MW; ++m) wf0[m] = __builtin_bit_cast(u32x4, mx_frag(VIA ? wl[m][0] : w[0][m][0], sf[m]));
   for (int i = 0; i < ns; i += G) {
     [&]<int... J>(std::integer_sequence<int, J...>) {
       (slice(std::integral_constant<int, J>{}, i + J), ...);
@@ -657,17 +792,19 @@ int launch_tile(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R)
 // product's tiles, which have to fill the chip: 512 blocks of 64 or 128 rows are resident at once, 256 of 256 rows.  The tiled
 // loop takes reductions of 128 and more, and with 256 rows only multiples of 128.  Both products, us, by rows an expert
 // (routed; few-row form | 64 | 128 | 256 rows):
-//   E 8,   H 4096, F 14336   16: 224 | 326 | 381 | 616   32: 375 | 336 | 393 | 620   64: 628 | 440 | 405 | 631   128: - | 597 | 536 | 648
-//   E 128, H 2048, F 768     16: 106 | 114 | 145 | 244   32: 170 | 122 | 152 | 247   64: 303 | 171 | 160 | 257   256: - | 476 | 386 | 450
-//   E 8,   H 1024, F 4096    16: 25 | 53 | 68 | 104      32: 40 | 53 | 70 | 105      64: 70 | 63 | 72 | 106      256: - | 95 | 98 | 133
-// and at 512 rows 128 | 256: 1585 | 1516, 710 | 696, 150 | 163.
+//   E 8,   H 4096, F 14336   8: 160 | 237 | 342 | 539   16: 226 | 240 | 346 | 539   48: 519 | 245 | 361 | 555
+//                            96: 882 | 387 | 387 | 576  256: - | 816 | 807 | 893    512: - | 1480 | 1370 | 1381
+//   E 128, H 2048, F 768     8: 85 | 105 | 145 | 242    16: 113 | 108 | 148 | 253   48: 248 | 130 | 158 | 259
+//                            96: 440 | 192 | 170 | 269  256: - | 425 | 382 | 430    512: - | 782 | 684 | 703
+//   E 8,   H 1024, F 4096    16: 29 | 42 | 50 | 66      32: 38 | 44 | 53 | 68       64: 62 | 55 | 58 | 73
+//                            128: - | 68 | 79 | 80      256: - | 91 | 102 | 119     512: - | 151 | 143 | 160
 int mx_rows(int64_t R, int64_t H, int64_t F, int64_t E) {
   if (H < 128 || F < 128) return 0;
   const bool even = H % 128 == 0 && F % 128 == 0;
   const int64_t tn = (F + 127) / 128;
-  if (R <= (E * tn < 512 ? 40 : 24) * E) return 0;
-  if (even && R > 400 * E && R / 256 * tn >= 1024) return 256;
-  return R > 48 * E && std::max(R / 128, E) * tn >= 512 ? 128 : 64;
+  if (R <= (E * tn < 512 ? 40 : 16) * E) return 0;
+  if (even && R > 512 * E && R / 256 * tn >= 1024) return 256;
+  return R > 160 * E && std::max(R / 128, E) * tn >= 1024 ? 128 : 64;
 }
 
 // Room for the partial tiles of an XCD (tiles of bm rows, 256 columns): two rounds of parts, 8 a tile.  None for products of

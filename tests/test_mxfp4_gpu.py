@@ -130,6 +130,15 @@ def test_backward(H, F, counts):
 
 
 @pytest.mark.parametrize("H,F,counts", [
+    (160, 8224, [1500, 0, 700]),             # tiles of 128 rows, odd numbers of blocks
+    (4096, 14336, [1100, 1003]),
+    (128, 16384, [1000, 0, 1303]),           # of 256 rows
+], ids=lambda v: str(v)[:24])
+def test_forward_of_many_rows(H, F, counts):
+    test_forward(H, F, counts)
+
+
+@pytest.mark.parametrize("H,F,counts", [
     (160, 2080, [3000, 0, 1201]),            # tiles of 128 rows; reductions and columns of odd numbers of blocks
     (96, 544, [64, 70, 58] * 44),            # ... of many experts
     (8224, 2016, [4133, 101]),               # of 256 rows for dxp
