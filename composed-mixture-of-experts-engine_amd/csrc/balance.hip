@@ -15,6 +15,12 @@
 // run c and sequence s meet in row c + s, which is distinct for every pair that meets (along a walk one of the two grows by
 // one), and a sequence's rows are consecutive.  Its rows are then added in order (64 bits), so every result is the same from
 // run to run: by one block that also forms the losses where there are few rows, else by a block a sequence and a third launch.
+// Small batches are one block's altogether (k_balance_one).
+//
+// Measured, forward | sums | losses | backward, us: 65536 tokens, E 64, K 6, 16 sequences 10.7 | 7.1 | 4.4 | 13.1; 32768 tokens,
+// E 128, K 8, 700 sequences 15.0 | 4.9 | 4.4 | 13.8 (16.8 MB read a forward, 33.6 MB moved a backward: 1.6 and 2.6 TB/s; what is
+// left is launches and each kernel's chain of loads).  A ticket whose last block forms the losses, in place of the third
+// launch: sums 10.3 us, nothing won.
 #include <algorithm>
 
 #include "common.h"
@@ -26,6 +32,9 @@ constexpr int kMaxBalanceE = 256;
 constexpr int kBalanceNT = 512;  // threads of a block of the two kernels over tokens
 constexpr int kFewSeqs = 64;     // sequences, and rows of sums, that one block adds up
 constexpr int kFewRows = 128;
+constexpr int kOneSeqs = 16;     // sequences, experts and tokens a lane group of a batch that one block finishes
+constexpr int kOneE = 64;
+constexpr int kOneU = 4;
 
 struct BalanceArgs {
   const float* logits;    // [N][E]
@@ -439,6 +448,101 @@ __device__ __forceinline__ double sum_sequence(const BalanceSumArgs& a, int64_t 
   return l;
 }
 
+// A small batch, whole, by one block: its probabilities and choices go to LDS, a wave takes every eighth sequence, and the
+// losses follow behind a barrier.  1000 tokens of 8 experts in 8 sequences: 9.5 us, where runs and their sums took 6.5 and 8 in
+// two launches; the calls' own cost on the host is most of what is left of both directions' 19 us.
+template <int LPT, bool VEC>
+__global__ __launch_bounds__(kBalanceNT) void k_balance_one(BalanceArgs a, BalanceSumArgs o) {
+  constexpr int TEAMS = kBalanceNT / LPT, NW = kBalanceNT / 64, EW = LPT * 4, TOK = kOneU * TEAMS;
+  static_assert(EW <= 64);
+  __shared__ __attribute__((aligned(16))) float s_p[TOK * EW];  // 32 KB
+  __shared__ uint8_t s_id[TOK * (EW < 32 ? EW : 32)];           // K <= min(E, 32)
+  __shared__ float s_l[TOK];                                    // squared logsumexp, negative where the token is masked
+  __shared__ int s_c[NW][EW];
+  __shared__ double s_loss[kOneSeqs], s_z[kOneSeqs];
+  __shared__ int s_n[kOneSeqs];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, sub = lane % LPT, team = tid / LPT;
+  const int E = a.E, K = a.K, N = (int)a.N, S = (int)a.S;
+  f32x4 p[kOneU];
+  bool ok[kOneU];
+#pragma unroll
+  for (int u = 0; u < kOneU; ++u) {
+    const int64_t t = min(u * TEAMS + team, N - 1);
+    p[u] = load_logits<VEC>(a, t, sub * 4);
+    ok[u] = a.mask == nullptr || a.mask[t] != 0;
+  }
+  const int64_t bound = min(max(seq_off(a, min(lane, S)), (int64_t)0), a.N);
+  for (int i = tid; i < N * K; i += kBalanceNT) {
+    const int64_t v = a.idx[i];
+    s_id[i] = (uint8_t)(v >= 0 && v < E ? v : 255);
+  }
+#pragma unroll
+  for (int u = 0; u < kOneU; ++u) {
+    const int t = u * TEAMS + team;
+    const float lse = softmax_token<LPT>(p[u]);
+    if (t < N) {
+      *reinterpret_cast<f32x4*>(s_p + t * EW + sub * 4) = p[u];
+      if (sub == 0) s_l[t] = ok[u] ? lse * lse : -1.f;
+    }
+  }
+  __syncthreads();
+  const int el = lane % EW, rl = lane / EW;
+  for (int s = wv; s < S; s += NW) {
+    const int lo = (int)__shfl(bound, s), hi = (int)__shfl(bound, s + 1);
+    if (lane < EW) s_c[wv][lane] = 0;
+    __asm__ volatile("" ::: "memory");
+    double P = 0., z = 0.;
+    int n = 0;
+    for (int t = lo + rl; t < hi; t += 64 / EW) P += !(s_l[t] < 0.f) ? (double)s_p[t * EW + el] : 0.;
+    for (int t = lo + lane; t < hi; t += 64) {
+      const float l = s_l[t];
+      if (!(l < 0.f)) {
+        z += (double)l;
+        ++n;
+        for (int k = 0; k < K; ++k) {
+          const int e = s_id[t * K + k];
+          if (e < E) atomicAdd(&s_c[wv][e], 1);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = EW; x < 64; x <<= 1) P += __shfl_xor(P, x);
+    n = wave_sum_of(n);
+    z = wave_sum_of(z);
+    __asm__ volatile("" ::: "memory");
+    const double inv = n > 0 ? 1. / (double)n : 0.;
+    double l = 0.;
+    if (lane < E) {
+      const int c = s_c[wv][lane];
+      o.counts[s * E + lane] = c;
+      o.mean_p[s * E + lane] = (float)(P * inv);
+      l = (double)E * (double)c * inv / (double)K * (P * inv);
+    }
+    l = wave_sum_of(l);
+    if (lane == 0) {
+      o.tokens[s] = n;
+      s_loss[s] = l;
+      s_z[s] = z;
+      s_n[s] = n;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    double sum = 0., z = 0.;
+    int all = 0, used = 0;
+    for (int s = 0; s < S; ++s) {
+      sum += s_loss[s];
+      z += s_z[s];
+      all += s_n[s];
+      used += s_n[s] > 0;
+    }
+    o.tokens[S] = all;
+    o.tokens[S + 1] = used;
+    *o.balance = (float)((double)o.bcoef * sum / fmax((double)used, 1.));
+    *o.z = (float)((double)o.zcoef * z / fmax((double)all, 1.));
+  }
+}
+
 // This thread's share of the runs' z sums.
 __device__ __forceinline__ double z_share(const BalanceSumArgs& a) {
   double zs = 0.;
@@ -574,6 +678,16 @@ int balance_check(const char* what, int64_t N, int64_t E, int64_t K, int64_t S) 
       case 64 * 16 + 8: MOE_LAUNCH("k_balance_fwd", (k_balance_fwd<64, 8, VEC>), grid, block, 0, s, a); break;\
     }                                                                                                         \
   } while (0)
+#define MOE_BALANCE_ONE(VEC)                                                                                  \
+  do {                                                                                                        \
+    const dim3 grid(1), block(kBalanceNT);                                                                    \
+    switch (f.lpt) {                                                                                          \
+      case 2: MOE_LAUNCH("k_balance_one", (k_balance_one<2, VEC>), grid, block, 0, s, a, b); break;           \
+      case 4: MOE_LAUNCH("k_balance_one", (k_balance_one<4, VEC>), grid, block, 0, s, a, b); break;           \
+      case 8: MOE_LAUNCH("k_balance_one", (k_balance_one<8, VEC>), grid, block, 0, s, a, b); break;           \
+      case 16: MOE_LAUNCH("k_balance_one", (k_balance_one<16, VEC>), grid, block, 0, s, a, b); break;         \
+    }                                                                                                         \
+  } while (0)
 #define MOE_BALANCE_BWD(VEC)                                                                                  \
   do {                                                                                                        \
     const dim3 grid((unsigned)runs), block(kBalanceNT);                                                       \
@@ -631,9 +745,6 @@ extern "C" int moe_balance_fwd(const float* logits, const int64_t* idx, const in
   a.part_c = reinterpret_cast<int*>(ws + w.off_c);
   a.part_n = reinterpret_cast<int*>(ws + w.off_n);
   a.part_z = reinterpret_cast<float*>(ws + w.off_z);
-  if (E % 4 == 0 && al16b(logits)) MOE_BALANCE_FWD(true);
-  else MOE_BALANCE_FWD(false);
-  if (int rc = check_launch("k_balance_fwd")) return rc;
   BalanceSumArgs b{};
   b.off = seq_offsets;
   b.part_p = a.part_p;
@@ -654,6 +765,15 @@ extern "C" int moe_balance_fwd(const float* logits, const int64_t* idx, const in
   b.seq_loss = reinterpret_cast<double*>(ws + w.off_loss);
   b.balance = balance;
   b.z = z;
+  const bool vec = E % 4 == 0 && al16b(logits);
+  if (S <= kOneSeqs && E <= kOneE && N <= kOneU * (kBalanceNT / f.lpt)) {
+    if (vec) MOE_BALANCE_ONE(true);
+    else MOE_BALANCE_ONE(false);
+    return check_launch("moe_balance_fwd");
+  }
+  if (vec) MOE_BALANCE_FWD(true);
+  else MOE_BALANCE_FWD(false);
+  if (int rc = check_launch("k_balance_fwd")) return rc;
 #define MOE_BALANCE_SUM(KERNEL, name, grid, block, ...)                               \
   do {                                                                                \
     if (E <= 64) MOE_LAUNCH(name, KERNEL<1>, grid, block, 0, s, __VA_ARGS__);         \
