@@ -109,6 +109,21 @@ def test_against_the_oracle(shape, spread):
     assert bool((d.cpu()[left] == 0).all())
 
 
+@pytest.mark.parametrize("shape", [
+    (1024, 8, 8, (0, [64] * 16), False),                  # the most that one block takes, and one more of each
+    (1025, 8, 2, (1, [64] * 16), True),
+    (1024, 7, 3, (0, [0, 1024] + [0] * 14), True),
+    (1000, 8, 2, (0, [50] * 17), True),
+    (512, 16, 16, (12, [1, 0, 499]), True),
+    (128, 64, 32, (0, [8] * 16), False),
+    (129, 64, 6, (0, [129]), True),
+    (128, 65, 6, (0, [100, 28]), True),
+    (2, 3, 1, (0, [0, 2]), False),
+], ids=lambda s: f"N{s[0]}-E{s[1]}-K{s[2]}-S{len(s[3][1])}")
+def test_small_batches(shape):
+    test_against_the_oracle(shape, 2.0)
+
+
 def test_masks_of_the_lowest_value_and_minus_infinity():
     """Experts closed to a token by the type's lowest value or by -inf have probability 0; all closed by the lowest value is
     a uniform token."""
