@@ -306,9 +306,10 @@ __global__ __launch_bounds__(NW * 64, 2) void k_mx_small(MxArgs g) {
   else mx_pass<GU, NF, NW, 1>(g, e, m0, hi - m0, n0, tile, stage, red);
 }
 
-// 64 weight rows and four waves a block; where that leaves fewer than 256 blocks with rows, 32 rows and eight waves.  Down
-// projection, us, (4, 4) | (2, 8): one token at H 4096, F 14336 (128 blocks) 20 | 14; 16 tokens (512 blocks) 52 | 55; 64 rows of
-// E 128, H 2048, F 768 (2048 blocks, three units a row) 20 | 43.
+// 64 weight rows and four waves a block; two waves where a row has few units for them; where that leaves fewer than 256 blocks
+// with rows, 32 rows and eight waves.  Down projection, us, (4, 4) | (4, 2) | (2, 8), rows of all experts: one token at
+// H 4096, F 14336 (128 blocks, 56 units a row) 20 | 27 | 14; 16 tokens (512 blocks) 52 | 57 | 55; 512 rows of E 128, H 2048, F 768
+// (4608 blocks, 3 units) 26 | 23 | 57; both products, 512 rows of E 64, H 4096, F 1536 (6 units) 140 | 132.
 template <bool GU>
 int launch_small(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R) {
   a.E = (int)E;
@@ -316,7 +317,8 @@ int launch_small(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R
   const bool wide = cdiv(a.N, GU ? 32 : 64) * std::min(E, R) >= 256;
   a.Tn = cdiv(a.N, (GU ? 16 : 32) * (wide ? 2 : 1));
   if (a.Tn * slots > INT32_MAX) return fail_arg("%s: too many tiles", name);
-  if (wide) MOE_LAUNCH(name, (k_mx_small<GU, 4, 4>), dim3((unsigned)(a.Tn * slots)), dim3(256), 0, s, a);
+  if (wide && a.K <= 6 * 256) MOE_LAUNCH(name, (k_mx_small<GU, 4, 2>), dim3((unsigned)(a.Tn * slots)), dim3(128), 0, s, a);
+  else if (wide) MOE_LAUNCH(name, (k_mx_small<GU, 4, 4>), dim3((unsigned)(a.Tn * slots)), dim3(256), 0, s, a);
   else MOE_LAUNCH(name, (k_mx_small<GU, 2, 8>), dim3((unsigned)(a.Tn * slots)), dim3(512), 0, s, a);
   return check_launch(name);
 }
