@@ -250,6 +250,40 @@ def test_graph_replays_other_streams_and_threads():
     assert not fails, fails
 
 
+def test_two_graphs_of_split_products():
+    """Forms whose last tiles are split over the reduction: two graphs, each with its own workspaces, replayed in turn with
+    eager calls between."""
+    say("[mxfp4 two graphs]")
+    H, F, counts = 1024, 1056, [300, 213, 0, 500]
+    q, s, _ = _experts(4, F, H, 23)
+    offs = _offsets(counts).to(dev())
+    x = torch.randn(2, sum(counts), H, device=dev()).bfloat16()
+
+    def step(t):
+        hgu, y = ops.swiglu_forward_mxfp4(t, q, s, offs)
+        return hgu, y, ops.swiglu_backward_mxfp4(y, hgu, q, s, offs)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        buf = [x[0].clone(), x[1].clone()]
+        step(buf[0])
+    side.synchronize()
+    graphs, outs = [], []
+    for b in buf:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(step(b))
+        graphs.append(g)
+    for i in range(3):
+        for k in (1, 0):
+            buf[k].copy_(x[k] * (i + 1))
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[k], step(buf[k]))), (i, k)
+
+
 def test_refusals():
     H, F = 64, 96
     q, s, _ = _experts(2, F, H, 19)

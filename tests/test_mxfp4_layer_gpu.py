@@ -135,6 +135,31 @@ def test_decode_graph():
             assert torch.equal(out, layer.forward_mxfp4(buf)), i
 
 
+def test_training_step_graph():
+    """A training step of the router and the tokens around 4-bit experts, captured and replayed."""
+    say("[mxfp4 training graph]")
+    from test_graph_gpu import _replays_match_eager
+
+    layer = _layer(256, 512, 8, 2, layout="routed", check_numerics=False, seq_balance_coef=0.5, z_loss_coef=1e-3)
+    layer.quantize_mxfp4()
+    x = torch.randn(6, 50, 256, device=dev()).to(B).requires_grad_(True)
+    mask = torch.arange(50, device=dev()) < torch.tensor([[50], [3], [0], [17], [49], [1]], device=dev())
+    gout, one = torch.randn(6, 50, 256, device=dev()).to(B), torch.ones((), device=dev())
+    gate = layer.router.gate_w
+
+    def step():
+        out = layer.forward_mxfp4(x, token_mask=mask)
+        r = layer.router
+        bal, z = r.last_seq_balance_loss, r.last_z_loss
+        dx, dg = torch.autograd.grad((out, bal, z), (x, gate), grad_outputs=(gout, one, one))
+        res = out.detach(), bal.detach(), z.detach(), r.last_seq_counts, r.last_seq_tokens, dx, dg
+        # the layer keeps its last losses; drop them, and with them the step's autograd graph
+        r.last_seq_balance_loss = r.last_z_loss = r.last_aux_loss = None
+        return res
+
+    _replays_match_eager(step, ("out", "balance", "z", "counts", "tokens", "dx", "dgate"))
+
+
 def test_refusals():
     layer = _layer(64, 64, 4, 2)
     layer.quantize_mxfp4()
