@@ -359,7 +359,8 @@ __device__ __forceinline__ T wave_sum_of(T v) {
 
 // One sequence's rows, added by W waves of a block (a power of two; wave w of them).  Lanes lie side by side on a row's
 // experts, 64 at a time, and with fewer experts on several rows.  Every wave of the block calls it, with live false where
-// it has no sequence.  EJ: 64-wide pieces of a row.  sm: a row for each of the block's waves.  Returns the sequence's loss and valid tokens to wave 0's lanes.
+// it has no sequence.  EJ: 64-wide pieces of a row.  sm: a row for each of the block's waves.  Returns the sequence's loss and
+// valid tokens to wave 0's lanes.
 template <int EJ>
 __device__ __forceinline__ double sum_sequence(const BalanceSumArgs& a, int64_t s, bool live, int W, int w, int lane,
                                                double* sm_p, int64_t* sm_c, int64_t* sm_n, int64_t& n) {

@@ -21,8 +21,8 @@
 // Many rows (k_mx_tile): 64, 128 or 256 rows of an expert by 256 weight rows.  The rows go through LDS in 64-wide slices, two
 // at a time; a wave has weight rows of its own, dequantizes them between registers and feeds v_mfma_f32_32x32x16_bf16, half a
 // conversion to 2, 4 or 8 row fragments.  64 rows read a weight so rarely that the vector cache bounds them too: their weights
-// come by whole lines through the wave's LDS (1002 rows at the sizes above, tiles of 64 rows: 600 -> 500 us), and LDS bounds
-// them after that (7/8 of its rate).  128 and 256 rows load in the lanes' own order, whose accesses the matrix instructions
+// come by whole lines through the wave's LDS (1002 rows at the sizes above, tiles of 64 rows: 600 -> 500 us); after that
+// LDS moves 7/8 of what it can by count, and the MFMAs are 46% busy.  128 and 256 rows load in the lanes' own order, whose accesses the matrix instructions
 // cover; what bounds them is the matrix instructions' power (16384 rows: 4.76 ms, 5.77 TFLOP, 1210 TFLOP/s at 1.6 GHz).
 #include <algorithm>
 #include <utility>
