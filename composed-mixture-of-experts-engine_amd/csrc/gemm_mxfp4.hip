@@ -991,8 +991,8 @@ __device__ __forceinline__ BkTile bk_tile(const BkArgs& g, int L, int lane) {
 // that use them they are 64 cache accesses a load, and those bounded the products (5.4 ms for dxp below).
 //
 // What bounds them: matrix instructions and the conversion's issue with 256 rows (one wave a SIMD, MFMA busy 62%), the
-// epilogue's 3.8 GB in the product with Wd, whose two blocks a CU run under each other's.  16384 rows, E 8, H 4096, F 14336:
-// dact 2.17 ms, dxp 3.33 ms (1.92 TFLOP and 3.85: 890 and 1160 TFLOP/s); the products on bf16 weights 2.01 and 3.35.
+// epilogue's 1.9 GB in the product with Wd, whose two blocks a CU run under each other's.  16384 rows, E 8, H 4096, F 14336:
+// dact 2.0-2.2 ms, dxp 3.35 ms (1.92 TFLOP and 3.85: 920 and 1150 TFLOP/s); the products on bf16 weights 2.01 and 3.35.
 
 // A form: a wave has 32 TF rows by 32 NF columns, a block's four waves lie WT on the rows, WF on the columns and KS along the
 // reduction.
