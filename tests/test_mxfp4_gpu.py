@@ -250,6 +250,29 @@ def test_graph_replays_other_streams_and_threads():
     assert not fails, fails
 
 
+@pytest.mark.parametrize("rows", [3, 1200])
+def test_weights_of_more_than_2_gb(rows):
+    """Offsets past 32 bits: the last expert's weights lie behind 2^31 bytes of each matrix."""
+    say(f"[mxfp4 large] rows={rows}")
+    E, H, F = 76, 4096, 14336
+    g = torch.Generator(device=dev()).manual_seed(rows)
+    q, s = [], []
+    for r, c in ((F, H), (F, H), (H, F)):
+        q.append(torch.randint(0, 256, (E, r, c // 2), dtype=torch.uint8, device=dev(), generator=g))
+        s.append(torch.randint(117, 121, (E, r, c // 32), dtype=torch.uint8, device=dev(), generator=g))
+    assert q[0][-1].data_ptr() - q[0].data_ptr() > 2 ** 31
+    offs = _offsets([0] * (E - 1) + [rows])
+    x, dy = (torch.randn(rows, H, device=dev(), generator=g).bfloat16() for _ in range(2))
+    hgu, y = ops.swiglu_forward_mxfp4(x, q, s, offs.to(dev()))
+    dx = ops.swiglu_backward_mxfp4(dy, hgu, q, s, offs.to(dev()))
+    w = [OX.dequant(a[-1:], b[-1:]) for a, b in zip(q, s)]
+    rh, ry, th, ty = OX.swiglu_fwd(x, w, [0, rows])
+    _inside(hgu, rh, th, "hgu")
+    _inside(y, ry, ty, "y")
+    rx, tx = OX.swiglu_bwd(dy, hgu, w, [0, rows])
+    _inside(dx, rx, tx, "dxp")
+
+
 def test_two_graphs_of_split_products():
     """Forms whose last tiles are split over the reduction: two graphs, each with its own workspaces, replayed in turn with
     eager calls between."""
