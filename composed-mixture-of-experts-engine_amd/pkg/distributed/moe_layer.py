@@ -379,17 +379,19 @@ class DistributedMoELayer(nn.Module):
         return self._fp8_cache[1], self._fp8_cache[2]
 
     @torch.no_grad()
-    def forward_fp8(self, tokens: torch.Tensor) -> torch.Tensor:
+    def forward_fp8(self, tokens: torch.Tensor, seq_offsets: Optional[torch.Tensor] = None,
+                    token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The layer's forward with an e4m3 dispatch payload and e4m3 expert GEMMs (no autograd): router and
         planner as in ``forward``, the permute writes each token row quantized (one fp32 scale per row),
         the gate/up and down projections run on the fp8 MFMA with per-row x per-channel scales, the
         SwiGLU activations are quantized per row between them, and the combine is the bf16 one.  Needs
-        the fused bf16 expert layout (``self._fused()``) and hidden_dim % 16 == 0."""
+        the fused bf16 expert layout (``self._fused()``) and hidden_dim % 16 == 0.  ``seq_offsets`` and ``token_mask`` as in
+        :meth:`forward`."""
         if not self._fused() or self.w_gate.dtype != torch.bfloat16:
             raise NotImplementedError("forward_fp8 needs the built-in SwiGLU experts in bfloat16")
         shape = tokens.shape
         flat = tokens.reshape(-1, shape[-1])
-        idx, weights, _cnt = self.router(flat)
+        idx, weights, _cnt = self.router(flat, **self._seq_kwargs(tokens, seq_offsets, token_mask))
         N = flat.shape[0]
         capacity = (
             math.ceil(self.capacity_factor * N * self.top_k / self.num_experts) if self.capacity_dropping else -1
