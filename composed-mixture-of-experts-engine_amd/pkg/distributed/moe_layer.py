@@ -270,14 +270,12 @@ class DistributedMoELayer(nn.Module):
             and len(self.experts) == self.num_experts
         )
 
-    def _seq_kwargs(self, tokens: torch.Tensor, seq_offsets, token_mask) -> dict:
-        """The router's arguments for the balance loss of sequences, the rows of a [B, S, H] batch by default."""
-        r = self.router
-        if seq_offsets is None and token_mask is None and getattr(r, "seq_balance_coef", 0.0) == 0.0:
-            return {}
-        if seq_offsets is None and tokens.dim() == 3 and tokens.shape[0] > 0 and tokens.shape[1] > 0:
-            seq_offsets = torch.arange(0, tokens.shape[0] * tokens.shape[1] + 1, tokens.shape[1], device=tokens.device)
-        return {"seq_offsets": seq_offsets, "token_mask": token_mask}
+    def _router_args(self, flat: torch.Tensor, shape, seq_offsets, token_mask):
+        """The router's tokens and its arguments for the balance loss of sequences (the tokens then as [B, S, H]: by default
+        the rows are the sequences)."""
+        if seq_offsets is None and token_mask is None and getattr(self.router, "seq_balance_coef", 0.0) == 0.0:
+            return flat, {}
+        return (flat.view(shape) if len(shape) == 3 else flat), {"seq_offsets": seq_offsets, "token_mask": token_mask}
 
     def forward(self, tokens: torch.Tensor, seq_offsets: Optional[torch.Tensor] = None,
                 token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -288,8 +286,9 @@ class DistributedMoELayer(nn.Module):
             raise ValueError(f"tokens must be rank 2 or 3, got {tokens.dim()}")
         H = tokens.shape[-1]
         flat = tokens.reshape(-1, H)
+        routed, seq = self._router_args(flat, tokens.shape, seq_offsets, token_mask)
         with self._deferred_router_check(), self._linked_tokens():
-            idx, weights, _cnt = self.router(flat, **self._seq_kwargs(tokens, seq_offsets, token_mask))
+            idx, weights, _cnt = self.router(routed, **seq)
         # the router hands the tokens back as a linked output (a view of the same memory): the expert path's
         # gradient of the tokens then reaches the router's backward, which adds it inside its dx kernel, so
         # x's gradient is formed in one pass instead of autograd adding the two paths' gradients afterwards
@@ -329,9 +328,9 @@ class DistributedMoELayer(nn.Module):
             raise ValueError(f"tokens must be rank 2 or 3, got {tokens.dim()}")
         H = tokens.shape[-1]
         flat = tokens.reshape(-1, H)
+        routed, seq = self._router_args(flat, original_shape, seq_offsets, token_mask)
         with self._deferred_router_check():
-            xn, idx, weights, _cnt = self.router.forward_with_norm(flat, norm_weight, eps,
-                                                                   **self._seq_kwargs(tokens, seq_offsets, token_mask))
+            xn, idx, weights, _cnt = self.router.forward_with_norm(routed, norm_weight, eps, **seq)
         return self._experts_forward(xn, idx, weights).reshape(original_shape)
 
     def _experts_forward(self, flat: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor,
@@ -391,7 +390,8 @@ class DistributedMoELayer(nn.Module):
             raise NotImplementedError("forward_fp8 needs the built-in SwiGLU experts in bfloat16")
         shape = tokens.shape
         flat = tokens.reshape(-1, shape[-1])
-        idx, weights, _cnt = self.router(flat, **self._seq_kwargs(tokens, seq_offsets, token_mask))
+        routed, seq = self._router_args(flat, shape, seq_offsets, token_mask)
+        idx, weights, _cnt = self.router(routed, **seq)
         N = flat.shape[0]
         capacity = (
             math.ceil(self.capacity_factor * N * self.top_k / self.num_experts) if self.capacity_dropping else -1
@@ -434,8 +434,9 @@ class DistributedMoELayer(nn.Module):
         if tokens.dtype != torch.bfloat16:
             raise TypeError(f"forward_mxfp4 takes bfloat16 tokens, got {tokens.dtype}")
         flat = tokens.reshape(-1, tokens.shape[-1])
+        routed, seq = self._router_args(flat, tokens.shape, seq_offsets, token_mask)
         with self._deferred_router_check(), self._linked_tokens():
-            idx, weights, _cnt = self.router(flat, **self._seq_kwargs(tokens, seq_offsets, token_mask))
+            idx, weights, _cnt = self.router(routed, **seq)
         linked = self.router.take_linked_tokens()
         return self._experts_forward(flat if linked is None else linked, idx, weights, q).reshape(tokens.shape)
 

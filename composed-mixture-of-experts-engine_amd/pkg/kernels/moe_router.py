@@ -254,9 +254,9 @@ class MoERouter(torch.nn.Module):
         self._last_logits: Optional[torch.Tensor] = None
         self.last_aux_loss: Optional[torch.Tensor] = None
         self.last_z_loss: Optional[torch.Tensor] = None
-        self.last_seq_balance_loss: Optional[torch.Tensor] = None
-        self.last_seq_counts: Optional[torch.Tensor] = None
-        self.last_seq_tokens: Optional[torch.Tensor] = None
+        # (loss, counts, tokens) of last_seq_*, or what they are formed from when read: (shape of the tokens, logits, idx, coef)
+        self._seq_last: tuple = (None, None, None)
+        self._seq_later: Optional[tuple] = None
         self.last_stats: Optional[torch.Tensor] = None
         self.last_stats_host: Optional[torch.Tensor] = None
         self.last_num_tokens = 0
@@ -275,6 +275,23 @@ class MoERouter(torch.nn.Module):
         self._pending = None
         self._profile = value
 
+    def _seq_values(self) -> tuple:
+        if self._seq_later is None:
+            return self._seq_last
+        shape, logits, idx, coef = self._seq_later
+        with torch.no_grad():
+            loss, _z, counts, tokens, _ = balance_loss(logits, idx, self._row_offsets(shape, logits.device), None, coef, 0.0)
+        return loss, counts, tokens
+
+    def _set_seq_value(self, i: int, value) -> None:
+        values = list(self._seq_values())
+        values[i] = value
+        self._seq_later, self._seq_last = None, tuple(values)
+
+    last_seq_balance_loss = property(lambda self: self._seq_values()[0], lambda self, v: self._set_seq_value(0, v))
+    last_seq_counts = property(lambda self: self._seq_values()[1], lambda self, v: self._set_seq_value(1, v))
+    last_seq_tokens = property(lambda self: self._seq_values()[2], lambda self, v: self._set_seq_value(2, v))
+
     def forward(self, tokens: torch.Tensor, force_reference: bool = False,
                 seq_offsets: Optional[torch.Tensor] = None, token_mask: Optional[torch.Tensor] = None):
         """Returns ``(topk_idx [N,K] int64, topk_w [N,K] tokens.dtype, dispatch_cnt [E] int64)``.
@@ -284,7 +301,11 @@ class MoERouter(torch.nn.Module):
         (:func:`moe_mi355.ops.balance_loss_forward`).  ``seq_offsets`` [S + 1] bounds the sequences in the flattened tokens
         (None: the rows of a [B, S, H] batch, or one sequence); ``token_mask`` (bool, one value a token) marks the valid
         tokens.  With a mask ``last_z_loss`` is over the valid tokens; every token is routed and dispatched all the same,
-        and ``last_aux_loss``, the counts and the statistics are over all of them."""
+        and ``last_aux_loss``, the counts and the statistics are over all of them.
+
+        Where no gradient is recorded (``torch.no_grad()``) and neither argument is given, the forward launches nothing for
+        them: each read of a ``last_seq_*`` forms them, from the logits and the returned ``topk_idx`` as they are then (so
+        after a graph's replay they are the replay's)."""
         if tokens.dim() == 3:
             B, S, H = tokens.shape
             flat = tokens.reshape(B * S, H)
@@ -308,7 +329,7 @@ class MoERouter(torch.nn.Module):
         self._x_link = outs[7] if self._link_x else None
         if timing is not None:
             timing.stop()
-        z = self._seq_losses(seq, logits, idx, z)
+        z = self._seq_losses(seq, tokens.shape, logits, idx, z)
         return self._finish(flat, idx, w, aux, z, logits, cnt, stats, timing)
 
     def take_linked_tokens(self) -> Optional[torch.Tensor]:
@@ -316,28 +337,37 @@ class MoERouter(torch.nn.Module):
         x, self._x_link = self._x_link, None
         return x
 
+    @staticmethod
+    def _row_offsets(shape, device) -> Optional[torch.Tensor]:
+        """Bounds of the rows of a [B, S, H] batch in its flattened tokens (None: one sequence)."""
+        if len(shape) != 3 or shape[0] == 0:
+            return None
+        if shape[1] == 0:
+            return torch.zeros(shape[0] + 1, dtype=torch.int64, device=device)
+        return torch.arange(0, shape[0] * shape[1] + 1, shape[1], device=device)
+
     def _seq_args(self, shape, seq_offsets, token_mask, device):
         """(seq_offsets, token_mask) of a forward that forms the balance loss of sequences, else None."""
-        if self.seq_balance_coef == 0.0 and seq_offsets is None and token_mask is None:
-            self.last_seq_balance_loss = self.last_seq_counts = self.last_seq_tokens = None
+        self._seq_last, self._seq_later = (None, None, None), None
+        if seq_offsets is None and token_mask is None and (self.seq_balance_coef == 0.0 or not torch.is_grad_enabled()):
             return None
-        if seq_offsets is None and len(shape) == 3 and shape[0] > 0:
-            seq_offsets = torch.arange(0, shape[0] * shape[1] + 1, max(shape[1], 1), device=device)[: shape[0] + 1]
-            if shape[1] == 0:
-                seq_offsets = torch.zeros(shape[0] + 1, dtype=torch.int64, device=device)
+        if seq_offsets is None:
+            seq_offsets = self._row_offsets(shape, device)
         return seq_offsets, token_mask
 
     def _kernel_z_coef(self, seq) -> float:
         """The z-loss over valid tokens is formed with the sequences' balance; the kernel's is over every token."""
         return 0.0 if seq is not None and seq[1] is not None else self.z_loss_coef
 
-    def _seq_losses(self, seq, logits, idx, z):
+    def _seq_losses(self, seq, shape, logits, idx, z):
         if seq is None:
+            if self.seq_balance_coef != 0.0:
+                self._seq_later = (tuple(shape), logits, idx, self.seq_balance_coef)
             return z
         masked = seq[1] is not None
-        balance, z_valid, self.last_seq_counts, self.last_seq_tokens, _ = balance_loss(
+        balance, z_valid, counts, tokens, _ = balance_loss(
             logits, idx, seq[0], seq[1], self.seq_balance_coef, self.z_loss_coef if masked else 0.0)
-        self.last_seq_balance_loss = balance
+        self._seq_last = (balance, counts, tokens)
         return z_valid if masked else z
 
     def forward_with_norm(self, tokens: torch.Tensor, norm_weight: torch.Tensor, eps: float,
@@ -356,7 +386,7 @@ class MoERouter(torch.nn.Module):
         )
         if timing is not None:
             timing.stop()
-        z = self._seq_losses(seq, logits, idx, z)
+        z = self._seq_losses(seq, tokens.shape, logits, idx, z)
         idx, w, cnt = self._finish(flat, idx, w, aux, z, logits, cnt, stats, timing)
         return xn, idx, w, cnt
 
