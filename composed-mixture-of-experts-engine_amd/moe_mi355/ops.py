@@ -510,8 +510,8 @@ def dequant_mxfp4(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = tor
     return L.native().dequant_mxfp4(q, scale, dtype == torch.bfloat16)
 
 
-def _mxfp4_experts(what: str, wq, wscale, H: int, offsets: torch.Tensor):
-    """Checks of the three quantized matrices (gate, up [E, F, H]; down [E, H, F]) and the row offsets [E + 1]."""
+def mxfp4_weights(what: str, wq, wscale, H: int):
+    """Checks of the three quantized matrices (gate, up [E, F, H]; down [E, H, F]) and their scales."""
     wg, wu, wd = wq
     sg, su, sd = wscale
     for t in (wg, wu, wd, sg, su, sd):
@@ -525,9 +525,16 @@ def _mxfp4_experts(what: str, wq, wscale, H: int, offsets: torch.Tensor):
                            ("down scale", sd, (E, H, F // 32))):
         if tuple(t.shape) != shape:
             raise ValueError(f"{what}: {name} must be {list(shape)}, got {list(t.shape)}")
+    return [wg, wu, wd], [sg, su, sd], F
+
+
+def _mxfp4_experts(what: str, wq, wscale, H: int, offsets: torch.Tensor):
+    """The weights' checks, and those of the row offsets [E + 1]."""
+    wq, wscale, F = mxfp4_weights(what, wq, wscale, H)
+    E = wq[0].shape[0]
     if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or not offsets.is_contiguous():
         raise ValueError(f"{what}: offsets must be contiguous int32 [{E + 1}]")
-    return [wg, wu, wd], [sg, su, sd], F
+    return wq, wscale, F
 
 
 def swiglu_forward_mxfp4(xp, wq, wscale, offsets, keep_preact: bool = True):

@@ -122,6 +122,9 @@ def compute_capacity_drop_mask(idx: torch.Tensor, num_experts: int, capacity: in
     return p.drop
 
 
+_MXFP4 = ("mxfp4_gate", "mxfp4_up", "mxfp4_down", "mxfp4_gate_scale", "mxfp4_up_scale", "mxfp4_down_scale")
+
+
 class _ExpertWeight(nn.Module):
     """``.weight`` of one expert projection: a view of the layer's stacked tensor."""
 
@@ -133,7 +136,10 @@ class _ExpertWeight(nn.Module):
 
     @property
     def weight(self) -> torch.Tensor:
-        return getattr(self._owner(), self._name)[self._index]
+        stacked = getattr(self._owner(), self._name)
+        if stacked is None:
+            raise RuntimeError(f"the layer's {self._name} was dropped: only forward_mxfp4 runs")
+        return stacked[self._index]
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return F.linear(x, self.weight)
@@ -190,6 +196,10 @@ class DistributedMoELayer(nn.Module):
         self.w_gate = nn.Parameter(torch.empty(E, ffn_dim, hidden_dim, device=dev, dtype=dtype))
         self.w_up = nn.Parameter(torch.empty(E, ffn_dim, hidden_dim, device=dev, dtype=dtype))
         self.w_down = nn.Parameter(torch.empty(E, hidden_dim, ffn_dim, device=dev, dtype=dtype))
+        # the experts in 4 bits (quantize_mxfp4, load_mxfp4): they move with the layer and are not in its state_dict, whose
+        # keys are the reference's
+        for name in _MXFP4:
+            self.register_buffer(name, None, persistent=False)
         nn.init.normal_(self.w_gate, mean=0.0, std=1.0 / math.sqrt(hidden_dim))
         nn.init.normal_(self.w_up, mean=0.0, std=1.0 / math.sqrt(hidden_dim))
         nn.init.normal_(self.w_down, mean=0.0, std=1.0 / math.sqrt(ffn_dim))
@@ -226,6 +236,8 @@ class DistributedMoELayer(nn.Module):
     def _from_reference_keys(module, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
                              error_msgs):
         for name in ("w_gate", "w_up", "w_down"):
+            if getattr(module, name) is None:  # dropped for serving from 4-bit weights
+                continue
             keys = [f"{prefix}experts.{i}.{name}.weight" for i in range(getattr(module, name).shape[0])]
             if all(k in state_dict for k in keys):
                 state_dict[prefix + name] = torch.stack([state_dict.pop(k) for k in keys])
@@ -263,7 +275,8 @@ class DistributedMoELayer(nn.Module):
     def _fused(self) -> bool:
         return (
             # the grouped GEMM's shapes: bf16 H % 8 == 0, fp32 H % 4 == 0, both F % 32 == 0
-            self.w_gate.dtype in (torch.bfloat16, torch.float32)
+            self.w_gate is not None
+            and self.w_gate.dtype in (torch.bfloat16, torch.float32)
             and self.w_gate.shape[-1] % (8 if self.w_gate.dtype == torch.bfloat16 else 4) == 0
             and self.w_gate.shape[1] % 32 == 0
             and all(type(m) is _SwiGLUExpert and m.w_gate._owner() is self for m in self.experts)
@@ -411,22 +424,43 @@ class DistributedMoELayer(nn.Module):
     def quantize_mxfp4(self):
         """Quantize the expert weights to MXFP4 (:func:`moe_mi355.ops.quant_mxfp4`: 4-bit e2m1 values, one power-of-two scale
         per 32 along the reduction) for :meth:`forward_mxfp4`, on the GPU.  The quantized weights stay as they are until this
-        is called again, whatever becomes of the parameters.  Returns ``((gate, up, down), (their scales))``."""
+        is called again, whatever becomes of the parameters, and move with the layer.  Returns ``((gate, up, down), (their
+        scales))``, for :meth:`load_mxfp4` to take again: they are not in the layer's ``state_dict``."""
+        if any(t is None for t in (self.w_gate, self.w_up, self.w_down)):
+            raise RuntimeError("quantize_mxfp4: the layer's full-width weights were dropped")
         if self.w_gate.shape[-1] % ops.MXFP4_BLOCK or self.w_gate.shape[1] % ops.MXFP4_BLOCK:
             raise NotImplementedError(f"quantize_mxfp4 needs hidden and ffn dims that are multiples of {ops.MXFP4_BLOCK}")
         q = [ops.quant_mxfp4(t.detach()) for t in (self.w_gate, self.w_up, self.w_down)]
-        self._mxfp4 = (tuple(t for t, _ in q), tuple(s for _, s in q))
-        return self._mxfp4
+        return self.load_mxfp4([t for t, _ in q], [s for _, s in q])
+
+    def load_mxfp4(self, weights, scales):
+        """Take ``(gate, up, down)`` and their scales for :meth:`forward_mxfp4`: what :meth:`quantize_mxfp4` returned, or
+        weights quantized elsewhere to the layout of :func:`moe_mi355.ops.quant_mxfp4` ([E, F, H / 2], [E, F, H / 2] and
+        [E, H, F / 2] bytes; the last dims of the scales H / 32, H / 32 and F / 32).  They are kept as they are, on the router's
+        device.  A layer that only serves them may drop its full-width parameters (``layer.w_gate = layer.w_up =
+        layer.w_down = None``).  Returns them."""
+        wq, ws, F_ = ops.mxfp4_weights("load_mxfp4", weights, scales, self.hidden_dim)
+        if wq[0].shape[0] != len(self.local_expert_ids) or F_ != self.ffn_dim:
+            raise ValueError(f"load_mxfp4: the layer has {len(self.local_expert_ids)} experts of ffn_dim {self.ffn_dim}, got "
+                             f"{wq[0].shape[0]} of {F_}")
+        dev = self.router.gate_w.device
+        for name, t in zip(_MXFP4, wq + ws):
+            setattr(self, name, t.detach().to(dev))
+        return self._mxfp4_weights()
+
+    def _mxfp4_weights(self):
+        q = tuple(getattr(self, name) for name in _MXFP4)
+        return q[:3], q[3:]
 
     def forward_mxfp4(self, tokens: torch.Tensor, seq_offsets: Optional[torch.Tensor] = None,
                       token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """``forward`` with the experts' weights as :meth:`quantize_mxfp4` left them: bf16 rows, 4-bit weights, from one
-        decoded token to a long prefill.  Differentiable in the tokens and the router; the 4-bit weights are constants (the
+        """``forward`` with the experts' weights as :meth:`quantize_mxfp4` or :meth:`load_mxfp4` left them: bf16 rows, 4-bit
+        weights, from one decoded token to a long prefill.  Differentiable in the tokens and the router; the 4-bit weights are constants (the
         layer's own expert parameters get no gradient), so a router, or what lies before the layer, can be trained around
         experts in the form that they are served in.  Needs the built-in SwiGLU experts and bfloat16 tokens."""
-        q = getattr(self, "_mxfp4", None)
-        if q is None:
-            raise RuntimeError("forward_mxfp4: call quantize_mxfp4() first")
+        q = self._mxfp4_weights()
+        if q[0][0] is None:
+            raise RuntimeError("forward_mxfp4: call quantize_mxfp4() or load_mxfp4() first")
         if not all(type(m) is _SwiGLUExpert and m.w_gate._owner() is self for m in self.experts):
             raise NotImplementedError("forward_mxfp4 needs the built-in SwiGLU experts")
         if tokens.dim() not in (2, 3):
