@@ -124,6 +124,31 @@ def test_small_batches(shape):
     test_against_the_oracle(shape, 2.0)
 
 
+@pytest.mark.parametrize("N,E,lengths,one", [
+    (384, 8, None, True), (385, 8, None, False), (1000, 8, None, False),  # one sequence: 8 tokens a step
+    (768, 8, [700, 68], True), (769, 8, [700, 69], False),
+    (1024, 8, [256] * 4, True), (1024, 8, [64] * 16, True), (1024, 8, [60] * 17, False), (1025, 8, [64] * 16, False),
+    (192, 16, None, True), (193, 16, None, False), (48, 64, None, True), (49, 64, None, False), (128, 64, [64, 64], False),
+    (96, 64, [1, 95], True), (20, 65, None, False),
+], ids=str)
+def test_which_form_a_small_batch_takes(N, E, lengths, one):
+    """One block only where its waves' sequences are short on average; either form against the oracle."""
+    from moe_mi355 import _lib
+
+    logits, idx, offs, mask = _case(N, E, min(E, 4), None if lengths is None else (0, lengths), True, seed=7)
+    torch.cuda.synchronize()
+    _lib.prof_enable(True)
+    try:
+        f, _ = _run(logits, idx, offs, mask)
+    finally:
+        _lib.prof_enable(False)
+    names = set(_lib.prof_summary())
+    assert ("k_balance_one" in names) == one and ("k_balance_fwd" in names) != one, names
+    test_against_the_oracle((N, E, min(E, 4), None if lengths is None else (0, lengths), True), 2.0)
+    ref = OB.balance(logits, idx, offs, mask, BC, ZC, GB, GZ)
+    assert torch.equal(f[2].cpu(), ref["counts"]) and torch.equal(f[3].cpu(), ref["tokens"])
+
+
 def test_masks_of_the_lowest_value_and_minus_infinity():
     """Experts closed to a token by the type's lowest value or by -inf have probability 0; all closed by the lowest value is
     a uniform token."""
