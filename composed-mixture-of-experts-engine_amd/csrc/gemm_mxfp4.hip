@@ -923,44 +923,35 @@ template <int NF>
 struct __attribute__((aligned(NF * 2))) BkCols {
   uint32_t d[NF / 2];
 };
-// They leave: dxp as they are; dh = [da u silu'(g) | da silu(g)] from fp32 da, the pre-activations gv, uv in hand.
-template <int NF>
-__device__ __forceinline__ void bk_put(const BkArgs& g, int64_t row, int col, const float (&v)[NF]) {
-  BkCols<NF> o;
-#pragma unroll
-  for (int d = 0; d < NF / 2; ++d) o.d[d] = pack2bf(v[2 * d], v[2 * d + 1]);
-  *reinterpret_cast<BkCols<NF>*>(g.C + row * g.N + col) = o;
-}
-template <int NF>
-__device__ __forceinline__ void bk_put(const BkArgs& g, int64_t row, int col, const float (&v)[NF], const BkCols<NF>& gv,
-                                       const BkCols<NF>& uv) {
-  BkCols<NF> dg, du;
-#pragma unroll
-  for (int d = 0; d < NF / 2; ++d) {
-    float o[2], p[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float x = __uint_as_float(h ? gv.d[d] & 0xffff0000u : gv.d[d] << 16);
-      const float u = __uint_as_float(h ? uv.d[d] & 0xffff0000u : uv.d[d] << 16);
-      const float sg = sig_mx(x), t = v[2 * d + h] * sg;
-      o[h] = t * u * (1.f + x * (1.f - sg));
-      p[h] = t * x;
-    }
-    dg.d[d] = pack2bf(o[0], o[1]);
-    du.d[d] = pack2bf(p[0], p[1]);
-  }
-  const int64_t at = row * 2 * (int64_t)g.N + col;
-  *reinterpret_cast<BkCols<NF>*>(g.C + at) = dg;
-  *reinterpret_cast<BkCols<NF>*>(g.C + at + g.N) = du;
-}
+// They leave: dxp as they are; dh = [da u silu'(g) | da silu(g)] from fp32 da and the pre-activations.
 template <bool DACT, int NF>
 __device__ __forceinline__ void bk_store(const BkArgs& g, int64_t row, int col, const float (&v)[NF]) {
   if constexpr (DACT) {
-    const uint16_t* const x = g.X + row * 2 * (int64_t)g.N + col;
-    const BkCols<NF> gv = *reinterpret_cast<const BkCols<NF>*>(x), uv = *reinterpret_cast<const BkCols<NF>*>(x + g.N);
-    bk_put<NF>(g, row, col, v, gv, uv);
+    const uint16_t* const pre = g.X + row * 2 * (int64_t)g.N + col;
+    const BkCols<NF> gv = *reinterpret_cast<const BkCols<NF>*>(pre), uv = *reinterpret_cast<const BkCols<NF>*>(pre + g.N);
+    BkCols<NF> dg, du;
+#pragma unroll
+    for (int d = 0; d < NF / 2; ++d) {
+      float o[2], p[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = __uint_as_float(h ? gv.d[d] & 0xffff0000u : gv.d[d] << 16);
+        const float u = __uint_as_float(h ? uv.d[d] & 0xffff0000u : uv.d[d] << 16);
+        const float sg = sig_mx(x), t = v[2 * d + h] * sg;
+        o[h] = t * u * (1.f + x * (1.f - sg));
+        p[h] = t * x;
+      }
+      dg.d[d] = pack2bf(o[0], o[1]);
+      du.d[d] = pack2bf(p[0], p[1]);
+    }
+    const int64_t at = row * 2 * (int64_t)g.N + col;
+    *reinterpret_cast<BkCols<NF>*>(g.C + at) = dg;
+    *reinterpret_cast<BkCols<NF>*>(g.C + at + g.N) = du;
   } else {
-    bk_put<NF>(g, row, col, v);
+    BkCols<NF> o;
+#pragma unroll
+    for (int d = 0; d < NF / 2; ++d) o.d[d] = pack2bf(v[2 * d], v[2 * d + 1]);
+    *reinterpret_cast<BkCols<NF>*>(g.C + row * g.N + col) = o;
   }
 }
 
@@ -1236,23 +1227,7 @@ __global__ __launch_bounds__(256, Form::BLOCKS) void k_mx_back(BkArgs g) {
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) __asm__ volatile("" ::"v"(w[s][j]));
-  // The pre-activations that the epilogue starts with are on their way while the product runs, the others' while it works on
-  // the ones in front of them: 16 rows each.
-  constexpr bool AHEAD = DACT && KS == 1 && Form::BLOCKS == 1;
   const int col = n0 + i32 * NF;
-  BkCols<NF> pg[AHEAD ? 2 : 1][16], pu[AHEAD ? 2 : 1][16];
-  auto fetch = [&](int t) {
-    const uint8_t* const x = reinterpret_cast<const uint8_t*>(g.X + (int64_t)tl.mbase * 2 * N);
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const int r = tw * (32 * TF) + t * 32 + (v & 3) + (v >> 2) * 8 + 4 * h;
-      const uint32_t o = (uint32_t)min(r, tl.mlen - 1) * (uint32_t)N * 4u + (uint32_t)min(col, N - NF) * 2u;
-      pg[t & 1][v] = *reinterpret_cast<const BkCols<NF>*>(x + o);
-      pu[t & 1][v] = *reinterpret_cast<const BkCols<NF>*>(x + (int64_t)N * 2 + o);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  if constexpr (AHEAD) fetch(0);
   for (int i = 0; i < rounds; ++i) {
     step(S0{}, x0, f0, x1, f1, i);
     step(S1{}, x1, f1, x0, f0, i);
@@ -1286,16 +1261,10 @@ __global__ __launch_bounds__(256, Form::BLOCKS) void k_mx_back(BkArgs g) {
     }
 #pragma unroll
     for (int t = 0; t < TF; ++t) {
-      if constexpr (AHEAD) {
-        if (t + 1 < TF) fetch(t + 1);
-      }
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const int r = tw * (32 * TF) + t * 32 + (v & 3) + (v >> 2) * 8 + 4 * h;
-        if (r >= tl.mlen || col >= N) continue;
-        const Cols o = cols(16 * t + v);
-        if constexpr (AHEAD) bk_put<NF>(g, tl.mbase + r, col, o.v, pg[t & 1][v], pu[t & 1][v]);
-        else bk_store<DACT, NF>(g, tl.mbase + r, col, o.v);
+        if (r < tl.mlen && col < N) bk_store<DACT, NF>(g, tl.mbase + r, col, cols(16 * t + v).v);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -1392,9 +1361,11 @@ int launch_back_as(const char* name, hipStream_t s, BkArgs a, int64_t E, int64_t
 }
 template <bool DACT>
 int launch_back(const char* name, hipStream_t s, const BkArgs& a, int64_t E, int64_t R, int bm) {
-  return bm == 256   ? launch_back_as<BkForm<4, 4, 2, 2, 1>, DACT>(name, s, a, E, R)
-         : bm == 128 ? launch_back_as<BkForm<2, 4, 2, 2, 1>, DACT>(name, s, a, E, R)
-                     : launch_back_as<BkForm<2, 8, 1, 1, 4>, DACT>(name, s, a, E, R);
+  if constexpr (!DACT) {
+    if (bm == 256) return launch_back_as<BkForm<4, 4, 2, 2, 1>, DACT>(name, s, a, E, R);
+  }
+  return bm == 128 ? launch_back_as<BkForm<2, 4, 2, 2, 1>, DACT>(name, s, a, E, R)
+                   : launch_back_as<BkForm<2, 8, 1, 1, 4>, DACT>(name, s, a, E, R);
 }
 }  // namespace
 }  // namespace moe
