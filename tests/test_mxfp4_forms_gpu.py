@@ -7,9 +7,9 @@ import pytest
 import torch
 
 from gpu_util import dev, say
-from test_mxfp4_gpu import _inside, _offsets
+from test_mxfp4_gpu import _experts, _inside, _offsets
 
-from moe_mi355 import _lib
+from moe_mi355 import _lib, ops
 from oracle import mxfp4 as OX
 
 pytestmark = pytest.mark.gpu
@@ -92,3 +92,56 @@ def test_weights_of_more_than_2_gb_in_every_form(large, rows, fwd, bwd):
     _inside(y[pick], ry, ty, "y")
     rx, tx = OX.swiglu_bwd(dy[pick], hgu[pick], w, n)
     _inside(dx[pick], rx, tx, "dxp")
+
+
+@pytest.mark.parametrize("H,F,counts,fwd,dxp,split", [
+    (1024, 4096, [300, 0, 513, 1], 64, 64, (True, True)),          # the down projection and dxp split
+    (4096, 4096, [700, 600], 64, 64, (False, True)),               # dact and dxp
+    (160, 2080, [3000, 0, 1201], 64, 128, (True, True)),           # dxp of 128 rows, odd numbers of blocks
+    (256, 8192, [1300, 1400], 128, 128, (True, True)),
+    (128, 16384, [1000, 0, 1303], 256, 128, (True, True)),
+    (8192, 2048, [4200], 64, 256, (True, True)),                   # dact of 128 rows, dxp of 256
+], ids=lambda v: str(v)[:24])
+def test_two_graphs_of_products_that_are_split(H, F, counts, fwd, dxp, split):
+    """Products whose last tiles are split over the reduction: two graphs, each with its own partial tiles, replayed in turn
+    with eager calls between; and either product against the oracle."""
+    say(f"[mxfp4 split graphs] H={H} F={F} {counts}")
+    E, R = len(counts), sum(counts)
+    q, s, w = _experts(E, F, H, H + F)
+    offs = _offsets(counts).to(dev())
+    g = torch.Generator(device=dev()).manual_seed(R)
+    x, dy = (torch.randn(2, R, H, device=dev(), generator=g).bfloat16() for _ in range(2))
+    hgu, y, p = _forward(x[0], q, s, offs, F)
+    tiles = lambda bm: sum(-(-c // bm) for c in counts)  # noqa: E731
+    assert p.tiles() == tiles(fwd) and p.split() == split[0]
+    dx, p = _backward(dy[0], hgu, q, s, offs, F)
+    assert p.tiles() == tiles(dxp) and p.split() == split[1]
+    rh, ry, th, ty = OX.swiglu_fwd(x[0], w, offs.tolist())
+    _inside(hgu, rh, th, "hgu")
+    _inside(y, ry, ty, "y")
+    rx, tx = OX.swiglu_bwd(dy[0], hgu, w, offs.tolist())
+    _inside(dx, rx, tx, "dxp")
+
+    def step(t, d):
+        h, o = ops.swiglu_forward_mxfp4(t, q, s, offs)
+        return h, o, ops.swiglu_backward_mxfp4(d, h, q, s, offs)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        buf = [(x[k].clone(), dy[k].clone()) for k in range(2)]
+        assert all(torch.equal(a, b) for a, b in zip(step(*buf[0]), (hgu, y, dx)))
+    side.synchronize()
+    graphs, outs = [], []
+    for b in buf:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            outs.append(step(*b))
+        graphs.append(gr)
+    for i in range(3):
+        for k in (1, 0):
+            buf[k][0].copy_(x[k] * (i + 1))
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[k], step(*buf[k]))), (i, k)
