@@ -119,7 +119,8 @@ __global__ __launch_bounds__(256) void k_dequant_mxfp4(const uint32_t* __restric
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t i = i0 + j * 512 + lane * 8;
-      if (i < n) store8(dst + i, w[j], __uint_as_float(b[j] << 23));  // byte 255: an infinite scale, NaNs
+      // the instruction takes the scale's exponent field: byte 0, as a float 0.0, is 2^-127, and 255 gives NaNs
+      if (i < n) store8(dst + i, w[j], __uint_as_float(b[j] << 23));
     }
   }
 }

@@ -341,3 +341,45 @@ def test_refusals():
         ops.dequant_mxfp4(q[0], s[0][:, :, :1])
     hgu, y = f(x[:0], q, s, _offsets([0, 0]).to(dev()))
     assert hgu.shape == (0, 2 * F) and y.shape == (0, H)
+
+
+def test_scale_bytes_at_the_ranges_ends():
+    """Bytes that ``quant_mxfp4`` never writes: 0 stands for 2^-127, with values down to 2^-128 (subnormal in bf16 and fp32)."""
+    q = (torch.arange(16) | (15 - torch.arange(16)) << 4).to(torch.uint8)  # every value, twice
+    q, s = q.expand(6, 16).contiguous(), torch.tensor([[0], [1], [2], [3], [252], [255]], dtype=torch.uint8)
+    for dt in (torch.bfloat16, torch.float32):
+        assert _same(ops.dequant_mxfp4(q.to(dev()), s.to(dev()), dt).cpu().double(), OX.dequant(q, s))
+
+
+@pytest.mark.parametrize("H,F,rows", [(64, 64, 3), (1568, 96, 40), (256, 256, 700), (160, 8224, 1500), (128, 16384, 1100)],
+                         ids=str)
+@pytest.mark.parametrize("byte", [0, 1, 2, 252])
+def test_products_of_scale_bytes_at_the_ranges_ends(H, F, rows, byte):
+    """Weights of one such byte against rows that bring the product back into range: a subnormal operand of a matrix
+    instruction counts in full."""
+    say(f"[mxfp4 scale byte] {byte} H={H} F={F} rows={rows}")
+    g = torch.Generator(device=dev()).manual_seed(byte + H)
+    q = [torch.randint(0, 256, (1, r, c // 2), dtype=torch.uint8, device=dev(), generator=g)
+         for r, c in ((F, H), (F, H), (H, F))]
+    r = 2.0 ** (115 - byte if byte < 3 else -122)  # rows x weights: some 2^-12 (2^3)
+    x = (torch.randn(rows, H, device=dev(), generator=g) * r).bfloat16()
+    offs = torch.tensor([0, rows], dtype=torch.int32, device=dev())
+
+    def scales(gate, up, down):
+        return [torch.full((*t.shape[:2], t.shape[2] // 16), b, dtype=torch.uint8, device=dev())
+                for t, b in zip(q, (gate, up, down))]
+
+    for gate, up in ((byte, 127), (127, byte)):  # (only the half of the matrix with that byte is looked at)
+        s = scales(gate, up, 127 if byte < 3 else 100)
+        t = torch.where(torch.arange(H, device=dev()) < 32, x, 0).bfloat16()  # one block a row: sums stay finite
+        hgu, _ = ops.swiglu_forward_mxfp4(t, q, s, offs)
+        w = [OX.dequant(a, b) for a, b in zip(q, s)]
+        rh, _, th, _ = OX.swiglu_fwd(t, w, [0, rows])
+        half = slice(0, F) if gate == byte else slice(F, 2 * F)
+        _inside(hgu[:, half], rh[:, half], th[:, half], "hgu")
+        assert float(rh[:, half].abs().median()) > 0
+    s = scales(125, 125, byte)
+    hgu = torch.randn(rows, 2 * F, device=dev(), generator=g).bfloat16()
+    dx = ops.swiglu_backward_mxfp4(x, hgu, q, s, offs)
+    rx, tx = OX.swiglu_bwd(x, hgu, [OX.dequant(a, b) for a, b in zip(q, s)], [0, rows])
+    _inside(dx, rx, tx, "dxp")
