@@ -130,7 +130,7 @@ def test_small_batches(shape):
     (1024, 8, [256] * 4, True), (1024, 8, [64] * 16, True), (1024, 8, [60] * 17, False), (1025, 8, [64] * 16, False),
     (192, 16, None, True), (193, 16, None, False), (48, 64, None, True), (49, 64, None, False), (128, 64, [64, 64], False),
     (96, 64, [1, 95], True), (20, 65, None, False),
-], ids=str)
+], ids=lambda v: str(v)[:24])
 def test_which_form_a_small_batch_takes(N, E, lengths, one):
     """One block only where its waves' sequences are short on average; either form against the oracle."""
     from moe_mi355 import _lib
@@ -283,3 +283,13 @@ def test_refusals():
         ops.balance_loss_backward(lg, out[2][:, :4], out[3], 2)
     with pytest.raises(ValueError):
         ops.balance_loss_backward(lg, out[2], out[3], 0)
+
+
+@pytest.mark.parametrize("N,E,K,lengths", [
+    (66000, 8, 2, [40000, 0, 25990]), (66000, 16, 4, [30000, 1, 0, 35000]), (66001, 15, 4, None),
+    (65700, 32, 4, [1000] * 65), (65701, 30, 8, [65700]), (33000, 64, 6, [32999]), (33001, 62, 6, [100] * 330),
+    (32900, 128, 8, [16000, 16000, 1]), (32901, 126, 32, None), (16500, 256, 8, [5] * 3300), (16501, 254, 3, [16000, 501]),
+], ids=lambda v: str(v)[:24])
+def test_long_batches(N, E, K, lengths):
+    """Batches that give every lane group several tokens: each number of lanes a token, with and without 16-byte loads."""
+    test_against_the_oracle((N, E, K, None if lengths is None else (0, lengths), True), 2.0)
