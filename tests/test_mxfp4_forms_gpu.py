@@ -145,3 +145,25 @@ def test_two_graphs_of_products_that_are_split(H, F, counts, fwd, dxp, split):
         torch.cuda.synchronize()
         for k in (0, 1):
             assert all(torch.equal(a, b) for a, b in zip(outs[k], step(*buf[k]))), (i, k)
+
+
+@pytest.mark.parametrize("H,F,E,sizes", [
+    (544, 1056, 2, (1, 16, 17, 33, 40)),           # few blocks: eight waves share a weight row's units, at any rows
+    (2048, 2048, 8, (8, 16, 17, 33, 40)),          # four waves, from 8 rows on
+    (1024, 1024, 16, (16, 17, 33, 40)),            # two waves, from 16 rows on
+], ids=["8-waves", "4-waves", "2-waves"])
+def test_a_rows_bits_within_one_few_row_form(H, F, E, sizes):
+    """With as many waves to a weight row a row's sums run in one order, whatever rows are beside it.  (How many waves there are
+    goes by the batch's rows: between those a row's last bits may differ.)"""
+    say(f"[mxfp4 row bits] H={H} F={F}")
+    q, s, _ = _experts(E, F, H, 29)
+    x = torch.randn(sizes[-1], H, device=dev(), generator=torch.Generator(device=dev()).manual_seed(1)).bfloat16()
+
+    def run(n):
+        offs = _offsets([0] * (E - 1) + [n]).to(dev())
+        return ops.swiglu_forward_mxfp4(x[:n], q, s, offs)
+
+    hgu, y = run(sizes[-1])
+    for n in sizes[:-1]:
+        a, b = run(n)
+        assert torch.equal(a, hgu[:n]) and torch.equal(b, y[:n]), n
