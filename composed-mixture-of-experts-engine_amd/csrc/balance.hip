@@ -638,8 +638,8 @@ BalanceForm balance_form(int64_t N, int64_t E, bool fwd) {
 // lpt), so with one or two sequences the other waves wait for it: up to 48 steps on average, which is all that the host knows.
 // A call in a graph of 20, us, one block | runs and their sums: E 8, one sequence of 256 tokens 7.6 | 10.5, 512 (64 steps) 11.6 | 10.7,
 // 1024 19.2 | 11.3; two, 768 tokens (48 steps) 10.0 | 11.3, 1024 12.2 | 11.3; four, 1024 9.0 | 11.5; eight 7.5 | 12.5; sixteen
-// 8.7 | 14.2.  E 16, 32 and 64 are within 0.7 us of these at the same steps.  (One of several sequences with all the
-// tokens costs what one sequence does.)
+// 8.7 | 14.2.  At the same steps E 16, 32 and 64 are within 1 us of these in the first column and 2 in the second.  (One of
+// several sequences that has nearly all the tokens costs what one sequence does.)
 bool balance_in_one(int64_t N, int64_t E, int64_t S, int lpt) {
   return S <= kOneSeqs && E <= kOneE && N <= kOneU * (kBalanceNT / lpt) && N * lpt <= 768 * S;
 }

@@ -800,6 +800,9 @@ int launch_tile(const char* name, hipStream_t s, MxArgs a, int64_t E, int64_t R)
 //                            96: 440 | 192 | 170 | 269  256: - | 425 | 382 | 430    512: - | 782 | 684 | 703
 //   E 8,   H 1024, F 4096    16: 29 | 42 | 50 | 66      32: 38 | 44 | 53 | 68       64: 62 | 55 | 58 | 73
 //                            128: - | 68 | 79 | 80      256: - | 91 | 102 | 119     512: - | 151 | 143 | 160
+// A batch that goes to one expert pays for the average, as each 32 rows read its weights again (all rows to one expert, few-row
+// form | the same in tiles of 64): 128 rows of E 8, H 4096, F 14336: 171 | 106; 2048 rows of E 128, H 2048, F 768: 71 | 45; 1200
+// rows of E 76, H 4096, F 14336: 1166 | 448 (spread evenly the same batches take 188, 86 and 1699 in the few-row form).
 int mx_rows(int64_t R, int64_t H, int64_t F, int64_t E) {
   if (H < 128 || F < 128) return 0;
   const bool even = H % 128 == 0 && F % 128 == 0;
@@ -981,9 +984,12 @@ __device__ __forceinline__ BkTile bk_tile(const BkArgs& g, int L, int lane) {
 // registers, and rows leave in whole segments.  The rows go through LDS in 64-wide slices, as in k_mx_tile: fetched by the lanes
 // that use them they are 64 cache accesses a load, and those bounded the products (5.4 ms for dxp below).
 //
-// What bounds them: matrix instructions and the conversion's issue with 256 rows (one wave a SIMD, MFMA busy 62%), the
-// epilogue's 1.9 GB in the product with Wd, whose two blocks a CU run under each other's.  16384 rows, E 8, H 4096, F 14336:
-// dact 2.0-2.2 ms, dxp 3.35 ms (1.92 TFLOP and 3.85: 920 and 1150 TFLOP/s); the products on bf16 weights 2.01 and 3.35.
+// What bounds them: with 256 rows no one part of the loop (one wave a SIMD, MFMA busy 62% at 1.77 GHz).  In a copy that leaves a
+// part out at a time dxp takes, of 3.10 ms: without the conversions 2.79, the weights' loads 2.74, the rows' refills of LDS
+// 2.60, the scales 3.00, all four 2.10 (each a little flattered, as constant operands draw less power); dact, of 1.95 ms:
+// 1.81, 1.65, 1.68, 1.79 and 1.16, with its epilogue's 1.9 GB, which two blocks a CU run under each other's loops, inside.
+// 16384 rows, E 8, H 4096, F 14336: dact 1.95-2.2 ms, dxp 3.1-3.35 ms (1.92 TFLOP and 3.85: 920-985 and 1150-1240 TFLOP/s);
+// the products on bf16 weights 2.01 and 3.35.
 
 // A form: a wave has 32 TF rows by 32 NF columns, a block's four waves lie WT on the rows, WF on the columns and KS along the
 // reduction.
