@@ -279,6 +279,8 @@ class MoERouter(torch.nn.Module):
         if self._seq_later is None:
             return self._seq_last
         shape, logits, idx, coef = self._seq_later
+        for t in (logits, idx):  # a read on another stream than the forward's: the next forward frees them
+            t.record_stream(torch.cuda.current_stream(t.device))
         with torch.no_grad():
             loss, _z, counts, tokens, _ = balance_loss(logits, idx, self._row_offsets(shape, logits.device), None, coef, 0.0)
         return loss, counts, tokens

@@ -133,3 +133,25 @@ def test_values_of_the_last_forward_can_be_set():
         r.seq_balance_coef = 0.0
         layer(_tokens())
     assert r.last_seq_balance_loss is None and r.last_seq_counts is None and r.last_seq_tokens is None
+
+
+def test_read_on_another_stream_than_the_forwards():
+    """The read's kernels wait behind other work while later forwards, on their own stream, take and fill new memory."""
+    say("[seq balance streams]")
+    layer = _layer(check_numerics=False)
+    r, side = layer.router, torch.cuda.Stream()
+    xs = [_tokens(20 + i) for i in range(8)]
+    with torch.no_grad():
+        layer.forward_mxfp4(xs[0])
+        want = r.last_seq_balance_loss, r.last_seq_counts, r.last_seq_tokens
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            layer.forward_mxfp4(xs[0])
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(20_000_000)
+        got = r.last_seq_balance_loss, r.last_seq_counts, r.last_seq_tokens
+        with torch.cuda.stream(side):
+            for x in xs[1:]:
+                layer.forward_mxfp4(x)
+        torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
