@@ -444,8 +444,9 @@ class DistributedMoELayer(nn.Module):
             raise ValueError(f"load_mxfp4: the layer has {len(self.local_expert_ids)} experts of ffn_dim {self.ffn_dim}, got "
                              f"{wq[0].shape[0]} of {F_}")
         dev = self.router.gate_w.device
-        for name, t in zip(_MXFP4, wq + ws):
-            setattr(self, name, t.detach().to(dev))
+        with torch.inference_mode(False):  # tensors of inference mode could not be saved for a backward
+            for name, t in zip(_MXFP4, wq + ws):
+                setattr(self, name, (t.clone() if t.is_inference() else t.detach()).to(dev))
         return self._mxfp4_weights()
 
     def _mxfp4_weights(self):

@@ -46,6 +46,15 @@ def test_state_dict_keeps_the_references_keys():
     assert a.mxfp4_gate is not None and b.mxfp4_gate is None
 
 
+def test_taken_in_inference_mode_they_can_be_trained_around():
+    layer = _layer()
+    with torch.inference_mode():
+        q, s = _weights()
+        got = layer.load_mxfp4(q, s)
+    assert not any(t.is_inference() for t in got[0] + got[1])
+    assert all(torch.equal(a, b) for a, b in zip(got[0] + got[1], q + s))
+
+
 def test_dropped_full_width_weights():
     layer = _layer()
     layer.load_mxfp4(*_weights())

@@ -47,3 +47,17 @@ def test_moved_handed_in_and_alone():
     a = torch.autograd.grad(other.forward_mxfp4(y).float().square().sum(), [y, other.router.gate_w])
     b = torch.autograd.grad(layer.forward_mxfp4(y).float().square().sum(), [y, layer.router.gate_w])
     assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_quantized_and_served_in_inference_mode_then_trained():
+    say("[mxfp4 weights inference mode]")
+    layer = _layer(2)
+    x = torch.randn(5, H, device=dev()).to(B)
+    with torch.inference_mode():
+        layer.quantize_mxfp4()
+        want = layer.forward_mxfp4(x)
+    y = x.clone().requires_grad_(True)
+    out = layer.forward_mxfp4(y)
+    assert torch.equal(out, want)
+    out.float().square().sum().backward()
+    assert float(y.grad.abs().max()) > 0 and float(layer.router.gate_w.grad.abs().max()) > 0
