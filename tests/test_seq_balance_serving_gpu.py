@@ -155,3 +155,18 @@ def test_read_on_another_stream_than_the_forwards():
                 layer.forward_mxfp4(x)
         torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_served_in_inference_mode_read_outside():
+    say("[seq balance inference mode]")
+    layer = _layer(check_numerics=False)
+    r, x = layer.router, _tokens(40)
+    with torch.inference_mode():
+        layer.forward_mxfp4(x)
+    got = r.last_seq_balance_loss, r.last_seq_counts, r.last_seq_tokens
+    with torch.inference_mode():
+        inside = r.last_seq_balance_loss, r.last_seq_counts, r.last_seq_tokens
+    layer.forward_mxfp4(x)  # a gradient is recorded: formed at once
+    want = r.last_seq_balance_loss, r.last_seq_counts, r.last_seq_tokens
+    assert want[0].requires_grad and not got[0].requires_grad
+    assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(got, want, inside))
