@@ -185,6 +185,10 @@ int check_launch(const char* what);
 int quant_rows_fp8(const void* src, int src_dtype, int64_t rows, int64_t cols, int64_t ld, void* dst, float* scale,
                    const int* row_limit, hipStream_t s);
 
+// ---- int8 row quantization (csrc/int8.hip), row_limit as above ----
+int quant_rows_int8(const void* src, int src_dtype, int64_t rows, int64_t cols, int64_t ld, void* dst, float* scale,
+                    const int* row_limit, hipStream_t s);
+
 // ---- the forward products for few rows per expert (csrc/gemm_small.hip); elem: bytes of a value (2 bf16, 4 fp32) ----
 bool swiglu_small_takes(int64_t R, int64_t H, int64_t F, int64_t E, int elem);
 int swiglu_small_fwd(bool f32, const void* xp, const void* w_gate, const void* w_up, const void* w_down,

@@ -1,10 +1,7 @@
 // e4m3 (OCP fp8) payloads of the expert FFN forward.
 //
-// Each row gets one fp32 scale, absmax / 448 (448 is the largest e4m3 value), and its elements are
-// multiplied by inv = 448 / absmax (one division per row) in fp32 and rounded to nearest even by
-// v_cvt_pk_fp8_f32.  A row whose absmax is below 2^-118 -- all-zero rows, and rows so small that 448 / absmax
-// would overflow fp32 (it does below 448 / FLT_MAX ~ 1.3e-36), turning 0 * inv into NaN -- is treated as a
-// zero row: scale 1, inv 1 (its elements, all below 2^-118, round to +-0).
+// Each row gets one fp32 scale and its elements are rounded to nearest even by v_cvt_pk_fp8_f32, by the rule in quant8.h
+// (one division per row).
 //
 // k_permute_fp8     the dispatch payload: each token row is quantized once and written to the rows of its
 //                   slots (the rows k_permute fills) at one byte per element -- half the bytes of the bf16
@@ -15,18 +12,9 @@
 // one 8-byte word.  bf16 rows of up to 16K elements stay in registers between the passes (one read of the
 // row from memory); longer rows and fp32 rows are read twice.
 #include "common.h"
+#include "quant8.h"
 
 namespace moe {
-
-constexpr float kE4M3Max = 448.f;
-constexpr float kQuantTiny = 0x1p-118f;  // smallest absmax quantized with its own scale: 448 / 2^-118 < FLT_MAX
-
-__device__ __forceinline__ void row_scale(float amax, float& sc, float& inv) {
-  const bool live = amax >= kQuantTiny;
-  sc = live ? amax / kE4M3Max : 1.f;
-  inv = live ? kE4M3Max / amax : 1.f;
-}
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <typename T>
 __device__ __forceinline__ void q_load8(const T* p, float (&v)[8]);
@@ -61,7 +49,7 @@ __device__ __forceinline__ void quant_row(const T* __restrict__ src, int cols, u
   }
   amax = wave_max(amax);
   float sc, inv;
-  row_scale(amax, sc, inv);
+  e4m3_row_scale(amax, sc, inv);
   if (lane == 0) *scale = sc;
   for (int c = lane * 8; c < cols; c += 512) {
     float v[8];
@@ -96,7 +84,7 @@ __device__ __forceinline__ void quant_row_reg(const uint16_t* __restrict__ src, 
 #pragma unroll
   for (int j = 0; j < NCH; ++j) __asm__ volatile("" : "+v"(w[j]));
   float sc, inv;
-  row_scale(amax, sc, inv);
+  e4m3_row_scale(amax, sc, inv);
   if (lane == 0) *scale = sc;
 #pragma unroll
   for (int j = 0; j < NCH; ++j) {
@@ -165,7 +153,7 @@ __global__ __launch_bounds__(256) void k_permute_fp8(const T* __restrict__ x, co
     }
     amax = wave_max(amax);
     float sc, inv;
-    row_scale(amax, sc, inv);
+    e4m3_row_scale(amax, sc, inv);
     for (int kw = 0; kw < K; kw += 64) {
       const int kn = min(K - kw, 64);
       const int mine = lane < kn ? slot_row[t * K + kw + lane] : -1;

@@ -23,10 +23,13 @@
 //                   (EP = 0) or u = dxn + G wg^T (EP = 8/16: the router's gradient of xn formed in place from
 //                   G = dL/dlogits, never written to HBM), u rounded to the storage type.  dgamma += u xhat
 //                   is kept per lane in registers, folded over the block's waves in LDS and over blocks by
-//                   k_rmsnorm_dgamma.
+//                   k_rmsnorm_dgamma.  EP = 2 adds a further gradient of x to dx.
+// k_rmsnorm_ext     the norm between two blocks: h = x + residual (rounded to the storage type and written), the norm of h,
+//                   and its output in the storage type, in 8 bits with a scale a row (quant8.h), or in both.
 #include <type_traits>
 
 #include "common.h"
+#include "quant8.h"
 #include "router_fin.h"
 
 namespace moe {
@@ -337,6 +340,137 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(NormFwdArgs a) {
   }
 }
 
+// The norm with the residual's addition and outputs in 8 bits.
+//   RES  h = x + residual, rounded to the storage type and written; the norm is of those rounded values
+//   Q    0: xn (and rstd); 1 / 2: xn's fp32 values in int8 / e4m3 with a scale a row, and xn too where the caller keeps it
+// One pass over memory: a row and its residual are held in registers, and the next row's pieces are requested as soon as this
+// row's are used for the last time.
+struct NormExtArgs {
+  const void* x;
+  const void* res;
+  const void* gamma;
+  int gamma_dt;
+  float eps;
+  int N, H;
+  void* h;
+  void* xn;      // Q: may be null
+  float* rstd;   // Q: null
+  uint8_t* q;
+  float* scale;
+};
+
+template <typename TX, int NCH, bool RES, int Q>
+__global__ __launch_bounds__(256) void k_rmsnorm_ext(NormExtArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t nsm[];
+  f32x4* s_gam = reinterpret_cast<f32x4*>(nsm);  // [NCH * 2][64]
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wv = norm_wave();
+  const int N = a.N, H = a.H;
+  const TX* __restrict__ x = static_cast<const TX*>(a.x);
+  const TX* __restrict__ res = static_cast<const TX*>(a.res);
+  const int rowbytes = H * (int)sizeof(TX);
+  const int nwt = gridDim.x * 4;
+  int t = blockIdx.x * 4 + wv;
+  auto rows = [&](const TX* base, int row) { return buf_rsrc(base + (int64_t)row * H, row < N ? rowbytes : 0); };
+  RowFrag<TX, NCH> f, fr;
+  if (t < N) {
+    frag_load_all(f, rows(x, t), lane);
+    if constexpr (RES) frag_load_all(fr, rows(res, t), lane);
+  }
+  if (a.gamma_dt == MOE_F32) stage_gamma<float, NCH>(s_gam, static_cast<const float*>(a.gamma), H, tid, 256);
+  else stage_gamma<uint16_t, NCH>(s_gam, static_cast<const uint16_t*>(a.gamma), H, tid, 256);
+  __syncthreads();
+  for (; t < N; t += nwt) {
+    row_fence();
+    const int tn = t + nwt;
+    const buf_rsrc_t rn = rows(x, tn);
+    if constexpr (RES) {
+      const buf_rsrc_t rr = rows(res, tn);
+      TX* hrow = static_cast<TX*>(a.h) + (int64_t)t * H;
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        float v[8], u[8];
+        frag_get(f, j, v);
+        frag_get(fr, j, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += u[i];
+        const int c = lane + 64 * j;
+        u32x4 pk;
+        chunk_store<TX>(hrow, c, 8 * c < H, v, pk);
+        if constexpr (std::is_same<TX, uint16_t>::value) {
+          f.w[j] = pk;
+        } else {
+          f.w[2 * j] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+          f.w[2 * j + 1] = u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+        }
+        frag_load(fr, rr, j, lane);
+        chunk_fence();
+      }
+    }
+    const float r = rsqrtf(frag_sumsq(f) / (float)H + a.eps);
+    if constexpr (Q == 0) {
+      if (lane == 0) a.rstd[t] = r;
+    }
+    TX* const orow = static_cast<TX*>(a.xn) + (int64_t)t * H;
+    auto normed = [&](int j, float(&o)[8]) {
+      float v[8], g[8];
+      frag_get(f, j, v);
+      gamma_get<NCH>(s_gam, j, lane, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = (v[i] * r) * g[i];
+    };
+    uint32_t mb = 0;
+    float amax = 0.f;
+    if constexpr (Q != 0) {
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        float o[8];
+        normed(j, o);
+        if (a.xn != nullptr) {
+          u32x4 pk;
+          chunk_store<TX>(orow, lane + 64 * j, 8 * (lane + 64 * j) < H, o, pk);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (Q == 1) mb = max(mb, abs_bits(o[i]));
+          else amax = fmaxf(amax, fabsf(o[i]));
+        }
+        chunk_fence();
+      }
+    }
+    Int8Row qr{};
+    float inv = 0.f;
+    if constexpr (Q == 1) {
+      mb = row16_max_u32(mb);
+      mb = max(mb, (uint32_t)__shfl_xor((int)mb, 16));
+      qr = int8_row(max(mb, (uint32_t)__shfl_xor((int)mb, 32)));
+      if (lane == 0) a.scale[t] = qr.scale;
+    } else if constexpr (Q == 2) {
+      float sc;
+      e4m3_row_scale(wave_max(amax), sc, inv);
+      if (lane == 0) a.scale[t] = sc;
+    }
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      float o[8];
+      normed(j, o);
+      const int c = lane + 64 * j;
+      if constexpr (Q == 0) {
+        u32x4 pk;
+        chunk_store<TX>(orow, c, 8 * c < H, o, pk);
+      } else {
+        u32x2 p;
+        if constexpr (Q == 1) p = int8_pack8(o, qr);
+        else p = e4m3_pack8(o, inv);
+        if (8 * c < H) *reinterpret_cast<u32x2*>(a.q + (int64_t)t * H + 8 * c) = p;
+      }
+      frag_load(f, rn, j, lane);
+      chunk_fence();
+    }
+  }
+}
+
 // Forward with the router fused in (bf16 x and gate, E <= EP in {8, 16}).  One block per CU (the gate image
 // fills most of the LDS).  Each wave takes R rows at a time, t_r = t0 + r * stride: one LDS read of the gate
 // serves all R rows' dot products and one reduce-scatter + routing pass serves all R tokens (token r is
@@ -526,6 +660,7 @@ struct NormBwdArgs {
   const float* rstd;
   const void* dxn;    // may be null (no gradient of xn from the expert path)
   const void* dxn2;   // MODE 1: a second gradient of xn
+  const void* dh;     // MODE 2: a gradient of x itself
   const uint16_t* G;  // MODE 8 / 16: dL/dlogits, bf16 [N][MODE]
   const uint16_t* wg;  // MODE 8 / 16: gate [H, E] bf16
   int E;
@@ -534,7 +669,7 @@ struct NormBwdArgs {
   float* part_dg;  // [gridDim.x][H]
 };
 
-// MODE: 0 = dxn, 1 = dxn + dxn2, 8 / 16 = dxn + G wg^T with E <= MODE experts.
+// MODE: 0 = dxn, 1 = dxn + dxn2, 2 = dxn with dh added to dx, 8 / 16 = dxn + G wg^T with E <= MODE experts.
 template <int NCH, int MODE>
 constexpr size_t norm_bwd_lds() { return (size_t)NCH * 4096 + (MODE >= 8 ? (size_t)MODE * NCH * 1024 : 0); }
 
@@ -547,6 +682,7 @@ template <typename TX, typename TG, int NCH, int MODE>
 __global__ __launch_bounds__(norm_bwd_waves<MODE>() * 64) __attribute__((amdgpu_waves_per_eu(NCH <= 8 ? 2 : 1)))
 void k_rmsnorm_bwd(NormBwdArgs a) {
   constexpr bool TWO = MODE == 1;
+  constexpr bool DH = MODE == 2;
   constexpr int EP = MODE >= 8 ? MODE : 0;
   constexpr int NWV = norm_bwd_waves<MODE>();
   constexpr int NT = NWV * 64;
@@ -569,11 +705,13 @@ void k_rmsnorm_bwd(NormBwdArgs a) {
   auto rows = [&](const TX* base, int row) {
     return buf_rsrc(base ? base + (int64_t)row * H : x, (base && row < N) ? rowbytes : 0);
   };
-  RowFrag<TX, NCH> fx, fg, fg2;  // the first row is requested before the LDS staging (latencies overlap)
+  const TX* __restrict__ dh = static_cast<const TX*>(a.dh);
+  RowFrag<TX, NCH> fx, fg, fg2, fh;  // the first row is requested before the LDS staging (latencies overlap)
   if (t < N) {
     frag_load_all(fx, rows(x, t), lane);
     frag_load_all(fg, rows(dxn, t), lane);
     if constexpr (TWO) frag_load_all(fg2, rows(dxn2, t), lane);
+    if constexpr (DH) frag_load_all(fh, rows(dh, t), lane);
   }
   stage_gamma<TG, NCH>(s_gam, static_cast<const TG*>(a.gamma), H, tid, NT);
   if constexpr (EP > 0)
@@ -589,6 +727,7 @@ void k_rmsnorm_bwd(NormBwdArgs a) {
     row_fence();
     const int tn = t + nwt;
     const buf_rsrc_t rx = rows(x, tn), rg = rows(dxn, tn), rg2 = rows(TWO ? dxn2 : nullptr, tn);
+    const buf_rsrc_t rh = rows(DH ? dh : nullptr, tn);
     const float r = a.rstd[t];
     u32x4 gt[EP >= 8 ? EP / 8 : 1];
     if constexpr (EP > 0) {
@@ -656,6 +795,13 @@ void k_rmsnorm_bwd(NormBwdArgs a) {
       gamma_get<NCH>(s_gam, j, lane, gm);
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = r * (gm[i] * uu[i] - (v[i] * r) * c);
+      if constexpr (DH) {
+        float hh[8];
+        frag_get(fh, j, hh);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] += hh[i];
+        frag_load(fh, rh, j, lane);
+      }
       const int cc = lane + 64 * j;
       u32x4 pk;
       chunk_store<TX>(drow, cc, 8 * cc < H, o, pk);
@@ -798,6 +944,19 @@ int launch_norm_fwd(int nblk, hipStream_t s, const NormFwdArgs& a) {
   return check_launch("k_rmsnorm_fwd");
 }
 
+template <typename TX, int NCH>
+int launch_norm_ext(int q, bool res, int nblk, hipStream_t s, const NormExtArgs& a) {
+  constexpr size_t lds = norm_fwd_lds<NCH>();  // at most 32 KB
+#define MOE_EXT(RES, Q, NAME) MOE_LAUNCH(NAME, (k_rmsnorm_ext<TX, NCH, RES, Q>), dim3(nblk), dim3(256), lds, s, a)
+  if (q == 0) MOE_EXT(true, 0, "k_rmsnorm_residual");
+  else if (q == 1 && res) MOE_EXT(true, 1, "k_rmsnorm_residual_int8");
+  else if (q == 1) MOE_EXT(false, 1, "k_rmsnorm_int8");
+  else if (res) MOE_EXT(true, 2, "k_rmsnorm_residual_e4m3");
+  else MOE_EXT(false, 2, "k_rmsnorm_e4m3");
+#undef MOE_EXT
+  return check_launch("k_rmsnorm_ext");
+}
+
 template <typename TG, int NCH, int EP>
 int launch_norm_route(int nblk, hipStream_t s, const NormFwdArgs& a) {
   constexpr size_t lds = norm_route_lds<NCH, EP, kRouteRows>();
@@ -846,6 +1005,53 @@ extern "C" int moe_rmsnorm_fwd(const void* x, int x_dtype, const void* gamma, in
   int rc = 0;
   MOE_NORM_DT(x_dtype, gamma_dtype, MOE_NCH(norm_nch(H), rc = (launch_norm_fwd<TX, TG, NCHv>(nblk, s, a))));
   return rc;
+}
+
+namespace {
+int norm_ext(const char* what, int q, const void* x, const void* res, int x_dtype, const void* gamma, int gamma_dtype, float eps,
+             int64_t N, int64_t H, void* h, void* xn, float* rstd, void* q_out, float* scale, void* stream) {
+  if (int rc = norm_check(what, N, H, x_dtype, gamma_dtype)) return rc;
+  if (q != 0 && H % 16) return fail_arg("%s: H=%lld: rows in 8 bits need H %% 16 == 0", what, (long long)H);
+  if (N == 0) return 0;
+  if (!x || !gamma || (res && !h) || (q == 0 && (!res || !xn || !rstd)) || (q != 0 && (!q_out || !scale)))
+    return fail_arg("%s: null pointer argument", what);
+  if (!al16p(x) || !al16p(res) || !al16p(gamma) || !al16p(h) || !al16p(xn) || !al16p(q_out))
+    return fail_arg("%s: misaligned pointer", what);
+  NormExtArgs a{};
+  a.x = x;
+  a.res = res;
+  a.gamma = gamma;
+  a.gamma_dt = gamma_dtype;
+  a.eps = eps;
+  a.N = (int)N;
+  a.H = (int)H;
+  a.h = h;
+  a.xn = xn;
+  a.rstd = rstd;
+  a.q = static_cast<uint8_t*>(q_out);
+  a.scale = scale;
+  const int nblk = norm_fwd_blocks(N);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  int rc = 0;
+  if (x_dtype == MOE_BF16) MOE_NCH(norm_nch(H), rc = (launch_norm_ext<uint16_t, NCHv>(q, res != nullptr, nblk, s, a)));
+  else MOE_NCH(norm_nch(H), rc = (launch_norm_ext<float, NCHv>(q, res != nullptr, nblk, s, a)));
+  return rc;
+}
+}  // namespace
+
+extern "C" int moe_rmsnorm_residual_fwd(const void* x, const void* residual, int x_dtype, const void* gamma, int gamma_dtype,
+                                        float eps, int64_t N, int64_t H, void* h_out, void* xn_out, float* rstd_out,
+                                        void* stream) {
+  return norm_ext("moe_rmsnorm_residual_fwd", 0, x, residual, x_dtype, gamma, gamma_dtype, eps, N, H, h_out, xn_out, rstd_out,
+                  nullptr, nullptr, stream);
+}
+
+extern "C" int moe_rmsnorm_quant(const void* x, const void* residual, int x_dtype, const void* gamma, int gamma_dtype,
+                                 float eps, int64_t N, int64_t H, int q_format, void* q_out, float* scale_out, void* h_out,
+                                 void* xn_out, void* stream) {
+  if (q_format != MOE_INT8 && q_format != MOE_E4M3) return fail_arg("moe_rmsnorm_quant: rows in int8 or e4m3, got %d", q_format);
+  return norm_ext("moe_rmsnorm_quant", q_format == MOE_INT8 ? 1 : 2, x, residual, x_dtype, gamma, gamma_dtype, eps, N, H,
+                  residual ? h_out : nullptr, xn_out, nullptr, q_out, scale_out, stream);
 }
 
 extern "C" size_t moe_rmsnorm_router_fwd_workspace(int64_t N, int64_t H, int64_t E, int64_t K, int x_dtype,
@@ -960,6 +1166,36 @@ extern "C" int moe_rmsnorm_bwd(const void* x, int x_dtype, const void* gamma, in
     MOE_NORM_DT(x_dtype, gamma_dtype, MOE_NCH(norm_nch(H), rc = (launch_norm_bwd<TX, TG, NCHv, 0>(nblk, s, a))));
   if (rc) return rc;
   return launch_dgamma(s, part, nblk, H, dgamma_out, gamma_dtype);
+}
+
+extern "C" int moe_rmsnorm_residual_bwd(const void* h, int x_dtype, const void* gamma, int gamma_dtype, const float* rstd,
+                                        const void* dxn, const void* dh, int64_t N, int64_t H, void* d_out, void* dgamma_out,
+                                        void* workspace, size_t ws_bytes, void* stream) {
+  if (!dh) return moe_rmsnorm_bwd(h, x_dtype, gamma, gamma_dtype, rstd, dxn, nullptr, N, H, d_out, dgamma_out, workspace,
+                                  ws_bytes, stream);
+  if (int rc = norm_check("moe_rmsnorm_residual_bwd", N, H, x_dtype, gamma_dtype)) return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (!gamma || !dgamma_out) return fail_arg("moe_rmsnorm_residual_bwd: null pointer argument");
+  if (N == 0) return launch_dgamma(s, nullptr, 0, H, dgamma_out, gamma_dtype);
+  if (!h || !rstd || !d_out || !al16p(h) || !al16p(gamma) || !al16p(dxn) || !al16p(dh) || !al16p(d_out))
+    return fail_arg("moe_rmsnorm_residual_bwd: null or misaligned pointer");
+  const int nblk = norm_bwd_blocks(N);
+  if (ws_bytes < moe_rmsnorm_bwd_workspace(N, H) || !workspace)
+    return set_error("moe_rmsnorm_residual_bwd: workspace too small"), MOE_EWORKSPACE;
+  NormBwdArgs a{};
+  a.x = h;
+  a.gamma = gamma;
+  a.rstd = rstd;
+  a.dxn = dxn;
+  a.dh = dh;
+  a.N = (int)N;
+  a.H = (int)H;
+  a.dx = d_out;
+  a.part_dg = static_cast<float*>(workspace);
+  int rc = 0;
+  MOE_NORM_DT(x_dtype, gamma_dtype, MOE_NCH(norm_nch(H), rc = (launch_norm_bwd<TX, TG, NCHv, 2>(nblk, s, a))));
+  if (rc) return rc;
+  return launch_dgamma(s, a.part_dg, nblk, H, dgamma_out, gamma_dtype);
 }
 
 namespace {

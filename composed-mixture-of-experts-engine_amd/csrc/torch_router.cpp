@@ -519,6 +519,235 @@ at::Tensor op_swiglu_backward_mxfp4(const at::Tensor& dy_in, const at::Tensor& h
   return dxp;
 }
 
+// ---- rows in 8 bits, the norm that gives them, int8 products ----
+// With one decoded token these calls' kernels are a few microseconds, so their arguments are checked here.
+
+// All given tensors on one GPU (the messages of _lib.require_device).
+void one_gpu(std::initializer_list<const at::Tensor*> ts) {
+  const at::Tensor* first = nullptr;
+  for (const at::Tensor* t : ts) {
+    if (t == nullptr || !t->defined()) continue;
+    if (!t->is_cuda())
+      throw std::runtime_error("moe_mi355 runs on an AMD Instinct GPU (gfx950) only; got a tensor on " + t->device().str() +
+                               ". Move the module and inputs to the GPU.");
+    if (first == nullptr) first = t;
+    else if (t->device() != first->device())
+      throw std::runtime_error("moe_mi355: tensors on different devices (" + first->device().str() + " vs " +
+                               t->device().str() + ")");
+  }
+}
+const at::Tensor* opt(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
+
+std::string shape_of(const at::Tensor& t) {
+  std::string s = "[";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + "]";
+}
+void need(bool ok, const char* what, const std::string& msg) {
+  if (!ok) throw pybind11::value_error(std::string(what) + ": " + msg);
+}
+void need_type(bool ok, const char* what, const std::string& msg) {
+  if (!ok) throw pybind11::type_error(std::string(what) + ": " + msg);
+}
+bool is_float(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
+void need_shape(const at::Tensor& t, at::IntArrayRef want, const char* what, const char* name) {
+  if (t.sizes() == want) return;
+  std::string s = "[";
+  for (size_t i = 0; i < want.size(); ++i) s += (i ? ", " : "") + std::to_string(want[i]);
+  throw pybind11::value_error(std::string(what) + ": " + name + " must be " + s + "], got " + shape_of(t));
+}
+
+std::tuple<at::Tensor, at::Tensor> op_quant_rows_int8(const at::Tensor& t_in) {
+  const char* const what = "quant_rows_int8";
+  one_gpu({&t_in});
+  need_type(is_float(t_in), what, "rows are float32 or bfloat16");
+  need(t_in.dim() >= 1 && t_in.size(-1) >= 16 && t_in.size(-1) % 16 == 0, what,
+       "the last dim must be a positive multiple of 16, got " + shape_of(t_in));
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(t_in.device());
+  const at::Tensor t = t_in.contiguous();
+  const int64_t cols = t.size(-1), rows = t.numel() / cols;
+  at::Tensor q = at::empty(t.sizes(), t.options().dtype(at::kChar));
+  at::Tensor sc = at::empty(t.sizes().slice(0, t.dim() - 1), t.options().dtype(at::kFloat));
+  check_rc(moe_quant_rows_int8(t.data_ptr(), code_of(t), rows, cols, cols, q.data_ptr(), sc.data_ptr<float>(), stream_of(t)),
+           "moe_quant_rows_int8");
+  return {q, sc};
+}
+
+at::Tensor op_dequant_rows(const at::Tensor& q_in, const at::Tensor& sc_in, bool bf16) {
+  const char* const what = "dequant_rows";
+  one_gpu({&q_in, &sc_in});
+  need_type(q_in.scalar_type() == at::kChar || q_in.scalar_type() == at::kByte, what, "q is int8, or uint8 (e4m3 bytes)");
+  need_type(sc_in.scalar_type() == at::kFloat, what, "scale is float32");
+  need(q_in.dim() >= 1 && q_in.size(-1) >= 16 && q_in.size(-1) % 16 == 0, what,
+       "the last dim must be a positive multiple of 16, got " + shape_of(q_in));
+  need_shape(sc_in, q_in.sizes().slice(0, q_in.dim() - 1), what, "scale");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q_in.device());
+  const at::Tensor q = q_in.contiguous(), sc = sc_in.contiguous();
+  at::Tensor v = at::empty(q.sizes(), q.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  const int64_t cols = q.size(-1);
+  check_rc(moe_dequant_rows(q.data_ptr(), q.scalar_type() == at::kChar ? MOE_INT8 : MOE_E4M3, sc.data_ptr<float>(),
+                            q.numel() / cols, cols, v.data_ptr(), code_of(v), stream_of(q)),
+           "moe_dequant_rows");
+  return v;
+}
+
+void need_rows_int8(const at::Tensor& q, const at::Tensor& sc, const char* what) {
+  need_type(q.scalar_type() == at::kChar && sc.scalar_type() == at::kFloat, what, "rows are int8 and their scales float32");
+  need(q.dim() >= 1, what, "rows must have a dim to sum over");
+  need_shape(sc, q.sizes().slice(0, q.dim() - 1), what, "the rows' scales");
+}
+void need_weight_int8(const at::Tensor& w, const at::Tensor& sw, const char* what) {
+  need_type(w.scalar_type() == at::kChar && sw.scalar_type() == at::kFloat, what,
+            "weights are int8 and their scales float32");
+  need(w.is_contiguous() && sw.is_contiguous(), what, "weights and their scales must be contiguous");
+}
+void need_offsets(const at::Tensor& o, int64_t E, const char* what) {
+  need(o.scalar_type() == at::kInt && o.dim() == 1 && o.size(0) == E + 1 && o.is_contiguous(), what,
+       "offsets must be contiguous int32 [" + std::to_string(E + 1) + "]");
+}
+
+at::Tensor op_matmul_int8(const at::Tensor& q_in, const at::Tensor& sc_in, const at::Tensor& wq, const at::Tensor& wsc,
+                          const OptTensor& offsets, bool bf16) {
+  const char* const what = "matmul_int8";
+  one_gpu({&q_in, &sc_in, &wq, &wsc, opt(offsets)});
+  need_rows_int8(q_in, sc_in, what);
+  need_weight_int8(wq, wsc, what);
+  const bool grouped = offsets.has_value();
+  need(wq.dim() == (grouped ? 3 : 2), what,
+       std::string("wq must be ") + (grouped ? "[E, N, K] with offsets" : "[N, K] without offsets") + ", got " + shape_of(wq));
+  need_shape(wsc, wq.sizes().slice(0, wq.dim() - 1), what, "wscale");
+  const int64_t K = wq.size(-1), N = wq.size(-2), E = grouped ? wq.size(0) : 1;
+  need(q_in.size(-1) == K && (!grouped || q_in.dim() == 2), what,
+       "rows " + shape_of(q_in) + " do not go with weights " + shape_of(wq));
+  if (grouped) need_offsets(*offsets, E, what);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q_in.device());
+  const at::Tensor q = q_in.contiguous(), sc = sc_in.contiguous();
+  std::vector<int64_t> ys = q.sizes().vec();
+  ys.back() = N;
+  at::Tensor y = at::empty(ys, q.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  check_rc(moe_matmul_int8(q.data_ptr(), sc.data_ptr<float>(), wq.data_ptr(), wsc.data_ptr<float>(),
+                           static_cast<const int*>(ptr(offsets)), sc.numel(), K, N, E, y.data_ptr(), code_of(y), stream_of(q)),
+           "moe_matmul_int8");
+  return y;
+}
+
+at::Tensor op_swiglu_forward_int8(const at::Tensor& xq_in, const at::Tensor& sx_in, const std::vector<at::Tensor>& wq,
+                                  const std::vector<at::Tensor>& ws, const at::Tensor& offsets, const OptTensor& row_slot,
+                                  int64_t top_k) {
+  const char* const what = "swiglu_forward_int8";
+  need(wq.size() == 3 && ws.size() == 3, what, "wq and wscale are (gate, up, down)");
+  one_gpu({&xq_in, &sx_in, &wq[0], &wq[1], &wq[2], &ws[0], &ws[1], &ws[2], &offsets, opt(row_slot)});
+  need_rows_int8(xq_in, sx_in, what);
+  for (int i = 0; i < 3; ++i) need_weight_int8(wq[i], ws[i], what);
+  need(xq_in.dim() == 2 && wq[0].dim() == 3, what, "rows are [T, H] and weights of rank 3");
+  const int64_t T = xq_in.size(0), H = xq_in.size(1), E = wq[0].size(0), F = wq[0].size(1);
+  need_shape(wq[0], {E, F, H}, what, "gate");
+  need_shape(wq[1], {E, F, H}, what, "up");
+  need_shape(wq[2], {E, H, F}, what, "down");
+  need_shape(ws[0], {E, F}, what, "gate scale");
+  need_shape(ws[1], {E, F}, what, "up scale");
+  need_shape(ws[2], {E, H}, what, "down scale");
+  need_offsets(offsets, E, what);
+  int64_t R = T;
+  if (row_slot.has_value()) {
+    need(row_slot->scalar_type() == at::kInt && row_slot->dim() == 1 && row_slot->is_contiguous() && top_k >= 1, what,
+         "row_slot must be contiguous int32 [R], with top_k >= 1");
+    R = row_slot->size(0);
+  }
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(xq_in.device());
+  const at::Tensor xq = xq_in.contiguous(), sx = sx_in.contiguous();
+  at::Tensor y = at::empty({R, H}, xq.options().dtype(at::kBFloat16));
+  if (R == 0) return y;
+  const size_t nbytes = moe_swiglu_fwd_int8_workspace(R, F);
+  const at::Tensor w = scratch(nbytes, xq);
+  check_rc(moe_swiglu_fwd_int8(xq.data_ptr(), sx.data_ptr<float>(), T, static_cast<const int*>(ptr(row_slot)), top_k,
+                               wq[0].data_ptr(), ws[0].data_ptr<float>(), wq[1].data_ptr(), ws[1].data_ptr<float>(),
+                               wq[2].data_ptr(), ws[2].data_ptr<float>(), offsets.data_ptr<int>(), R, H, F, E, y.data_ptr(),
+                               w.data_ptr(), nbytes, stream_of(xq)),
+           "moe_swiglu_fwd_int8");
+  return y;
+}
+
+void need_norm(const at::Tensor& x, const at::Tensor& weight, const char* what) {
+  need_type(is_float(x) && is_float(weight), what, "tensors are float32 or bfloat16");
+  need(x.dim() == 2 && weight.dim() == 1 && weight.size(0) == x.size(1), what,
+       "x must be [N, H] and weight [H], got " + shape_of(x) + " and " + shape_of(weight));
+}
+void need_like(const at::Tensor& t, const at::Tensor& x, const char* what, const char* name) {
+  need_type(t.scalar_type() == x.scalar_type(), what, std::string(name) + " must have x's dtype");
+  need_shape(t, x.sizes(), what, name);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> op_rmsnorm_residual_forward(const at::Tensor& x_in, const at::Tensor& r_in,
+                                                                           const at::Tensor& weight_in, double eps) {
+  const char* const what = "rmsnorm_residual_forward";
+  one_gpu({&x_in, &r_in, &weight_in});
+  need_norm(x_in, weight_in, what);
+  need_like(r_in, x_in, what, "residual");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x_in.device());
+  const at::Tensor x = x_in.contiguous(), r = r_in.contiguous(), weight = weight_in.contiguous();
+  at::Tensor xn = at::empty(x.sizes(), x.options()), h = at::empty(x.sizes(), x.options());
+  at::Tensor rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  check_rc(moe_rmsnorm_residual_fwd(x.data_ptr(), r.data_ptr(), code_of(x), weight.data_ptr(), code_of(weight), (float)eps,
+                                    x.size(0), x.size(1), h.data_ptr(), xn.data_ptr(), rstd.data_ptr<float>(), stream_of(x)),
+           "moe_rmsnorm_residual_fwd");
+  return {xn, h, rstd};
+}
+
+std::tuple<at::Tensor, at::Tensor> op_rmsnorm_residual_backward(const at::Tensor& h_in, const at::Tensor& weight_in,
+                                                                const at::Tensor& rstd_in, const OptTensor& dxn_in,
+                                                                const OptTensor& dh_in) {
+  const char* const what = "rmsnorm_residual_backward";
+  one_gpu({&h_in, &weight_in, &rstd_in, opt(dxn_in), opt(dh_in)});
+  need_norm(h_in, weight_in, what);
+  need(rstd_in.scalar_type() == at::kFloat && rstd_in.dim() == 1 && rstd_in.size(0) == h_in.size(0), what,
+       "rstd must be float32 [" + std::to_string(h_in.size(0)) + "]");
+  need(dxn_in.has_value() || dh_in.has_value(), what, "needs a gradient of xn or of h");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(h_in.device());
+  const at::Tensor h = h_in.contiguous(), weight = weight_in.contiguous(), rstd = rstd_in.contiguous();
+  OptTensor dxn, dh;
+  if (dxn_in.has_value()) {
+    need_like(*dxn_in, h, what, "dxn");
+    dxn = dxn_in->contiguous();
+  }
+  if (dh_in.has_value()) {
+    need_like(*dh_in, h, what, "dh");
+    dh = dh_in->contiguous();
+  }
+  at::Tensor d = at::empty(h.sizes(), h.options()), dw = at::empty(weight.sizes(), weight.options());
+  const size_t nbytes = moe_rmsnorm_bwd_workspace(h.size(0), h.size(1));
+  const at::Tensor ws = scratch(nbytes, h);
+  check_rc(moe_rmsnorm_residual_bwd(h.data_ptr(), code_of(h), weight.data_ptr(), code_of(weight), rstd.data_ptr<float>(),
+                                    ptr(dxn), ptr(dh), h.size(0), h.size(1), d.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes,
+                                    stream_of(h)),
+           "moe_rmsnorm_residual_bwd");
+  return {d, dw};
+}
+
+std::tuple<at::Tensor, at::Tensor, OptTensor, OptTensor> op_rmsnorm_quant(const at::Tensor& x_in, const at::Tensor& weight_in,
+                                                                          double eps, const OptTensor& r_in, bool e4m3,
+                                                                          bool keep_norm) {
+  const char* const what = "rmsnorm_quant";
+  one_gpu({&x_in, &weight_in, opt(r_in)});
+  need_norm(x_in, weight_in, what);
+  if (r_in.has_value()) need_like(*r_in, x_in, what, "residual");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x_in.device());
+  const at::Tensor x = x_in.contiguous(), weight = weight_in.contiguous();
+  OptTensor r, xn, h;
+  if (r_in.has_value()) {
+    r = r_in->contiguous();
+    h = at::empty(x.sizes(), x.options());
+  }
+  if (keep_norm) xn = at::empty(x.sizes(), x.options());
+  at::Tensor q = at::empty(x.sizes(), x.options().dtype(e4m3 ? at::kByte : at::kChar));
+  at::Tensor sc = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  check_rc(moe_rmsnorm_quant(x.data_ptr(), ptr(r), code_of(x), weight.data_ptr(), code_of(weight), (float)eps, x.size(0),
+                             x.size(1), e4m3 ? MOE_E4M3 : MOE_INT8, q.data_ptr(), sc.data_ptr<float>(),
+                             const_cast<void*>(ptr(h)), const_cast<void*>(ptr(xn)), stream_of(x)),
+           "moe_rmsnorm_quant");
+  return {q, sc, xn, h};
+}
+
 // ---- the balance loss of sequences ----
 
 std::vector<at::Tensor> op_balance_forward(const at::Tensor& logits_in, const at::Tensor& idx_in, const OptTensor& off_in,
@@ -586,6 +815,13 @@ PYBIND11_MODULE(_moe_torch, m) {
   m.def("dequant_mxfp4", &op_dequant_mxfp4, nogil);
   m.def("swiglu_forward_mxfp4", &op_swiglu_forward_mxfp4, nogil);
   m.def("swiglu_backward_mxfp4", &op_swiglu_backward_mxfp4, nogil);
+  m.def("quant_rows_int8", &op_quant_rows_int8, nogil);
+  m.def("dequant_rows", &op_dequant_rows, nogil);
+  m.def("matmul_int8", &op_matmul_int8, nogil);
+  m.def("swiglu_forward_int8", &op_swiglu_forward_int8, nogil);
+  m.def("rmsnorm_residual_forward", &op_rmsnorm_residual_forward, nogil);
+  m.def("rmsnorm_residual_backward", &op_rmsnorm_residual_backward, nogil);
+  m.def("rmsnorm_quant", &op_rmsnorm_quant, nogil);
   m.def("balance_forward", &op_balance_forward, nogil);
   m.def("balance_backward", &op_balance_backward, nogil);
 }

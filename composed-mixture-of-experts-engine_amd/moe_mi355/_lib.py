@@ -92,6 +92,17 @@ _SIGNATURES = {
     "moe_swiglu_fwd_fp8": (
         _I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ, _P]
     ),
+    "moe_rmsnorm_residual_fwd": (_I32, [_P, _P, _I32, _P, _I32, _F32, _I64, _I64, _P, _P, _P, _P]),
+    "moe_rmsnorm_residual_bwd": (_I32, [_P, _I32, _P, _I32, _P, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
+    "moe_rmsnorm_quant": (_I32, [_P, _P, _I32, _P, _I32, _F32, _I64, _I64, _I32, _P, _P, _P, _P, _P]),
+    "moe_quant_rows_int8": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "moe_dequant_rows": (_I32, [_P, _I32, _P, _I64, _I64, _P, _I32, _P]),
+    "moe_matmul_int8": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I32, _P]),
+    "moe_swiglu_fwd_int8_workspace": (_SZ, [_I64, _I64]),
+    "moe_swiglu_fwd_int8": (
+        _I32,
+        [_P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _SZ, _P],
+    ),
     "moe_quant_mxfp4": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P]),
     "moe_dequant_mxfp4": (_I32, [_P, _P, _I64, _I64, _P, _I32, _P]),
     "moe_swiglu_fwd_mxfp4_workspace": (_SZ, [_I64, _I64, _I64, _I64]),

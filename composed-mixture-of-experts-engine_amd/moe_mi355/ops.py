@@ -265,6 +265,34 @@ def rmsnorm_router_backward(
                                                     grad_z, float(aux_coef), float(z_coef), grad_logits))
 
 
+def rmsnorm_residual_forward(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                             eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``h = x + residual`` (both [N, H] of one dtype, the sum rounded to it) and :func:`rmsnorm_forward` of ``h`` in one
+    kernel: ``(xn [N, H], h [N, H], rstd f32 [N])``."""
+    return L.native().rmsnorm_residual_forward(x, residual, weight, eps)
+
+
+def rmsnorm_residual_backward(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, dxn: Optional[torch.Tensor],
+                              dh: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Backward of :func:`rmsnorm_residual_forward` for the gradients of ``xn`` and of ``h`` (either may be None):
+    ``(d, dweight)``, ``d`` the gradient of ``x`` and of ``residual`` alike."""
+    return L.native().rmsnorm_residual_backward(h, weight, rstd, dxn, dh)
+
+
+ROW_FORMATS = ("int8", "e4m3")
+
+
+def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None,
+                  fmt: str = "int8", keep_norm: bool = False):
+    """The norm of ``x`` [N, H] (of ``h = x + residual`` if given) with its rows in 8 bits, from the normalised values in
+    fp32, for serving: ``(q, scale f32 [N], xn or None, h or None)``.  ``q`` [N, H] is int8 (:func:`quant_rows_int8`'s rule) or,
+    for ``fmt="e4m3"``, uint8 e4m3 bytes (:func:`quant_rows_fp8`'s); ``keep_norm`` also returns the rows in ``x``'s dtype,
+    e.g. for the router."""
+    if fmt not in ROW_FORMATS:
+        raise ValueError(f"rmsnorm_quant: fmt must be one of {ROW_FORMATS}, got {fmt!r}")
+    return L.native().rmsnorm_quant(x, weight, eps, residual, fmt == "e4m3", keep_norm)
+
+
 # ---------------------------------------------------------------------------
 # Dispatch planner, permute, combine
 # ---------------------------------------------------------------------------
@@ -478,6 +506,41 @@ def swiglu_backward(dy, xp, act, hgu, w_gate, w_up, w_down, offsets):
     _, _ = xp.shape
     _, _, _ = w_gate.shape
     return tuple(L.native().swiglu_backward(dy, xp, act, hgu, w_gate, w_up, w_down, offsets))
+
+
+# ---------------------------------------------------------------------------
+# int8 rows and weights, their products, the experts on them
+# ---------------------------------------------------------------------------
+def quant_rows_int8(t: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of ``t`` [..., cols] (bf16 / fp32, cols % 16 == 0) -> (int8 [..., cols], fp32 scale [...]): with
+    ``a = max(absmax(row), 2^-100)``, scale = a / 127 and each element is the whole number nearest to 127 x / a, ties to even.
+    A row with an infinity or a NaN has the scale NaN and elements 0.  For activations (a scale a token) and weights (a scale
+    an output channel) alike."""
+    return L.native().quant_rows_int8(t)
+
+
+def dequant_rows(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [..., cols] of rows in 8 bits, q * scale: ``q`` int8, or uint8 for e4m3 bytes (:func:`quant_rows_fp8`)."""
+    return L.native().dequant_rows(q, scale, L.dtype_code(dtype) == L.MOE_BF16)
+
+
+def matmul_int8(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor,
+                offsets: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``y[..., n] = scale[...] wscale[n] sum_k q[..., k] wq[n, k]``: int8 rows ``q`` [..., K] times int8 weights [N, K] with a
+    scale each token and output channel (:func:`quant_rows_int8`), y bf16 or fp32.  With ``offsets`` (int32 [E + 1]) the rows
+    [R, K] are grouped by expert and ``wq`` is [E, N, K], ``wscale`` [E, N]; rows past offsets[E] are left unwritten.  The sum is
+    exact, so a row's result is the same in any batch."""
+    return L.native().matmul_int8(q, scale, wq, wscale, offsets, L.dtype_code(out_dtype) == L.MOE_BF16)
+
+
+def swiglu_forward_int8(xq, sx, wq, wscale, offsets, row_slot: Optional[torch.Tensor] = None, top_k: int = 1):
+    """Forward of the SwiGLU experts on int8 rows and weights (:func:`quant_rows_int8`): ``wq`` = (gate [E, F, H], up
+    [E, F, H], down [E, H, F]) with ``wscale`` = (sg [E, F], su [E, F], sd [E, H]); ``act = silu(g) u`` is rounded to bf16 and
+    quantized by row between the projections -> y [R, H] bf16, rows grouped by expert (``offsets`` [E + 1] int32).  ``xq``
+    [T, H] with scales ``sx`` [T] holds the tokens, and row r reads token ``row_slot[r] // top_k`` (a plan's ``row_slot``: no
+    copy of a token per expert), or the rows themselves where ``row_slot`` is None.  From one row to many; rows past offsets[E]
+    are left unwritten."""
+    return L.native().swiglu_forward_int8(xq, sx, wq, wscale, offsets, row_slot, top_k)
 
 
 # ---------------------------------------------------------------------------

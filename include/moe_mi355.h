@@ -29,6 +29,9 @@ extern "C" {
 
 enum moe_dtype { MOE_F32 = 0, MOE_BF16 = 1 };
 
+/* Formats of rows held in 8 bits with one fp32 scale each. */
+enum moe_row_format { MOE_INT8 = 0, MOE_E4M3 = 1 };
+
 enum moe_status {
   MOE_OK = 0,
   MOE_EINVAL = -1,   /* bad shape / dtype / pointer argument */
@@ -335,6 +338,39 @@ int moe_swiglu_fwd_fp8(const void* xq, const float* sx, const void* wg_q, const 
                        size_t ws_bytes, void* stream);
 
 /* ----------------------------------------------------------------------
+ * int8: rows and weights in 8-bit integers with one fp32 scale a row (a weight row is an output channel), their products,
+ * and the SwiGLU experts on them; a variant of moe_quant_rows_fp8 / moe_swiglu_fwd_fp8 (the expert loop, moe_layer.py
+ * L:166-198, L:326-337).  The reference has no integer path: its results are the bf16 path's up to the quantization.
+ *
+ * moe_quant_rows_int8: src [rows, ld] (MOE_BF16 / MOE_F32, first `cols` columns) -> dst [rows, cols] int8, scale [rows] f32.
+ * With a = max(absmax of the row, 2^-100): scale = a / 127 and each element is the whole number nearest to 127 x / a, ties to
+ * even (the quotient taken exactly).  A row with an infinity or a NaN has the scale NaN and elements 0.  cols % 16 == 0,
+ * ld % 8 == 0.
+ * moe_dequant_rows: q * scale in fp32, rounded to dst_dtype, for rows in int8 or e4m3 (moe_quant_rows_fp8, moe_rmsnorm_quant).
+ * cols % 16 == 0.
+ * moe_matmul_int8: y[m, n] = sx[m] sw[n] sum_k xq[m, k] wq[n, k], xq [R, K], sx [R], and wq [N, K], sw [N] (E = 1, offsets
+ * NULL) or wq [E, N, K], sw [E, N] for rows grouped by expert ([offsets[e], offsets[e + 1]); rows in no segment are not
+ * written).  y [R, N] MOE_BF16 or MOE_F32.  The sum is a whole number in 32 bits, so a row's result is the same in any batch.
+ * K % 16 == 0, K <= 131056, N % 8 == 0, N K < 2^32, E <= 1024.
+ * moe_swiglu_fwd_int8: for each expert's rows  g = Wg x, u = Wu x, act = silu(g) u (rounded to bf16, then quantized by row as
+ * above), y = Wd act, y [R, H] bf16.  Row m's x is row row_slot[m] / top_k of xq [T, H] (moe_plan's row_slot: tokens are
+ * quantized once and not copied), or row m where row_slot is NULL (T == R).  wg_q, wu_q [E, F, H] (scales sg, su [E, F]), wd_q
+ * [E, H, F] (sd [E, H]).  Rows past offsets[E] are not written.  H % 16 == 0, F % 16 == 0.
+ * Pointers to rows and weights are 16-byte aligned.
+ * ---------------------------------------------------------------------- */
+int moe_quant_rows_int8(const void* src, int src_dtype, int64_t rows, int64_t cols, int64_t ld, void* dst, float* scale,
+                        void* stream);
+int moe_dequant_rows(const void* q, int q_format, const float* scale, int64_t rows, int64_t cols, void* dst, int dst_dtype,
+                     void* stream);
+int moe_matmul_int8(const void* xq, const float* sx, const void* wq, const float* sw, const int32_t* offsets, int64_t R,
+                    int64_t K, int64_t N, int64_t E, void* y, int y_dtype, void* stream);
+size_t moe_swiglu_fwd_int8_workspace(int64_t R, int64_t F);
+int moe_swiglu_fwd_int8(const void* xq, const float* sx, int64_t T, const int32_t* row_slot, int64_t top_k, const void* wg_q,
+                        const float* sg, const void* wu_q, const float* su, const void* wd_q, const float* sd,
+                        const int32_t* offsets, int64_t R, int64_t H, int64_t F, int64_t E, void* y, void* workspace,
+                        size_t ws_bytes, void* stream);
+
+/* ----------------------------------------------------------------------
  * MXFP4 experts: weights held in 4 bits (e2m1: 0, 1/2, 1, 3/2, 2, 3, 4, 6 and negatives), every 32 consecutive
  * elements of a row with one power-of-two scale (OCP MX, E8M0 byte e + 127); a variant of moe_quant_rows_fp8 /
  * moe_swiglu_fwd_fp8 (the expert loop, moe_layer.py L:166-198, L:326-337) with bf16 rows.  The reference has no 4-bit
@@ -419,6 +455,17 @@ int moe_balance_bwd(const float* logits, const int64_t* counts, const int64_t* t
  * xn is formed inside the norm kernel from dL/dlogits and never reaches HBM;
  * otherwise moe_router_bwd writes it to the workspace and moe_rmsnorm_bwd
  * adds it.
+ *
+ * moe_rmsnorm_residual_fwd: h = x + residual (the sum of L:125-126, left by one
+ * block to the next one's norm), rounded to x's dtype, and moe_rmsnorm_fwd of
+ * h, in one kernel.  moe_rmsnorm_residual_bwd: d = dh + the norm's gradient,
+ * the gradient of x and of residual alike (workspace: moe_rmsnorm_bwd's; dxn
+ * or dh may be null, not both).
+ *
+ * moe_rmsnorm_quant: the norm of x (residual null) or of h = x + residual, its
+ * fp32 values quantized by row: int8 (moe_quant_rows_int8) or e4m3
+ * (moe_quant_rows_fp8), q [N, H] and scale [N]; xn_out (the rows in x's dtype)
+ * may be null, h_out goes with residual.  H % 16 == 0.
  * ---------------------------------------------------------------------- */
 int moe_rmsnorm_fwd(const void* x, int x_dtype, const void* gamma, int gamma_dtype, float eps, int64_t N,
                     int64_t H, void* xn_out, float* rstd_out, void* stream);
@@ -433,6 +480,15 @@ size_t moe_rmsnorm_bwd_workspace(int64_t N, int64_t H);
 int moe_rmsnorm_bwd(const void* x, int x_dtype, const void* gamma, int gamma_dtype, const float* rstd,
                     const void* dxn, const void* dxn2, int64_t N, int64_t H, void* dx_out, void* dgamma_out,
                     void* workspace, size_t ws_bytes, void* stream);
+int moe_rmsnorm_residual_fwd(const void* x, const void* residual, int x_dtype, const void* gamma, int gamma_dtype,
+                             float eps, int64_t N, int64_t H, void* h_out, void* xn_out, float* rstd_out,
+                             void* stream);
+int moe_rmsnorm_residual_bwd(const void* h, int x_dtype, const void* gamma, int gamma_dtype, const float* rstd,
+                             const void* dxn, const void* dh, int64_t N, int64_t H, void* d_out, void* dgamma_out,
+                             void* workspace, size_t ws_bytes, void* stream);
+int moe_rmsnorm_quant(const void* x, const void* residual, int x_dtype, const void* gamma, int gamma_dtype, float eps,
+                      int64_t N, int64_t H, int q_format, void* q_out, float* scale_out, void* h_out, void* xn_out,
+                      void* stream);
 size_t moe_rmsnorm_router_bwd_workspace(int64_t N, int64_t H, int64_t E, int64_t K, int x_dtype, int wg_dtype);
 int moe_rmsnorm_router_bwd(const void* x, int x_dtype, const void* gamma, int gamma_dtype, const float* rstd,
                            const void* xn, const void* wg, int wg_dtype, const float* logits, const int64_t* idx,

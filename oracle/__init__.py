@@ -15,6 +15,7 @@ algorithm of the reference moe-engine hot path:
   (this build's own variant: the reference has no fp8 path).
 * ``oracle.mxfp4``   -- the experts held in 4 bits, forward and backward to the rows
   (likewise without a counterpart).
+* ``oracle.int8``    -- rows and weights in int8, their products and the experts on them (likewise).
 * ``oracle.balance`` -- the balance loss of sequences and the z-loss over valid tokens.
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and ``bench.py``'s CPU-baseline

@@ -10,6 +10,7 @@ Pinning (each checked in ``tests/test_oracle_norm.py``):
   the output has RMS ~1 before ``weight``; and ``torch.rsqrt`` / ``mean`` in float64 (library routines).
 * ``rmsnorm_bwd`` -- the closed-form gradient below against torch autograd through the float64 forward, and
   against central finite differences on a tiny case.
+* ``rmsnorm_residual_fwd`` / ``_bwd`` -- the two above on a rounded sum: autograd of the float64 formula.
 * ``rmsnorm_to`` -- the dtype cast of the reference (``.to(x.dtype)``): bf16 rounding of the float64 value.
 """
 
@@ -52,3 +53,21 @@ def rmsnorm_bwd(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, eps: fl
     dx = r * (g - xhat * (g * xhat).mean(-1, keepdim=True))
     dweight = (g_out * xhat).sum(0)
     return dx, dweight
+
+
+def rmsnorm_residual_fwd(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5):
+    """``h = x + residual`` rounded to x's dtype (the sum of moe.py L:126, left to the next block's norm) and
+    ``rmsnorm_fwd(h)``: ``(xn float64, h, rstd float64)``."""
+    h = (x.to(_F64) + residual.to(_F64)).to(x.dtype)
+    y, rstd = rmsnorm_fwd(h, weight, eps)
+    return y, h, rstd
+
+
+def rmsnorm_residual_bwd(h: torch.Tensor, weight: torch.Tensor, dxn, dh, eps: float = 1e-5):
+    """``(d, dweight)`` in float64 for gradients of ``xn`` and of ``h`` (either may be None): ``d = dh + rmsnorm_bwd``, of x and
+    of residual alike."""
+    d = torch.zeros(h.shape, dtype=_F64, device=h.device) if dh is None else dh.to(_F64)
+    if dxn is None:
+        return d, torch.zeros(h.shape[1], dtype=_F64, device=h.device)
+    dx, dweight = rmsnorm_bwd(h, weight, dxn, eps)
+    return d + dx, dweight
