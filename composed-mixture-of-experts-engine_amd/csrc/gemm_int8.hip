@@ -17,6 +17,7 @@
 // weights.  Blocks start their chunks at different columns: rows lie a power of two apart, and blocks that walk them in step
 // ask the same few memory channels.
 #include <algorithm>
+#include <utility>
 
 #include "common.h"
 #include "quant8.h"
@@ -248,9 +249,271 @@ int launch_small(const char* name, hipStream_t s, I8Args a) {
   return check_launch(name);
 }
 
+// ---- many rows ----
+typedef __attribute__((address_space(1))) const u32x4 g_u32x4;
+__device__ __forceinline__ u32x4 ldg16(const uint8_t* p) {
+  return *reinterpret_cast<g_u32x4*>(reinterpret_cast<uintptr_t>(p));
+}
+struct __attribute__((packed, aligned(4))) Scale4 { float v[4]; };
+__device__ __attribute__((aligned(16))) const uint8_t g_i8_zero[16] = {0};
+
+// One tile of BM rows of an expert by BN weight rows (GU: BN / 2 gate rows and the matching up rows, 32 by 32), four waves
+// WR x WC of MI x NI fragments of v_mfma_i32_32x32x32_i8.  Both operands go through LDS in slices of 128 bytes of a row (whole
+// cache lines), two slices at a time, a row's eight 16-byte chunks swizzled so that the 16 rows a fragment read touches at
+// once lie in distinct banks.  While slice kt is computed, each wave writes its share of slice kt + 1 (in registers since the
+// slice before) into the free half and loads its share of slice kt + 2 into the same registers, one 16-byte piece a lane at a
+// time between the matrix instructions; one barrier a slice.
+template <bool GU, typename OT, int WR, int MI, int NI>
+__global__ __launch_bounds__(256, MI * NI <= 4 ? 2 : 1) void k_i8_tile(I8Args g) {
+  constexpr int WC = 4 / WR;
+  constexpr int BM = WR * MI * 32, BN = WC * NI * 32;
+  constexpr int SA = BM * 128, SB = BN * 128;          // LDS bytes of a slice of either operand
+  constexpr int QA = BM / 32, QB = BN / 32, NP = QA + QB;  // 16-byte pieces of a wave's share of a slice
+  constexpr int CW = GU ? BN / 2 : BN;                 // output columns of the tile
+  constexpr int WCOLS = CW / WC;                       // ... and of a wave
+  constexpr int CP = GU ? (WCOLS + 8) / 2 : WCOLS + 4; // words a row of a wave's output strip of 32 rows
+  constexpr int SMEM = std::max(2 * (SA + SB), 4 * 32 * CP * 4);
+  __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm0 = wv / WC * (MI * 32), wn0 = wv % WC * (NI * 32);
+  const int i32 = lane & 31, h = lane >> 5;
+
+  // XCD-contiguous logical order over a 1-D grid sized for the most tiles any routing can produce: the tiles that there are,
+  // split into 8 contiguous ranges (blockIdx mod 8)
+  auto row_tiles = [&](int e) {
+    return e < g.E ? (int)((seg(g, e + 1) - seg(g, e) + BM - 1) / BM) : 0;
+  };
+  int sum = 0;
+  for (int e0 = 0; e0 < g.E; e0 += 64) sum += max(row_tiles(e0 + lane), 0);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  const int total = __builtin_amdgcn_readfirstlane(sum) * g.Tn;
+  const int chunk = (total + 7) >> 3, slot = (int)(blockIdx.x >> 3), L = (int)(blockIdx.x & 7) * chunk + slot;
+  if (slot >= chunk || L >= total) return;
+  int e = 0, before = 0, cnt = 0;  // row tiles of the experts before e, and of e
+  for (int e0 = 0;; e0 += 64) {
+    const int c = max(row_tiles(e0 + lane), 0);
+    int upto = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o);
+      upto += lane >= o ? v : 0;
+    }
+    const unsigned long long past = __ballot(L < (before + upto) * g.Tn);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      e = e0 + l;
+      cnt = __shfl(c, l);
+      before += __shfl(upto, l) - cnt;
+      break;
+    }
+    before += __shfl(upto, 63);
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
+  cnt = __builtin_amdgcn_readfirstlane(cnt);
+  const int local = L - __builtin_amdgcn_readfirstlane(before) * g.Tn;
+  constexpr int GM = 8;
+  const int grp = local / (GM * g.Tn), rest = local - grp * GM * g.Tn, gm = min(cnt - grp * GM, GM);
+  const int nt = rest / gm, mt = grp * GM + rest - nt * gm;
+  const int64_t mbase = seg(g, e) + (int64_t)mt * BM;
+  const int mlen = (int)min(seg(g, e + 1) - mbase, (int64_t)BM);
+  const int n0 = nt * CW, K = g.K, nk = (K + 127) / 128;
+
+  // piece p of a wave's share: instruction j fills rows 8 j + lane / 8 of its operand's tile, slot lane % 8 of the row
+  const uint8_t* const b_base[2] = {g.B + (int64_t)e * g.N * K, GU ? g.B2 + (int64_t)e * g.N * K : g.B + (int64_t)e * g.N * K};
+  const uint8_t* a_src[QA];
+  uint32_t b_off[QB];
+  auto chunk_of = [&](int j) { return (lane & 7) ^ ((4 * j + (lane >> 4)) & 7); };
+#pragma unroll
+  for (int q = 0; q < QA; ++q) {
+    const int j = QA * wv + q;
+    a_src[q] = g.A + source_row(g, mbase + min(8 * j + (lane >> 3), mlen - 1)) * K + chunk_of(j) * 16;
+  }
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const int j = QB * wv + q, i = 8 * j + (lane >> 3);
+    const int n = GU ? n0 + (i >> 6) * 32 + (i & 31) : n0 + i;
+    b_off[q] = (uint32_t)min(n, g.N - 1) * (uint32_t)K + chunk_of(j) * 16;
+  }
+  u32x4 st[NP];
+  // piece p of slice kt; past the row's end A is zeros and B anything
+  auto gload = [&](int kt, int p, bool full) {
+    if (p < QA) {
+      const uint8_t* s = a_src[p] + kt * 128;
+      if (!full) s = kt * 128 + chunk_of(QA * wv + p) * 16 < K ? s : g_i8_zero;
+      st[p] = ldg16(s);
+    } else {
+      const int q = p - QA, j = QB * wv + q;
+      const uint8_t* const base = b_base[GU ? (8 * j >> 5) & 1 : 0];
+      uint32_t o = b_off[q];
+      if (full) {
+        st[p] = ldg16(base + (uint32_t)kt * 128u + o);
+      } else {
+        const int k = kt * 128 + chunk_of(j) * 16;
+        st[p] = ldg16(base + (o - chunk_of(j) * 16) + (k < K ? (uint32_t)k : 0u));
+      }
+    }
+  };
+  auto half = [&](int kt) { return smem + (kt & 1) * (SA + SB); };
+  auto lwrite = [&](int kt, int p) {
+    uint8_t* const d = half(kt) + (p < QA ? (QA * wv + p) * 1024 : SA + (QB * wv + p - QA) * 1024);
+    __asm__ volatile("" ::: "memory");
+    *reinterpret_cast<u32x4*>(d + lane * 16) = st[p];
+    __asm__ volatile("" ::: "memory");
+  };
+  auto frag = [&](const uint8_t* t, int row, int ks) {
+    return *reinterpret_cast<const i32x4*>(t + row * 128 + (((2 * ks + h) ^ ((row >> 1) & 7)) << 4));
+  };
+  auto read_frag = [&](int kt, int ks, int f, i32x4(&fa)[MI], i32x4(&fb)[NI]) {
+    if (f < MI) fa[f] = frag(half(kt), wm0 + f * 32 + i32, ks);
+    else fb[f - MI] = frag(half(kt) + SA, wn0 + (f - MI) * 32 + i32, ks);
+  };
+
+  i32x16 acc[MI][NI];
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[mi][ni][j] = 0;
+
+  // One 32-wide quarter of slice kt: MI NI matrix instructions, after each at most a fragment read of the next quarter (the
+  // first ones) and a refill piece of [PLO, PHI) (the last ones).  MODE 0: write slice kt + 1, load the whole slice kt + 2;
+  // 1: the slice loaded may end inside; 2: write only; 3: neither.
+  constexpr int SLOTS = MI * NI;
+  auto quarter = [&](auto mode_c, auto plo_c, auto phi_c, const i32x4(&ca)[MI], const i32x4(&cb)[NI], int nkt, int nks,
+                     bool read_next, i32x4(&na)[MI], i32x4(&nb)[NI], int kt, bool lfull) {
+    constexpr int MODE = decltype(mode_c)::value, PLO = decltype(plo_c)::value, PHI = decltype(phi_c)::value;
+    static_assert(PHI - PLO <= SLOTS && MI + NI <= SLOTS);
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      (([&] {
+         constexpr int mi = I / NI, ni = I % NI;
+         acc[mi][ni] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cb[ni], ca[mi], acc[mi][ni], 0, 0, 0);
+         __builtin_amdgcn_sched_barrier(0);
+         if constexpr (I < MI + NI) {
+           if (read_next) read_frag(nkt, nks, I, na, nb);
+         }
+         constexpr int p = PHI - SLOTS + I;
+         if constexpr (MODE < 3 && p >= PLO) {
+           lwrite(kt + 1, p);
+           if constexpr (MODE == 0) gload(kt + 2, p, true);
+           else if constexpr (MODE == 1) gload(kt + 2, p, lfull);
+         }
+         __builtin_amdgcn_sched_barrier(0);
+       }()), ...);
+    }(std::make_integer_sequence<int, SLOTS>{});
+  };
+  using P0 = std::integral_constant<int, 0>;
+  using P1 = std::integral_constant<int, (NP + 2) / 3>;
+  using P2 = std::integral_constant<int, (2 * NP + 2) / 3>;
+  using P3 = std::integral_constant<int, NP>;
+  using M3 = std::integral_constant<int, 3>;
+  i32x4 fa0[MI], fb0[NI], fa1[MI], fb1[NI];
+  const int whole = K / 128;  // whole slices
+  auto slice = [&](auto mode_c, int kt) {
+    const bool lfull = kt + 2 < whole;
+    quarter(mode_c, P0{}, P1{}, fa0, fb0, kt, 1, true, fa1, fb1, kt, lfull);
+    quarter(mode_c, P1{}, P2{}, fa1, fb1, kt, 2, true, fa0, fb0, kt, lfull);
+    quarter(mode_c, P2{}, P3{}, fa0, fb0, kt, 3, true, fa1, fb1, kt, lfull);
+    lds_sync();  // this wave's pieces of slice kt + 1 are written and its reads of slice kt done, and every other wave's
+    __builtin_amdgcn_sched_barrier(0);
+    quarter(M3{}, P3{}, P3{}, fa1, fb1, kt + 1, 0, kt + 1 < nk, fa0, fb0, kt, true);
+  };
+  for (int p = 0; p < NP; ++p) gload(0, p, 0 < whole);
+  for (int p = 0; p < NP; ++p) lwrite(0, p);
+  if (nk > 1) {
+    for (int p = 0; p < NP; ++p) gload(1, p, 1 < whole);
+  }
+  __syncthreads();
+  for (int f = 0; f < MI + NI; ++f) read_frag(0, 0, f, fa0, fb0);
+  int kt = 0;
+  for (; kt + 2 < whole; ++kt) slice(std::integral_constant<int, 0>{}, kt);
+  for (; kt + 2 < nk; ++kt) slice(std::integral_constant<int, 1>{}, kt);
+  if (kt + 1 < nk) slice(std::integral_constant<int, 2>{}, kt++);
+  if (kt < nk) slice(M3{}, kt);
+  __syncthreads();
+
+  // The matrix instructions take the weights as their M operand, so a lane holds one row of C and, in each four accumulators,
+  // four columns in a row: acc[mi][ni][j] = C[wm0 + 32 mi + lane % 32][wn0 + 32 ni + 8 (j / 4) + 4 (lane / 32) + j % 4].  Each
+  // wave turns its strips of 32 rows over through LDS of its own, so that rows leave in whole lines.
+  uint32_t* const cs = reinterpret_cast<uint32_t*>(smem) + wv * 32 * CP;
+  const int c0 = n0 + wv % WC * WCOLS;  // the wave's first column
+  const float* const sb = g.sb + (int64_t)e * g.N;
+  const float* const sb2 = GU ? g.sb2 + (int64_t)e * g.N : nullptr;
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    const int r0 = wm0 + mi * 32;  // the strip's first row of the tile
+    if (r0 >= mlen) break;
+    const float sx = g.sa[source_row(g, mbase + min(r0 + i32, mlen - 1))];
+    __asm__ volatile("" ::: "memory");
+    if constexpr (GU) {
+#pragma unroll
+      for (int pr = 0; pr < NI / 2; ++pr)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int c = pr * 32 + v * 8 + h * 4, n = min(c0 + c, g.N - 4);
+          const Scale4 sg = *reinterpret_cast<const Scale4*>(sb + n), su = *reinterpret_cast<const Scale4*>(sb2 + n);
+          float o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float gv = (float)acc[mi][2 * pr][4 * v + j] * sx * sg.v[j];
+            o[j] = gv * sig_i8(gv) * ((float)acc[mi][2 * pr + 1][4 * v + j] * sx * su.v[j]);
+          }
+          *reinterpret_cast<uint2*>(cs + i32 * CP + c / 2) = uint2{pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+        }
+    } else {
+#pragma unroll
+      for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int c = ni * 32 + v * 8 + h * 4, n = min(c0 + c, g.N - 4);
+          const Scale4 s = *reinterpret_cast<const Scale4*>(sb + n);
+          f32x4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = (float)acc[mi][ni][4 * v + j] * sx * s.v[j];
+          *reinterpret_cast<f32x4*>(cs + i32 * CP + c) = o;
+        }
+    }
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int PER = GU || sizeof(OT) == 2 ? 8 : 4;  // columns of a 16-byte store
+    constexpr int LPR = WCOLS / PER;                    // lanes a row
+#pragma unroll
+    for (int u = 0; u < 32 * LPR / 64; ++u) {
+      const int r = u * (64 / LPR) + lane / LPR, c = lane % LPR * PER;
+      u32x4 o;
+      if constexpr (GU) {
+        o = *reinterpret_cast<const u32x4*>(cs + r * CP + c / 2);
+      } else if constexpr (sizeof(OT) == 4) {
+        o = *reinterpret_cast<const u32x4*>(cs + r * CP + c);
+      } else {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(cs + r * CP + c), hi = *reinterpret_cast<const f32x4*>(cs + r * CP + c + 4);
+        o = u32x4{pack2bf(lo[0], lo[1]), pack2bf(lo[2], lo[3]), pack2bf(hi[0], hi[1]), pack2bf(hi[2], hi[3])};
+      }
+      if (r0 + r < mlen && c0 + c < g.N)
+        *reinterpret_cast<u32x4*>(static_cast<OT*>(g.C) + (mbase + r0 + r) * g.N + c0 + c) = o;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <bool GU, typename OT, int WR, int MI, int NI>
+int launch_tile(const char* name, hipStream_t s, I8Args a) {
+  constexpr int BM = WR * MI * 32, CW = (4 / WR) * NI * 32 / (GU ? 2 : 1);
+  a.Tn = cdiv(a.N, CW);
+  const int64_t tiles = (a.offsets ? a.R / BM + a.E : cdiv(a.R, BM)) * a.Tn;  // the most that any routing can produce
+  MOE_LAUNCH(name, (k_i8_tile<GU, OT, WR, MI, NI>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0, s, a);
+  return check_launch(name);
+}
+
 template <bool GU, typename OT>
 int product(const char* name, hipStream_t s, const I8Args& a) {
-  return launch_small<GU, OT>(name, s, a);
+  const int64_t r = a.R / a.E;
+  const int form = r <= 24 ? 0 : r <= 64 ? 1 : r <= 192 ? 2 : 3;
+  if (form == 0) return launch_small<GU, OT>(name, s, a);
+  if (form == 1) return launch_tile<GU, OT, 1, 2, 2>(name, s, a);
+  if (form == 2) return launch_tile<GU, OT, 2, 2, 4>(name, s, a);
+  return launch_tile<GU, OT, 2, 4, 4>(name, s, a);
 }
 
 bool al16_i8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
