@@ -15,8 +15,14 @@
 // loads bytes [16 q, 16 q + 16) of a 64-byte half chunk of row r.  The k slot that a value lands in is free as long as both
 // operands agree.  The waves' partial sums meet in LDS.  Every 64 rows of an expert are a pass of their own blocks over its
 // weights.  Blocks start their chunks at different columns: rows lie a power of two apart, and blocks that walk them in step
-// ask the same few memory channels.
+// ask the same few memory channels.  One token, two experts, H 4096, F 14336: 45 us for gate and up (235 MB, 5.2 TB/s), 24 for
+// the down projection (117 MB).
+//
+// More rows (k_i8_tile): both operands from memory straight to LDS.  128 rows on 8 experts of that layer: 160 us for gate and up
+// (940 MB, 5.9 TB/s: all the card reads), 80 for the down projection; 16384 rows: 1.83 ms for gate and up (3.85 Tops, 2.1 Pops/s)
+// and 0.93 ms, where the matrix instructions' power sets the clock (8192^3: 2.39 Pops/s, a library's product 2.41).
 #include <algorithm>
+#include <type_traits>
 #include <utility>
 
 #include "common.h"
@@ -45,6 +51,9 @@ struct I8Args {
   int N;                // output columns
   int Tn;               // column tiles
   int E;
+  bool scan;            // k_i8_small: blocks for the passes that there are alone
+  bool tails;           // tiles: experts' last rows behind all whole tiles
+  int parts;            // tiles: blocks that a tile's reduction is split over; their sums go to C as int32 [parts][R][columns]
 };
 
 __device__ __forceinline__ i32x4 mma_i8(const u32x4& w, const u32x4& a, const i32x4& c) {
@@ -200,14 +209,16 @@ template <bool GU, typename OT, int NF, int NW>
 __global__ __launch_bounds__(NW * 64, 8 / NW) void k_i8_small(I8Args g) {
   __shared__ __attribute__((aligned(16))) int red[NW * 16 * (NF * 16 + 4)];
   const int slot = (int)(blockIdx.x / g.Tn), nt = (int)(blockIdx.x % g.Tn);
+  // Block slots: every expert's first pass, then the passes past those.  With far fewer rows than experts (g.scan) the slots are
+  // the passes that there are, experts one after the other: E 128, 8 rows 32 -> 21 us, but 64 rows 56 -> 63.
   int e = slot, pass = 0;
-  if (slot >= g.E) {  // the (slot - E)-th of the passes past the experts' first ones
-    const int lane = threadIdx.x & 63;
-    int x = slot - g.E;
+  const int lane = threadIdx.x & 63, skip = g.scan ? 0 : 1;
+  if (g.scan || slot >= g.E) {
+    int x = g.scan ? slot : slot - g.E;
     for (int e0 = 0;; e0 += 64) {
       if (e0 >= g.E) return;
       const int i = e0 + lane;
-      const int c = i < g.E ? max((int)(seg(g, i + 1) - seg(g, i) + kI8Pass - 1) / kI8Pass - 1, 0) : 0;
+      const int c = i < g.E ? max((int)((seg(g, i + 1) - seg(g, i) + kI8Pass - 1) / kI8Pass) - skip, 0) : 0;
       int upto = c;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -218,7 +229,7 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void k_i8_small(I8Args g) {
       if (past) {
         const int l = __builtin_ctzll(past);
         e = e0 + l;
-        pass = x - (__shfl(upto, l) - __shfl(c, l)) + 1;
+        pass = x - (__shfl(upto, l) - __shfl(c, l)) + skip;
         break;
       }
       x -= __shfl(upto, 63);
@@ -237,62 +248,292 @@ __global__ __launch_bounds__(NW * 64, 8 / NW) void k_i8_small(I8Args g) {
 }
 
 template <bool GU, typename OT>
-int launch_small(const char* name, hipStream_t s, I8Args a) {
-  const int64_t slots = a.E + a.R / kI8Pass;  // every expert's first pass, and as many more as R rows can need
-  if (cdiv(a.N, GU ? 32 : 64) * (int64_t)a.E >= 512) {
+int launch_small(hipStream_t s, I8Args a) {
+  constexpr const char* name = GU ? "k_i8_small_gu" : "k_i8_small";
+  const int64_t live = std::min<int64_t>(a.E, a.R);  // experts with rows, at most
+  a.scan = a.R * 4 <= a.E;
+  const int64_t slots = (a.scan ? live : a.E) + a.R / kI8Pass;  // the most passes that any routing can take
+  if (cdiv(a.N, GU ? 32 : 64) * live >= 512) {
     a.Tn = cdiv(a.N, GU ? 32 : 64);
     MOE_LAUNCH(name, (k_i8_small<GU, OT, 4, 4>), dim3((unsigned)(a.Tn * slots)), dim3(256), 0, s, a);
-  } else {
+  } else if (GU || cdiv(a.N, 32) * live >= 256) {
     a.Tn = cdiv(a.N, GU ? 16 : 32);
     MOE_LAUNCH(name, (k_i8_small<GU, OT, 2, 8>), dim3((unsigned)(a.Tn * slots)), dim3(512), 0, s, a);
+  } else if constexpr (!GU) {
+    a.Tn = cdiv(a.N, 16);
+    MOE_LAUNCH(name, (k_i8_small<GU, OT, 1, 8>), dim3((unsigned)(a.Tn * slots)), dim3(512), 0, s, a);
   }
   return check_launch(name);
 }
 
 // ---- many rows ----
-typedef __attribute__((address_space(1))) const u32x4 g_u32x4;
-__device__ __forceinline__ u32x4 ldg16(const uint8_t* p) {
-  return *reinterpret_cast<g_u32x4*>(reinterpret_cast<uintptr_t>(p));
-}
-struct __attribute__((packed, aligned(4))) Scale4 { float v[4]; };
-__device__ __attribute__((aligned(16))) const uint8_t g_i8_zero[16] = {0};
+//
+// A tile (i8_tile): up to 256 rows of an expert by 256 weight rows (GU: 128 gate rows and the matching up rows, 32 by 32) on
+// v_mfma_i32_32x32x32_i8, four waves, one a SIMD.  Both operands go from memory straight to LDS (global_load_lds) in slices of
+// 128 bytes of a row, whole cache lines, a row's eight 16-byte chunks swizzled so that the 16 rows a fragment read touches at
+// once lie in distinct banks.
+struct I8Place {
+  int e;
+  int64_t mbase;  // the tile's first row
+  int mlen, n0;   // its rows; its first output column
+  int k0, klen;   // the columns of A and B to sum over
+  int part;
+};
 
-// One tile of BM rows of an expert by BN weight rows (GU: BN / 2 gate rows and the matching up rows, 32 by 32), four waves
-// WR x WC of MI x NI fragments of v_mfma_i32_32x32x32_i8.  Both operands go through LDS in slices of 128 bytes of a row (whole
-// cache lines), two slices at a time, a row's eight 16-byte chunks swizzled so that the 16 rows a fragment read touches at
-// once lie in distinct banks.  While slice kt is computed, each wave writes its share of slice kt + 1 (in registers since the
-// slice before) into the free half and loads its share of slice kt + 2 into the same registers, one 16-byte piece a lane at a
-// time between the matrix instructions; one barrier a slice.
-template <bool GU, typename OT, int WR, int MI, int NI>
-__global__ __launch_bounds__(256, MI * NI <= 4 ? 2 : 1) void k_i8_tile(I8Args g) {
-  constexpr int WC = 4 / WR;
-  constexpr int BM = WR * MI * 32, BN = WC * NI * 32;
-  constexpr int SA = BM * 128, SB = BN * 128;          // LDS bytes of a slice of either operand
+__device__ __attribute__((aligned(16))) const uint8_t g_i8_zero[16] = {0};
+struct __attribute__((packed, aligned(4))) Scale4 { float v[4]; };
+typedef __attribute__((address_space(3))) void lds_i8_t;
+
+// s_waitcnt vmcnt(n), and lgkmcnt(0) or unconstrained.
+template <int N, bool LGKM0>
+__device__ __forceinline__ void i8_wait() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (LGKM0 ? 0 : 15 << 8));
+}
+
+// LDS of a tile of WR MI 32 rows: NS stages of a slice of both operands.
+template <int WR, int MI, int NI>
+constexpr int i8_stage() { return (WR * MI + 4 / WR * NI) * 32 * 128; }
+
+// WR x (4 / WR) waves of MI x NI fragments.  The ring holds NS slices: while slice kt is multiplied the next NS - 1 are on their
+// way.  A slice is four 32-wide quarters of MI NI matrix instructions, each followed by at most a fragment read of the next
+// quarter and a refill piece or two (16 bytes a lane).  The slice's one barrier lies inside its last quarter, when the wave's
+// own LDS reads of the slice have long drained under matrix instructions: behind it slice kt + 1 is complete and slice kt's
+// stage is free for slice kt + NS.
+template <bool GU, typename OT, int WR, int MI, int NI, int NS>
+__device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint8_t* smem) {
+  constexpr int WC = 4 / WR, BM = WR * MI * 32, BN = WC * NI * 32;
+  constexpr int SA = BM * 128, STAGE = i8_stage<WR, MI, NI>();
   constexpr int QA = BM / 32, QB = BN / 32, NP = QA + QB;  // 16-byte pieces of a wave's share of a slice
-  constexpr int CW = GU ? BN / 2 : BN;                 // output columns of the tile
-  constexpr int WCOLS = CW / WC;                       // ... and of a wave
-  constexpr int CP = GU ? (WCOLS + 8) / 2 : WCOLS + 4; // words a row of a wave's output strip of 32 rows
-  constexpr int SMEM = std::max(2 * (SA + SB), 4 * 32 * CP * 4);
-  __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr bool PART = std::is_same_v<OT, int>;           // int32 sums of a part of the reduction
+  constexpr int CW = GU ? BN / 2 : BN, WCOLS = CW / WC;    // output columns of the tile and of a wave
+  constexpr int CP = (WCOLS * (int)sizeof(OT) + 16) / 4;   // words a row of a wave's output strip of 32 rows
+  static_assert(!(GU && PART), "gate and up sums meet in one block");
+  static_assert(4 * 32 * CP * 4 <= NS * STAGE, "the output strips reuse the ring");
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm0 = wv / WC * (MI * 32), wn0 = wv % WC * (NI * 32);
   const int i32 = lane & 31, h = lane >> 5;
+  const int K = at.klen, nk = (K + 127) / 128, whole = K / 128;
 
-  // XCD-contiguous logical order over a 1-D grid sized for the most tiles any routing can produce: the tiles that there are,
-  // split into 8 contiguous ranges (blockIdx mod 8)
-  auto row_tiles = [&](int e) {
-    return e < g.E ? (int)((seg(g, e + 1) - seg(g, e) + BM - 1) / BM) : 0;
+  // piece p of a wave's share: instruction j fills rows 8 j + lane / 8 of its operand's tile, slot lane % 8 of the row.  Rows
+  // past the tile repeat the last one.
+  const int64_t eb = (int64_t)at.e * g.N * g.K + at.k0;
+  const uint8_t* const b_base[2] = {g.B + eb, (GU ? g.B2 : g.B) + eb};
+  const uint8_t* a_src[QA];
+  uint32_t b_off[QB];
+  auto chunk_of = [&](int j) { return (lane & 7) ^ ((4 * j + (lane >> 4)) & 7); };
+#pragma unroll
+  for (int q = 0; q < QA; ++q) {
+    const int j = QA * wv + q;
+    a_src[q] = g.A + source_row(g, at.mbase + min(8 * j + (lane >> 3), at.mlen - 1)) * g.K + at.k0 + chunk_of(j) * 16;
+  }
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const int j = QB * wv + q, i = 8 * j + (lane >> 3);
+    const int n = GU ? at.n0 + (i >> 6) * 32 + (i & 31) : at.n0 + i;
+    b_off[q] = (uint32_t)min(n, g.N - 1) * (uint32_t)g.K + chunk_of(j) * 16;
+  }
+  // Piece p of slice kt to the stage at byte s; past the row's end A is zeros and B anything.  Issued from asm: the compiler
+  // would make every LDS read that it cannot tell apart wait for all of them; the waits are the loop's own.  (m0 is written by
+  // the scalar unit: one wait state.)
+  auto fill = [&](int kt, int s, int p, bool full) {
+    const uint8_t* src;
+    int to;
+    if (p < QA) {
+      const int j = QA * wv + p;
+      src = a_src[p] + kt * 128;
+      if (!full) src = kt * 128 + chunk_of(j) * 16 < K ? src : g_i8_zero;
+      to = j * 1024;
+    } else {
+      const int q = p - QA, j = QB * wv + q;
+      const uint8_t* const base = b_base[GU ? (8 * j >> 5) & 1 : 0];
+      const int k = kt * 128 + chunk_of(j) * 16;
+      src = full || k < K ? base + ((uint32_t)kt * 128u + b_off[q]) : base + (b_off[q] - chunk_of(j) * 16);
+      to = SA + j * 1024;
+    }
+    __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                     :
+                     : "v"(src), "{m0}"((uint32_t)(uintptr_t)(lds_i8_t*)(smem + s + to))
+                     : "memory");
   };
+  // fragment f of quarter ks of the slice in stage s, in the order in which the quarter's matrix instructions need them
+  auto read_frag = [&](int s, int ks, int f, i32x4(&fa)[MI], i32x4(&fb)[NI]) {
+    const bool is_a = f == 0 || f > NI;
+    const int x = is_a ? (f ? f - NI : 0) : f - 1, row = (is_a ? wm0 : wn0) + x * 32 + i32;
+    const i32x4 v = *reinterpret_cast<const i32x4*>(smem + s + (is_a ? 0 : SA) + row * 128 +
+                                                    (((2 * ks + h) ^ ((row >> 1) & 7)) << 4));
+    if (is_a) fa[x] = v;
+    else fb[x] = v;
+  };
+
+  i32x16 acc[MI][NI];
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[mi][ni][j] = 0;
+
+  // Refill pieces: the first PD from the barrier on, the others in the next slice's first quarter.
+  constexpr int SLOTS = MI * NI, NF = MI + NI, SLACK = std::max(std::min(SLOTS - NF, 4), 0), PD = std::min(NP, SLOTS - SLACK);
+  // FILL 0: none; 1: whole slices; 2: the slice may end inside.  PLO, PHI: pieces, spread over the slots from RLO on.  VM: loads
+  // that may still be on their way at the barrier (-1: no barrier).
+  auto quarter = [&](auto fill_c, auto plo_c, auto phi_c, auto rlo_c, auto vm_c, const i32x4(&ca)[MI], const i32x4(&cb)[NI],
+                     int ns, int nks, bool read_next, i32x4(&na)[MI], i32x4(&nb)[NI], int fkt, int fs) {
+    constexpr int FILL = decltype(fill_c)::value, PLO = decltype(plo_c)::value, PHI = decltype(phi_c)::value;
+    constexpr int RLO = decltype(rlo_c)::value, VM = decltype(vm_c)::value;
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      (([&] {
+         constexpr int mi = I / NI, ni = I % NI;
+         if constexpr (VM >= 0 && I == RLO) {
+           i8_wait<VM, true>();
+           __asm__ volatile("" ::: "memory");
+           __builtin_amdgcn_s_barrier();
+           __asm__ volatile("" ::: "memory");
+           __builtin_amdgcn_sched_barrier(0);
+         }
+         acc[mi][ni] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cb[ni], ca[mi], acc[mi][ni], 0, 0, 0);
+         __builtin_amdgcn_sched_barrier(0);
+         // (reads: one a slot, or as many as it takes to end with the quarter)
+         if constexpr (I >= RLO) {
+           constexpr int N = SLOTS - RLO, R0 = N >= NF ? std::min(I - RLO, NF) : NF * (I - RLO) / N;
+           constexpr int R1 = N >= NF ? std::min(I - RLO + 1, NF) : NF * (I - RLO + 1) / N;
+           if (read_next) {
+             [&]<int... X>(std::integer_sequence<int, X...>) {
+               (read_frag(ns, nks, R0 + X, na, nb), ...);
+             }(std::make_integer_sequence<int, R1 - R0>{});
+           }
+         }
+         if constexpr (FILL > 0 && I >= RLO) {
+           constexpr int P0 = PLO + (PHI - PLO) * (I - RLO) / (SLOTS - RLO), P1 = PLO + (PHI - PLO) * (I - RLO + 1) / (SLOTS - RLO);
+           [&]<int... P>(std::integer_sequence<int, P...>) {
+             (fill(fkt, fs, P0 + P, FILL == 1 || fkt < whole), ...);
+           }(std::make_integer_sequence<int, P1 - P0>{});
+         }
+         __builtin_amdgcn_sched_barrier(0);
+       }()), ...);
+    }(std::make_integer_sequence<int, SLOTS>{});
+  };
+  using C0 = std::integral_constant<int, 0>;
+  using C1 = std::integral_constant<int, 1>;
+  using C2 = std::integral_constant<int, 2>;
+  using CN = std::integral_constant<int, -1>;
+  using CD = std::integral_constant<int, PD>;
+  using CP_ = std::integral_constant<int, NP>;
+  using CS = std::integral_constant<int, SLACK>;
+  i32x4 fa0[MI], fb0[NI], fa1[MI], fb1[NI];
+  auto next = [&](int s) { return s + STAGE == NS * STAGE ? 0 : s + STAGE; };
+  auto prev = [&](int s) { return s == 0 ? (NS - 1) * STAGE : s - STAGE; };
+  // Slice kt, in stage s.  F0: fills of the rest of slice kt + NS - 1, F1: of the first of slice kt + NS; VM as above.
+  auto slice = [&](auto f0, auto f1, auto vm, int kt, int s) {
+    quarter(f0, CD{}, CP_{}, C0{}, CN{}, fa0, fb0, s, 1, true, fa1, fb1, kt + NS - 1, prev(s));
+    quarter(C0{}, C0{}, C0{}, C0{}, CN{}, fa1, fb1, s, 2, true, fa0, fb0, 0, 0);
+    quarter(C0{}, C0{}, C0{}, C0{}, CN{}, fa0, fb0, s, 3, true, fa1, fb1, 0, 0);
+    quarter(f1, C0{}, CD{}, CS{}, vm, fa1, fb1, next(s), 0, kt + 1 < nk, fa0, fb0, kt + NS, s);
+  };
+  for (int t = 0; t < NS && t < nk; ++t)
+    for (int p = 0; p < (t < NS - 1 ? NP : PD); ++p) fill(t, t * STAGE, p, t < whole);
+  if (nk >= NS) i8_wait<(NS - 2) * NP + PD, false>();  // slice 0 is there
+  else i8_wait<0, false>();
+  lds_sync();
+  for (int f = 0; f < NF; ++f) read_frag(0, 0, f, fa0, fb0);
+  int kt = 0, s = 0;
+  using CV = std::integral_constant<int, (NS - 2) * NP>;
+  for (; kt + NS < whole; ++kt, s = next(s)) slice(C1{}, C1{}, CV{}, kt, s);
+  for (; kt + NS < nk; ++kt, s = next(s)) slice(C2{}, C2{}, CV{}, kt, s);
+  if (kt + NS - 1 < nk) {
+    slice(C2{}, C0{}, CV{}, kt, s);
+    ++kt, s = next(s);
+  }
+  for (; kt < nk; ++kt, s = next(s)) slice(C0{}, C0{}, C0{}, kt, s);
+  __syncthreads();
+
+  // The matrix instructions take the weights as their M operand, so a lane holds one row of C and, in each four accumulators,
+  // four columns in a row: acc[mi][ni][j] = C[wm0 + 32 mi + lane % 32][wn0 + 32 ni + 8 (j / 4) + 4 (lane / 32) + j % 4].  Each
+  // wave turns its strips of 32 rows over through LDS of its own, so that rows leave in whole lines.
+  uint32_t* const cs = reinterpret_cast<uint32_t*>(smem) + wv * 32 * CP;
+  const int c0 = at.n0 + wv % WC * WCOLS;  // the wave's first column
+  const float* const sb = g.sb + (int64_t)at.e * g.N;
+  const float* const sb2 = GU ? g.sb2 + (int64_t)at.e * g.N : nullptr;
+  // the lane's scales, all asked for before the first is used: [0] of every accumulator column (GU: of the gate), [1] of the up
+  constexpr int NS4 = GU ? NI * 2 : NI * 4;
+  Scale4 sc[GU ? 2 : 1][NS4];
+  float sx[MI];
+  if constexpr (!PART) {
+#pragma unroll
+    for (int u = 0; u < NS4; ++u) {
+      const int n = min(c0 + u * 8 + h * 4, g.N - 4);
+      sc[0][u] = *reinterpret_cast<const Scale4*>(sb + n);
+      if constexpr (GU) sc[1][u] = *reinterpret_cast<const Scale4*>(sb2 + n);
+    }
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) sx[mi] = g.sa[source_row(g, at.mbase + min(wm0 + mi * 32 + i32, at.mlen - 1))];
+  }
+  OT* const out = static_cast<OT*>(g.C) + (PART ? (int64_t)at.part * g.R * g.N : 0);
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    const int r0 = wm0 + mi * 32;  // the strip's first row of the tile
+    if (r0 >= at.mlen) break;
+    __asm__ volatile("" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < NS4; ++u) {
+      const int c = u * 8 + h * 4, v = u % 4;  // the lane's column of the strip
+      if constexpr (PART) {
+        const i32x16& t = acc[mi][u / 4];
+        *reinterpret_cast<i32x4*>(cs + i32 * CP + c) = i32x4{t[4 * v], t[4 * v + 1], t[4 * v + 2], t[4 * v + 3]};
+      } else {
+        f32x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (GU) {
+            const float gv = (float)acc[mi][u / 4 * 2][4 * v + j] * sx[mi] * sc[0][u].v[j];
+            o[j] = gv * sig_i8(gv) * ((float)acc[mi][u / 4 * 2 + 1][4 * v + j] * sx[mi] * sc[1][u].v[j]);
+          } else {
+            o[j] = (float)acc[mi][u / 4][4 * v + j] * sx[mi] * sc[0][u].v[j];
+          }
+        }
+        if constexpr (sizeof(OT) == 2)
+          *reinterpret_cast<uint2*>(cs + i32 * CP + c / 2) = uint2{pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+        else *reinterpret_cast<f32x4*>(cs + i32 * CP + c) = o;
+      }
+    }
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int PER = 16 / sizeof(OT);  // columns of a 16-byte store
+    constexpr int LPR = WCOLS / PER;      // lanes a row
+#pragma unroll
+    for (int u = 0; u < 32 * LPR / 64; ++u) {
+      const int r = u * (64 / LPR) + lane / LPR, c = lane % LPR * PER;
+      const u32x4 o = *reinterpret_cast<const u32x4*>(cs + r * CP + c * (int)sizeof(OT) / 4);
+      if (r0 + r < at.mlen && c0 + c < g.N)
+        *reinterpret_cast<u32x4*>(out + (at.mbase + r0 + r) * g.N + c0 + c) = o;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The number of row tiles of expert e: all (KIND 0), those of more than 3/4 BM rows (1) or a shorter one behind them (2).
+template <int BM, int KIND>
+__device__ __forceinline__ int i8_row_tiles(const I8Args& g, int e) {
+  if (e >= g.E) return 0;
+  const int64_t r = max(seg(g, e + 1) - seg(g, e), (int64_t)0);
+  const int all = (int)((r + BM - 1) / BM), tall = (int)((r + BM / 4 - 1) / BM);
+  return KIND == 0 ? all : KIND == 1 ? tall : all - tall;
+}
+template <int BM, int KIND>
+__device__ __forceinline__ int i8_total(const I8Args& g, int lane) {
   int sum = 0;
-  for (int e0 = 0; e0 < g.E; e0 += 64) sum += max(row_tiles(e0 + lane), 0);
+  for (int e0 = 0; e0 < g.E; e0 += 64) sum += i8_row_tiles<BM, KIND>(g, e0 + lane);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  const int total = __builtin_amdgcn_readfirstlane(sum) * g.Tn;
-  const int chunk = (total + 7) >> 3, slot = (int)(blockIdx.x >> 3), L = (int)(blockIdx.x & 7) * chunk + slot;
-  if (slot >= chunk || L >= total) return;
+  return __builtin_amdgcn_readfirstlane(sum) * g.Tn;
+}
+// Tile number L (below the total) of that kind: experts one after the other, within an expert groups of up to 8 row tiles with the
+// columns walked inside a group, so that the tiles that run at once share few operand panels.
+template <int BM, int KIND>
+__device__ __forceinline__ I8Place i8_place(const I8Args& g, int L, int cw, int lane) {
   int e = 0, before = 0, cnt = 0;  // row tiles of the experts before e, and of e
   for (int e0 = 0;; e0 += 64) {
-    const int c = max(row_tiles(e0 + lane), 0);
+    const int c = i8_row_tiles<BM, KIND>(g, e0 + lane);
     int upto = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -309,211 +550,184 @@ __global__ __launch_bounds__(256, MI * NI <= 4 ? 2 : 1) void k_i8_tile(I8Args g)
     }
     before += __shfl(upto, 63);
   }
-  e = __builtin_amdgcn_readfirstlane(e);
+  I8Place p;
+  p.e = __builtin_amdgcn_readfirstlane(e);
   cnt = __builtin_amdgcn_readfirstlane(cnt);
   const int local = L - __builtin_amdgcn_readfirstlane(before) * g.Tn;
   constexpr int GM = 8;
   const int grp = local / (GM * g.Tn), rest = local - grp * GM * g.Tn, gm = min(cnt - grp * GM, GM);
-  const int nt = rest / gm, mt = grp * GM + rest - nt * gm;
-  const int64_t mbase = seg(g, e) + (int64_t)mt * BM;
-  const int mlen = (int)min(seg(g, e + 1) - mbase, (int64_t)BM);
-  const int n0 = nt * CW, K = g.K, nk = (K + 127) / 128;
+  const int nt = rest / gm;
+  int mt = grp * GM + rest - nt * gm;
+  const int64_t lo = seg(g, p.e), hi = seg(g, p.e + 1);
+  if (KIND == 2) mt = i8_row_tiles<BM, 1>(g, p.e);
+  p.mbase = lo + (int64_t)mt * BM;
+  p.mlen = (int)min(hi - p.mbase, (int64_t)BM);
+  p.n0 = nt * cw;
+  p.k0 = 0;
+  p.klen = g.K;
+  p.part = 0;
+  return p;
+}
 
-  // piece p of a wave's share: instruction j fills rows 8 j + lane / 8 of its operand's tile, slot lane % 8 of the row
-  const uint8_t* const b_base[2] = {g.B + (int64_t)e * g.N * K, GU ? g.B2 + (int64_t)e * g.N * K : g.B + (int64_t)e * g.N * K};
-  const uint8_t* a_src[QA];
-  uint32_t b_off[QB];
-  auto chunk_of = [&](int j) { return (lane & 7) ^ ((4 * j + (lane >> 4)) & 7); };
-#pragma unroll
-  for (int q = 0; q < QA; ++q) {
-    const int j = QA * wv + q;
-    a_src[q] = g.A + source_row(g, mbase + min(8 * j + (lane >> 3), mlen - 1)) * K + chunk_of(j) * 16;
-  }
-#pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    const int j = QB * wv + q, i = 8 * j + (lane >> 3);
-    const int n = GU ? n0 + (i >> 6) * 32 + (i & 31) : n0 + i;
-    b_off[q] = (uint32_t)min(n, g.N - 1) * (uint32_t)K + chunk_of(j) * 16;
-  }
-  u32x4 st[NP];
-  // piece p of slice kt; past the row's end A is zeros and B anything
-  auto gload = [&](int kt, int p, bool full) {
-    if (p < QA) {
-      const uint8_t* s = a_src[p] + kt * 128;
-      if (!full) s = kt * 128 + chunk_of(QA * wv + p) * 16 < K ? s : g_i8_zero;
-      st[p] = ldg16(s);
+// Tiles of up to BM rows by BN weight rows, each as tall as its rows need.  One dimension of blocks, sized for the most tiles any
+// routing can produce; the tiles that there are lie in 8 contiguous ranges, one an XCD (blockIdx mod 8).
+//   256 x 256: many rows.  g.tails: the short tiles of experts' last rows come behind all others, so that they fill the last round.
+//   192 x 128, 64 x 256: few enough that the weights' stream bounds the product; two blocks a CU, for more of it on its way.
+//     DEEP: one block a CU with more slices on their way, where there are no more tiles than CUs.
+template <bool GU, typename OT, int BM, int BN, bool DEEP>
+__global__ __launch_bounds__(256, BM == 256 || DEEP ? 1 : 2) void k_i8_tile(I8Args g) {
+  constexpr int SMEM = BM == 256 ? std::max(3 * i8_stage<1, 4, 2>(), 2 * i8_stage<2, 4, 4>())
+                       : DEEP ? 6 * i8_stage<2, 1, 2>() : BM == 192 ? 2 * i8_stage<2, 3, 2>() : 2 * i8_stage<1, 2, 2>();
+  __shared__ __attribute__((aligned(16))) uint8_t smem[SMEM];
+  const int lane = threadIdx.x & 63;
+  constexpr int CW = GU ? BN / 2 : BN;
+  const int xcd = (int)(blockIdx.x & 7), slot = (int)(blockIdx.x >> 3);
+  I8Place at;
+  if (BM == 256 && g.tails) {
+    const int n1 = i8_total<BM, 1>(g, lane), n2 = i8_total<BM, 2>(g, lane), c1 = (n1 + 7) >> 3, c2 = (n2 + 7) >> 3;
+    if (slot < c1) {
+      const int L = xcd * c1 + slot;
+      if (L >= n1) return;
+      at = i8_place<BM, 1>(g, L, CW, lane);
     } else {
-      const int q = p - QA, j = QB * wv + q;
-      const uint8_t* const base = b_base[GU ? (8 * j >> 5) & 1 : 0];
-      uint32_t o = b_off[q];
-      if (full) {
-        st[p] = ldg16(base + (uint32_t)kt * 128u + o);
-      } else {
-        const int k = kt * 128 + chunk_of(j) * 16;
-        st[p] = ldg16(base + (o - chunk_of(j) * 16) + (k < K ? (uint32_t)k : 0u));
-      }
+      const int L = xcd * c2 + slot - c1;
+      if (slot - c1 >= c2 || L >= n2) return;
+      at = i8_place<BM, 2>(g, L, CW, lane);
     }
-  };
-  auto half = [&](int kt) { return smem + (kt & 1) * (SA + SB); };
-  auto lwrite = [&](int kt, int p) {
-    uint8_t* const d = half(kt) + (p < QA ? (QA * wv + p) * 1024 : SA + (QB * wv + p - QA) * 1024);
-    __asm__ volatile("" ::: "memory");
-    *reinterpret_cast<u32x4*>(d + lane * 16) = st[p];
-    __asm__ volatile("" ::: "memory");
-  };
-  auto frag = [&](const uint8_t* t, int row, int ks) {
-    return *reinterpret_cast<const i32x4*>(t + row * 128 + (((2 * ks + h) ^ ((row >> 1) & 7)) << 4));
-  };
-  auto read_frag = [&](int kt, int ks, int f, i32x4(&fa)[MI], i32x4(&fb)[NI]) {
-    if (f < MI) fa[f] = frag(half(kt), wm0 + f * 32 + i32, ks);
-    else fb[f - MI] = frag(half(kt) + SA, wn0 + (f - MI) * 32 + i32, ks);
-  };
-
-  i32x16 acc[MI][NI];
-#pragma unroll
-  for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-    for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) acc[mi][ni][j] = 0;
-
-  // One 32-wide quarter of slice kt: MI NI matrix instructions, after each at most a fragment read of the next quarter (the
-  // first ones) and a refill piece of [PLO, PHI) (the last ones).  MODE 0: write slice kt + 1, load the whole slice kt + 2;
-  // 1: the slice loaded may end inside; 2: write only; 3: neither.
-  constexpr int SLOTS = MI * NI;
-  auto quarter = [&](auto mode_c, auto plo_c, auto phi_c, const i32x4(&ca)[MI], const i32x4(&cb)[NI], int nkt, int nks,
-                     bool read_next, i32x4(&na)[MI], i32x4(&nb)[NI], int kt, bool lfull) {
-    constexpr int MODE = decltype(mode_c)::value, PLO = decltype(plo_c)::value, PHI = decltype(phi_c)::value;
-    static_assert(PHI - PLO <= SLOTS && MI + NI <= SLOTS);
-    [&]<int... I>(std::integer_sequence<int, I...>) {
-      (([&] {
-         constexpr int mi = I / NI, ni = I % NI;
-         acc[mi][ni] = __builtin_amdgcn_mfma_i32_32x32x32_i8(cb[ni], ca[mi], acc[mi][ni], 0, 0, 0);
-         __builtin_amdgcn_sched_barrier(0);
-         if constexpr (I < MI + NI) {
-           if (read_next) read_frag(nkt, nks, I, na, nb);
-         }
-         constexpr int p = PHI - SLOTS + I;
-         if constexpr (MODE < 3 && p >= PLO) {
-           lwrite(kt + 1, p);
-           if constexpr (MODE == 0) gload(kt + 2, p, true);
-           else if constexpr (MODE == 1) gload(kt + 2, p, lfull);
-         }
-         __builtin_amdgcn_sched_barrier(0);
-       }()), ...);
-    }(std::make_integer_sequence<int, SLOTS>{});
-  };
-  using P0 = std::integral_constant<int, 0>;
-  using P1 = std::integral_constant<int, (NP + 2) / 3>;
-  using P2 = std::integral_constant<int, (2 * NP + 2) / 3>;
-  using P3 = std::integral_constant<int, NP>;
-  using M3 = std::integral_constant<int, 3>;
-  i32x4 fa0[MI], fb0[NI], fa1[MI], fb1[NI];
-  const int whole = K / 128;  // whole slices
-  auto slice = [&](auto mode_c, int kt) {
-    const bool lfull = kt + 2 < whole;
-    quarter(mode_c, P0{}, P1{}, fa0, fb0, kt, 1, true, fa1, fb1, kt, lfull);
-    quarter(mode_c, P1{}, P2{}, fa1, fb1, kt, 2, true, fa0, fb0, kt, lfull);
-    quarter(mode_c, P2{}, P3{}, fa0, fb0, kt, 3, true, fa1, fb1, kt, lfull);
-    lds_sync();  // this wave's pieces of slice kt + 1 are written and its reads of slice kt done, and every other wave's
-    __builtin_amdgcn_sched_barrier(0);
-    quarter(M3{}, P3{}, P3{}, fa1, fb1, kt + 1, 0, kt + 1 < nk, fa0, fb0, kt, true);
-  };
-  for (int p = 0; p < NP; ++p) gload(0, p, 0 < whole);
-  for (int p = 0; p < NP; ++p) lwrite(0, p);
-  if (nk > 1) {
-    for (int p = 0; p < NP; ++p) gload(1, p, 1 < whole);
+  } else {
+    const int n = i8_total<BM, 0>(g, lane) * g.parts, chunk = (n + 7) >> 3, L = xcd * chunk + slot;
+    if (slot >= chunk || L >= n) return;
+    at = i8_place<BM, 0>(g, L / g.parts, CW, lane);
+    if constexpr (std::is_same_v<OT, int>) {
+      const int nk = (g.K + 127) / 128;
+      at.part = L % g.parts;
+      at.k0 = nk * at.part / g.parts * 128;
+      at.klen = min(nk * (at.part + 1) / g.parts * 128, g.K) - at.k0;
+    }
   }
-  __syncthreads();
-  for (int f = 0; f < MI + NI; ++f) read_frag(0, 0, f, fa0, fb0);
-  int kt = 0;
-  for (; kt + 2 < whole; ++kt) slice(std::integral_constant<int, 0>{}, kt);
-  for (; kt + 2 < nk; ++kt) slice(std::integral_constant<int, 1>{}, kt);
-  if (kt + 1 < nk) slice(std::integral_constant<int, 2>{}, kt++);
-  if (kt < nk) slice(M3{}, kt);
-  __syncthreads();
-
-  // The matrix instructions take the weights as their M operand, so a lane holds one row of C and, in each four accumulators,
-  // four columns in a row: acc[mi][ni][j] = C[wm0 + 32 mi + lane % 32][wn0 + 32 ni + 8 (j / 4) + 4 (lane / 32) + j % 4].  Each
-  // wave turns its strips of 32 rows over through LDS of its own, so that rows leave in whole lines.
-  uint32_t* const cs = reinterpret_cast<uint32_t*>(smem) + wv * 32 * CP;
-  const int c0 = n0 + wv % WC * WCOLS;  // the wave's first column
-  const float* const sb = g.sb + (int64_t)e * g.N;
-  const float* const sb2 = GU ? g.sb2 + (int64_t)e * g.N : nullptr;
-#pragma unroll
-  for (int mi = 0; mi < MI; ++mi) {
-    const int r0 = wm0 + mi * 32;  // the strip's first row of the tile
-    if (r0 >= mlen) break;
-    const float sx = g.sa[source_row(g, mbase + min(r0 + i32, mlen - 1))];
-    __asm__ volatile("" ::: "memory");
-    if constexpr (GU) {
-#pragma unroll
-      for (int pr = 0; pr < NI / 2; ++pr)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int c = pr * 32 + v * 8 + h * 4, n = min(c0 + c, g.N - 4);
-          const Scale4 sg = *reinterpret_cast<const Scale4*>(sb + n), su = *reinterpret_cast<const Scale4*>(sb2 + n);
-          float o[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float gv = (float)acc[mi][2 * pr][4 * v + j] * sx * sg.v[j];
-            o[j] = gv * sig_i8(gv) * ((float)acc[mi][2 * pr + 1][4 * v + j] * sx * su.v[j]);
-          }
-          *reinterpret_cast<uint2*>(cs + i32 * CP + c / 2) = uint2{pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
-        }
-    } else {
-#pragma unroll
-      for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int c = ni * 32 + v * 8 + h * 4, n = min(c0 + c, g.N - 4);
-          const Scale4 s = *reinterpret_cast<const Scale4*>(sb + n);
-          f32x4 o;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[j] = (float)acc[mi][ni][4 * v + j] * sx * s.v[j];
-          *reinterpret_cast<f32x4*>(cs + i32 * CP + c) = o;
-        }
-    }
-    __asm__ volatile("" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
-    constexpr int PER = GU || sizeof(OT) == 2 ? 8 : 4;  // columns of a 16-byte store
-    constexpr int LPR = WCOLS / PER;                    // lanes a row
-#pragma unroll
-    for (int u = 0; u < 32 * LPR / 64; ++u) {
-      const int r = u * (64 / LPR) + lane / LPR, c = lane % LPR * PER;
-      u32x4 o;
-      if constexpr (GU) {
-        o = *reinterpret_cast<const u32x4*>(cs + r * CP + c / 2);
-      } else if constexpr (sizeof(OT) == 4) {
-        o = *reinterpret_cast<const u32x4*>(cs + r * CP + c);
-      } else {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(cs + r * CP + c), hi = *reinterpret_cast<const f32x4*>(cs + r * CP + c + 4);
-        o = u32x4{pack2bf(lo[0], lo[1]), pack2bf(lo[2], lo[3]), pack2bf(hi[0], hi[1]), pack2bf(hi[2], hi[3])};
-      }
-      if (r0 + r < mlen && c0 + c < g.N)
-        *reinterpret_cast<u32x4*>(static_cast<OT*>(g.C) + (mbase + r0 + r) * g.N + c0 + c) = o;
-    }
-    __builtin_amdgcn_wave_barrier();
+  if constexpr (BM == 256) {
+    if (at.mlen > 192) i8_tile<GU, OT, 2, 4, 4, 2>(g, at, smem);
+    else if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 4, 2>(g, at, smem);
+    else if (at.mlen > 64) i8_tile<GU, OT, 1, 4, 2, 3>(g, at, smem);
+    else i8_tile<GU, OT, 1, 2, 2, 3>(g, at, smem);
+  } else if constexpr (BM == 192) {
+    if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 2, DEEP ? 3 : 2>(g, at, smem);
+    else if (at.mlen > 64) i8_tile<GU, OT, 2, 2, 2, DEEP ? 4 : 2>(g, at, smem);
+    else i8_tile<GU, OT, 2, 1, 2, DEEP ? 6 : 3>(g, at, smem);
+  } else {
+    i8_tile<GU, OT, 1, 2, 2, 2>(g, at, smem);
   }
 }
 
-template <bool GU, typename OT, int WR, int MI, int NI>
-int launch_tile(const char* name, hipStream_t s, I8Args a) {
-  constexpr int BM = WR * MI * 32, CW = (4 / WR) * NI * 32 / (GU ? 2 : 1);
-  a.Tn = cdiv(a.N, CW);
-  const int64_t tiles = (a.offsets ? a.R / BM + a.E : cdiv(a.R, BM)) * a.Tn;  // the most that any routing can produce
-  MOE_LAUNCH(name, (k_i8_tile<GU, OT, WR, MI, NI>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0, s, a);
+template <bool GU, typename OT, int BM, int BN, bool DEEP = false>
+int launch_tile(hipStream_t s, I8Args a, int parts) {
+  constexpr const char* name = BM == 64    ? (GU ? "k_i8_tile64_gu" : "k_i8_tile64")
+                               : BM == 256 ? (GU ? "k_i8_tile256_gu" : "k_i8_tile256")
+                               : DEEP      ? (GU ? "k_i8_tile192_deep_gu" : "k_i8_tile192_deep")
+                                           : (GU ? "k_i8_tile192_gu" : "k_i8_tile192");
+  a.Tn = cdiv(a.N, GU ? BN / 2 : BN);
+  a.tails = parts == 1 && a.R >= 512 * (int64_t)a.E;
+  a.parts = parts;
+  // the most tiles that any routing can produce, and what rounding two ranges up may add
+  const int64_t tiles = (a.offsets ? a.R / BM + std::min<int64_t>(a.E, a.R) : cdiv(a.R, BM)) * a.Tn * parts;
+  MOE_LAUNCH(name, (k_i8_tile<GU, OT, BM, BN, DEEP>), dim3((unsigned)((tiles + 7) / 8 * 8 + 8)), dim3(256), 0, s, a);
   return check_launch(name);
 }
 
+// y of a product whose reduction was split: the parts' sums added (whole numbers: in any order) and scaled.  A block a row.
+template <typename OT>
+__global__ __launch_bounds__(256) void k_i8_join(I8Args g, const int* __restrict__ part) {
+  const int64_t row = blockIdx.x;
+  int e = 0;
+  if (g.offsets != nullptr) {  // the row's expert: those whose rows all come before it
+    const int lane = threadIdx.x & 63;
+    for (int e0 = 0; e0 < g.E; e0 += 64) {
+      const int n = __popcll(__ballot(e0 + lane < g.E && seg(g, min(e0 + lane, g.E - 1) + 1) <= row));
+      e += n;
+      if (n < 64) break;
+    }
+    e = __builtin_amdgcn_readfirstlane(e);
+    if (e >= g.E || row < seg(g, e)) return;
+  }
+  const float sx = g.sa[source_row(g, row)];
+  const float* const sb = g.sb + (int64_t)e * g.N;
+  for (int c = threadIdx.x * 4; c < g.N; c += 1024) {
+    i32x4 v = {0, 0, 0, 0};
+    for (int p = 0; p < g.parts; ++p) v += *reinterpret_cast<const i32x4*>(part + ((int64_t)p * g.R + row) * g.N + c);
+    const Scale4 sc = *reinterpret_cast<const Scale4*>(sb + c);
+    f32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (float)v[j] * sx * sc.v[j];
+    OT* const y = static_cast<OT*>(g.C) + row * g.N + c;
+    if constexpr (sizeof(OT) == 4) *reinterpret_cast<f32x4*>(y) = o;
+    else *reinterpret_cast<uint2*>(y) = uint2{pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+  }
+}
+
+// The form of a product, by its sizes alone (the host does not know the rows of each expert).  r: rows an expert that can have
+// any; tiles: of 192 x 128.  Measured (us; E, H, F for both products of the experts, K x N for one):
+//   small | 192 x 128    E 8, H 4096, F 14336, r 2, 8, 16: 222 | 228, 249 | 250, 284 | 249.  E 32, H 2048, F 4096, r 4, 8, 16:
+//                        142 | 163, 149 | 167, 175 | 171
+//   small | 64 x 256     E 128, H 2048, F 768, r 1, 2, 4, 8: 79 | 80, 111 | 119, 122 | 124, 126 | 127; routed with a Zipf(1.1)
+//                        bias, r 2, 4, 8: 54 | 46, 66 | 52, 98 | 78: with many experts an even routing is the exception
+//   64 x 256 | 192 x 128 the same layer, r 16, 32: 131 | 138, 140 | 147; biased 8, 16, 32: 78 | 90, 106 | 100, 120 | 121
+//   small | 192 x 128    little work: 4096 x 4096, 16, 32, 64 rows 6.3 | 13, 9 | 13, 13 | 13; 2048 x 2048, 128, 256 rows 8 | 11,
+//                        13 | 14; E 8, 1024 x 512, r 64, 128: 5.8 | 7.4, 8.8 | 8.6; E 8, 528 x 3088, r 16, 32: 6.7 | 6.8, 9 | 7
+//   192 | deep | 256     E 8, H 4096, F 14336, r 32: 263 | 278 | 298; 64: 334 | 295 | 316; 128: 376 | 351 | 417; 256: 520 | 606 |
+//                        547; 512: 887 | 924 | 904; 1024: 1601 | 1785 | 1554.  E 128, H 2048, F 768 (16 and 6 slices), r 128:
+//                        205 | 244 | 210.  4096 x 14336, 96 to 256 rows 25 | 18 | 26 to 30 | 25 | 45, 512: 40 | 47 | 48,
+//                        1024: 71 | 79 | 60; 4096 x 4096, 2048 rows 43 | 50 | 50
+//   parts 1 | 2 | 4      14336 x 4096, 64 rows: 35 | 26 | 21; 256: 58 | 39 | 36; 512: 58 | 45 | 54; 4096 x 4096, 64: 13 | 14 | 15
+enum { kSmall, kTile64, kTile192, kTile192Deep, kTile256 };
+struct I8Form {
+  int kind;
+  int parts;  // blocks that a tile's reduction is split over
+};
+I8Form i8_form(int64_t R, int64_t K, int64_t N, int64_t E, bool gu) {
+  const int64_t live = std::min(E, R), r = R / live, nk = (K + 127) / 128, cols = gu ? 2 * N : N;
+  if (E < 64 ? r <= 8 : r < 2) return {kSmall, 1};
+  if (live * N * K <= (int64_t)1 << 26 && R * K * N <= (int64_t)1 << (live == 1 ? 30 : 28) && (nk < 64 || r <= 16))
+    return {kSmall, 1};
+  if (r > 512 && (r + 255) / 256 * live * ((cols + 255) / 256) >= 192) return {kTile256, 1};
+  if (E >= 64 && r <= 24) return {kTile64, 1};
+  const int64_t tiles = (r + 191) / 192 * live * ((cols + 127) / 128);
+  const int parts = !gu && tiles <= 128 && nk >= 64 ? (int)std::min<int64_t>(4, 256 / tiles) : 1;
+  const bool deep = tiles * parts <= 256 || (r > 48 && r <= 160 && nk >= 32);
+  return {deep ? kTile192Deep : kTile192, parts};
+}
+
 template <bool GU, typename OT>
-int product(const char* name, hipStream_t s, const I8Args& a) {
-  const int64_t r = a.R / a.E;
-  const int form = r <= 24 ? 0 : r <= 64 ? 1 : r <= 192 ? 2 : 3;
-  if (form == 0) return launch_small<GU, OT>(name, s, a);
-  if (form == 1) return launch_tile<GU, OT, 1, 2, 2>(name, s, a);
-  if (form == 2) return launch_tile<GU, OT, 2, 2, 4>(name, s, a);
-  return launch_tile<GU, OT, 2, 4, 4>(name, s, a);
+int launch_form(hipStream_t s, const I8Args& a, const I8Form& f) {
+  switch (f.kind) {
+    case kTile64: return launch_tile<GU, OT, 64, 256>(s, a, f.parts);
+    case kTile192: return launch_tile<GU, OT, 192, 128>(s, a, f.parts);
+    case kTile192Deep: return launch_tile<GU, OT, 192, 128, true>(s, a, f.parts);
+    default: return launch_tile<GU, OT, 256, 256>(s, a, f.parts);
+  }
+}
+
+template <bool GU, typename OT>
+int product(hipStream_t s, const I8Args& a, void* ws) {
+  const I8Form f = i8_form(a.R, a.K, a.N, a.E, GU);
+  if (f.kind == kSmall) return launch_small<GU, OT>(s, a);
+  if constexpr (!GU) {
+    if (f.parts > 1) {
+      I8Args p = a;
+      p.C = ws;
+      if (int rc = launch_form<false, int>(s, p, f)) return rc;
+      p = a;
+      p.parts = f.parts;
+      MOE_LAUNCH("k_i8_join", k_i8_join<OT>, dim3((unsigned)a.R), dim3(256), 0, s, p, static_cast<const int*>(ws));
+      return check_launch("k_i8_join");
+    }
+  }
+  return launch_form<GU, OT>(s, a, f);
+}
+
+// Bytes of the parts' sums.
+size_t i8_part_bytes(int64_t R, int64_t K, int64_t N, int64_t E) {
+  const I8Form f = i8_form(R, K, N, E, false);
+  return f.parts > 1 ? (size_t)f.parts * R * N * 4 : 0;
 }
 
 bool al16_i8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -530,8 +744,14 @@ bool i8_sizes(int64_t R, int64_t K, int64_t N, int64_t E) {
 
 using namespace moe;
 
+extern "C" size_t moe_matmul_int8_workspace(int64_t R, int64_t K, int64_t N, int64_t E) {
+  if (R <= 0 || !i8_sizes(R, K, N, E)) return 0;
+  return i8_part_bytes(R, K, N, E);
+}
+
 extern "C" int moe_matmul_int8(const void* xq, const float* sx, const void* wq, const float* sw, const int32_t* offsets,
-                               int64_t R, int64_t K, int64_t N, int64_t E, void* y, int y_dtype, void* stream) {
+                               int64_t R, int64_t K, int64_t N, int64_t E, void* y, int y_dtype, void* workspace,
+                               size_t ws_bytes, void* stream) {
   if (!i8_sizes(R, K, N, E) || (y_dtype != MOE_BF16 && y_dtype != MOE_F32) || (!offsets && E != 1))
     return fail_arg("moe_matmul_int8: bad arguments R=%lld K=%lld N=%lld E=%lld (need K %% 16 == 0, K <= %lld, N %% 8 == 0, "
                     "N K < 2^32, E <= 1024, bf16 or fp32 y; E == 1 without offsets)", (long long)R, (long long)K, (long long)N,
@@ -539,6 +759,9 @@ extern "C" int moe_matmul_int8(const void* xq, const float* sx, const void* wq, 
   if (R == 0) return 0;
   if (!xq || !sx || !wq || !sw || !y || !al16_i8(xq) || !al16_i8(wq) || !al16_i8(y))
     return fail_arg("moe_matmul_int8: null or misaligned pointer");
+  const size_t need = moe_matmul_int8_workspace(R, K, N, E);
+  if (need > 0 && (!workspace || !al16_i8(workspace) || ws_bytes < need))
+    return set_error("moe_matmul_int8: workspace %zu < %zu bytes, or misaligned", ws_bytes, need), MOE_EWORKSPACE;
   I8Args a{};
   a.A = static_cast<const uint8_t*>(xq);
   a.sa = sx;
@@ -553,13 +776,14 @@ extern "C" int moe_matmul_int8(const void* xq, const float* sx, const void* wq, 
   a.N = (int)N;
   a.E = (int)E;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return y_dtype == MOE_BF16 ? product<false, uint16_t>("k_matmul_int8", s, a) : product<false, float>("k_matmul_int8", s, a);
+  return y_dtype == MOE_BF16 ? product<false, uint16_t>(s, a, workspace)
+                             : product<false, float>(s, a, workspace);
 }
 
-// act (bf16), then act in int8 and its scales
-extern "C" size_t moe_swiglu_fwd_int8_workspace(int64_t R, int64_t F) {
-  if (R <= 0 || F <= 0) return 0;
-  return up256((size_t)R * F * 2) + up256((size_t)R * F) + up256((size_t)R * 4);
+// act (bf16), then act in int8 and its scales; the down projection's partial sums lie where act was
+extern "C" size_t moe_swiglu_fwd_int8_workspace(int64_t R, int64_t H, int64_t F, int64_t E) {
+  if (R <= 0 || !i8_sizes(R, H, F, E) || !i8_sizes(R, F, H, E)) return 0;
+  return up256(std::max((size_t)R * F * 2, i8_part_bytes(R, F, H, E))) + up256((size_t)R * F) + up256((size_t)R * 4);
 }
 
 extern "C" int moe_swiglu_fwd_int8(const void* xq, const float* sx, int64_t T, const int32_t* row_slot, int64_t top_k,
@@ -575,11 +799,11 @@ extern "C" int moe_swiglu_fwd_int8(const void* xq, const float* sx, int64_t T, c
   if (!xq || !sx || !wg_q || !sg || !wu_q || !su || !wd_q || !sd || !offsets || !y || !al16_i8(xq) || !al16_i8(wg_q) ||
       !al16_i8(wu_q) || !al16_i8(wd_q) || !al16_i8(y) || !al16_i8(workspace))
     return fail_arg("moe_swiglu_fwd_int8: null or misaligned pointer");
-  if (!workspace || ws_bytes < moe_swiglu_fwd_int8_workspace(R, F))
-    return set_error("moe_swiglu_fwd_int8: workspace %zu < %zu bytes", ws_bytes, moe_swiglu_fwd_int8_workspace(R, F)),
-           MOE_EWORKSPACE;
+  const size_t need = moe_swiglu_fwd_int8_workspace(R, H, F, E);
+  if (!workspace || ws_bytes < need)
+    return set_error("moe_swiglu_fwd_int8: workspace %zu < %zu bytes", ws_bytes, need), MOE_EWORKSPACE;
   uint8_t* const act = static_cast<uint8_t*>(workspace);
-  uint8_t* const aq = act + up256((size_t)R * F * 2);
+  uint8_t* const aq = act + up256(std::max((size_t)R * F * 2, i8_part_bytes(R, F, H, E)));
   float* const as = reinterpret_cast<float*>(aq + up256((size_t)R * F));
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   I8Args a{};
@@ -598,7 +822,7 @@ extern "C" int moe_swiglu_fwd_int8(const void* xq, const float* sx, int64_t T, c
   a.K = (int)H;
   a.N = (int)F;
   a.E = (int)E;
-  if (int rc = product<true, uint16_t>("k_i8_gate_up", s, a)) return rc;
+  if (int rc = product<true, uint16_t>(s, a, nullptr)) return rc;
   if (int rc = quant_rows_int8(act, MOE_BF16, R, F, F, aq, as, offsets + E, s)) return rc;
   I8Args b{};
   b.A = aq;
@@ -613,5 +837,5 @@ extern "C" int moe_swiglu_fwd_int8(const void* xq, const float* sx, int64_t T, c
   b.K = (int)F;
   b.N = (int)H;
   b.E = (int)E;
-  return product<false, uint16_t>("k_i8_down", s, b);
+  return product<false, uint16_t>(s, b, act);
 }

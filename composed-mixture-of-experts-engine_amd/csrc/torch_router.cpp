@@ -625,8 +625,12 @@ at::Tensor op_matmul_int8(const at::Tensor& q_in, const at::Tensor& sc_in, const
   std::vector<int64_t> ys = q.sizes().vec();
   ys.back() = N;
   at::Tensor y = at::empty(ys, q.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  const size_t nbytes = moe_matmul_int8_workspace(sc.numel(), K, N, E);
+  at::Tensor ws;
+  if (nbytes > 0) ws = scratch(nbytes, q);
   check_rc(moe_matmul_int8(q.data_ptr(), sc.data_ptr<float>(), wq.data_ptr(), wsc.data_ptr<float>(),
-                           static_cast<const int*>(ptr(offsets)), sc.numel(), K, N, E, y.data_ptr(), code_of(y), stream_of(q)),
+                           static_cast<const int*>(ptr(offsets)), sc.numel(), K, N, E, y.data_ptr(), code_of(y),
+                           nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, stream_of(q)),
            "moe_matmul_int8");
   return y;
 }
@@ -658,7 +662,7 @@ at::Tensor op_swiglu_forward_int8(const at::Tensor& xq_in, const at::Tensor& sx_
   const at::Tensor xq = xq_in.contiguous(), sx = sx_in.contiguous();
   at::Tensor y = at::empty({R, H}, xq.options().dtype(at::kBFloat16));
   if (R == 0) return y;
-  const size_t nbytes = moe_swiglu_fwd_int8_workspace(R, F);
+  const size_t nbytes = moe_swiglu_fwd_int8_workspace(R, H, F, E);
   const at::Tensor w = scratch(nbytes, xq);
   check_rc(moe_swiglu_fwd_int8(xq.data_ptr(), sx.data_ptr<float>(), T, static_cast<const int*>(ptr(row_slot)), top_k,
                                wq[0].data_ptr(), ws[0].data_ptr<float>(), wq[1].data_ptr(), ws[1].data_ptr<float>(),

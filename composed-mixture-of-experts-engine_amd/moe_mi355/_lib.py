@@ -97,8 +97,9 @@ _SIGNATURES = {
     "moe_rmsnorm_quant": (_I32, [_P, _P, _I32, _P, _I32, _F32, _I64, _I64, _I32, _P, _P, _P, _P, _P]),
     "moe_quant_rows_int8": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
     "moe_dequant_rows": (_I32, [_P, _I32, _P, _I64, _I64, _P, _I32, _P]),
-    "moe_matmul_int8": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I32, _P]),
-    "moe_swiglu_fwd_int8_workspace": (_SZ, [_I64, _I64]),
+    "moe_matmul_int8_workspace": (_SZ, [_I64, _I64, _I64, _I64]),
+    "moe_matmul_int8": (_I32, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I32, _P, _SZ, _P]),
+    "moe_swiglu_fwd_int8_workspace": (_SZ, [_I64, _I64, _I64, _I64]),
     "moe_swiglu_fwd_int8": (
         _I32,
         [_P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _SZ, _P],

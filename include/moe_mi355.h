@@ -356,15 +356,16 @@ int moe_swiglu_fwd_fp8(const void* xq, const float* sx, const void* wg_q, const 
  * above), y = Wd act, y [R, H] bf16.  Row m's x is row row_slot[m] / top_k of xq [T, H] (moe_plan's row_slot: tokens are
  * quantized once and not copied), or row m where row_slot is NULL (T == R).  wg_q, wu_q [E, F, H] (scales sg, su [E, F]), wd_q
  * [E, H, F] (sd [E, H]).  Rows past offsets[E] are not written.  H % 16 == 0, F % 16 == 0.
- * Pointers to rows and weights are 16-byte aligned.
+ * Pointers to rows, weights and workspaces are 16-byte aligned; a workspace of 0 bytes may be NULL.
  * ---------------------------------------------------------------------- */
 int moe_quant_rows_int8(const void* src, int src_dtype, int64_t rows, int64_t cols, int64_t ld, void* dst, float* scale,
                         void* stream);
 int moe_dequant_rows(const void* q, int q_format, const float* scale, int64_t rows, int64_t cols, void* dst, int dst_dtype,
                      void* stream);
+size_t moe_matmul_int8_workspace(int64_t R, int64_t K, int64_t N, int64_t E);
 int moe_matmul_int8(const void* xq, const float* sx, const void* wq, const float* sw, const int32_t* offsets, int64_t R,
-                    int64_t K, int64_t N, int64_t E, void* y, int y_dtype, void* stream);
-size_t moe_swiglu_fwd_int8_workspace(int64_t R, int64_t F);
+                    int64_t K, int64_t N, int64_t E, void* y, int y_dtype, void* workspace, size_t ws_bytes, void* stream);
+size_t moe_swiglu_fwd_int8_workspace(int64_t R, int64_t H, int64_t F, int64_t E);
 int moe_swiglu_fwd_int8(const void* xq, const float* sx, int64_t T, const int32_t* row_slot, int64_t top_k, const void* wg_q,
                         const float* sg, const void* wu_q, const float* su, const void* wd_q, const float* sd,
                         const int32_t* offsets, int64_t R, int64_t H, int64_t F, int64_t E, void* y, void* workspace,

@@ -155,8 +155,10 @@ def _into(entry, y, *args):
 
 def _product_into(q, s, wq, ws, offs, y):
     E = wq.shape[0] if wq.dim() == 3 else 1
+    n = _lib.load().moe_matmul_int8_workspace(q.shape[0], q.shape[1], wq.shape[-2], E)
+    w = _lib.workspace(n, dev())
     _into("moe_matmul_int8", y, q.data_ptr(), s.data_ptr(), wq.data_ptr(), ws.data_ptr(), _lib.ptr(offs), q.shape[0],
-          q.shape[1], wq.shape[-2], E, y.data_ptr(), _lib.dtype_code(y.dtype))
+          q.shape[1], wq.shape[-2], E, y.data_ptr(), _lib.dtype_code(y.dtype), w.data_ptr(), n)
 
 
 @pytest.mark.parametrize("counts", [[3, 0, 9], [200, 0, 90], [700, 0, 600]], ids=str)
@@ -279,7 +281,7 @@ def test_experts_leave_rows_of_no_segment_alone():
         offs = torch.tensor([0, counts[0], sum(counts)], dtype=torch.int32, device=dev())
         q, s = _rows(R, H, 3)
         y = torch.full((R, H), 7.5, device=dev(), dtype=torch.bfloat16)
-        n = _lib.load().moe_swiglu_fwd_int8_workspace(R, F)
+        n = _lib.load().moe_swiglu_fwd_int8_workspace(R, H, F, E)
         w = _lib.workspace(n, dev())
         w.fill_(255)  # NaNs behind the last segment's rows
         _into("moe_swiglu_fwd_int8", y, q.data_ptr(), s.data_ptr(), R, None, 1, wq[0].data_ptr(), ws[0].data_ptr(),
