@@ -2,6 +2,8 @@
 
 ``RMSNormFn``       xn = ((x * rsqrt(mean(x^2) + eps)) * weight).to(x.dtype) and its backward
                     (moe-engine/pkg/models/moe.py L:83-86, the norm of ToyMoEBlock L:125-126).
+``RMSNormResidualFn``  h = x + residual and its norm in one kernel (the residual sum of ToyMoEBlock L:126, left to the next
+                    block's norm); one gradient for x and residual, formed with the norm's in one kernel.
 ``NormRouterCore``  the norm with the router forward fused onto its output: one read of the hidden state
                     for both (bf16 x and gate, E <= 16), returning ``xn`` for the expert path together with
                     everything :class:`moe_mi355.router.RouterCore` returns.  Its backward is one call
@@ -15,6 +17,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -33,6 +36,27 @@ class RMSNormFn(torch.autograd.Function):
         x, weight, rstd = ctx.saved_tensors
         dx, dweight = ops.rmsnorm_backward(x, weight, rstd, dxn)
         return (dx if ctx.needs_input_grad[0] else None), (dweight if ctx.needs_input_grad[1] else None), None
+
+
+class RMSNormResidualFn(torch.autograd.Function):
+    """(x [N,H], residual [N,H], weight [H], eps) -> (xn [N,H], h [N,H])."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps: float):
+        xn, h, rstd = ops.rmsnorm_residual_forward(x, residual, weight, eps)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.set_materialize_grads(False)
+        return xn, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dxn, dh):
+        if dxn is None and dh is None:
+            return None, None, None, None
+        h, weight, rstd = ctx.saved_tensors
+        d, dweight = ops.rmsnorm_residual_backward(h, weight, rstd, dxn, dh)
+        need_x, need_r, need_w, _ = ctx.needs_input_grad
+        return (d if need_x else None), (d if need_r else None), (dweight if need_w else None), None
 
 
 class NormRouterCore(torch.autograd.Function):

@@ -123,6 +123,7 @@ def compute_capacity_drop_mask(idx: torch.Tensor, num_experts: int, capacity: in
 
 
 _MXFP4 = ("mxfp4_gate", "mxfp4_up", "mxfp4_down", "mxfp4_gate_scale", "mxfp4_up_scale", "mxfp4_down_scale")
+_INT8 = ("int8_gate", "int8_up", "int8_down", "int8_gate_scale", "int8_up_scale", "int8_down_scale")
 
 
 class _ExpertWeight(nn.Module):
@@ -199,6 +200,9 @@ class DistributedMoELayer(nn.Module):
         # the experts in 4 bits (quantize_mxfp4, load_mxfp4): they move with the layer and are not in its state_dict, whose
         # keys are the reference's
         for name in _MXFP4:
+            self.register_buffer(name, None, persistent=False)
+        # and in int8 (quantize_int8, load_int8), the fp32 scales as int32 words: a change of the layer's dtype leaves them alone
+        for name in _INT8:
             self.register_buffer(name, None, persistent=False)
         nn.init.normal_(self.w_gate, mean=0.0, std=1.0 / math.sqrt(hidden_dim))
         nn.init.normal_(self.w_up, mean=0.0, std=1.0 / math.sqrt(hidden_dim))
@@ -347,7 +351,7 @@ class DistributedMoELayer(nn.Module):
         return self._experts_forward(xn, idx, weights).reshape(original_shape)
 
     def _experts_forward(self, flat: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor,
-                         mxfp4=None) -> torch.Tensor:
+                         mxfp4=None, int8=None) -> torch.Tensor:
         N = flat.shape[0]
         capacity = (
             math.ceil(self.capacity_factor * N * self.top_k / self.num_experts) if self.capacity_dropping else -1
@@ -358,6 +362,15 @@ class DistributedMoELayer(nn.Module):
             train = torch.is_grad_enabled() and (flat.requires_grad or weights.requires_grad)
             timer = _ExpertTimer.new(flat)
             out = ExpertsMxfp4Fn.apply(flat, weights, *mxfp4, p, train, timer)
+        elif int8 is not None:
+            q, scale, wq, ws = int8
+            timer = _ExpertTimer.new(flat)
+            if timer is not None:
+                timer.start()
+            y = ops.swiglu_forward_int8(q, scale, wq, ws, p.offsets, row_slot=p.row_slot[:p.rows], top_k=self.top_k)
+            if timer is not None:
+                timer.stop()
+            out = ops.combine(y, weights, p)
         elif self._fused():
             train = torch.is_grad_enabled() and any(
                 t.requires_grad for t in (flat, weights, self.w_gate, self.w_up, self.w_down))
@@ -399,10 +412,13 @@ class DistributedMoELayer(nn.Module):
         SwiGLU activations are quantized per row between them, and the combine is the bf16 one.  Needs
         the fused bf16 expert layout (``self._fused()``) and hidden_dim % 16 == 0.  ``seq_offsets`` and ``token_mask`` as in
         :meth:`forward`."""
+        shape = tokens.shape
+        return self._forward_fp8(tokens.reshape(-1, shape[-1]), shape, seq_offsets, token_mask).reshape(shape)
+
+    def _forward_fp8(self, flat, shape, seq_offsets, token_mask, quantized=None):
+        """``quantized``: the rows in e4m3 with their scales, where something before the layer has made them."""
         if not self._fused() or self.w_gate.dtype != torch.bfloat16:
             raise NotImplementedError("forward_fp8 needs the built-in SwiGLU experts in bfloat16")
-        shape = tokens.shape
-        flat = tokens.reshape(-1, shape[-1])
         routed, seq = self._router_args(flat, shape, seq_offsets, token_mask)
         idx, weights, _cnt = self.router(routed, **seq)
         N = flat.shape[0]
@@ -412,10 +428,14 @@ class DistributedMoELayer(nn.Module):
         p = ops.plan(idx, self.num_experts, capacity=capacity, layout=_LAYOUTS[self.layout])
         self.last_plan = p
         wq, ws = self.quantize_fp8()
-        xq, sx = ops.permute_fp8(flat, p)
+        if quantized is None:
+            xq, sx = ops.permute_fp8(flat, p)
+        else:
+            q, scale = quantized
+            xq = ops.permute(q, p)
+            sx = scale[p.row_slot[:p.rows] // self.top_k]  # (rows that no slot has: -1, any scale)
         _act, _hgu, y = ops.swiglu_forward_fp8(xq, sx, wq, ws, p.offsets, keep_preact=False)
-        out = ops.combine(y, weights, p)
-        return out.reshape(shape)
+        return ops.combine(y, weights, p)
 
     # ------------------------------------------------------------------
     # experts held in 4 bits (MXFP4), new: serving, and training around frozen experts
@@ -474,6 +494,71 @@ class DistributedMoELayer(nn.Module):
             idx, weights, _cnt = self.router(routed, **seq)
         linked = self.router.take_linked_tokens()
         return self._experts_forward(flat if linked is None else linked, idx, weights, q).reshape(tokens.shape)
+
+    # ------------------------------------------------------------------
+    # experts held in int8, new: serving
+    # ------------------------------------------------------------------
+    @torch.no_grad()
+    def quantize_int8(self):
+        """Quantize the expert weights to int8 with one fp32 scale per output channel (:func:`moe_mi355.ops.quant_rows_int8`)
+        for :meth:`forward_int8`, on the GPU.  As :meth:`quantize_mxfp4`: they stay as they are until this is called again, move
+        with the layer and are not in its ``state_dict``.  Returns ``((gate, up, down), (their scales))``."""
+        if any(t is None for t in (self.w_gate, self.w_up, self.w_down)):
+            raise RuntimeError("quantize_int8: the layer's full-width weights were dropped")
+        if self.w_gate.shape[-1] % 16 or self.w_gate.shape[1] % 16:
+            raise NotImplementedError("quantize_int8 needs hidden and ffn dims that are multiples of 16")
+        q = [ops.quant_rows_int8(t.detach()) for t in (self.w_gate, self.w_up, self.w_down)]
+        return self.load_int8([t for t, _ in q], [s for _, s in q])
+
+    def load_int8(self, weights, scales):
+        """Take ``(gate, up, down)`` and their scales for :meth:`forward_int8`: what :meth:`quantize_int8` returned, or weights
+        quantized elsewhere (int8 [E, F, H], [E, F, H] and [E, H, F]; float32 [E, F], [E, F] and [E, H]).  They are kept as they
+        are, on the router's device.  A layer that only serves them may drop its full-width parameters.  Returns them."""
+        E, F_, H = len(self.local_expert_ids), self.ffn_dim, self.hidden_dim
+        for name, w, s, shape in zip(("gate", "up", "down"), weights, scales, ((E, F_, H), (E, F_, H), (E, H, F_))):
+            if w.dtype != torch.int8 or s.dtype != torch.float32:
+                raise TypeError(f"load_int8: {name} must be int8 with float32 scales, got {w.dtype} and {s.dtype}")
+            if tuple(w.shape) != shape or tuple(s.shape) != shape[:2]:
+                raise ValueError(f"load_int8: {name} must be {list(shape)} with scales {list(shape[:2])}, got {list(w.shape)} and "
+                                 f"{list(s.shape)}")
+        dev = self.router.gate_w.device
+        with torch.inference_mode(False):
+            for name, t in zip(_INT8, [*weights, *scales]):
+                t = t.clone() if t.is_inference() else t.detach()
+                t = t.contiguous().to(dev)
+                setattr(self, name, t.view(torch.int32) if t.dtype == torch.float32 else t)
+        return self._int8_weights()
+
+    def _int8_weights(self):
+        q = tuple(getattr(self, name) for name in _INT8)
+        return q[:3], tuple(None if t is None else t.view(torch.float32) for t in q[3:])
+
+    @torch.no_grad()
+    def forward_int8(self, tokens: torch.Tensor, seq_offsets: Optional[torch.Tensor] = None,
+                     token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``forward`` for serving (no autograd) on the weights as :meth:`quantize_int8` or :meth:`load_int8` left them: router,
+        planner and combine as in ``forward``; the tokens are quantized to int8 once, the experts read them through the plan,
+        and the SwiGLU activations are quantized per row between the projections.  From one decoded token to a long prompt; a
+        token's experts give the same bits in any batch.  Needs the built-in SwiGLU experts and bfloat16 tokens."""
+        if tokens.dim() not in (2, 3):
+            raise ValueError(f"tokens must be rank 2 or 3, got {tokens.dim()}")
+        flat = tokens.reshape(-1, tokens.shape[-1])
+        return self._forward_int8(flat, tokens.shape, seq_offsets, token_mask).reshape(tokens.shape)
+
+    def _forward_int8(self, flat, shape, seq_offsets, token_mask, quantized=None):
+        """``quantized``: the rows in int8 with their scales, where something before the layer has made them."""
+        wq, ws = self._int8_weights()
+        if wq[0] is None:
+            raise RuntimeError("forward_int8: call quantize_int8() or load_int8() first")
+        if not all(type(m) is _SwiGLUExpert and m.w_gate._owner() is self for m in self.experts):
+            raise NotImplementedError("forward_int8 needs the built-in SwiGLU experts")
+        if flat.dtype != torch.bfloat16:
+            raise TypeError(f"forward_int8 takes bfloat16 tokens, got {flat.dtype}")
+        q, scale = ops.quant_rows_int8(flat) if quantized is None else quantized
+        routed, seq = self._router_args(flat, shape, seq_offsets, token_mask)
+        with self._deferred_router_check():
+            idx, weights, _cnt = self.router(routed, **seq)
+        return self._experts_forward(flat, idx, weights, int8=(q, scale, wq, ws))
 
     def _forward_per_expert(self, flat: torch.Tensor, weights: torch.Tensor, p: ops.Plan,
                             timer: Optional["_ExpertTimer"] = None) -> torch.Tensor:

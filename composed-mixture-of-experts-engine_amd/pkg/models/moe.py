@@ -5,14 +5,22 @@ operation (:class:`moe_mi355.norm.NormRouterCore`): the hidden state is read onc
 routes the bf16-rounded normalised rows exactly as it would route ``norm(x)``, and the expert path takes
 those same rows.  Modules whose experts are not the built-in SwiGLU, or shapes the norm kernels do not
 take, use the plain composition ``moe(norm(x))``.
+
+In a stack the sum ``x + moe(norm(x))`` is read again by the next block's norm.  With ``residual`` the sum is left to that norm:
+``out, h = block(x, residual=r)`` is ``h = x + r``, ``out = moe(norm(h))``, the addition inside the norm's kernel; the next block
+takes ``(out, residual=h)`` and the last norm (``RMSNorm.forward(out, residual=h)``) adds the last one.  ``forward_int8`` and
+``forward_fp8`` serve a block on experts in 8 bits, whose rows the norm writes quantized.
 """
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 from torch import nn
 
-from moe_mi355.norm import RMSNormFn
+from moe_mi355 import ops
+from moe_mi355.norm import RMSNormFn, RMSNormResidualFn
 from pkg.distributed.moe_layer import DistributedMoELayer
 
 _NORM_MAX_H = 8192
@@ -32,9 +40,26 @@ class RMSNorm(nn.Module):
     def extra_repr(self) -> str:
         return f"dim={self.weight.shape[0]}, eps={self.eps}"
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        """The normalised ``x``; with ``residual`` (of x's shape and dtype) ``(norm(h), h)`` for ``h = x + residual``."""
         H = x.shape[-1]
-        return RMSNormFn.apply(x.reshape(-1, H), self.weight, self.eps).reshape(x.shape)
+        if residual is None:
+            return RMSNormFn.apply(x.reshape(-1, H), self.weight, self.eps).reshape(x.shape)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must be {list(x.shape)}, got {list(residual.shape)}")
+        xn, h = RMSNormResidualFn.apply(x.reshape(-1, H), residual.reshape(-1, H), self.weight, self.eps)
+        return xn.reshape(x.shape), h.reshape(x.shape)
+
+    @torch.no_grad()
+    def quantized(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, fmt: str = "int8"):
+        """For serving: ``(q, scale, norm(h), h)`` with the normalised rows in 8 bits too (:func:`moe_mi355.ops.rmsnorm_quant`;
+        ``q`` [N, H], ``scale`` [N] over the flattened rows, the others in x's shape); h is x without ``residual``."""
+        H = x.shape[-1]
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError(f"residual must be {list(x.shape)}, got {list(residual.shape)}")
+        q, scale, xn, h = ops.rmsnorm_quant(x.reshape(-1, H), self.weight, self.eps,
+                                            None if residual is None else residual.reshape(-1, H), fmt=fmt, keep_norm=True)
+        return q, scale, xn.reshape(x.shape), (x if h is None else h.reshape(x.shape))
 
 
 class ToyMoEBlock(nn.Module):
@@ -74,11 +99,32 @@ class ToyMoEBlock(nn.Module):
             and self.moe.router.gate_w.dtype == x.dtype
         )
 
-    def forward(self, x: torch.Tensor, seq_offsets=None, token_mask=None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, seq_offsets=None, token_mask=None, residual: Optional[torch.Tensor] = None):
         """``seq_offsets`` and ``token_mask``: the sequences and valid tokens of the router's balance loss
-        (:meth:`DistributedMoELayer.forward`)."""
+        (:meth:`DistributedMoELayer.forward`).  With ``residual``, ``(moe(norm(h)), h)`` for ``h = x + residual``."""
+        if residual is not None:
+            xn, h = self.norm(x, residual)
+            return self.moe(xn, seq_offsets, token_mask), h
         if self._fused(x):
             out = self.moe.forward_normed(x, self.norm.weight, self.norm.eps, seq_offsets, token_mask)
         else:
             out = self.moe(self.norm(x), seq_offsets, token_mask)
         return x + out
+
+    @torch.no_grad()
+    def forward_int8(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, seq_offsets=None, token_mask=None):
+        """``forward`` for serving on the layer's int8 weights (:meth:`DistributedMoELayer.forward_int8`), the experts' rows
+        quantized by the norm from its fp32 values: ``x + moe(norm(x))``, or with ``residual`` ``(moe(norm(h)), h)``."""
+        return self._serve(self.moe._forward_int8, "int8", x, residual, seq_offsets, token_mask)
+
+    @torch.no_grad()
+    def forward_fp8(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, seq_offsets=None, token_mask=None):
+        """The same on e4m3 rows and weights (:meth:`DistributedMoELayer.forward_fp8`)."""
+        return self._serve(self.moe._forward_fp8, "e4m3", x, residual, seq_offsets, token_mask)
+
+    def _serve(self, layer, fmt, x, residual, seq_offsets, token_mask):
+        if x.dim() not in (2, 3):
+            raise ValueError(f"tokens must be rank 2 or 3, got {x.dim()}")
+        q, scale, xn, h = self.norm.quantized(x, residual, fmt)
+        out = layer(xn.reshape(-1, x.shape[-1]), x.shape, seq_offsets, token_mask, quantized=(q, scale)).reshape(x.shape)
+        return x + out if residual is None else (out, h)
