@@ -23,7 +23,7 @@
 //                   (EP = 0) or u = dxn + G wg^T (EP = 8/16: the router's gradient of xn formed in place from
 //                   G = dL/dlogits, never written to HBM), u rounded to the storage type.  dgamma += u xhat
 //                   is kept per lane in registers, folded over the block's waves in LDS and over blocks by
-//                   k_rmsnorm_dgamma.  EP = 2 adds a further gradient of x to dx.
+//                   k_rmsnorm_dgamma.  EP = 2 adds a further gradient of x to dx (H <= 512; wider rows: k_rmsnorm_residual_bwd).
 // k_rmsnorm_ext     the norm between two blocks: h = x + residual (rounded to the storage type and written), the norm of h,
 //                   and its output in the storage type, in 8 bits with a scale a row (quant8.h), or in both.
 #include <type_traits>
@@ -831,6 +831,92 @@ void k_rmsnorm_bwd(NormBwdArgs a) {
   }
 }
 
+// The backward with a gradient dh of h beside the norm's (MODE 2's mathematics) for rows of more than 512 elements: a block a
+// row, so that a lane holds 8 NCH of its elements (NCH = 1, 2, 4 as H <= 2048, 4096, 8192), gamma and dgamma of the same columns
+// in registers, and the whole next row on its way while it computes on one.  With a wave a row, three operands and dgamma take
+// more registers than there are from H = 4096 on (16384 x 4096 bf16: 169 us with 33 of them spilled, 3.2 TB/s).
+template <typename TX, int NCH>
+__global__ __launch_bounds__(256) void k_rmsnorm_residual_bwd(NormBwdArgs a, int gamma_dt) {
+  constexpr int CW = chunk_words<TX>();
+  __shared__ float red[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wv = norm_wave();
+  const int N = a.N, H = a.H, rowbytes = H * (int)sizeof(TX);
+  float gm[NCH][8], dg[NCH][8];
+#pragma unroll
+  for (int j = 0; j < NCH; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int h = 8 * (tid + 256 * j) + i;
+      gm[j][i] = h < H ? load_f(a.gamma, gamma_dt, h) : 0.f;
+      dg[j][i] = 0.f;
+    }
+  struct Row {
+    RowFrag<TX, NCH> x, u, h;
+    float r;
+  };
+  auto load = [&](Row& w, int t) {
+    const bool in = t < N;
+    auto one = [&](RowFrag<TX, NCH>& f, const void* base) {  // a null gradient, or a row past N, reads as zeros
+      const buf_rsrc_t rs = buf_rsrc(base ? static_cast<const TX*>(base) + (int64_t)t * H : a.x, base && in ? rowbytes : 0);
+#pragma unroll
+      for (int j = 0; j < NCH; ++j)
+#pragma unroll
+        for (int q = 0; q < CW; ++q)
+          f.w[j * CW + q] = __builtin_bit_cast(
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (tid + 256 * j) * 8 * (int)sizeof(TX) + 16 * q, 0, kNormStream));
+    };
+    one(w.x, a.x);
+    one(w.u, a.dxn);
+    one(w.h, a.dh);
+    w.r = in ? a.rstd[t] : 0.f;
+  };
+  Row cur, nxt;
+  int t = blockIdx.x, par = 0;
+  load(cur, t);
+  for (; t < N; t += gridDim.x, par ^= 1) {
+    load(nxt, t + gridDim.x);
+    float c = 0.f;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      float v[8], u[8];
+      frag_get(cur.x, j, v);
+      frag_get(cur.u, j, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float xh = v[i] * cur.r;
+        c = fmaf(gm[j][i] * u[i], xh, c);
+        dg[j][i] = fmaf(u[i], xh, dg[j][i]);
+      }
+    }
+    c = wave_total(c);
+    if (lane == 0) red[par][wv] = c;
+    lds_sync();  // (the other half is this row's; a wave is at most one row ahead)
+    c = (red[par][0] + red[par][1] + red[par][2] + red[par][3]) / (float)H;
+    TX* const row = static_cast<TX*>(a.dx) + (int64_t)t * H;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      float v[8], u[8], d[8], o[8];
+      frag_get(cur.x, j, v);
+      frag_get(cur.u, j, u);
+      frag_get(cur.h, j, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = cur.r * (gm[j][i] * u[i] - (v[i] * cur.r) * c) + d[i];
+      u32x4 pk;
+      chunk_store<TX>(row, tid + 256 * j, 8 * (tid + 256 * j) < H, o, pk);
+    }
+    cur = nxt;
+  }
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    const int h0 = 8 * (tid + 256 * j);
+    if (h0 < H) {
+      float* const d = a.part_dg + (int64_t)blockIdx.x * H + h0;
+      reinterpret_cast<f32x4*>(d)[0] = f32x4{dg[j][0], dg[j][1], dg[j][2], dg[j][3]};
+      reinterpret_cast<f32x4*>(d)[1] = f32x4{dg[j][4], dg[j][5], dg[j][6], dg[j][7]};
+    }
+  }
+}
+
 // dgamma[h] = sum over blocks b of part_dg[b][h] in a fixed order.  Block = 32 columns x 32 groups of
 // blocks: thread (g, cq) sums blocks g, g + 32, ... of columns 4 cq .. 4 cq + 3 (16-byte loads, four in
 // flight), then the group sums are added in group order.
@@ -874,6 +960,8 @@ int norm_route_blocks(int64_t N) {
 }
 // the backward writes one dgamma partial row per block: about two blocks per CU
 int norm_bwd_blocks(int64_t N) { return (int)std::min<int64_t>(512, std::max<int64_t>(1, (N + 3) / 4)); }
+// a block a row: four blocks of four waves a CU (a partial row of dgamma each)
+int residual_bwd_blocks(int64_t N) { return (int)std::min<int64_t>(1024, std::max<int64_t>(1, N)); }
 // the fused backward: one block of eight waves per CU
 int norm_route_bwd_blocks(int64_t N) { return (int)std::min<int64_t>(256, std::max<int64_t>(1, (N + 7) / 8)); }
 int norm_route_ep(int64_t E) { return E <= 8 ? 8 : 16; }
@@ -973,6 +1061,17 @@ int launch_norm_bwd(int nblk, hipStream_t s, const NormBwdArgs& a) {
   if (int rc = allow_lds(k_rmsnorm_bwd<TX, TG, NCH, MODE>, lds)) return rc;
   MOE_LAUNCH(name, (k_rmsnorm_bwd<TX, TG, NCH, MODE>), dim3(nblk), dim3(norm_bwd_waves<MODE>() * 64), lds, s, a);
   return check_launch(name);
+}
+
+template <typename TX>
+int launch_residual_bwd(int nblk, hipStream_t s, const NormBwdArgs& a, int gamma_dt) {
+#define MOE_RB(NCH) \
+  MOE_LAUNCH("k_rmsnorm_residual_bwd", (k_rmsnorm_residual_bwd<TX, NCH>), dim3(nblk), dim3(256), 0, s, a, gamma_dt)
+  if (a.H <= 2048) MOE_RB(1);
+  else if (a.H <= 4096) MOE_RB(2);
+  else MOE_RB(4);
+#undef MOE_RB
+  return check_launch("k_rmsnorm_residual_bwd");
 }
 
 int launch_dgamma(hipStream_t s, const float* part, int nblk, int64_t H, void* dgamma, int g_dt) {
@@ -1168,6 +1267,11 @@ extern "C" int moe_rmsnorm_bwd(const void* x, int x_dtype, const void* gamma, in
   return launch_dgamma(s, part, nblk, H, dgamma_out, gamma_dtype);
 }
 
+extern "C" size_t moe_rmsnorm_residual_bwd_workspace(int64_t N, int64_t H) {
+  if (N <= 0 || H <= 0) return 0;
+  return std::max(moe_rmsnorm_bwd_workspace(N, H), align256n((size_t)residual_bwd_blocks(N) * H * 4));
+}
+
 extern "C" int moe_rmsnorm_residual_bwd(const void* h, int x_dtype, const void* gamma, int gamma_dtype, const float* rstd,
                                         const void* dxn, const void* dh, int64_t N, int64_t H, void* d_out, void* dgamma_out,
                                         void* workspace, size_t ws_bytes, void* stream) {
@@ -1179,8 +1283,8 @@ extern "C" int moe_rmsnorm_residual_bwd(const void* h, int x_dtype, const void* 
   if (N == 0) return launch_dgamma(s, nullptr, 0, H, dgamma_out, gamma_dtype);
   if (!h || !rstd || !d_out || !al16p(h) || !al16p(gamma) || !al16p(dxn) || !al16p(dh) || !al16p(d_out))
     return fail_arg("moe_rmsnorm_residual_bwd: null or misaligned pointer");
-  const int nblk = norm_bwd_blocks(N);
-  if (ws_bytes < moe_rmsnorm_bwd_workspace(N, H) || !workspace)
+  const int nblk = H <= 512 ? norm_bwd_blocks(N) : residual_bwd_blocks(N);
+  if (ws_bytes < moe_rmsnorm_residual_bwd_workspace(N, H) || !workspace)
     return set_error("moe_rmsnorm_residual_bwd: workspace too small"), MOE_EWORKSPACE;
   NormBwdArgs a{};
   a.x = h;
@@ -1193,7 +1297,9 @@ extern "C" int moe_rmsnorm_residual_bwd(const void* h, int x_dtype, const void* 
   a.dx = d_out;
   a.part_dg = static_cast<float*>(workspace);
   int rc = 0;
-  MOE_NORM_DT(x_dtype, gamma_dtype, MOE_NCH(norm_nch(H), rc = (launch_norm_bwd<TX, TG, NCHv, 2>(nblk, s, a))));
+  if (H <= 512) MOE_NORM_DT(x_dtype, gamma_dtype, rc = (launch_norm_bwd<TX, TG, 1, 2>(nblk, s, a)));
+  else if (x_dtype == MOE_BF16) rc = launch_residual_bwd<uint16_t>(nblk, s, a, gamma_dtype);
+  else rc = launch_residual_bwd<float>(nblk, s, a, gamma_dtype);
   if (rc) return rc;
   return launch_dgamma(s, a.part_dg, nblk, H, dgamma_out, gamma_dtype);
 }

@@ -719,7 +719,7 @@ std::tuple<at::Tensor, at::Tensor> op_rmsnorm_residual_backward(const at::Tensor
     dh = dh_in->contiguous();
   }
   at::Tensor d = at::empty(h.sizes(), h.options()), dw = at::empty(weight.sizes(), weight.options());
-  const size_t nbytes = moe_rmsnorm_bwd_workspace(h.size(0), h.size(1));
+  const size_t nbytes = moe_rmsnorm_residual_bwd_workspace(h.size(0), h.size(1));
   const at::Tensor ws = scratch(nbytes, h);
   check_rc(moe_rmsnorm_residual_bwd(h.data_ptr(), code_of(h), weight.data_ptr(), code_of(weight), rstd.data_ptr<float>(),
                                     ptr(dxn), ptr(dh), h.size(0), h.size(1), d.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes,

@@ -93,6 +93,7 @@ _SIGNATURES = {
         _I32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _SZ, _P]
     ),
     "moe_rmsnorm_residual_fwd": (_I32, [_P, _P, _I32, _P, _I32, _F32, _I64, _I64, _P, _P, _P, _P]),
+    "moe_rmsnorm_residual_bwd_workspace": (_SZ, [_I64, _I64]),
     "moe_rmsnorm_residual_bwd": (_I32, [_P, _I32, _P, _I32, _P, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
     "moe_rmsnorm_quant": (_I32, [_P, _P, _I32, _P, _I32, _F32, _I64, _I64, _I32, _P, _P, _P, _P, _P]),
     "moe_quant_rows_int8": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),

@@ -460,8 +460,7 @@ int moe_balance_bwd(const float* logits, const int64_t* counts, const int64_t* t
  * moe_rmsnorm_residual_fwd: h = x + residual (the sum of L:125-126, left by one
  * block to the next one's norm), rounded to x's dtype, and moe_rmsnorm_fwd of
  * h, in one kernel.  moe_rmsnorm_residual_bwd: d = dh + the norm's gradient,
- * the gradient of x and of residual alike (workspace: moe_rmsnorm_bwd's; dxn
- * or dh may be null, not both).
+ * the gradient of x and of residual alike (dxn or dh may be null, not both).
  *
  * moe_rmsnorm_quant: the norm of x (residual null) or of h = x + residual, its
  * fp32 values quantized by row: int8 (moe_quant_rows_int8) or e4m3
@@ -484,6 +483,7 @@ int moe_rmsnorm_bwd(const void* x, int x_dtype, const void* gamma, int gamma_dty
 int moe_rmsnorm_residual_fwd(const void* x, const void* residual, int x_dtype, const void* gamma, int gamma_dtype,
                              float eps, int64_t N, int64_t H, void* h_out, void* xn_out, float* rstd_out,
                              void* stream);
+size_t moe_rmsnorm_residual_bwd_workspace(int64_t N, int64_t H);
 int moe_rmsnorm_residual_bwd(const void* h, int x_dtype, const void* gamma, int gamma_dtype, const float* rstd,
                              const void* dxn, const void* dh, int64_t N, int64_t H, void* d_out, void* dgamma_out,
                              void* workspace, size_t ws_bytes, void* stream);

@@ -83,8 +83,11 @@ def test_backward(N, H, dtype, wdtype, grads):
     dot = (g * xhat).mean(-1, keepdim=True)
     slack = rr * (g * (e + 4 * F32) + xhat * dot * (2 * e + 2 * e + 8 * F32)) + (rd.abs() + rr * (g + xhat * dot)) * 3 * F32
     assert _off(d, rd, slack + rd.abs() * _step(dtype) + 1e-37) <= 1
-    # dweight: sums of N terms, each off by e and a rounding, in lanes, waves and blocks: at most N / 2048 + 8 + 40 in a row
-    sdw = (u * v * rr).abs().sum(0) * (e + (N / 2048 + 52) * F32)
+    # dweight: sums of N terms, each off by e and two roundings.  The longest chain of additions that a term goes through: a
+    # lane's rows (up to 512 elements a wave a row, 2048 of them at once: N / 2048 + 1, then 3 waves; past that a block a row,
+    # 1024 of them: N / 1024 + 1), the blocks' partial sums (at most 1024 / 32 in a row, then 31 more), the last rounding: at
+    # most N / 1024 + 66, and 2 for the term itself
+    sdw = (u * v * rr).abs().sum(0) * (e + (N / 1024 + 68) * F32)
     assert _off(dw, rdw, sdw + rdw.abs() * _step(wdtype) + 1e-37) <= 1
 
 
