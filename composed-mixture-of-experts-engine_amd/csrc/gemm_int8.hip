@@ -299,7 +299,7 @@ constexpr int i8_stage() { return (WR * MI + 4 / WR * NI) * 32 * 128; }
 // quarter and a refill piece or two (16 bytes a lane).  The slice's one barrier lies inside its last quarter, when the wave's
 // own LDS reads of the slice have long drained under matrix instructions: behind it slice kt + 1 is complete and slice kt's
 // stage is free for slice kt + NS.
-template <bool GU, typename OT, int WR, int MI, int NI, int NS>
+template <bool GU, typename OT, int WR, int MI, int NI, int NS, bool NT>
 __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint8_t* smem) {
   constexpr int WC = 4 / WR, BM = WR * MI * 32, BN = WC * NI * 32;
   constexpr int SA = BM * 128, STAGE = i8_stage<WR, MI, NI>();
@@ -350,10 +350,9 @@ __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint
       src = full || k < K ? base + ((uint32_t)kt * 128u + b_off[q]) : base + (b_off[q] - chunk_of(j) * 16);
       to = SA + j * 1024;
     }
-    __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                     :
-                     : "v"(src), "{m0}"((uint32_t)(uintptr_t)(lds_i8_t*)(smem + s + to))
-                     : "memory");
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_i8_t*)(smem + s + to);
+    if (NT && p >= QA) __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(src), "{m0}"(lds) : "memory");
+    else __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds) : "memory");
   };
   // fragment f of quarter ks of the slice in stage s, in the order in which the quarter's matrix instructions need them
   auto read_frag = [&](int s, int ks, int f, i32x4(&fa)[MI], i32x4(&fb)[NI]) {
@@ -511,12 +510,12 @@ __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint
   }
 }
 
-// The number of row tiles of expert e: all (KIND 0), those of more than 3/4 BM rows (1) or a shorter one behind them (2).
+// The number of row tiles of expert e: all (KIND 0), those of more than 64 rows (1) or a shorter one behind them (2).
 template <int BM, int KIND>
 __device__ __forceinline__ int i8_row_tiles(const I8Args& g, int e) {
   if (e >= g.E) return 0;
   const int64_t r = max(seg(g, e + 1) - seg(g, e), (int64_t)0);
-  const int all = (int)((r + BM - 1) / BM), tall = (int)((r + BM / 4 - 1) / BM);
+  const int all = (int)((r + BM - 1) / BM), tall = (int)((r + BM - 65) / BM);
   return KIND == 0 ? all : KIND == 1 ? tall : all - tall;
 }
 template <int BM, int KIND>
@@ -606,16 +605,16 @@ __global__ __launch_bounds__(256, BM == 256 || DEEP ? 1 : 2) void k_i8_tile(I8Ar
     }
   }
   if constexpr (BM == 256) {
-    if (at.mlen > 192) i8_tile<GU, OT, 2, 4, 4, 2>(g, at, smem);
-    else if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 4, 2>(g, at, smem);
-    else if (at.mlen > 64) i8_tile<GU, OT, 1, 4, 2, 3>(g, at, smem);
-    else i8_tile<GU, OT, 1, 2, 2, 3>(g, at, smem);
+    if (at.mlen > 192) i8_tile<GU, OT, 2, 4, 4, 2, BM != 256>(g, at, smem);
+    else if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 4, 2, BM != 256>(g, at, smem);
+    else if (at.mlen > 64) i8_tile<GU, OT, 1, 4, 2, 3, BM != 256>(g, at, smem);
+    else i8_tile<GU, OT, 1, 2, 2, 3, BM != 256>(g, at, smem);
   } else if constexpr (BM == 192) {
-    if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 2, DEEP ? 3 : 2>(g, at, smem);
-    else if (at.mlen > 64) i8_tile<GU, OT, 2, 2, 2, DEEP ? 4 : 2>(g, at, smem);
-    else i8_tile<GU, OT, 2, 1, 2, DEEP ? 6 : 3>(g, at, smem);
+    if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 2, DEEP ? 3 : 2, BM != 256>(g, at, smem);
+    else if (at.mlen > 64) i8_tile<GU, OT, 2, 2, 2, DEEP ? 4 : 2, BM != 256>(g, at, smem);
+    else i8_tile<GU, OT, 2, 1, 2, DEEP ? 6 : 3, BM != 256>(g, at, smem);
   } else {
-    i8_tile<GU, OT, 1, 2, 2, 2>(g, at, smem);
+    i8_tile<GU, OT, 1, 2, 2, 2, BM != 256>(g, at, smem);
   }
 }
 
