@@ -315,44 +315,52 @@ __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint
   const int K = at.klen, nk = (K + 127) / 128, whole = K / 128;
 
   // piece p of a wave's share: instruction j fills rows 8 j + lane / 8 of its operand's tile, slot lane % 8 of the row.  Rows
-  // past the tile repeat the last one.
+  // past the tile repeat the last one.  A lane's address is a scalar base and an offset of 32 bits of its own that no slice
+  // changes; the instruction's own offset moves both the address and the place in LDS, so four pieces share m0 (the offsets are
+  // off by as much, and kBias keeps them positive).
+  constexpr uint32_t kBias = 3 * 1024;
   const int64_t eb = (int64_t)at.e * g.N * g.K + at.k0;
   const uint8_t* const b_base[2] = {g.B + eb, (GU ? g.B2 : g.B) + eb};
-  const uint8_t* a_src[QA];
-  uint32_t b_off[QB];
+  const uint8_t* const a_base = g.A + (g.row_slot == nullptr ? at.mbase * g.K : (int64_t)0) + at.k0;
+  uint32_t a_off[QA], b_off[QB];
   auto chunk_of = [&](int j) { return (lane & 7) ^ ((4 * j + (lane >> 4)) & 7); };
 #pragma unroll
   for (int q = 0; q < QA; ++q) {
-    const int j = QA * wv + q;
-    a_src[q] = g.A + source_row(g, at.mbase + min(8 * j + (lane >> 3), at.mlen - 1)) * g.K + at.k0 + chunk_of(j) * 16;
+    const int j = QA * wv + q, r = min(8 * j + (lane >> 3), at.mlen - 1);
+    a_off[q] = (uint32_t)(g.row_slot == nullptr ? (int64_t)r : source_row(g, at.mbase + r)) * (uint32_t)g.K + chunk_of(j) * 16 +
+               (kBias - q % 4 * 1024);
   }
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
     const int j = QB * wv + q, i = 8 * j + (lane >> 3);
     const int n = GU ? at.n0 + (i >> 6) * 32 + (i & 31) : at.n0 + i;
-    b_off[q] = (uint32_t)min(n, g.N - 1) * (uint32_t)g.K + chunk_of(j) * 16;
+    b_off[q] = (uint32_t)min(n, g.N - 1) * (uint32_t)g.K + chunk_of(j) * 16 + (kBias - q % 4 * 1024);
   }
-  // Piece p of slice kt to the stage at byte s; past the row's end A is zeros and B anything.  Issued from asm: the compiler
-  // would make every LDS read that it cannot tell apart wait for all of them; the waits are the loop's own.  (m0 is written by
-  // the scalar unit: one wait state.)
-  auto fill = [&](int kt, int s, int p, bool full) {
-    const uint8_t* src;
-    int to;
-    if (p < QA) {
-      const int j = QA * wv + p;
-      src = a_src[p] + kt * 128;
-      if (!full) src = kt * 128 + chunk_of(j) * 16 < K ? src : g_i8_zero;
-      to = j * 1024;
+  // Piece p of slice kt to the stage at byte s; past the row's end A is zeros and B the row's first bytes.  Issued from asm: the
+  // compiler would make every LDS read that it cannot tell apart wait for all of them; the waits are the loop's own.  (m0 is
+  // written by the scalar unit: one wait state.)
+  auto fill = [&](int kt, int s, auto p_c, bool full) {
+    constexpr int p = decltype(p_c)::value;
+    constexpr bool IS_A = p < QA;
+    constexpr int q = IS_A ? p : p - QA;
+    const int j = (IS_A ? QA : QB) * wv + q;
+    const uint8_t* const base = IS_A ? a_base : b_base[GU ? (8 * j >> 5) & 1 : 0];
+    uint32_t off;
+    if constexpr (IS_A) off = a_off[q];
+    else off = b_off[q];
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_i8_t*)(smem + s + (IS_A ? 0 : SA) + (j - q % 4) * 1024);
+    if (full) {
+      const uint8_t* const at_kt = base - kBias + (int64_t)kt * 128;
+      if constexpr (NT && !IS_A)
+        __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%2 nt" : : "v"(off), "s"(at_kt), "n"(q % 4 * 1024), "{m0}"(lds) : "memory");
+      else
+        __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%2" : : "v"(off), "s"(at_kt), "n"(q % 4 * 1024), "{m0}"(lds) : "memory");
     } else {
-      const int q = p - QA, j = QB * wv + q;
-      const uint8_t* const base = b_base[GU ? (8 * j >> 5) & 1 : 0];
       const int k = kt * 128 + chunk_of(j) * 16;
-      src = full || k < K ? base + ((uint32_t)kt * 128u + b_off[q]) : base + (b_off[q] - chunk_of(j) * 16);
-      to = SA + j * 1024;
+      const uint8_t* const row = base + (off - (kBias - q % 4 * 1024) - chunk_of(j) * 16);
+      const uint8_t* const src = k < K ? row + k : IS_A ? g_i8_zero : row;
+      __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds + q % 4 * 1024) : "memory");
     }
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_i8_t*)(smem + s + to);
-    if (NT && p >= QA) __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(src), "{m0}"(lds) : "memory");
-    else __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds) : "memory");
   };
   // fragment f of quarter ks of the slice in stage s, in the order in which the quarter's matrix instructions need them
   auto read_frag = [&](int s, int ks, int f, i32x4(&fa)[MI], i32x4(&fb)[NI]) {
@@ -405,7 +413,7 @@ __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint
          if constexpr (FILL > 0 && I >= RLO) {
            constexpr int P0 = PLO + (PHI - PLO) * (I - RLO) / (SLOTS - RLO), P1 = PLO + (PHI - PLO) * (I - RLO + 1) / (SLOTS - RLO);
            [&]<int... P>(std::integer_sequence<int, P...>) {
-             (fill(fkt, fs, P0 + P, FILL == 1 || fkt < whole), ...);
+             (fill(fkt, fs, std::integral_constant<int, P0 + P>{}, FILL == 1 || fkt < whole), ...);
            }(std::make_integer_sequence<int, P1 - P0>{});
          }
          __builtin_amdgcn_sched_barrier(0);
@@ -429,8 +437,13 @@ __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint
     quarter(C0{}, C0{}, C0{}, C0{}, CN{}, fa0, fb0, s, 3, true, fa1, fb1, 0, 0);
     quarter(f1, C0{}, CD{}, CS{}, vm, fa1, fb1, next(s), 0, kt + 1 < nk, fa0, fb0, kt + NS, s);
   };
-  for (int t = 0; t < NS && t < nk; ++t)
-    for (int p = 0; p < (t < NS - 1 ? NP : PD); ++p) fill(t, t * STAGE, p, t < whole);
+  // nothing of the compiler's own may be on its way in the loop: it would wait there for everything that is
+  i8_wait<0, true>();
+  for (int t = 0; t < NS && t < nk; ++t) {
+    [&]<int... P>(std::integer_sequence<int, P...>) {
+      ((P < PD || t < NS - 1 ? fill(t, t * STAGE, std::integral_constant<int, P>{}, t < whole) : void()), ...);
+    }(std::make_integer_sequence<int, NP>{});
+  }
   if (nk >= NS) i8_wait<(NS - 2) * NP + PD, false>();  // slice 0 is there
   else i8_wait<0, false>();
   lds_sync();
@@ -736,7 +749,7 @@ size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 constexpr int64_t kI8MaxK = 131056;
 bool i8_sizes(int64_t R, int64_t K, int64_t N, int64_t E) {
   return R >= 0 && R <= INT32_MAX / 2 && K >= 16 && K % 16 == 0 && K <= kI8MaxK && N >= 8 && N % 8 == 0 && E >= 1 && E <= 1024 &&
-         N * K < ((int64_t)1 << 32) && (E + R / kI8Pass + 1) * ((N + 15) / 16) < INT32_MAX;
+         N * K < ((int64_t)1 << 32) - 4096 && (E + R / kI8Pass + 1) * ((N + 15) / 16) < INT32_MAX;
 }
 }  // namespace
 }  // namespace moe
@@ -795,6 +808,8 @@ extern "C" int moe_swiglu_fwd_int8(const void* xq, const float* sx, int64_t T, c
                     (long long)H, (long long)F, (long long)E, (long long)top_k, (long long)kI8MaxK);
   if (R == 0) return 0;
   if (T == 0) return fail_arg("moe_swiglu_fwd_int8: rows of no token");
+  if (row_slot && T * H >= ((int64_t)1 << 32) - 4096)
+    return fail_arg("moe_swiglu_fwd_int8: T H must be below 2^32 with row_slot, got T=%lld H=%lld", (long long)T, (long long)H);
   if (!xq || !sx || !wg_q || !sg || !wu_q || !su || !wd_q || !sd || !offsets || !y || !al16_i8(xq) || !al16_i8(wg_q) ||
       !al16_i8(wu_q) || !al16_i8(wd_q) || !al16_i8(y) || !al16_i8(workspace))
     return fail_arg("moe_swiglu_fwd_int8: null or misaligned pointer");
