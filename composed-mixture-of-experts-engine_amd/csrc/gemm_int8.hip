@@ -15,12 +15,14 @@
 // loads bytes [16 q, 16 q + 16) of a 64-byte half chunk of row r.  The k slot that a value lands in is free as long as both
 // operands agree.  The waves' partial sums meet in LDS.  Every 64 rows of an expert are a pass of their own blocks over its
 // weights.  Blocks start their chunks at different columns: rows lie a power of two apart, and blocks that walk them in step
-// ask the same few memory channels.  One token, two experts, H 4096, F 14336: 45 us for gate and up (235 MB, 5.2 TB/s), 24 for
-// the down projection (117 MB).
+// ask the same few memory channels.  One token, two experts, H 4096, F 14336: 19 us for the down projection (117 MB, 6.1 TB/s);
+// 4096 x 4096, 64 rows: 9.7 us, where a block's start and its waves' meeting count.
 //
-// More rows (k_i8_tile): both operands from memory straight to LDS.  128 rows on 8 experts of that layer: 160 us for gate and up
-// (940 MB, 5.9 TB/s: all the card reads), 80 for the down projection; 16384 rows: 1.83 ms for gate and up (3.85 Tops, 2.1 Pops/s)
-// and 0.93 ms, where the matrix instructions' power sets the clock (8192^3: 2.39 Pops/s, a library's product 2.41).
+// More rows (k_i8_tile): both operands from memory straight to LDS.  That token's gate and up products: 38 us (235 MB, 6.2
+// TB/s).  128 rows on 8 experts of that layer: 145 us for gate and up (940 MB, 6.5 TB/s: all the card reads), 75 for the down
+// projection; 1024 rows: 230 and 106 us (4.1 TB/s), between the weights' stream and the matrix instructions; 16384 rows: 1.83 ms
+// for gate and up (3.85 Tops, 2.1 Pops/s) and 0.87 ms (2.2), where the matrix instructions' power sets the clock (8192^3: 2.39
+// Pops/s, a library's product 2.41).
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -678,17 +680,19 @@ __global__ __launch_bounds__(256) void k_i8_join(I8Args g, const int* __restrict
 
 // The form of a product, by its sizes alone (the host does not know the rows of each expert).  r: rows an expert that can have
 // any; tiles: of 192 x 128.  Measured (us; E, H, F for both products of the experts, K x N for one):
-//   small | 192 x 128    E 8, H 4096, F 14336, r 2, 8, 16: 222 | 228, 249 | 250, 284 | 249.  E 32, H 2048, F 4096, r 4, 8, 16:
-//                        142 | 163, 149 | 167, 175 | 171
-//   small | 64 x 256     E 128, H 2048, F 768, r 1, 2, 4, 8: 79 | 80, 111 | 119, 122 | 124, 126 | 127; routed with a Zipf(1.1)
-//                        bias, r 2, 4, 8: 54 | 46, 66 | 52, 98 | 78: with many experts an even routing is the exception
-//   64 x 256 | 192 x 128 the same layer, r 16, 32: 131 | 138, 140 | 147; biased 8, 16, 32: 78 | 90, 106 | 100, 120 | 121
-//   small | 192 x 128    little work: 4096 x 4096, 16, 32, 64 rows 6.3 | 13, 9 | 13, 13 | 13; 2048 x 2048, 128, 256 rows 8 | 11,
-//                        13 | 14; E 8, 1024 x 512, r 64, 128: 5.8 | 7.4, 8.8 | 8.6; E 8, 528 x 3088, r 16, 32: 6.7 | 6.8, 9 | 7
-//   192 | deep | 256     E 8, H 4096, F 14336, r 32: 263 | 278 | 298; 64: 334 | 295 | 316; 128: 376 | 351 | 417; 256: 520 | 606 |
-//                        547; 512: 887 | 924 | 904; 1024: 1601 | 1785 | 1554.  E 128, H 2048, F 768 (16 and 6 slices), r 128:
-//                        205 | 244 | 210.  4096 x 14336, 96 to 256 rows 25 | 18 | 26 to 30 | 25 | 45, 512: 40 | 47 | 48,
-//                        1024: 71 | 79 | 60; 4096 x 4096, 2048 rows 43 | 50 | 50
+//   small | 192 x 128    few tiles: E 8, H 4096, F 14336, one token: gate and up (448 tiles) 45 | 36, down (64) 23 | 52.  E 128,
+//                        H 2048, F 768, 8, 16 rows (96 and 128, 192 and 256 tiles): 21 | 24, 27 | 25.  4096 x 4096, 16 rows (32)
+//                        6.3 | 13; 4096 x 14336 (112) 15 | 14
+//   small | 192 x 128    little work: 4096 x 4096, 32, 64 rows 9 | 13, 13 | 13; 2048 x 2048, 128, 256 rows 8 | 11, 13 | 14; E 8,
+//                        1024 x 512, r 64, 128: 5.8 | 7.4, 8.8 | 8.6; E 8, 528 x 3088, r 16, 32: 6.7 | 6.8, 9 | 7
+//   small | 192 | 64     E 8, H 4096, F 14336, r 1, 4, 16: 191 | 182 | 267, 241 | 216 | 284, 282 | 222 | 290.  E 128, H 2048, F 768,
+//                        r 2, 4, 8, 32: 110 | 108 | 107, 122 | 119 | 112, 126 | 122 | 114, 191 | 133 | 125; routed with a Zipf(1.1)
+//                        bias, r 4, 8, 16, 32: 65 | 60 | 55, 100 | 87 | 76, 126 | 95 | 101, 178 | 117 | 117.  E 64, H 2048, F 1408,
+//                        r 6, 24: 110 | 99 | 102, 153 | 106 | 108.  E 32, 1024 x 1024, r 32: 11 | 8 | 11
+//   192 | deep | 256     E 8, H 4096, F 14336, r 16: 222 | 237 | 279; 32: 239 | 254 | 296; 64: 319 | 287 | 316; 128: 374 | 354 |
+//                        411; 256: 520 | 606 | 547; 512: 887 | 924 | 904; 1024: 1601 | 1785 | 1554.  E 128, H 2048, F 768 (16 and
+//                        6 slices), r 128: 205 | 244 | 210.  4096 x 14336, 96 to 256 rows 25 | 18 | 26 to 30 | 25 | 45, 512: 40 |
+//                        47 | 48, 1024: 71 | 79 | 60; 4096 x 4096, 2048 rows 43 | 50 | 50
 //   parts 1 | 2 | 4      14336 x 4096, 64 rows: 35 | 26 | 21; 256: 58 | 39 | 36; 512: 58 | 45 | 54; 4096 x 4096, 64: 13 | 14 | 15
 enum { kSmall, kTile64, kTile192, kTile192Deep, kTile256 };
 struct I8Form {
@@ -697,14 +701,14 @@ struct I8Form {
 };
 I8Form i8_form(int64_t R, int64_t K, int64_t N, int64_t E, bool gu) {
   const int64_t live = std::min(E, R), r = R / live, nk = (K + 127) / 128, cols = gu ? 2 * N : N;
-  if (E < 64 ? r <= 8 : r < 2) return {kSmall, 1};
+  const int64_t tiles = (r + 191) / 192 * live * ((cols + 127) / 128);
+  if (r <= 16 && tiles < 192) return {kSmall, 1};
   if (live * N * K <= (int64_t)1 << 26 && R * K * N <= (int64_t)1 << (live == 1 ? 30 : 28) && (nk < 64 || r <= 16))
     return {kSmall, 1};
   if (r > 512 && (r + 255) / 256 * live * ((cols + 255) / 256) >= 192) return {kTile256, 1};
-  if (E >= 64 && r <= 24) return {kTile64, 1};
-  const int64_t tiles = (r + 191) / 192 * live * ((cols + 127) / 128);
+  if (N * K <= (int64_t)1 << 21 && live * N * K >= (int64_t)1 << 27 && r <= 24) return {kTile64, 1};
   const int parts = !gu && tiles <= 128 && nk >= 64 ? (int)std::min<int64_t>(4, 256 / tiles) : 1;
-  const bool deep = tiles * parts <= 256 || (r > 48 && r <= 160 && nk >= 32);
+  const bool deep = r > 48 && (tiles * parts <= 256 || (r <= 160 && nk >= 32));
   return {deep ? kTile192Deep : kTile192, parts};
 }
 

@@ -20,8 +20,10 @@ FORMS = [
     ("k_i8_small", 144, 264, [1] + [0] * 200 + [1]),  # blocks for the experts with rows alone
     ("k_i8_small", 400, 264, [9, 3, 0, 21] * 20),     # many experts, little to do
     ("k_i8_tile192", 1040, 1032, [9, 3, 0, 21, 64, 65] * 12),
-    ("k_i8_tile64", 1040, 1032, [9, 3, 0, 21, 64, 1, 65, 2] * 9),
-    ("k_i8_tile64", 2048, 768, [2, 0, 200, 1] + [2] * 60),
+    ("k_i8_tile192", 1040, 1032, [9, 3, 0, 21, 64, 1, 65, 2] * 9),
+    ("k_i8_tile192", 2048, 768, [2, 0, 200, 1] + [2] * 60),
+    ("k_i8_tile64", 2048, 1016, [9, 3, 0, 21, 64, 1, 65, 2] * 9),
+    ("k_i8_tile64", 2064, 776, [2, 0, 200, 1] + [3] * 124),
     ("k_i8_tile192", 1040, 4104, [20, 0, 193, 65, 1, 128, 10, 40]),
     ("k_i8_tile192", 2048, 4104, [300, 0, 383, 192, 129, 64, 500, 200]),
     ("k_i8_tile192_deep", 1024, 1032, [400, 0, 129, 64]),   # fewer tiles than CUs
@@ -69,7 +71,8 @@ def test_product(form, K, N, counts, dtype):
 GATE_UP = [
     ("k_i8_small_gu", 144, 80, [8, 0, 7, 1]),
     ("k_i8_small_gu", 272, 144, [9, 3, 0, 21] * 20),
-    ("k_i8_tile64_gu", 1040, 1040, [9, 3, 0, 21, 64, 1] * 12),
+    ("k_i8_tile192_gu", 1040, 1040, [9, 3, 0, 21, 64, 1] * 12),
+    ("k_i8_tile64_gu", 2048, 1008, [9, 3, 0, 21, 64, 1] * 12),
     ("k_i8_tile192_gu", 528, 3088, [20, 0, 193, 65, 1, 128, 10, 40]),
     ("k_i8_small_gu", 528, 1040, [300, 0, 65, 64]),
     ("k_i8_tile192_deep_gu", 528, 2064, [300, 0, 365, 64]),
