@@ -547,6 +547,7 @@ template <int BM, int KIND>
 __device__ __forceinline__ I8Place i8_place(const I8Args& g, int L, int cw, int lane) {
   int e = 0, before = 0, cnt = 0;  // row tiles of the experts before e, and of e
   for (int e0 = 0;; e0 += 64) {
+    if (e0 >= g.E) return I8Place{};  // (only where offsets decrease and the total has overflowed: no rows)
     const int c = i8_row_tiles<BM, KIND>(g, e0 + lane);
     int upto = c;
 #pragma unroll
@@ -619,6 +620,7 @@ __global__ __launch_bounds__(256, BM == 256 || DEEP ? 1 : 2) void k_i8_tile(I8Ar
       at.klen = min(nk * (at.part + 1) / g.parts * 128, g.K) - at.k0;
     }
   }
+  if (at.mlen <= 0) return;
   if constexpr (BM == 256) {
     if (at.mlen > 192) i8_tile<GU, OT, 2, 4, 4, 2, BM != 256>(g, at, smem);
     else if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 4, 2, BM != 256>(g, at, smem);

@@ -235,7 +235,7 @@ extern "C" int moe_dequant_rows(const void* q, int q_format, const float* scale,
     if (dst_dtype == MOE_BF16) MOE_DQ(F8, uint16_t, LPR);       \
     else MOE_DQ(F8, float, LPR);                                \
   } while (0)
-  // lanes a row: 64, 128 or 256, by its 16-element pieces (e4m3, 65536 rows of 2048: 256 lanes 101 us, 128 the better part of it)
+  // lanes a row: 64, 128 or 256, by its 16-element pieces (65536 rows of 2048 e4m3: 256 lanes 101 us, 128 88)
   if (q_format == MOE_E4M3) {
     if (cols <= 1024) MOE_DQ_T(true, 64);
     else if (cols <= 2048) MOE_DQ_T(true, 128);
