@@ -20,7 +20,7 @@
 //
 // More rows (k_i8_tile): both operands from memory straight to LDS.  That token's gate and up products: 38 us (235 MB, 6.2
 // TB/s).  128 rows on 8 experts of that layer: 145 us for gate and up (940 MB, 6.5 TB/s: all the card reads), 75 for the down
-// projection; 1024 rows: 230 and 106 us (4.1 TB/s), between the weights' stream and the matrix instructions; 16384 rows: 1.83 ms
+// projection; 1002 rows: 225 and 105 us (4.2 TB/s), between the weights' stream and the matrix instructions; 16384 rows: 1.83 ms
 // for gate and up (3.85 Tops, 2.1 Pops/s) and 0.87 ms (2.2), where the matrix instructions' power sets the clock (8192^3: 2.39
 // Pops/s, a library's product 2.41).
 #include <algorithm>
@@ -280,6 +280,7 @@ struct I8Place {
   int mlen, n0;   // its rows; its first output column
   int k0, klen;   // the columns of A and B to sum over
   int part;
+  int turn;       // TURN: the eighth of the reduction that it starts with
 };
 
 __device__ __attribute__((aligned(16))) const uint8_t g_i8_zero[16] = {0};
@@ -301,7 +302,7 @@ constexpr int i8_stage() { return (WR * MI + 4 / WR * NI) * 32 * 128; }
 // quarter and a refill piece or two (16 bytes a lane).  The slice's one barrier lies inside its last quarter, when the wave's
 // own LDS reads of the slice have long drained under matrix instructions: behind it slice kt + 1 is complete and slice kt's
 // stage is free for slice kt + NS.
-template <bool GU, typename OT, int WR, int MI, int NI, int NS, bool NT>
+template <bool GU, typename OT, int WR, int MI, int NI, int NS, bool NT, bool TURN>
 __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint8_t* smem) {
   constexpr int WC = 4 / WR, BM = WR * MI * 32, BN = WC * NI * 32;
   constexpr int SA = BM * 128, STAGE = i8_stage<WR, MI, NI>();
@@ -315,6 +316,7 @@ __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint
   const int wm0 = wv / WC * (MI * 32), wn0 = wv % WC * (NI * 32);
   const int i32 = lane & 31, h = lane >> 5;
   const int K = at.klen, nk = (K + 127) / 128, whole = K / 128;
+  const int turn = TURN && whole == nk ? at.turn * (nk / 8) : 0;
 
   // piece p of a wave's share: instruction j fills rows 8 j + lane / 8 of its operand's tile, slot lane % 8 of the row.  Rows
   // past the tile repeat the last one.  A lane's address is a scalar base and an offset of 32 bits of its own that no slice
@@ -352,7 +354,8 @@ __device__ __forceinline__ void i8_tile(const I8Args& g, const I8Place& at, uint
     else off = b_off[q];
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_i8_t*)(smem + s + (IS_A ? 0 : SA) + (j - q % 4) * 1024);
     if (full) {
-      const uint8_t* const at_kt = base - kBias + (int64_t)kt * 128;
+      const int kr = !TURN || kt + turn < nk ? kt + turn : kt + turn - nk;
+      const uint8_t* const at_kt = base - kBias + (int64_t)kr * 128;
       if constexpr (NT && !IS_A)
         __asm__ volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%2 nt" : : "v"(off), "s"(at_kt), "n"(q % 4 * 1024), "{m0}"(lds) : "memory");
       else
@@ -589,7 +592,10 @@ __device__ __forceinline__ I8Place i8_place(const I8Args& g, int L, int cw, int 
 //   256 x 256: many rows.  g.tails: the short tiles of experts' last rows come behind all others, so that they fill the last round.
 //   192 x 128, 64 x 256: few enough that the weights' stream bounds the product; two blocks a CU, for more of it on its way.
 //     DEEP: one block a CU with more slices on their way, where there are no more tiles than CUs.
-template <bool GU, typename OT, int BM, int BN, bool DEEP>
+//     TURN: an expert's tiles start their reductions at different eighths where all of its rows are in one row of tiles: in step,
+//     tiles whose weight rows lie a power of two apart ask the same few memory channels.  (Tiles that share weights stay in step:
+//     14336 x 4096, 512 rows 48 | 68 us.)
+template <bool GU, typename OT, int BM, int BN, bool DEEP, bool TURN>
 __global__ __launch_bounds__(256, BM == 256 || DEEP ? 1 : 2) void k_i8_tile(I8Args g) {
   constexpr int SMEM = BM == 256 ? std::max(3 * i8_stage<1, 4, 2>(), 2 * i8_stage<2, 4, 4>())
                        : DEEP ? 6 * i8_stage<2, 1, 2>() : BM == 192 ? 2 * i8_stage<2, 3, 2>() : 2 * i8_stage<1, 2, 2>();
@@ -621,24 +627,26 @@ __global__ __launch_bounds__(256, BM == 256 || DEEP ? 1 : 2) void k_i8_tile(I8Ar
     }
   }
   if (at.mlen <= 0) return;
+  at.turn = TURN && seg(g, at.e + 1) - seg(g, at.e) <= BM ? slot & 7 : 0;
   if constexpr (BM == 256) {
-    if (at.mlen > 192) i8_tile<GU, OT, 2, 4, 4, 2, BM != 256>(g, at, smem);
-    else if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 4, 2, BM != 256>(g, at, smem);
-    else if (at.mlen > 64) i8_tile<GU, OT, 1, 4, 2, 3, BM != 256>(g, at, smem);
-    else i8_tile<GU, OT, 1, 2, 2, 3, BM != 256>(g, at, smem);
+    if (at.mlen > 192) i8_tile<GU, OT, 2, 4, 4, 2, BM != 256, TURN>(g, at, smem);
+    else if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 4, 2, BM != 256, TURN>(g, at, smem);
+    else if (at.mlen > 64) i8_tile<GU, OT, 1, 4, 2, 3, BM != 256, TURN>(g, at, smem);
+    else i8_tile<GU, OT, 1, 2, 2, 3, BM != 256, TURN>(g, at, smem);
   } else if constexpr (BM == 192) {
-    if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 2, DEEP ? 3 : 2, BM != 256>(g, at, smem);
-    else if (at.mlen > 64) i8_tile<GU, OT, 2, 2, 2, DEEP ? 4 : 2, BM != 256>(g, at, smem);
-    else i8_tile<GU, OT, 2, 1, 2, DEEP ? 6 : 3, BM != 256>(g, at, smem);
+    if (at.mlen > 128) i8_tile<GU, OT, 2, 3, 2, DEEP ? 3 : 2, BM != 256, TURN>(g, at, smem);
+    else if (at.mlen > 64) i8_tile<GU, OT, 2, 2, 2, DEEP ? 4 : 2, BM != 256, TURN>(g, at, smem);
+    else i8_tile<GU, OT, 2, 1, 2, DEEP ? 6 : 3, BM != 256, TURN>(g, at, smem);
   } else {
-    i8_tile<GU, OT, 1, 2, 2, 2, BM != 256>(g, at, smem);
+    i8_tile<GU, OT, 1, 2, 2, 2, BM != 256, TURN>(g, at, smem);
   }
 }
 
-template <bool GU, typename OT, int BM, int BN, bool DEEP = false>
+template <bool GU, typename OT, int BM, int BN, bool DEEP = false, bool TURN = false>
 int launch_tile(hipStream_t s, I8Args a, int parts) {
   constexpr const char* name = BM == 64    ? (GU ? "k_i8_tile64_gu" : "k_i8_tile64")
                                : BM == 256 ? (GU ? "k_i8_tile256_gu" : "k_i8_tile256")
+                               : TURN      ? (GU ? "k_i8_tile192_turn_gu" : "k_i8_tile192_turn")
                                : DEEP      ? (GU ? "k_i8_tile192_deep_gu" : "k_i8_tile192_deep")
                                            : (GU ? "k_i8_tile192_gu" : "k_i8_tile192");
   a.Tn = cdiv(a.N, GU ? BN / 2 : BN);
@@ -646,7 +654,7 @@ int launch_tile(hipStream_t s, I8Args a, int parts) {
   a.parts = parts;
   // the most tiles that any routing can produce, and what rounding two ranges up may add
   const int64_t tiles = (a.offsets ? a.R / BM + std::min<int64_t>(a.E, a.R) : cdiv(a.R, BM)) * a.Tn * parts;
-  MOE_LAUNCH(name, (k_i8_tile<GU, OT, BM, BN, DEEP>), dim3((unsigned)((tiles + 7) / 8 * 8 + 8)), dim3(256), 0, s, a);
+  MOE_LAUNCH(name, (k_i8_tile<GU, OT, BM, BN, DEEP, TURN>), dim3((unsigned)((tiles + 7) / 8 * 8 + 8)), dim3(256), 0, s, a);
   return check_launch(name);
 }
 
@@ -695,8 +703,10 @@ __global__ __launch_bounds__(256) void k_i8_join(I8Args g, const int* __restrict
 //                        411; 256: 520 | 606 | 547; 512: 887 | 924 | 904; 1024: 1601 | 1785 | 1554.  E 128, H 2048, F 768 (16 and
 //                        6 slices), r 128: 205 | 244 | 210.  4096 x 14336, 96 to 256 rows 25 | 18 | 26 to 30 | 25 | 45, 512: 40 |
 //                        47 | 48, 1024: 71 | 79 | 60; 4096 x 4096, 2048 rows 43 | 50 | 50
+//   deep | turn          E 8, H 4096, F 14336, r 50, 64, 96, 128, 150: 270 | 274, 293 | 291, 331 | 327, 363 | 355, 385 | 376.  E 32, H
+//                        2048, F 4096: 176 | 163, 188 | 172, 213 | 203, 234 | 227, 251 | 240.  4096 x 28672, 64 rows 26 | 22
 //   parts 1 | 2 | 4      14336 x 4096, 64 rows: 35 | 26 | 21; 256: 58 | 39 | 36; 512: 58 | 45 | 54; 4096 x 4096, 64: 13 | 14 | 15
-enum { kSmall, kTile64, kTile192, kTile192Deep, kTile256 };
+enum { kSmall, kTile64, kTile192, kTile192Deep, kTile192Turn, kTile256 };
 struct I8Form {
   int kind;
   int parts;  // blocks that a tile's reduction is split over
@@ -711,7 +721,7 @@ I8Form i8_form(int64_t R, int64_t K, int64_t N, int64_t E, bool gu) {
   if (N * K <= (int64_t)1 << 21 && live * N * K >= (int64_t)1 << 27 && r <= 24) return {kTile64, 1};
   const int parts = !gu && tiles <= 128 && nk >= 64 ? (int)std::min<int64_t>(4, 256 / tiles) : 1;
   const bool deep = r > 48 && (tiles * parts <= 256 || (r <= 160 && nk >= 32));
-  return {deep ? kTile192Deep : kTile192, parts};
+  return {!deep ? kTile192 : r <= 192 ? kTile192Turn : kTile192Deep, parts};
 }
 
 template <bool GU, typename OT>
@@ -720,6 +730,7 @@ int launch_form(hipStream_t s, const I8Args& a, const I8Form& f) {
     case kTile64: return launch_tile<GU, OT, 64, 256>(s, a, f.parts);
     case kTile192: return launch_tile<GU, OT, 192, 128>(s, a, f.parts);
     case kTile192Deep: return launch_tile<GU, OT, 192, 128, true>(s, a, f.parts);
+    case kTile192Turn: return launch_tile<GU, OT, 192, 128, true, true>(s, a, f.parts);
     default: return launch_tile<GU, OT, 256, 256>(s, a, f.parts);
   }
 }

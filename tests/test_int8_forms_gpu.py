@@ -26,8 +26,10 @@ FORMS = [
     ("k_i8_tile64", 2064, 776, [2, 0, 200, 1] + [3] * 124),
     ("k_i8_tile192", 1040, 4104, [20, 0, 193, 65, 1, 128, 10, 40]),
     ("k_i8_tile192", 2048, 4104, [300, 0, 383, 192, 129, 64, 500, 200]),
-    ("k_i8_tile192_deep", 1024, 1032, [400, 0, 129, 64]),   # fewer tiles than CUs
-    ("k_i8_tile192_deep", 4112, 8200, [130, 70, 0, 50, 64, 60, 192, 100]),
+    ("k_i8_tile192_deep", 1024, 1032, [400, 0, 500, 64]),   # fewer tiles than CUs
+    ("k_i8_tile192_turn", 1024, 1032, [400, 0, 129, 64]),
+    ("k_i8_tile192_turn", 4096, 4104, [130, 70, 0, 50, 64, 60, 193, 100]),
+    ("k_i8_tile192_turn", 4112, 8200, [130, 70, 0, 50, 64, 60, 192, 100]),
     ("k_i8_tile256", 272, 8200, [513 + 255, 700, 0, 900]),
     ("k_i8_tile256", 1024, 14344, 1025),
     ("k_i8_join", 14336, 520, 130),
@@ -75,8 +77,9 @@ GATE_UP = [
     ("k_i8_tile64_gu", 2048, 1008, [9, 3, 0, 21, 64, 1] * 12),
     ("k_i8_tile192_gu", 528, 3088, [20, 0, 193, 65, 1, 128, 10, 40]),
     ("k_i8_small_gu", 528, 1040, [300, 0, 65, 64]),
-    ("k_i8_tile192_deep_gu", 528, 2064, [300, 0, 365, 64]),
-    ("k_i8_tile192_deep_gu", 4096, 4112, [130, 70, 0, 50, 64, 60, 192, 100]),
+    ("k_i8_tile192_deep_gu", 528, 1040, [300, 0, 565, 64]),
+    ("k_i8_tile192_turn_gu", 528, 2064, [300, 0, 365, 64]),
+    ("k_i8_tile192_turn_gu", 4096, 4112, [130, 70, 0, 50, 64, 60, 192, 100]),
     ("k_i8_tile256_gu", 272, 4112, [513 + 255, 700, 0, 900]),
 ]
 
