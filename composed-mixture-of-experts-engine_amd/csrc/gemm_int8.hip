@@ -20,7 +20,7 @@
 //
 // More rows (k_i8_tile): both operands from memory straight to LDS.  That token's gate and up products: 38 us (235 MB, 6.2
 // TB/s).  128 rows on 8 experts of that layer: 145 us for gate and up (940 MB, 6.5 TB/s: all the card reads), 75 for the down
-// projection; 1002 rows: 225 and 105 us (4.2 TB/s), between the weights' stream and the matrix instructions; 16384 rows: 1.83 ms
+// projection; 1002 rows: 235 and 98 us (4.0 and 4.8 TB/s), between the weights' stream and the matrix instructions; 16384 rows: 1.83 ms
 // for gate and up (3.85 Tops, 2.1 Pops/s) and 0.87 ms (2.2), where the matrix instructions' power sets the clock (8192^3: 2.39
 // Pops/s, a library's product 2.41).
 #include <algorithm>
