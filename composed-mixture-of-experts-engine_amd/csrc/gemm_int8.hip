@@ -591,7 +591,7 @@ __device__ __forceinline__ I8Place i8_place(const I8Args& g, int L, int cw, int 
 // routing can produce; the tiles that there are lie in 8 contiguous ranges, one an XCD (blockIdx mod 8).
 //   256 x 256: many rows.  g.tails: the short tiles of experts' last rows come behind all others, so that they fill the last round.
 //   192 x 128, 64 x 256: few enough that the weights' stream bounds the product; two blocks a CU, for more of it on its way.
-//     DEEP: one block a CU with more slices on their way, where there are no more tiles than CUs.
+//     DEEP: one block a CU with more slices on their way, where there are no more tiles than CUs, or 49 to 160 rows and long sums.
 //     TURN: an expert's tiles start their reductions at different eighths where all of its rows are in one row of tiles: in step,
 //     tiles whose weight rows lie a power of two apart ask the same few memory channels.  (Tiles that share weights stay in step:
 //     14336 x 4096, 512 rows 48 | 68 us.)
