@@ -421,7 +421,6 @@ __global__ __launch_bounds__(256) void k_rmsnorm_ext(NormExtArgs a) {
       for (int i = 0; i < 8; ++i) o[i] = (v[i] * r) * g[i];
     };
     uint32_t mb = 0;
-    float amax = 0.f;
     if constexpr (Q != 0) {
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
@@ -432,24 +431,21 @@ __global__ __launch_bounds__(256) void k_rmsnorm_ext(NormExtArgs a) {
           chunk_store<TX>(orow, lane + 64 * j, 8 * (lane + 64 * j) < H, o, pk);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if constexpr (Q == 1) mb = max(mb, abs_bits(o[i]));
-          else amax = fmaxf(amax, fabsf(o[i]));
-        }
+        for (int i = 0; i < 8; ++i) mb = max(mb, abs_bits(o[i]));
         chunk_fence();
       }
-    }
-    Int8Row qr{};
-    float inv = 0.f;
-    if constexpr (Q == 1) {
       mb = row16_max_u32(mb);
       mb = max(mb, (uint32_t)__shfl_xor((int)mb, 16));
-      qr = int8_row(max(mb, (uint32_t)__shfl_xor((int)mb, 32)));
+      mb = max(mb, (uint32_t)__shfl_xor((int)mb, 32));
+    }
+    Int8Row qr{};
+    E4M3Row er{};
+    if constexpr (Q == 1) {
+      qr = int8_row(mb);
       if (lane == 0) a.scale[t] = qr.scale;
     } else if constexpr (Q == 2) {
-      float sc;
-      e4m3_row_scale(wave_max(amax), sc, inv);
-      if (lane == 0) a.scale[t] = sc;
+      er = e4m3_row(mb);
+      if (lane == 0) a.scale[t] = er.scale;
     }
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
@@ -462,7 +458,7 @@ __global__ __launch_bounds__(256) void k_rmsnorm_ext(NormExtArgs a) {
       } else {
         u32x2 p;
         if constexpr (Q == 1) p = int8_pack8(o, qr);
-        else p = e4m3_pack8(o, inv);
+        else p = e4m3_pack8(o, er);
         if (8 * c < H) *reinterpret_cast<u32x2*>(a.q + (int64_t)t * H + 8 * c) = p;
       }
       frag_load(f, rn, j, lane);

@@ -4,7 +4,11 @@
 // e4m3: scale = absmax / 448 (the largest e4m3 value), element = x * (448 / absmax) in fp32, rounded to nearest even.  A row
 // whose absmax is below 2^-118 -- all-zero rows, and rows so small that 448 / absmax would overflow fp32 (it does below
 // 448 / FLT_MAX ~ 1.3e-36), turning 0 * inv into NaN -- is treated as a zero row: scale 1, inv 1 (its elements, all below
-// 2^-118, round to +-0).
+// 2^-118, round to +-0).  A row of
+// the norm (csrc/norm.hip) that holds an infinity or a NaN has the scale NaN and elements 0, as in int8: an infinity in h makes
+// 1 / rms and every other element zero, and a maximum that passed the NaN over would let the row read back as zeros.
+// (csrc/fp8.hip quantizes rows as they are given: a NaN stays in its element, an infinity gives the scale infinity, and 0 times
+// that reads back as NaN.)
 //
 // int8: scale = a / 127 with a = max(absmax, 2^-100), element = the whole number nearest to 127 x / a, ties to even.  The
 // quotient is taken exactly: x = a / 2 lies on the border between 63 and 64 (common in bf16), and products by a rounded
@@ -31,13 +35,26 @@ __device__ __forceinline__ void e4m3_row_scale(float amax, float& sc, float& inv
   inv = live ? kE4M3Max / amax : 1.f;
 }
 
-__device__ __forceinline__ u32x2 e4m3_pack8(const float (&v)[8], float inv) {
+struct E4M3Row {
+  float scale, inv;
+  uint32_t keep;  // all ones, or 0 for a row that holds an infinity or a NaN
+};
+__device__ __forceinline__ E4M3Row e4m3_row(uint32_t amax_bits) {
+  E4M3Row r;
+  const bool ok = amax_bits < 0x7f800000u;
+  e4m3_row_scale(__uint_as_float(ok ? amax_bits : 0u), r.scale, r.inv);
+  r.scale = ok ? r.scale : __uint_as_float(0x7fc00000u);
+  r.keep = ok ? ~0u : 0u;
+  return r;
+}
+
+__device__ __forceinline__ u32x2 e4m3_pack8(const float (&v)[8], const E4M3Row& r) {
   uint32_t lo = 0, hi = 0;
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, lo, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, lo, true);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, hi, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, hi, true);
-  return u32x2{lo, hi};
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * r.inv, v[1] * r.inv, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * r.inv, v[3] * r.inv, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * r.inv, v[5] * r.inv, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * r.inv, v[7] * r.inv, hi, true);
+  return u32x2{lo & r.keep, hi & r.keep};
 }
 
 // Magnitude bits: their unsigned order is the order of the magnitudes, infinities and NaNs on top (fmaxf drops a NaN).

@@ -286,8 +286,8 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: O
                   fmt: str = "int8", keep_norm: bool = False):
     """The norm of ``x`` [N, H] (of ``h = x + residual`` if given) with its rows in 8 bits, from the normalised values in
     fp32, for serving: ``(q, scale f32 [N], xn or None, h or None)``.  ``q`` [N, H] is int8 (:func:`quant_rows_int8`'s rule) or,
-    for ``fmt="e4m3"``, uint8 e4m3 bytes (:func:`quant_rows_fp8`'s); ``keep_norm`` also returns the rows in ``x``'s dtype,
-    e.g. for the router."""
+    for ``fmt="e4m3"``, uint8 e4m3 bytes (:func:`quant_rows_fp8`'s); in either, a row whose values are not all finite has the
+    scale NaN and elements 0.  ``keep_norm`` also returns the rows in ``x``'s dtype, e.g. for the router."""
     if fmt not in ROW_FORMATS:
         raise ValueError(f"rmsnorm_quant: fmt must be one of {ROW_FORMATS}, got {fmt!r}")
     return L.native().rmsnorm_quant(x, weight, eps, residual, fmt == "e4m3", keep_norm)

@@ -464,8 +464,9 @@ int moe_balance_bwd(const float* logits, const int64_t* counts, const int64_t* t
  *
  * moe_rmsnorm_quant: the norm of x (residual null) or of h = x + residual, its
  * fp32 values quantized by row: int8 (moe_quant_rows_int8) or e4m3
- * (moe_quant_rows_fp8), q [N, H] and scale [N]; xn_out (the rows in x's dtype)
- * may be null, h_out goes with residual.  H % 16 == 0.
+ * (moe_quant_rows_fp8), q [N, H] and scale [N]; a row whose values are not all
+ * finite has the scale NaN and elements 0 in either format.  xn_out (the rows in
+ * x's dtype) may be null, h_out goes with residual.  H % 16 == 0.
  * ---------------------------------------------------------------------- */
 int moe_rmsnorm_fwd(const void* x, int x_dtype, const void* gamma, int gamma_dtype, float eps, int64_t N,
                     int64_t H, void* xn_out, float* rstd_out, void* stream);

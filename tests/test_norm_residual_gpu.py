@@ -247,3 +247,34 @@ def test_refusals():
         ops.rmsnorm_residual_backward(h, w, rstd[:2], dxn, dh)
     with pytest.raises(RuntimeError, match="AMD Instinct"):
         ops.rmsnorm_quant(x.cpu(), w.cpu(), EPS)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
+@pytest.mark.parametrize("H", [64, 512, 2064, 8192])
+def test_rows_in_8_bits_that_are_not_finite(H, dtype, fmt):
+    """A row with an infinity or a NaN, before or after the residual's addition or made by the weight, has the scale NaN and
+    elements 0, so that all of it reads back as NaNs; the others keep their bits."""
+    x, r, _, _, w = _case(11, H, dtype, seed=3)
+    x[1] = 0
+    r[1] = 0
+    clean = ops.rmsnorm_quant(x, w, EPS, residual=r, fmt=fmt, keep_norm=True)
+    x[4, 7] = float("nan")
+    r[6, 1] = float("inf")
+    x[7, H - 1] = -float("inf")
+    x[8, 0], r[8, 0] = float("inf"), -float("inf")
+    x[9, :] = float("nan")
+    q, s, xn, h = ops.rmsnorm_quant(x, w, EPS, residual=r, fmt=fmt, keep_norm=True)
+    bad = torch.zeros(11, dtype=torch.bool, device=dev())
+    bad[[4, 6, 7, 8, 9]] = True
+    assert torch.isnan(s[bad]).all() and (q[bad] == 0).all()
+    assert torch.isnan(ops.dequant_rows(q, s, torch.float32)[bad]).all()
+    for a, b in zip((q, s, xn, h), clean):
+        assert torch.equal(a[~bad], b[~bad])
+    # the rows kept beside them are those of the norm alone
+    assert torch.equal(torch.nan_to_num(xn.float(), nan=777.0), torch.nan_to_num(ops.rmsnorm_forward(h, w, EPS)[0].float(), nan=777.0))
+    # finite rows whose normalised values are not
+    wbad = w.clone()
+    wbad[5] = float("inf")
+    q, s, _, _ = ops.rmsnorm_quant(r[:4], wbad, EPS, fmt=fmt)
+    assert torch.isnan(s).all() and (q == 0).all()  # (row 1: 0 times infinity)
