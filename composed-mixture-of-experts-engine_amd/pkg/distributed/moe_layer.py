@@ -514,6 +514,9 @@ class DistributedMoELayer(nn.Module):
         """Take ``(gate, up, down)`` and their scales for :meth:`forward_int8`: what :meth:`quantize_int8` returned, or weights
         quantized elsewhere (int8 [E, F, H], [E, F, H] and [E, H, F]; float32 [E, F], [E, F] and [E, H]).  They are kept as they
         are, on the router's device.  A layer that only serves them may drop its full-width parameters.  Returns them."""
+        weights, scales = list(weights), list(scales)
+        if len(weights) != 3 or len(scales) != 3:
+            raise ValueError(f"load_int8: takes (gate, up, down) and three scales, got {len(weights)} and {len(scales)}")
         E, F_, H = len(self.local_expert_ids), self.ffn_dim, self.hidden_dim
         for name, w, s, shape in zip(("gate", "up", "down"), weights, scales, ((E, F_, H), (E, F_, H), (E, H, F_))):
             if w.dtype != torch.int8 or s.dtype != torch.float32:

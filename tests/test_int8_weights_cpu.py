@@ -137,3 +137,19 @@ def test_c_abi_refuses_before_it_launches():
     bad(lib.moe_rmsnorm_quant(P, None, 1, P, 0, 1e-5, 4, 64, 5, P, P, None, None, None), "int8 or e4m3")
     bad(lib.moe_rmsnorm_quant(P, None, 1, P, 0, 1e-5, 4, 24, 0, P, P, None, None, None), "H % 16")
     bad(lib.moe_rmsnorm_quant(P, P, 1, P, 0, 1e-5, 4, 64, 0, P, P, None, None, None), "null")  # a residual without h
+
+
+def test_load_takes_three_weights_and_three_scales():
+    layer = _layer()
+    q, s = _weights()
+    for weights, scales in ((q[:2], s[:2]), (q, s[:2]), (q[:2], s), ([*q, q[2]], s), (q, [*s, s[2]]), ([*q, q[2]], [*s, s[2]]),
+                            ((), ())):
+        with pytest.raises(ValueError, match="load_int8"):
+            layer.load_int8(weights, scales)
+        assert all(t is None for n, t in layer._buffers.items() if "int8" in n)
+    got = layer.load_int8(iter(q), iter(s))
+    assert all(torch.equal(a, b) for a, b in zip(got[0] + got[1], q + s))
+    with pytest.raises(ValueError, match="load_int8"):  # what is there stays
+        layer.load_int8(q[:2], s[:2])
+    got = layer._int8_weights()
+    assert all(torch.equal(a, b) for a, b in zip(got[0] + got[1], q + s))
