@@ -852,8 +852,8 @@ __global__ __launch_bounds__(256) void k_rmsnorm_residual_bwd(NormBwdArgs a, int
   };
   auto load = [&](Row& w, int t) {
     const bool in = t < N;
-    auto one = [&](RowFrag<TX, NCH>& f, const void* base) {  // a null gradient, or a row past N, reads as zeros
-      const buf_rsrc_t rs = buf_rsrc(base ? static_cast<const TX*>(base) + (int64_t)t * H : a.x, base && in ? rowbytes : 0);
+    auto one = [&](RowFrag<TX, NCH>& f, const void* base) {  // a row past N reads as zeros
+      const buf_rsrc_t rs = buf_rsrc(static_cast<const TX*>(base) + (int64_t)t * H, in ? rowbytes : 0);
 #pragma unroll
       for (int j = 0; j < NCH; ++j)
 #pragma unroll
@@ -911,6 +911,12 @@ __global__ __launch_bounds__(256) void k_rmsnorm_residual_bwd(NormBwdArgs a, int
       reinterpret_cast<f32x4*>(d)[1] = f32x4{dg[j][4], dg[j][5], dg[j][6], dg[j][7]};
     }
   }
+}
+
+// n 16-byte words.
+__global__ __launch_bounds__(256) void k_copy16(const u32x4* __restrict__ src, u32x4* __restrict__ dst, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    __builtin_nontemporal_store(__builtin_nontemporal_load(src + i), dst + i);
 }
 
 // dgamma[h] = sum over blocks b of part_dg[b][h] in a fixed order.  Block = 32 columns x 32 groups of
@@ -1282,6 +1288,13 @@ extern "C" int moe_rmsnorm_residual_bwd(const void* h, int x_dtype, const void* 
   const int nblk = H <= 512 ? norm_bwd_blocks(N) : residual_bwd_blocks(N);
   if (ws_bytes < moe_rmsnorm_residual_bwd_workspace(N, H) || !workspace)
     return set_error("moe_rmsnorm_residual_bwd: workspace too small"), MOE_EWORKSPACE;
+  if (!dxn) {  // d = dh and dgamma = 0, whatever h holds (zeros times an infinity would not be zeros)
+    const int64_t n = N * H * (x_dtype == MOE_BF16 ? 2 : 4) / 16;
+    MOE_LAUNCH("k_copy16", k_copy16, dim3((unsigned)std::min<int64_t>(2048, (n + 255) / 256)), dim3(256), 0, s,
+               static_cast<const u32x4*>(dh), static_cast<u32x4*>(d_out), n);
+    if (int rc = check_launch("k_copy16")) return rc;
+    return launch_dgamma(s, nullptr, 0, H, dgamma_out, gamma_dtype);
+  }
   NormBwdArgs a{};
   a.x = h;
   a.gamma = gamma;

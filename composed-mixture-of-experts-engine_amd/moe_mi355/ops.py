@@ -275,7 +275,8 @@ def rmsnorm_residual_forward(x: torch.Tensor, residual: torch.Tensor, weight: to
 def rmsnorm_residual_backward(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, dxn: Optional[torch.Tensor],
                               dh: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
     """Backward of :func:`rmsnorm_residual_forward` for the gradients of ``xn`` and of ``h`` (either may be None):
-    ``(d, dweight)``, ``d`` the gradient of ``x`` and of ``residual`` alike."""
+    ``(d, dweight)``, ``d`` the gradient of ``x`` and of ``residual`` alike.  Without ``dxn``, ``d`` is ``dh`` and ``dweight``
+    zero, whatever ``h`` holds."""
     return L.native().rmsnorm_residual_backward(h, weight, rstd, dxn, dh)
 
 

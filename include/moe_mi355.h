@@ -460,7 +460,8 @@ int moe_balance_bwd(const float* logits, const int64_t* counts, const int64_t* t
  * moe_rmsnorm_residual_fwd: h = x + residual (the sum of L:125-126, left by one
  * block to the next one's norm), rounded to x's dtype, and moe_rmsnorm_fwd of
  * h, in one kernel.  moe_rmsnorm_residual_bwd: d = dh + the norm's gradient,
- * the gradient of x and of residual alike (dxn or dh may be null, not both).
+ * the gradient of x and of residual alike (dxn or dh may be null, not both;
+ * without dxn d is dh and dgamma zero, whatever h holds).
  *
  * moe_rmsnorm_quant: the norm of x (residual null) or of h = x + residual, its
  * fp32 values quantized by row: int8 (moe_quant_rows_int8) or e4m3

@@ -278,3 +278,18 @@ def test_rows_in_8_bits_that_are_not_finite(H, dtype, fmt):
     wbad[5] = float("inf")
     q, s, _, _ = ops.rmsnorm_quant(r[:4], wbad, EPS, fmt=fmt)
     assert torch.isnan(s).all() and (q == 0).all()  # (row 1: 0 times infinity)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f32"])
+@pytest.mark.parametrize("N,H", [(1, 8), (7, 64), (6, 520), (1030, 2048), (5, 8192)], ids=str)
+def test_backward_of_the_sum_alone(N, H, dtype):
+    """Without a gradient of the norm's output d is dh and dweight zero, whatever h holds (a padded row's values, say)."""
+    x, r, _, dh, w = _case(N, H, dtype, seed=8)
+    x[0, 0] = float("nan")
+    r[N // 2, H - 1] = float("inf")
+    r[N - 1, 3] = -float("inf")
+    _, h, rstd = ops.rmsnorm_residual_forward(x, r, w, EPS)
+    for wd in (w, w.bfloat16()):
+        d, dw = ops.rmsnorm_residual_backward(h, wd, rstd, None, dh)
+        assert torch.equal(d, dh) and d.data_ptr() != dh.data_ptr()
+        assert dw.dtype == wd.dtype and (dw == 0).all()
