@@ -649,6 +649,7 @@ int launch_tile(hipStream_t s, I8Args a, int parts) {
                                : TURN      ? (GU ? "k_i8_tile192_turn_gu" : "k_i8_tile192_turn")
                                : DEEP      ? (GU ? "k_i8_tile192_deep_gu" : "k_i8_tile192_deep")
                                            : (GU ? "k_i8_tile192_gu" : "k_i8_tile192");
+  static_assert(BM == 192 || !std::is_same_v<OT, int>, "no product splits the reduction of other tiles");
   a.Tn = cdiv(a.N, GU ? BN / 2 : BN);
   a.tails = parts == 1 && a.R >= 512 * (int64_t)a.E;
   a.parts = parts;
@@ -724,15 +725,19 @@ I8Form i8_form(int64_t R, int64_t K, int64_t N, int64_t E, bool gu) {
   return {!deep ? kTile192 : r <= 192 ? kTile192Turn : kTile192Deep, parts};
 }
 
+// A product's tiles; a split reduction's int32 sums (OT int) are made by the 192 x 128 forms alone, i8_form's only ones with parts.
 template <bool GU, typename OT>
 int launch_form(hipStream_t s, const I8Args& a, const I8Form& f) {
   switch (f.kind) {
-    case kTile64: return launch_tile<GU, OT, 64, 256>(s, a, f.parts);
     case kTile192: return launch_tile<GU, OT, 192, 128>(s, a, f.parts);
     case kTile192Deep: return launch_tile<GU, OT, 192, 128, true>(s, a, f.parts);
     case kTile192Turn: return launch_tile<GU, OT, 192, 128, true, true>(s, a, f.parts);
-    default: return launch_tile<GU, OT, 256, 256>(s, a, f.parts);
   }
+  if constexpr (!std::is_same_v<OT, int>) {
+    if (f.kind == kTile64) return launch_tile<GU, OT, 64, 256>(s, a, f.parts);
+    if (f.kind == kTile256) return launch_tile<GU, OT, 256, 256>(s, a, f.parts);
+  }
+  return fail_arg("int8 product: no tiles for form %d in %d parts", f.kind, f.parts);
 }
 
 template <bool GU, typename OT>
