@@ -407,3 +407,35 @@ def test_refusals():
     with pytest.raises(ValueError, match="row_slot must be"):
         ops.swiglu_forward_int8(q, s, eq, es, offs, row_slot=torch.zeros(8, dtype=torch.int32, device=dev()), top_k=0)
     assert ops.swiglu_forward_int8(q[:0], s[:0], eq, es, offs * 0).shape == (0, 96)
+
+
+def _lowest(shape, seed):
+    """Any int8 values, -128 (which quantization never writes) often among them."""
+    q = torch.randint(-128, 128, shape, device=dev(), generator=_gen(seed), dtype=torch.int8)
+    return torch.where(torch.rand(shape, device=dev(), generator=_gen(seed + 1)) < 0.25, -128, q.int()).to(torch.int8)
+
+
+@pytest.mark.parametrize("R,K,N", [(1, 4096, 4096), (16, 48, 16), (64, 4096, 4096), (300, 2048, 1032), (1100, 1024, 1544),
+                                   (64, 14336, 520), (3, 131056, 16), (70, 131056, 1024)], ids=str)
+def test_product_of_the_lowest_values(R, K, N):
+    """Weights and rows of -128: scales of 1, so the result is the sum, rounded to fp32 once.  Its largest, 128 * 128 * 131056, is
+    below 2^31."""
+    say(f"[int8 -128] R={R} K={K} N={N}")
+    q, wq = _lowest((R, K), 1), _lowest((N, K), 2)
+    q[0] = wq[0] = wq[N - 1] = -128
+    y = ops.matmul_int8(q, torch.ones(R, device=dev()), wq, torch.ones(N, device=dev()), out_dtype=torch.float32)
+    want = (q.double() @ wq.double().T).float()  # whole numbers below 2^53: exact
+    assert torch.equal(y, want)
+
+
+def test_experts_on_the_lowest_values():
+    E, H, F, counts = 4, 272, 144, [3, 0, 70, 17]
+    wq = [_lowest(sh, 3 + i) for i, sh in enumerate(((E, F, H), (E, F, H), (E, H, F)))]
+    ws = [torch.rand(t.shape[:2], device=dev(), generator=_gen(9)) * 1e-3 + 1e-4 for t in wq]
+    for t in wq:
+        t[:, 1] = -128
+    offs = torch.tensor([0] + list(torch.tensor(counts).cumsum(0)), dtype=torch.int32)
+    q, s = _lowest((sum(counts), H), 20), torch.rand(sum(counts), device=dev(), generator=_gen(21)) * 0.02 + 1e-3
+    y = ops.swiglu_forward_int8(q, s, wq, ws, offs.to(dev()))
+    want, tol = OI.swiglu_fwd(q, s, wq, ws, offs.tolist())
+    assert float(((y.double() - want).abs() / tol).max()) <= 1.0

@@ -291,3 +291,68 @@ def test_sequences_and_masks_pass_through():
             call(x, residual=x, token_mask=mask)
             losses.append(float(block.moe.router.last_seq_balance_loss))
     assert losses[0] == losses[1] == losses[2] > 0.0
+
+
+def _block(H, F, E, K, layout, drops):
+    torch.manual_seed(11)
+    block = ToyMoEBlock(H, F, E, K, build_topology(), dtype=B, layout=layout, capacity_dropping=drops, capacity_factor=1.0,
+                        check_numerics=False).to(dev())
+    with torch.no_grad():
+        block.norm.weight.add_(0.1 * torch.randn(H, device=dev(), generator=_gen(5)))
+    return block
+
+
+LAYOUTS = [("routed", False), ("reference", False), ("routed", True), ("reference", True)]
+
+
+@pytest.mark.parametrize("layout,drops", LAYOUTS)
+@pytest.mark.parametrize("N", [1, 37, 600])
+def test_block_in_e4m3_is_its_parts(N, layout, drops):
+    """The block on the norm's e4m3 rows: each slot's row and scale placed where the plan says, the experts' products and the
+    combine, bit for bit.  Every row has a largest value, and so a scale, of its own: another row's would show."""
+    H, F, E, K = 256, 384, 8, 2
+    say(f"[block e4m3] N={N} {layout} drops={drops}")
+    block = _block(H, F, E, K, layout, drops)
+    x = torch.randn(N, H, device=dev(), generator=_gen(N)).to(B)
+    r = torch.randn(N, H, device=dev(), generator=_gen(N + 1)).to(B)
+    r[:, 0] += torch.exp2(torch.arange(N, device=dev()) % 9.0).to(B) * 4  # the largest of a row by another factor each
+    out, h = block.forward_fp8(x, residual=r)
+    p = block.moe.last_plan
+    q, s, xn, hq = ops.rmsnorm_quant(x, block.norm.weight, block.norm.eps, residual=r, fmt="e4m3", keep_norm=True)
+    assert torch.equal(h, hq)
+    with torch.no_grad():
+        w = block.moe.router(xn)[1]
+    row = p.slot_row.long().reshape(N, K)
+    used = int(p.offsets[-1])
+    xq, sx = torch.zeros(p.rows, H, dtype=torch.uint8, device=dev()), torch.ones(p.rows, device=dev())
+    for k in range(K):
+        live = (row[:, k] >= 0) & (row[:, k] < used)
+        xq[row[live, k]], sx[row[live, k]] = q[live], s[live]
+    if drops and N > 1:
+        assert bool(p.drop.any()) if p.drop is not None else used < N * K
+    wq, ws = block.moe.quantize_fp8()
+    y = ops.swiglu_forward_fp8(xq, sx, wq, ws, p.offsets, keep_preact=False)[2]
+    want = ops.combine(y, w, p)
+    assert torch.equal(out, want)
+    if N >= 37:
+        assert len(s.unique()) >= 9  # rows that differ
+
+
+@pytest.mark.parametrize("layout,drops", LAYOUTS)
+@pytest.mark.parametrize("N", [1, 37, 600])
+def test_block_in_int8_with_layouts_and_drops(N, layout, drops):
+    H, F, E, K = 256, 384, 8, 2
+    say(f"[block int8] N={N} {layout} drops={drops}")
+    block = _block(H, F, E, K, layout, drops)
+    block.moe.quantize_int8()
+    x = torch.randn(N, H, device=dev(), generator=_gen(N)).to(B)
+    r = torch.randn(N, H, device=dev(), generator=_gen(N + 1)).to(B)
+    r[:, 0] += torch.exp2(torch.arange(N, device=dev()) % 9.0).to(B) * 4
+    out, h = block.forward_int8(x, residual=r)
+    p = block.moe.last_plan
+    q, s, xn, hq = ops.rmsnorm_quant(x, block.norm.weight, block.norm.eps, residual=r, keep_norm=True)
+    assert torch.equal(h, hq)
+    with torch.no_grad():
+        w = block.moe.router(xn)[1]
+    ref, tol = _combined(block.moe, p, w, *_experts(block.moe, q, s, p))
+    assert float(((out.double() - ref).abs() / tol).max()) <= 1.0
