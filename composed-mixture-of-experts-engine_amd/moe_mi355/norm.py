@@ -39,11 +39,17 @@ class RMSNormFn(torch.autograd.Function):
 
 
 class RMSNormResidualFn(torch.autograd.Function):
-    """(x [N,H], residual [N,H], weight [H], eps) -> (xn [N,H], h [N,H])."""
+    """(x [..., H], residual of x's shape, weight [H], eps) -> (xn, h) of x's shape.
+
+    x and residual have one gradient, returned as one tensor: autograd then sees that it is shared and copies it before a leaf
+    keeps it.  (Views of it, which reshapes outside would make, are taken over by both leaves: the next backward would add to
+    the same memory twice.)"""
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps: float):
-        xn, h, rstd = ops.rmsnorm_residual_forward(x, residual, weight, eps)
+        H = x.shape[-1]
+        xn, h, rstd = ops.rmsnorm_residual_forward(x.reshape(-1, H), residual.reshape(-1, H), weight, eps)
+        xn.resize_(x.shape), h.resize_(x.shape)  # (not views: a view made in here could not be written in place)
         ctx.save_for_backward(h, weight, rstd)
         ctx.set_materialize_grads(False)
         return xn, h
@@ -54,7 +60,10 @@ class RMSNormResidualFn(torch.autograd.Function):
         if dxn is None and dh is None:
             return None, None, None, None
         h, weight, rstd = ctx.saved_tensors
-        d, dweight = ops.rmsnorm_residual_backward(h, weight, rstd, dxn, dh)
+        rows = (rstd.shape[0], h.shape[-1])
+        d, dweight = ops.rmsnorm_residual_backward(h.reshape(rows), weight, rstd, None if dxn is None else dxn.reshape(rows),
+                                                   None if dh is None else dh.reshape(rows))
+        d = d.reshape(h.shape)
         need_x, need_r, need_w, _ = ctx.needs_input_grad
         return (d if need_x else None), (d if need_r else None), (dweight if need_w else None), None
 

@@ -47,8 +47,7 @@ class RMSNorm(nn.Module):
             return RMSNormFn.apply(x.reshape(-1, H), self.weight, self.eps).reshape(x.shape)
         if residual.shape != x.shape:
             raise ValueError(f"residual must be {list(x.shape)}, got {list(residual.shape)}")
-        xn, h = RMSNormResidualFn.apply(x.reshape(-1, H), residual.reshape(-1, H), self.weight, self.eps)
-        return xn.reshape(x.shape), h.reshape(x.shape)
+        return RMSNormResidualFn.apply(x, residual, self.weight, self.eps)
 
     @torch.no_grad()
     def quantized(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, fmt: str = "int8"):

@@ -356,3 +356,49 @@ def test_block_in_int8_with_layouts_and_drops(N, layout, drops):
         w = block.moe.router(xn)[1]
     ref, tol = _combined(block.moe, p, w, *_experts(block.moe, q, s, p))
     assert float(((out.double() - ref).abs() / tol).max()) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", [B, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape", [(6, 64), (2, 3, 64), (2, 1, 5, 528)], ids=str)
+def test_gradients_accumulate_apart(shape, dtype):
+    """x and the residual have one gradient; as leaves each keeps its own, and a second backward adds to each once."""
+    norm = RMSNorm(shape[-1]).to(dev())
+    x, r, gx, gh = (torch.randn(shape, device=dev(), generator=_gen(i)).to(dtype) for i in range(4))
+    for run in (lambda a, b: norm(a, residual=b), lambda a, b: norm(a, residual=b)[1:], lambda a, b: norm(a, residual=b)[:1]):
+        x, r = x.detach().requires_grad_(), r.detach().requires_grad_()
+        outs = run(x, r)
+        once = torch.autograd.grad(outs, [x, r], ([gx, gh] if len(outs) == 2 else [gx]))
+        assert torch.equal(once[0], once[1])
+        for _ in range(2):
+            outs = run(x, r)
+            torch.autograd.backward(outs, [gx, gh] if len(outs) == 2 else [gx])
+        assert x.grad.untyped_storage().data_ptr() != r.grad.untyped_storage().data_ptr()
+        assert torch.equal(x.grad, once[0] + once[0]) and torch.equal(r.grad, once[0] + once[0])
+        x.grad.zero_()
+        assert torch.equal(r.grad, once[0] + once[0])
+
+
+def test_a_blocks_gradients_accumulate_apart():
+    blocks, _ = _stack(1, 128, 96, 4, 2, torch.float32)
+    x, r = (torch.randn(2, 20, 128, device=dev(), generator=_gen(i)).requires_grad_() for i in range(2))
+    g = torch.randn(2, 20, 128, device=dev(), generator=_gen(3))
+    once = torch.autograd.grad(blocks[0](x, residual=r), [x, r], [g, g])
+    for _ in range(2):
+        torch.autograd.backward(blocks[0](x, residual=r), [g, g])
+    for t in (x, r):
+        assert float((t.grad - 2 * once[0]).abs().max()) <= 1e-5 * float(once[0].abs().max())
+
+
+@pytest.mark.parametrize("shape", [(6, 64), (2, 3, 64)], ids=str)
+def test_outputs_written_in_place(shape):
+    """The normalised rows may be written in place; writing the sum, which the backward reads, is noticed."""
+    norm = RMSNorm(shape[-1]).to(dev())
+    x, r, g = (torch.randn(shape, device=dev(), generator=_gen(i)) for i in range(3))
+    x.requires_grad_()
+    want = torch.autograd.grad(norm(x, residual=r)[0], x, 3 * g)[0]
+    y = norm(x, residual=r)[0].mul_(3)
+    assert torch.equal(torch.autograd.grad(y, x, g)[0], want)
+    y, h = norm(x, residual=r)
+    h.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward(g)
