@@ -15,14 +15,15 @@
 // loads bytes [16 q, 16 q + 16) of a 64-byte half chunk of row r.  The k slot that a value lands in is free as long as both
 // operands agree.  The waves' partial sums meet in LDS.  Every 64 rows of an expert are a pass of their own blocks over its
 // weights.  Blocks start their chunks at different columns: rows lie a power of two apart, and blocks that walk them in step
-// ask the same few memory channels.  One token, two experts, H 4096, F 14336: 19 us for the down projection (117 MB, 6.1 TB/s);
-// 4096 x 4096, 64 rows: 9.7 us, where a block's start and its waves' meeting count.
+// ask the same few memory channels.  One token, two experts, H 4096, F 14336: 24 us for the down projection (117 MB, 5.0 TB/s),
+// 19 us on the experts of the call before, which the 256 MB cache still holds in part; 4096 x 4096, 16, 32, 64 rows: 7, 10, 14 us,
+// where a block's start and its waves' meeting count.
 //
-// More rows (k_i8_tile): both operands from memory straight to LDS.  That token's gate and up products: 38 us (235 MB, 6.2
-// TB/s).  128 rows on 8 experts of that layer: 145 us for gate and up (940 MB, 6.5 TB/s: all the card reads), 75 for the down
-// projection; 1002 rows: 235 and 98 us (4.0 and 4.8 TB/s), between the weights' stream and the matrix instructions; 16384 rows: 1.83 ms
-// for gate and up (3.85 Tops, 2.1 Pops/s) and 0.87 ms (2.2), where the matrix instructions' power sets the clock (8192^3: 2.39
-// Pops/s, a library's product 2.41).
+// More rows (k_i8_tile): both operands from memory straight to LDS.  That token's gate and up products: 40 us (235 MB, 5.9
+// TB/s), 38 us on the same experts again.  128 rows on 8 experts of that layer: 145 us for gate and up (940 MB, 6.5 TB/s: all the
+// card reads), 75 for the down projection; 1002 rows: 235 and 98 us (4.0 and 4.8 TB/s), between the weights' stream and the matrix
+// instructions; 16384 rows: 1.83 ms for gate and up (3.85 Tops, 2.1 Pops/s) and 0.87 ms (2.2), where the matrix instructions' power
+// sets the clock (8192^3: 2.39 Pops/s, a library's product 2.41).
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -691,15 +692,23 @@ __global__ __launch_bounds__(256) void k_i8_join(I8Args g, const int* __restrict
 
 // The form of a product, by its sizes alone (the host does not know the rows of each expert).  r: rows an expert that can have
 // any; tiles: of 192 x 128.  Measured (us; E, H, F for both products of the experts, K x N for one):
-//   small | 192 x 128    few tiles: E 8, H 4096, F 14336, one token: gate and up (448 tiles) 45 | 36, down (64) 23 | 52.  E 128,
+//   small | 192 x 128    few tiles: E 8, H 4096, F 14336, one token: gate and up (448 tiles) 47 | 40, down (64) 24 | 53.  E 128,
 //                        H 2048, F 768, 8, 16 rows (96 and 128, 192 and 256 tiles): 21 | 24, 27 | 25.  4096 x 4096, 16 rows (32)
-//                        6.3 | 13; 4096 x 14336 (112) 15 | 14
-//   small | 192 x 128    little work: 4096 x 4096, 32, 64 rows 9 | 13, 13 | 13; 2048 x 2048, 128, 256 rows 8 | 11, 13 | 14; E 8,
+//                        7 | 13; 4096 x 14336 (112) 15 | 14
+//   small | 192 x 128    little work: 4096 x 4096, 32, 64 rows 10 | 13, 14 | 13; 2048 x 2048, 128, 256 rows 8 | 11, 13 | 14; E 8,
 //                        1024 x 512, r 64, 128: 5.8 | 7.4, 8.8 | 8.6; E 8, 528 x 3088, r 16, 32: 6.7 | 6.8, 9 | 7
 //   small | 192 | 64     E 8, H 4096, F 14336, r 1, 4, 16: 191 | 182 | 267, 241 | 216 | 284, 282 | 222 | 290.  E 128, H 2048, F 768,
 //                        r 2, 4, 8, 32: 110 | 108 | 107, 122 | 119 | 112, 126 | 122 | 114, 191 | 133 | 125; routed with a Zipf(1.1)
 //                        bias, r 4, 8, 16, 32: 65 | 60 | 55, 100 | 87 | 76, 126 | 95 | 101, 178 | 117 | 117.  E 64, H 2048, F 1408,
 //                        r 6, 24: 110 | 99 | 102, 153 | 106 | 108.  E 32, 1024 x 1024, r 32: 11 | 8 | 11
+//   192 | 64             small experts, both products with r 2, 8, 16, 24: E 64, H 2048, F 1024: 69 | 62, 82 | 70, 83 | 72, 86 | 74;
+//                        E 96, 1024, 2048: 106 | 96, 119 | 108, 123 | 113, 130 | 120; E 128, 1024, 1024: 79 | 69, 86 | 76, 88 | 78,
+//                        92 | 82; E 160, 1536, 768: 108 | 96, 118 | 106, 123 | 111, 128 | 115; E 256, 2048, 512: 158 | 132, 171 | 148,
+//                        177 | 154, 182 | 160; E 512, 1024, 256: 140 | 97, 155 | 107, 162 | 113, 166 | 118; E 128, 4096, 512: 163 |
+//                        156, 178 | 176, 184 | 182, 187 | 185.  Routed with a Zipf(1.1) bias, r 2, 8, 24: E 128, 1024, 1024: 59 | 57,
+//                        85 | 71, 105 | 101; E 256, 2048, 512: 94 | 78, 156 | 133, 199 | 181; E 160, 1536, 768: 78 | 83, 112 | 100,
+//                        135 | 139.  Behind with columns that fill no whole tile (E 72, 2048, 1008: 85 | 83, 103 | 116, 105 | 118,
+//                        108 | 120) and with fewer weights than the rule asks for (E 64, 1408, 1408: 69 | 72, 75 | 77, 78 | 78, 82 | 81)
 //   192 | deep | 256     E 8, H 4096, F 14336, r 16: 222 | 237 | 279; 32: 239 | 254 | 296; 64: 319 | 287 | 316; 128: 374 | 354 |
 //                        411; 256: 520 | 606 | 547; 512: 887 | 924 | 904; 1024: 1601 | 1785 | 1554.  E 128, H 2048, F 768 (16 and
 //                        6 slices), r 128: 205 | 244 | 210.  4096 x 14336, 96 to 256 rows 25 | 18 | 26 to 30 | 25 | 45, 512: 40 |
